@@ -425,6 +425,74 @@ int qlin_get_device_error(void* stream, int clear, int* device_status);
 int qlin_gather_columns(int dtype, const void* src, void* dst, int64_t G, int64_t M,
                         int64_t n_shard, int64_t ld_dst, void* stream);
 
+/*
+ * 4-bit quaternion weights (OCP microscaling MXFP4): e2m1 elements, one E8M0
+ * scale for each 32 consecutive input quaternions of one component row
+ * W_p[o, :].  The scale is 2^(floor(log2 max|w|) - 2); elements are rounded to
+ * nearest, ties to even, and saturate at 6 scales.  A block that holds an
+ * infinity or a NaN stands for NaNs.
+ *
+ * qlin_mx_weights_size: bytes of the buffer of a layer (about 4.25 bits a
+ * weight); the buffer is 128-byte aligned, its contents opaque and the same
+ * on every device.
+ * qlin_mx_quantize: the four components [N_g, K_g] (leading dimension ld_w)
+ * into the buffer mx.
+ * qlin_mx_dequantize: the values that the codes stand for, rounded once to
+ * dtype, as four component tensors.
+ */
+int qlin_mx_weights_size(int64_t K_g, int64_t N_g, size_t* bytes);
+int qlin_mx_quantize(int dtype,
+                     const void* wr, const void* wi, const void* wj, const void* wk, int64_t ld_w,
+                     int64_t K_g, int64_t N_g, void* mx, void* stream);
+int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g,
+                       void* wr, void* wi, void* wj, void* wk, int64_t ld_w, void* stream);
+
+/*
+ * qlin_forward with 4-bit weights:
+ *     y = QuaternionLinear(x) (+ bias) (+ lora_scale * ((x A^T) B^T))
+ * with the weights that mx stands for.  x, bias, LoRA A/B and y share dtype;
+ * accumulation is fp32, outputs are rounded once.  Arguments as qlin_forward;
+ * workspace of at least qlin_mx_workspace_size() bytes, 256-byte aligned.
+ */
+int qlin_mx_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes);
+int qlin_mx_forward(int dtype,
+                    const void* x, int64_t ld_x, const void* mx, const void* bias,
+                    const void* lora_a, const void* lora_b, int rank, float lora_scale,
+                    void* y, int64_t ld_y,
+                    int64_t M, int64_t K_g, int64_t N_g,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of qlin_mx_forward for gy [M, ld_g] = dL/dy; the 4-bit weights
+ * are constants.  Null outputs are not computed:
+ *   dx    [M, ld_dx]      gy conj(W)^T + lora_scale * (gy B) A
+ *   da    [rank, 4 K_g]   lora_scale * (gy B)^T x
+ *   db    [4 N_g, rank]   lora_scale * gy^T (x A^T)
+ *   dbias [4 N_g]         sum over the tokens of gy
+ * x is read for da and db, mx for dx (either may be NULL where it is not).
+ * M = 0 leaves dx alone and zeroes the others.
+ */
+int qlin_mx_backward_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes);
+int qlin_mx_backward(int dtype,
+                     const void* gy, int64_t ld_g, const void* x, int64_t ld_x, const void* mx,
+                     const void* lora_a, const void* lora_b, int rank, float lora_scale,
+                     void* dx, int64_t ld_dx, void* da, void* db, void* dbias,
+                     int64_t M, int64_t K_g, int64_t N_g,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Global norm of `count` gradient tensors and their clipping, in place:
+ *     norm = sqrt(sum of all g^2),   g <- g * min(1, max_norm / (norm + 1e-6))
+ * grads, sizes (elements) and dtypes are host arrays; the tensors are
+ * contiguous and do not overlap, their types may differ.  norm: one fp32 on
+ * the device, written on the stream.  The sum runs in fp64 over fp32 squares,
+ * in a fixed order.  An infinite max_norm gives the norm and leaves the
+ * gradients.
+ */
+int qlin_grad_clip_workspace_size(int count, size_t* bytes);
+int qlin_grad_clip(int count, void* const* grads, const int64_t* sizes, const int* dtypes, float max_norm,
+                   float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,7 @@ The directory name is not a Python identifier, so import it with
 from . import ops
 from .convert import ConversionRecord, convert_model, eligible_modules, project_onto_quaternion
 from ._lib import device_error
+from .grad import clip_grad_norm
 from .linear import QuaternionLinear, fused_quaternion_linear, pack_quaternion_weights, quaternion_linear
 from .lora import (
     LoRAQuaternionLinear,
@@ -23,6 +24,13 @@ from .lora import (
     inject_lora,
     lora_parameters,
     mark_only_lora_trainable,
+)
+from .mx import (
+    MXQuaternionLinear,
+    MXQuaternionWeights,
+    mx_quaternion_linear,
+    quantize_model,
+    quantize_quaternion_weights,
 )
 from .packing import (
     build_block_matrix,
@@ -37,6 +45,12 @@ from .reparam import FactorizedQuaternionLinear, UnitQuaternionLinear, normalize
 from .sharded import ColumnParallelQuaternionLinear, MulticastOutputs, PeerOutputs, gather_columns, shard_bounds
 
 __all__ = [
+    "MXQuaternionWeights",
+    "MXQuaternionLinear",
+    "quantize_quaternion_weights",
+    "mx_quaternion_linear",
+    "quantize_model",
+    "clip_grad_norm",
     "QuaternionLinear",
     "quaternion_linear",
     "fused_quaternion_linear",

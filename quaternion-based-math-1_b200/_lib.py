@@ -63,6 +63,15 @@ EXPORTED = (
     "qlin_nccl_unique_id",
     "qlin_nccl_comm_init",
     "qlin_nccl_comm_destroy",
+    "qlin_mx_weights_size",
+    "qlin_mx_quantize",
+    "qlin_mx_dequantize",
+    "qlin_mx_workspace_size",
+    "qlin_mx_forward",
+    "qlin_mx_backward_workspace_size",
+    "qlin_mx_backward",
+    "qlin_grad_clip_workspace_size",
+    "qlin_grad_clip",
 )
 
 
@@ -137,6 +146,20 @@ def load(path: str | None = None):
         lib.qlin_nccl_comm_init.restype = I
         lib.qlin_nccl_comm_destroy.argtypes = [P]
         lib.qlin_nccl_comm_destroy.restype = I
+        SP = ctypes.POINTER(ctypes.c_size_t)
+        lib.qlin_mx_weights_size.argtypes = [I64, I64, SP]
+        lib.qlin_mx_quantize.argtypes = [I, P, P, P, P, I64, I64, I64, P, P]
+        lib.qlin_mx_dequantize.argtypes = [I, P, I64, I64, P, P, P, P, I64, P]
+        lib.qlin_mx_workspace_size.argtypes = [I, I64, I64, I64, I, SP]
+        lib.qlin_mx_forward.argtypes = [I, P, I64, P, P, P, P, I, ctypes.c_float, P, I64, I64, I64, I64, P,
+                                        ctypes.c_size_t, P]
+        lib.qlin_mx_backward_workspace_size.argtypes = [I, I64, I64, I64, I, SP]
+        lib.qlin_mx_backward.argtypes = [I, P, I64, P, I64, P, P, P, I, ctypes.c_float, P, I64, P, P, P, I64, I64,
+                                         I64, P, ctypes.c_size_t, P]
+        lib.qlin_grad_clip_workspace_size.argtypes = [I, SP]
+        lib.qlin_grad_clip.argtypes = [I, PP, ctypes.POINTER(I64), IP, ctypes.c_float, P, P, ctypes.c_size_t, P]
+        for name in EXPORTED[-9:]:
+            getattr(lib, name).restype = I
         if path is None:
             _lib = lib
             _load_fast(os.path.dirname(p))

@@ -14,24 +14,28 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libqlin_b200.so")
-SOURCES = [os.path.join(CSRC, "qlin_abi.cu")]
-DEPENDS = SOURCES + [os.path.join(CSRC, f) for f in ("qlin_common.cuh", "qlin_gemv.cuh", "qlin_pair.cuh",
-                                                      "qlin_simt.cuh", "qlin_tc.cuh")] + [
+SOURCES = [os.path.join(CSRC, f) for f in ("qlin_abi.cu", "qlin_mx.cu")]
+HEADERS = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cuh", ".h"))] + [
     os.path.join(REPO, "include", "qlin_b200.h")
 ]
+DEPENDS = SOURCES + HEADERS
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "-Xlinker", "-soname=libqlin_b200.so",
-    "-Xptxas", "-v",
+    "-Xcompiler", "-fPIC", "-Xptxas", "-v",
     "-I", os.path.join(REPO, "include"),
+]
+LINK_FLAGS = [
+    "-gencode", "arch=compute_100a,code=sm_100a",
+    "-shared", "-cudart", "static", "-Xlinker", "-soname=libqlin_b200.so",
 ]
 
 
@@ -47,8 +51,8 @@ PYCALL_SRC = os.path.join(CSRC, "qlin_pycall.c")
 PYCALL_PATH = os.path.join(LIB_DIR, "_qlin_call" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
-# torch extension: the modules' inference forward in C++
-TORCH_EXT_SRC = os.path.join(CSRC, "qlin_torch_ext.cpp")
+# torch extension: the modules' inference forward and the calls on 4-bit weights in C++
+TORCH_EXT_SRCS = [os.path.join(CSRC, f) for f in ("qlin_torch_ext.cpp", "qlin_torch_mx.cpp")]
 TORCH_EXT_PATH = os.path.join(LIB_DIR, "_qlin_torch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
@@ -57,29 +61,40 @@ def needs_build() -> bool:
     if not all(os.path.exists(p) for p in outs):
         return True
     t = min(os.path.getmtime(p) for p in outs)
-    return any(os.path.getmtime(p) > t for p in DEPENDS + [PYCALL_SRC, TORCH_EXT_SRC])
+    return any(os.path.getmtime(p) > t for p in DEPENDS + [PYCALL_SRC, *TORCH_EXT_SRCS])
 
 
-def build_torch_ext() -> None:
+def build_torch_ext(force: bool = False) -> None:
     import torch
     import torch.utils.cpp_extension as ce
 
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda_home = ce.CUDA_HOME or "/usr/local/cuda"
     cxx = os.environ.get("QLIN_CXX") or shutil.which("g++") or "c++"
-    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-DTORCH_EXTENSION_NAME=_qlin_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-I", os.path.join(os.path.dirname(torch.__file__), "include"),
-           "-I", os.path.join(os.path.dirname(torch.__file__), "include", "torch", "csrc", "api", "include"),
-           "-I", os.path.join(cuda_home, "include"), "-I", sysconfig.get_paths()["include"],
-           "-I", os.path.join(REPO, "include"),
-           "-o", TORCH_EXT_PATH + ".tmp", TORCH_EXT_SRC,
-           "-L", torch_lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
-           "-L", LIB_DIR, "-lqlin_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"building the torch extension failed:\n{res.stderr[-3000:]}")
+    flags = ["-O2", "-std=c++17", "-fPIC",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-DTORCH_EXTENSION_NAME=_qlin_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-I", os.path.join(os.path.dirname(torch.__file__), "include"),
+             "-I", os.path.join(os.path.dirname(torch.__file__), "include", "torch", "csrc", "api", "include"),
+             "-I", os.path.join(cuda_home, "include"), "-I", sysconfig.get_paths()["include"],
+             "-I", os.path.join(REPO, "include")]
+    objects, compiles = [], []
+    for src in TORCH_EXT_SRCS:
+        obj = os.path.join(LIB_DIR, os.path.basename(src) + ".o")
+        objects.append(obj)
+        if force or not os.path.exists(obj) or any(os.path.getmtime(f) > os.path.getmtime(obj)
+                                                   for f in (src, os.path.join(REPO, "include", "qlin_b200.h"))):
+            compiles.append([cxx, *flags, "-c", "-o", obj, src])
+    with ThreadPoolExecutor() as pool:
+        done = list(pool.map(lambda cmd: subprocess.run(cmd, capture_output=True, text=True), compiles))
+    link = [cxx, "-shared", "-o", TORCH_EXT_PATH + ".tmp", *objects,
+            "-L", torch_lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+            "-L", LIB_DIR, "-lqlin_b200", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
+    if all(res.returncode == 0 for res in done):
+        done.append(subprocess.run(link, capture_output=True, text=True))
+    for res in done:
+        if res.returncode != 0:
+            raise RuntimeError(f"building the torch extension failed:\n{res.stderr[-3000:]}")
     os.replace(TORCH_EXT_PATH + ".tmp", TORCH_EXT_PATH)
 
 
@@ -99,18 +114,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
-    cmd = [find_nvcc(), *NVCC_FLAGS, "-o", tmp, *SOURCES]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    objects = [os.path.join(LIB_DIR, os.path.basename(src) + ".o") for src in SOURCES]
+    compiles = []
+    for src, obj in zip(SOURCES, objects):
+        # an object newer than its source and every header is kept
+        if not force and os.path.exists(obj) and all(os.path.getmtime(f) < os.path.getmtime(obj)
+                                                     for f in [src, *HEADERS]):
+            continue
+        compiles.append([find_nvcc(), *NVCC_FLAGS, "-c", "-o", obj, src])
+    with ThreadPoolExecutor() as pool:
+        done = list(pool.map(lambda cmd: (cmd, subprocess.run(cmd, capture_output=True, text=True)), compiles))
+    if all(res.returncode == 0 for _, res in done):
+        cmd = [find_nvcc(), *LINK_FLAGS, "-o", tmp, *objects]
+        done.append((cmd, subprocess.run(cmd, capture_output=True, text=True)))
     log = os.path.join(LIB_DIR, "build.log")
     with open(log, "w") as f:
-        f.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}); see {log}\n{res.stderr[-4000:]}")
+        for cmd, res in done:
+            f.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+    for _, res in done:
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}); see {log}\n{res.stderr[-4000:]}")
     os.replace(tmp, LIB_PATH)
     build_pycall()
-    build_torch_ext()
+    build_torch_ext(force)
     if verbose:
-        print(res.stderr)
+        print("".join(res.stderr for _, res in done))
     return LIB_PATH
 
 

@@ -19,6 +19,7 @@
 
 #include "../../include/qlin_b200.h"
 #include "qlin_gemv.cuh"
+#include "qlin_host.h"
 #include "qlin_simt.cuh"
 #include "qlin_pair.cuh"
 #include "qlin_tc.cuh"
@@ -1181,6 +1182,15 @@ int allgather_common(int dtype, const void* x, int64_t ld_x, const void* wr, con
 
 }  // namespace
 
+int qlin_host_device(int* sms) {
+  DeviceInfo* dev = nullptr;
+  const int st = device_info(&dev);
+  if (st == QLIN_OK) *sms = dev->num_sms;
+  return st;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 qlin_host_encoder() { return get_encoder() == QLIN_OK ? g_encode : nullptr; }
+
 extern "C" {
 
 const char* qlin_status_string(int status) {
@@ -1199,7 +1209,7 @@ const char* qlin_status_string(int status) {
   }
 }
 
-int qlin_abi_version(void) { return 104; }
+int qlin_abi_version(void) { return 105; }
 
 int qlin_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes) {
   if (!bytes) return QLIN_ERR_ARG;
@@ -1422,7 +1432,10 @@ int qlin_get_device_error(void* stream, int clear, int* device_status) {
     const int zero = 0;
     if (cudaMemcpyToSymbol(qlin::g_device_error, &zero, sizeof(int)) != cudaSuccess) return QLIN_ERR_LAUNCH;
   }
-  *device_status = v;
+  int mx = 0;
+  const int st = qlin_mx_device_error(stream, clear, &mx);
+  if (st != QLIN_OK) return st;
+  *device_status = v != 0 ? v : mx;
   return QLIN_OK;
 }
 

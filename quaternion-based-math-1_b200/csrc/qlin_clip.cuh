@@ -1,0 +1,176 @@
+// Global norm of many gradient tensors, and their clipping:
+//
+//     norm = sqrt(sum over all tensors and elements of g^2)
+//     g   <- g * min(1, max_norm / (norm + 1e-6))
+//
+// Two launches over one table of tensors (a kernel parameter: no copy to the
+// device, so both can be captured into a graph).  The elements of all tensors
+// form one line of pieces of kClipPiece elements, no piece in two tensors;
+// every CTA takes an equal run of pieces in both launches.
+//
+// Bound by the bytes: read once for the norm, read and written once for the
+// product.  The second launch walks its run backwards, so that it begins with
+// what the first has left in L2 (sets of up to about 100 MB are read from
+// HBM once).
+//
+// Squares are summed in fp32 within a piece and thread (at most 16 terms) and
+// in fp64 from there on, in an order that depends only on the sizes: the same
+// gradients give the same bits.  A thread whose fp32 sum overflows sums its
+// piece again in fp64.
+#pragma once
+
+#include "qlin_common.cuh"
+
+namespace qlin {
+
+constexpr int kClipThreads = 512;
+constexpr int kClipPiece = kClipThreads * 16;  // elements
+constexpr int kClipTensors = 512;              // most table entries of a launch
+constexpr int kClipFewTensors = 64;            // entries of the small table (less to hand to a launch)
+constexpr int kClipCtasPerSm = 4;
+
+template <int CAP>
+struct ClipTable {
+  void* data[CAP];
+  long long first[CAP + 1];  // first piece of each tensor
+  long long size[CAP];       // elements
+  unsigned char type[CAP];   // QLIN_F32, QLIN_BF16, QLIN_F16
+  int count;
+};
+
+template <typename T>
+__device__ __forceinline__ double clip_piece_sum(const T* at, long long left) {
+  constexpr int V = 16 / (int)sizeof(T);  // elements of a 16-byte load
+  float s = 0.f;
+  if (left >= kClipPiece && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    uint4 q[16 / V];
+#pragma unroll
+    for (int u = 0; u < 16 / V; ++u)
+      q[u] = ld_cg_v4(at + ((long long)u * kClipThreads + threadIdx.x) * V);
+#pragma unroll
+    for (int u = 0; u < 16 / V; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float v = to_f32(reinterpret_cast<const T*>(&q[u])[j]);
+        s = fmaf(v, v, s);
+      }
+    if (s <= 3.0e38f) return (double)s;
+    double d = 0.0;
+#pragma unroll
+    for (int u = 0; u < 16 / V; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double v = (double)to_f32(reinterpret_cast<const T*>(&q[u])[j]);
+        d += v * v;
+      }
+    return d;
+  }
+  double d = 0.0;
+  for (long long k = threadIdx.x; k < min(left, (long long)kClipPiece); k += kClipThreads) {
+    const double v = (double)to_f32(at[k]);
+    d += v * v;
+  }
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ void clip_piece_scale(T* at, long long left, float f) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (left >= kClipPiece && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    uint4 q[16 / V];
+#pragma unroll
+    for (int u = 0; u < 16 / V; ++u)
+      q[u] = ld_cg_v4(at + ((long long)u * kClipThreads + threadIdx.x) * V);
+#pragma unroll
+    for (int u = 0; u < 16 / V; ++u) {
+      T* e = reinterpret_cast<T*>(&q[u]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = from_f32<T>(to_f32(e[j]) * f);
+      *reinterpret_cast<uint4*>(at + ((long long)u * kClipThreads + threadIdx.x) * V) = q[u];
+    }
+    return;
+  }
+  for (long long k = threadIdx.x; k < min(left, (long long)kClipPiece); k += kClipThreads)
+    at[k] = from_f32<T>(to_f32(at[k]) * f);
+}
+
+// The tensor that holds a piece: the last whose first piece is not past it.
+template <int CAP>
+__device__ __forceinline__ int clip_find(const ClipTable<CAP>& tab, long long piece) {
+  int lo = 0, hi = tab.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (tab.first[mid] <= piece) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Sum of 512 threads' values, the same in every thread (fixed order).
+__device__ __forceinline__ double clip_block_sum(double v, double* slots) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < kClipThreads / 32; ++w) s += slots[w];
+  return s;
+}
+
+// partials[blockIdx.x] = this CTA's share of the sum of squares.
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads)
+qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __restrict__ partials) {
+  __shared__ double slots[kClipThreads / 32];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const long long pieces = tab.first[tab.count];
+  const long long p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
+  double s = 0.0;
+  if (p0 < p1) {
+    int k = clip_find(tab, p0);
+    for (long long p = p0; p < p1; ++p) {
+      while (p >= tab.first[k + 1]) ++k;
+      const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
+      if (tab.type[k] == 0) s += clip_piece_sum(static_cast<const float*>(tab.data[k]) + at, left);
+      else if (tab.type[k] == 1) s += clip_piece_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, left);
+      else s += clip_piece_sum(static_cast<const __half*>(tab.data[k]) + at, left);
+    }
+  }
+  s = clip_block_sum(s, slots);
+  if (threadIdx.x == 0) partials[blockIdx.x] = s;
+}
+
+// Every CTA adds up all partial sums (in the same order) and scales its run.
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads)
+qlin_grad_scale_kernel(const __grid_constant__ ClipTable<CAP> tab, const double* __restrict__ partials, int n_partials,
+                       float max_norm, float* __restrict__ norm_out) {
+  __shared__ double slots[kClipThreads / 32];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  double s = 0.0;
+  for (int k = threadIdx.x; k < n_partials; k += kClipThreads) s += __ldcg(partials + k);
+  s = clip_block_sum(s, slots);
+  const float norm = (float)sqrt(s);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  // a NaN norm makes every gradient NaN, an infinite one zero (or NaN)
+  float f = max_norm / (norm + 1e-6f);
+  if (f > 1.f) f = 1.f;
+  if (isinf(max_norm)) return;  // the norm alone
+  const long long pieces = tab.first[tab.count];
+  const long long p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
+  if (p0 >= p1) return;
+  int k = clip_find(tab, p1 - 1);
+  for (long long p = p1 - 1; p >= p0; --p) {
+    while (p < tab.first[k]) --k;
+    const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
+    if (tab.type[k] == 0) clip_piece_scale(static_cast<float*>(tab.data[k]) + at, left, f);
+    else if (tab.type[k] == 1) clip_piece_scale(static_cast<__nv_bfloat16*>(tab.data[k]) + at, left, f);
+    else clip_piece_scale(static_cast<__half*>(tab.data[k]) + at, left, f);
+  }
+}
+
+}  // namespace qlin

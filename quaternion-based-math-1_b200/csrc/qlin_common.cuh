@@ -128,8 +128,8 @@ template <> __device__ __forceinline__ uint2 pack4<__half>(float a, float b, flo
 // ---------------------------------------------------------------------------
 // device error word (status codes from qlin_b200.h); bounded waits set it
 // ---------------------------------------------------------------------------
-// Defined here: the library is one translation unit (qlin_abi.cu).
-__device__ int g_device_error = 0;
+// One word per translation unit; qlin_get_device_error reads them all.
+static __device__ int g_device_error = 0;
 
 __device__ __forceinline__ void record_error(int code) { atomicCAS(&g_device_error, 0, code); }
 

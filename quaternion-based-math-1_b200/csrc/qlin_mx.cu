@@ -1,0 +1,376 @@
+// C ABI of the 4-bit (MXFP4) quaternion weights and of gradient clipping
+// (declarations: include/qlin_b200.h): argument checks, workspace pieces,
+// launches on the caller's stream.  No exception crosses the ABI, nothing
+// allocates.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/qlin_b200.h"
+#include "qlin_clip.cuh"
+#include "qlin_host.h"
+#include "qlin_mx.cuh"
+#include "qlin_mx_lora.cuh"
+
+namespace {
+
+using namespace qlin;
+
+inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+inline bool known(int dtype) { return dtype == QLIN_F32 || dtype == QLIN_BF16 || dtype == QLIN_F16; }
+inline int64_t elem(int dtype) { return dtype == QLIN_F32 ? 4 : 2; }
+
+int check_groups(int64_t K_g, int64_t N_g) {
+  if (K_g <= 0 || N_g <= 0 || K_g > INT32_MAX / 8 || N_g > INT32_MAX / 8) return QLIN_ERR_SHAPE;
+  return QLIN_OK;
+}
+
+int64_t mx_bytes(int64_t K_g, int64_t N_g) {
+  return kMxHeader + ceil_div(N_g, kMxRows) * ceil_div(K_g, kMxBlock) * kMxRecord;
+}
+
+int check_layer(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
+  if (!known(dtype)) return QLIN_ERR_DTYPE;
+  if (M < 0 || M > INT32_MAX || rank < 0) return QLIN_ERR_SHAPE;
+  return check_groups(K_g, N_g);
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? QLIN_OK : QLIN_ERR_LAUNCH; }
+
+// Calls f(element value of the type) for a known dtype.
+template <typename F>
+int by_type(int dtype, F f) {
+  switch (dtype) {
+    case QLIN_F32: return f(float());
+    case QLIN_BF16: return f(__nv_bfloat16());
+    default: return f(__half());
+  }
+}
+
+// Pieces of a workspace, 256-byte aligned.
+struct Carve {
+  size_t at = 0;
+  size_t take(int64_t bytes) {
+    const size_t p = at;
+    at = (size_t)round_up((int64_t)at + bytes, 256);
+    return p;
+  }
+};
+
+struct ForwardWs {
+  size_t planes = 0, inner = 0, inner_bytes = 0, total = 0;
+};
+
+ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
+  ForwardWs w;
+  Carve c;
+  w.planes = c.take(4 * K_g * N_g * elem(dtype));
+  qlin_workspace_size(dtype, M, K_g, N_g, rank, &w.inner_bytes);
+  w.inner = c.take((int64_t)w.inner_bytes);
+  w.total = c.at;
+  return w;
+}
+
+struct BackwardWs {
+  size_t planes = 0, at = 0, bt = 0, t = 0, up = 0, inner = 0, inner_bytes = 0, total = 0;
+};
+
+BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
+  BackwardWs w;
+  Carve c;
+  w.planes = c.take(4 * K_g * N_g * elem(dtype));
+  w.at = c.take(4 * K_g * rank * elem(dtype));
+  w.bt = c.take(4 * N_g * rank * elem(dtype));
+  w.t = c.take(M * rank * 4);
+  w.up = c.take(M * rank * 4);
+  qlin_workspace_size(dtype, M, N_g, K_g, rank, &w.inner_bytes);
+  w.inner = c.take((int64_t)w.inner_bytes);
+  w.total = c.at;
+  return w;
+}
+
+template <typename T>
+MxPlanes<T> planes_at(void* base, int64_t K_g, int64_t N_g) {
+  MxPlanes<T> p;
+  for (int c = 0; c < 4; ++c) p.w[c] = static_cast<T*>(base) + c * K_g * N_g;
+  return p;
+}
+
+// CTAs of the record kernels: eight records (one per warp) a step, at most
+// four CTAs per SM.
+unsigned record_ctas(int64_t K_g, int64_t N_g, int sms) {
+  const int64_t records = ceil_div(N_g, kMxRows) * ceil_div(K_g, kMxBlock);
+  return (unsigned)std::min<int64_t>(ceil_div(records, 8), 8ll * sms);
+}
+
+template <typename T>
+void launch_dequantize(const void* mx, const MxPlanes<T>& dst, int64_t ld, int64_t K_g, int64_t N_g, int sms,
+                       cudaStream_t s) {
+  bool vec = (ld * sizeof(T)) % 16 == 0;
+  for (int c = 0; c < 4; ++c) vec = vec && aligned(dst.w[c], 16);
+  qlin_mx_dequantize_kernel<T><<<record_ctas(K_g, N_g, sms), 256, 0, s>>>(static_cast<const uint8_t*>(mx), dst, ld,
+                                                                         (int)K_g, (int)N_g, vec);
+}
+
+template <typename TP, typename TQ, typename TC>
+void strided_gemm(const TP* P, int64_t pi, int64_t pl, const TQ* Q, int64_t qj, int64_t ql, TC* C, int64_t ld_c,
+                  int64_t I, int64_t J, int64_t L, float alpha, cudaStream_t s) {
+  const dim3 grid((unsigned)ceil_div(I, 32), (unsigned)ceil_div(J, 32));
+  qlin_mx_strided_gemm_kernel<TP, TQ, TC><<<grid, 256, 0, s>>>(P, pi, pl, Q, qj, ql, C, ld_c, I, J, L, alpha);
+}
+
+template <int CAP>
+void clip_tables(int count, void* const* grads, const int64_t* sizes, const int* dtypes, float max_norm, float* norm,
+                 double* partials, int ctas, cudaStream_t s) {
+  const int rounds = (int)std::max<int64_t>(1, ceil_div(count, CAP));
+  for (int pass = 0; pass < 2; ++pass)
+    for (int r = 0; r < rounds; ++r) {
+      ClipTable<CAP> tab;
+      std::memset(&tab, 0, sizeof(tab));
+      tab.count = std::min(CAP, count - r * CAP);
+      for (int k = 0; k < tab.count; ++k) {
+        tab.data[k] = grads[r * CAP + k];
+        tab.size[k] = sizes[r * CAP + k];
+        tab.type[k] = (unsigned char)dtypes[r * CAP + k];
+        tab.first[k + 1] = tab.first[k] + ceil_div(tab.size[k], kClipPiece);
+      }
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+      cfg.blockDim = dim3(kClipThreads, 1, 1);
+      cfg.stream = s;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (pass == 0)
+        cudaLaunchKernelEx(&cfg, qlin_grad_norm_kernel<CAP>, tab, partials + (int64_t)r * ctas);
+      else
+        cudaLaunchKernelEx(&cfg, qlin_grad_scale_kernel<CAP>, tab, (const double*)partials, rounds * ctas, max_norm,
+                           norm);
+    }
+}
+
+// CTAs of the clipping kernels for a set of tensors: a run of pieces each, at
+// most what the device holds at once.
+int clip_ctas(int64_t pieces, int sms) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(pieces, (int64_t)kClipCtasPerSm * sms));
+}
+
+// Upper bound of the SM count, to size a workspace without a device.
+constexpr int64_t kMostSms = 160;
+
+}  // namespace
+
+int qlin_mx_device_error(void* stream, int clear, int* device_status) {
+  (void)stream;
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, qlin::g_device_error, sizeof(int)) != cudaSuccess) return QLIN_ERR_LAUNCH;
+  if (clear && v != 0) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(qlin::g_device_error, &zero, sizeof(int)) != cudaSuccess) return QLIN_ERR_LAUNCH;
+  }
+  *device_status = v;
+  return QLIN_OK;
+}
+
+extern "C" {
+
+int qlin_mx_weights_size(int64_t K_g, int64_t N_g, size_t* bytes) {
+  if (!bytes) return QLIN_ERR_ARG;
+  const int st = check_groups(K_g, N_g);
+  if (st == QLIN_OK) *bytes = (size_t)mx_bytes(K_g, N_g);
+  return st;
+}
+
+int qlin_mx_quantize(int dtype, const void* wr, const void* wi, const void* wj, const void* wk, int64_t ld_w,
+                     int64_t K_g, int64_t N_g, void* mx, void* stream) {
+  int st = check_layer(dtype, 0, K_g, N_g, 0);
+  if (st != QLIN_OK) return st;
+  if (ld_w < K_g) return QLIN_ERR_SHAPE;
+  if (!wr || !wi || !wj || !wk || !mx) return QLIN_ERR_ARG;
+  if (!aligned(mx, 128)) return QLIN_ERR_ALIGN;
+  int sms = 0;
+  if ((st = qlin_host_device(&sms)) != QLIN_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaGetLastError();
+  if (cudaMemsetAsync(mx, 0, kMxHeader, s) != cudaSuccess) return QLIN_ERR_LAUNCH;
+  return by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    MxPlanes<const T> src;
+    const void* w[4] = {wr, wi, wj, wk};
+    bool vec = (ld_w * sizeof(T)) % 16 == 0;
+    for (int c = 0; c < 4; ++c) {
+      src.w[c] = static_cast<const T*>(w[c]);
+      vec = vec && aligned(w[c], 16);
+    }
+    qlin_mx_quantize_kernel<T><<<record_ctas(K_g, N_g, sms), 256, 0, s>>>(src, ld_w, (int)K_g, (int)N_g,
+                                                                         static_cast<uint8_t*>(mx), vec);
+    return launched();
+  });
+}
+
+int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g, void* wr, void* wi, void* wj, void* wk,
+                       int64_t ld_w, void* stream) {
+  int st = check_layer(dtype, 0, K_g, N_g, 0);
+  if (st != QLIN_OK) return st;
+  if (ld_w < K_g) return QLIN_ERR_SHAPE;
+  if (!wr || !wi || !wj || !wk || !mx) return QLIN_ERR_ARG;
+  if (!aligned(mx, 128)) return QLIN_ERR_ALIGN;
+  int sms = 0;
+  if ((st = qlin_host_device(&sms)) != QLIN_OK) return st;
+  cudaGetLastError();
+  return by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    const MxPlanes<T> dst = {{static_cast<T*>(wr), static_cast<T*>(wi), static_cast<T*>(wj), static_cast<T*>(wk)}};
+    launch_dequantize<T>(mx, dst, ld_w, K_g, N_g, sms, static_cast<cudaStream_t>(stream));
+    return launched();
+  });
+}
+
+int qlin_mx_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes) {
+  if (!bytes) return QLIN_ERR_ARG;
+  const int st = check_layer(dtype, M, K_g, N_g, rank);
+  if (st == QLIN_OK) *bytes = M == 0 ? 0 : forward_ws(dtype, M, K_g, N_g, rank).total;
+  return st;
+}
+
+int qlin_mx_forward(int dtype, const void* x, int64_t ld_x, const void* mx, const void* bias, const void* lora_a,
+                    const void* lora_b, int rank, float lora_scale, void* y, int64_t ld_y, int64_t M, int64_t K_g,
+                    int64_t N_g, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_layer(dtype, M, K_g, N_g, rank);
+  if (st != QLIN_OK) return st;
+  if (ld_x < 4 * K_g || ld_y < 4 * N_g) return QLIN_ERR_SHAPE;
+  if (M == 0) return QLIN_OK;
+  if (!x || !mx || !y || (rank > 0 && (!lora_a || !lora_b))) return QLIN_ERR_ARG;
+  if (!aligned(mx, 128)) return QLIN_ERR_ALIGN;
+  const ForwardWs w = forward_ws(dtype, M, K_g, N_g, rank);
+  if (w.total > 0 && (!workspace || workspace_bytes < w.total || !aligned(workspace, 256))) return QLIN_ERR_WORKSPACE;
+  int sms = 0;
+  if ((st = qlin_host_device(&sms)) != QLIN_OK) return st;
+  cudaGetLastError();
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    const MxPlanes<T> p = planes_at<T>(ws + w.planes, K_g, N_g);
+    launch_dequantize<T>(mx, p, K_g, K_g, N_g, sms, static_cast<cudaStream_t>(stream));
+    if (launched() != QLIN_OK) return (int)QLIN_ERR_LAUNCH;
+    return qlin_forward_ex(dtype, x, ld_x, p.w[0], p.w[1], p.w[2], p.w[3], K_g, bias, lora_a, lora_b, rank,
+                           lora_scale, y, ld_y, M, K_g, N_g, ws + w.inner, w.inner_bytes, QLIN_ALGO_AUTO, 0, stream);
+  });
+}
+
+int qlin_mx_backward_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes) {
+  if (!bytes) return QLIN_ERR_ARG;
+  const int st = check_layer(dtype, M, K_g, N_g, rank);
+  if (st == QLIN_OK) *bytes = M == 0 ? 0 : backward_ws(dtype, M, K_g, N_g, rank).total;
+  return st;
+}
+
+int qlin_mx_backward(int dtype, const void* gy, int64_t ld_g, const void* x, int64_t ld_x, const void* mx,
+                     const void* lora_a, const void* lora_b, int rank, float lora_scale, void* dx, int64_t ld_dx,
+                     void* da, void* db, void* dbias, int64_t M, int64_t K_g, int64_t N_g, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int st = check_layer(dtype, M, K_g, N_g, rank);
+  if (st != QLIN_OK) return st;
+  if (ld_g < 4 * N_g || (dx && ld_dx < 4 * K_g) || ((da || db) && ld_x < 4 * K_g)) return QLIN_ERR_SHAPE;
+  if ((da || db) && rank == 0) return QLIN_ERR_ARG;
+  if (M > 0 && (!gy || (dx && !mx) || ((da || db) && !x) || (rank > 0 && (!lora_a || !lora_b)))) return QLIN_ERR_ARG;
+  if (!aligned(mx, 128)) return QLIN_ERR_ALIGN;
+  const int64_t K = 4 * K_g, N = 4 * N_g;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M == 0) {  // empty sums
+    if (!da && !db && !dbias) return QLIN_OK;
+    cudaGetLastError();
+    if (da) cudaMemsetAsync(da, 0, rank * K * elem(dtype), s);
+    if (db) cudaMemsetAsync(db, 0, rank * N * elem(dtype), s);
+    if (dbias) cudaMemsetAsync(dbias, 0, N * elem(dtype), s);
+    return launched();
+  }
+  const BackwardWs w = backward_ws(dtype, M, K_g, N_g, rank);
+  if (w.total > 0 && (!workspace || workspace_bytes < w.total || !aligned(workspace, 256))) return QLIN_ERR_WORKSPACE;
+  int sms = 0;
+  if ((st = qlin_host_device(&sms)) != QLIN_OK) return st;
+  cudaGetLastError();
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    const T* g = static_cast<const T*>(gy);
+    const T* xt = static_cast<const T*>(x);
+    const T* a = static_cast<const T*>(lora_a);
+    const T* b = static_cast<const T*>(lora_b);
+    T* at = reinterpret_cast<T*>(ws + w.at);
+    T* bt = reinterpret_cast<T*>(ws + w.bt);
+    if (dx) {
+      const MxPlanes<T> p = planes_at<T>(ws + w.planes, K_g, N_g);
+      const int64_t steps = ceil_div(N_g, 64) * ceil_div(K_g, kMxBlock);
+      qlin_mx_adjoint_kernel<T><<<(unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s>>>(
+          static_cast<const uint8_t*>(mx), p, N_g, (int)K_g, (int)N_g);
+      if (rank > 0) {
+        qlin_mx_turn_kernel<T><<<(unsigned)ceil_div(rank * K, 256), 256, 0, s>>>(a, at, rank, K);
+        qlin_mx_turn_kernel<T><<<(unsigned)ceil_div(rank * N, 256), 256, 0, s>>>(b, bt, N, rank);
+      }
+      if (launched() != QLIN_OK) return (int)QLIN_ERR_LAUNCH;
+      const int e = qlin_forward_ex(dtype, gy, ld_g, p.w[0], p.w[1], p.w[2], p.w[3], N_g, nullptr, bt, at, rank,
+                                    lora_scale, dx, ld_dx, M, N_g, K_g, ws + w.inner, w.inner_bytes, QLIN_ALGO_AUTO,
+                                    0, stream);
+      if (e != QLIN_OK) return e;
+    }
+    float* t = reinterpret_cast<float*>(ws + w.t);
+    float* up = reinterpret_cast<float*>(ws + w.up);
+    if (da) {
+      strided_gemm<T, T, float>(g, ld_g, 1, b, 1, rank, up, rank, M, rank, N, lora_scale, s);
+      strided_gemm<float, T, T>(up, 1, rank, xt, 1, ld_x, static_cast<T*>(da), K, rank, K, M, 1.f, s);
+    }
+    if (db) {
+      strided_gemm<T, T, float>(xt, ld_x, 1, a, K, 1, t, rank, M, rank, K, lora_scale, s);
+      strided_gemm<T, float, T>(g, 1, ld_g, t, 1, rank, static_cast<T*>(db), rank, N, rank, M, 1.f, s);
+    }
+    if (dbias)
+      qlin_mx_column_sum_kernel<T><<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(g, ld_g, static_cast<T*>(dbias), M, N);
+    return launched();
+  });
+}
+
+int qlin_grad_clip_workspace_size(int count, size_t* bytes) {
+  if (!bytes) return QLIN_ERR_ARG;
+  if (count < 0) return QLIN_ERR_SHAPE;
+  *bytes = (size_t)(std::max<int64_t>(1, ceil_div(count, kClipTensors)) * kClipCtasPerSm * kMostSms * 8);
+  return QLIN_OK;
+}
+
+int qlin_grad_clip(int count, void* const* grads, const int64_t* sizes, const int* dtypes, float max_norm,
+                   float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+  if (count < 0) return QLIN_ERR_SHAPE;
+  if (!norm || (count > 0 && (!grads || !sizes || !dtypes)) || !(max_norm >= 0.f)) return QLIN_ERR_ARG;
+  int64_t pieces = 0;
+  for (int k = 0; k < count; ++k) {
+    if (sizes[k] < 0) return QLIN_ERR_SHAPE;
+    if (!known(dtypes[k])) return QLIN_ERR_DTYPE;
+    if (sizes[k] > 0 && !grads[k]) return QLIN_ERR_ARG;
+    if (!aligned(grads[k], (uintptr_t)elem(dtypes[k]))) return QLIN_ERR_ALIGN;
+    pieces += ceil_div(sizes[k], kClipPiece);
+  }
+  size_t need = 0;
+  qlin_grad_clip_workspace_size(count, &need);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return QLIN_ERR_WORKSPACE;
+  int sms = 0;
+  const int st = qlin_host_device(&sms);
+  if (st != QLIN_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaGetLastError();
+  const int ctas = clip_ctas(pieces, (int)std::min<int64_t>(sms, kMostSms));
+  double* partials = static_cast<double*>(workspace);
+  if (count <= kClipFewTensors)
+    clip_tables<kClipFewTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, s);
+  else
+    clip_tables<kClipTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, s);
+  return launched();
+}
+
+}  // extern "C"

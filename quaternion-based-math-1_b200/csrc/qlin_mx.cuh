@@ -1,0 +1,225 @@
+// 4-bit quaternion weights (OCP microscaling, MXFP4): layout, quantisation and
+// dequantisation.
+//
+// Element format e2m1 (sign, 2 exponent bits, 1 mantissa bit): +-{0, 0.5, 1,
+// 1.5, 2, 3, 4, 6}.  32 consecutive input quaternions of one component row
+// W_p[o, :] share one E8M0 scale 2^(E - 127):
+//
+//     E - 127 = floor(log2(max |w|)) - 2,   code = e2m1(w / 2^(E - 127))
+//
+// rounded to nearest, ties to the even code, saturating at 6 (the quotient is
+// below 8).  The power-of-two quotient is exact, so the codes are those of the
+// real-number definition.  E is clamped to [0, 254] (a block of zeros has
+// E = 0); a block that holds an infinity or a NaN gets E = 255 and zero codes
+// and stands for NaNs.
+//
+// Buffer: a header of kMxHeader bytes (word 0: the largest E below 255 of the
+// layer), then one record per 16 output quaternions (tile) and 32 input
+// quaternions (block), tile-major, blocks of one tile contiguous:
+//
+//     record (1088 bytes) = codes [16 rows][4 octets t][4 components p] words,
+//                           then scales [16 rows][4 components p] bytes
+//
+// Word (row, t, p) holds the codes of input quaternions 32 b + 8 t + j
+// (j = 0..7) of component p in nibble j.  So one 16-byte piece holds all four
+// components of eight input quaternions of a row, and the pieces that the 32
+// lanes of an m16 tensor-core operand need are two runs of 512 bytes.  Rows and
+// input quaternions past the layer's are zero codes with E = 0.
+#pragma once
+
+#include <type_traits>
+
+#include "qlin_common.cuh"
+
+namespace qlin {
+
+constexpr int kMxBlock = 32;           // input quaternions that share a scale
+constexpr int kMxRows = 16;            // output quaternions of a record
+constexpr int kMxCodeBytes = kMxRows * kMxBlock * 4 / 2;
+constexpr int kMxRecord = kMxCodeBytes + kMxRows * 4;
+constexpr int kMxHeader = 128;
+
+// 2^(E - 127) as fp32 (E = 0: the subnormal 2^-127; E = 255: NaN).
+__device__ __forceinline__ float mx_scale(uint32_t e) {
+  return __uint_as_float(e == 255u ? 0x7FC00000u : (e == 0u ? 0x00400000u : e << 23));
+}
+
+// e2m1 value of the low four bits of c.
+__device__ __forceinline__ float mx_value(uint32_t c) {
+  const uint32_t m = c & 7u;
+  // exponent field 0: 0 or 0.5; else 2^(e - 1) (1 + m / 2)
+  const uint32_t bits = m < 2u ? m * 0x3F000000u : ((126u + (m >> 1)) << 23 | (m & 1u) << 22);
+  return __uint_as_float(bits | (c & 8u) << 28);
+}
+
+// E of a block whose largest magnitude is amax (finite).
+__device__ __forceinline__ uint32_t mx_exponent(float amax) {
+  const uint32_t field = __float_as_uint(amax) >> 23;  // floor(log2) + 127; 0 for subnormals
+  return field <= 2u ? 0u : field - 2u;
+}
+
+// Code of the magnitude a = |w| / scale, by the midpoints between neighbouring
+// values (a tie goes to the even code).
+__device__ __forceinline__ uint32_t mx_code(float a) {
+  return (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
+}
+
+// Eight consecutive elements of a row from `at`, zero from `left` on (vec: the
+// row pieces are 16-byte aligned and whole).
+template <typename T>
+__device__ __forceinline__ void mx_load8(const T* at, int64_t left, bool vec, float (&v)[8]) {
+  if (vec && left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = ld_cg_f4(at), b = ld_cg_f4(at + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 q = ld_cg_v4(at);
+      const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(at[j]) : 0.f;
+}
+
+template <typename T>
+struct MxPlanes {
+  T* w[4];
+};
+
+// Quantisation: a warp makes a record at a time, two rows (four components of
+// four octets each) per step.  A lane holds eight elements of one block, the
+// four lanes of a block share its maximum.  Bound by the bytes read (2 or 4 a
+// weight) and written (0.53): one pass, everything else in registers.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_g, uint8_t* __restrict__ mx,
+                        bool vec) {
+  const int lane = threadIdx.x & 31;
+  const int t = lane & 3, p = (lane >> 2) & 3, half = lane >> 4;
+  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  uint32_t top = 0;
+  for (int64_t rec = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); rec < tiles * kb; rec += warps) {
+    const int64_t tile = rec / kb, b = rec - tile * kb;
+    uint8_t* out = mx + kMxHeader + rec * kMxRecord;
+    const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
+#pragma unroll
+    for (int step = 0; step < kMxRows / 2; ++step) {
+      const int row = 2 * step + half;
+      const int64_t o = tile * kMxRows + row;
+      float v[8];
+      if (o < N_g && left > 0) {
+        mx_load8(src.w[p] + o * ld + i, left, vec, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      }
+      // magnitudes as integers: the order of finite values, infinities and NaNs above them
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const bool bad = m >= 0x7F800000u;
+      const uint32_t e = bad ? 255u : mx_exponent(__uint_as_float(m));
+      uint32_t word = 0;
+      if (!bad) {
+        top = max(top, e);
+        const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - E): E is at most 252
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t sign = __float_as_uint(v[j]) >> 31;
+          word |= (mx_code(fabsf(v[j]) * inv) | sign << 3) << (4 * j);
+        }
+      }
+      *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = word;
+      if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)e;
+    }
+  }
+  __shared__ uint32_t tops[8];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) top = max(top, tops[w]);
+    atomicMax(reinterpret_cast<unsigned*>(mx), top);  // a maximum: the same in any order
+  }
+}
+
+// Dequantisation to the four component rows, mapped like the quantisation.
+// One rounding (none for fp32, or for bf16 in its normal range).
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
+                          bool vec) {
+  const int lane = threadIdx.x & 31;
+  const int t = lane & 3, p = (lane >> 2) & 3, half = lane >> 4;
+  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  for (int64_t rec = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); rec < tiles * kb; rec += warps) {
+    const int64_t tile = rec / kb, b = rec - tile * kb;
+    const uint8_t* in = mx + kMxHeader + rec * kMxRecord;
+    const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
+    if (left <= 0) continue;
+#pragma unroll
+    for (int step = 0; step < kMxRows / 2; ++step) {
+      const int row = 2 * step + half;
+      const int64_t o = tile * kMxRows + row;
+      if (o >= N_g) continue;
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4);
+      const float s = mx_scale(in[kMxCodeBytes + row * 4 + p]);
+      T* at = dst.w[p] + o * ld + i;
+      T v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(mx_value(word >> (4 * j)) * s);
+      if (vec && left >= 8) {
+#pragma unroll
+        for (int c = 0; c < (int)sizeof(T) / 2; ++c)
+          reinterpret_cast<uint4*>(at)[c] = reinterpret_cast<const uint4*>(v)[c];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < left) at[j] = v[j];
+      }
+    }
+  }
+}
+
+// The weights of the adjoint layer, conj(W)^T, as four component rows
+// [K_g, N_g]: 64 output quaternions x 32 input quaternions of one component
+// per CTA step, turned through shared memory.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_adjoint_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g) {
+  __shared__ T turn[4][kMxBlock][66];
+  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
+  const int64_t groups = (tiles + 3) / 4;
+  const int t = threadIdx.x & 3, p = (threadIdx.x >> 2) & 3, row = threadIdx.x >> 4;
+  for (int64_t step = blockIdx.x; step < groups * kb; step += gridDim.x) {
+    const int64_t g = step / kb, b = step - g * kb;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t tile = 4 * g + u;
+      if (tile >= tiles) break;
+      const uint8_t* in = mx + kMxHeader + (tile * kb + b) * kMxRecord;
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4);
+      const float s = mx_scale(in[kMxCodeBytes + row * 4 + p]) * (p == 0 ? 1.f : -1.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) turn[p][8 * t + j][16 * u + row] = from_f32<T>(mx_value(word >> (4 * j)) * s);
+    }
+    __syncthreads();
+    const int64_t o0 = 64 * g;
+    for (int k = threadIdx.x; k < 4 * kMxBlock * 64; k += 256) {
+      const int c = k & 63, i = (k >> 6) & 31, q = k >> 11;
+      if (o0 + c < N_g && b * kMxBlock + i < K_g) dst.w[q][(b * kMxBlock + i) * ld + o0 + c] = turn[q][i][c];
+    }
+  }
+}
+
+}  // namespace qlin

@@ -190,7 +190,10 @@ std::vector<at::Tensor> workspaces() {
 
 }  // namespace
 
+void register_mx(pybind11::module& m);  // qlin_torch_mx.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  register_mx(m);
   m.def("forward", &forward, "fused quaternion linear inference forward (see qlin_b200.h)", pybind11::arg("x"),
         pybind11::arg("wr"), pybind11::arg("wi"), pybind11::arg("wj"), pybind11::arg("wk"),
         pybind11::arg("bias") = pybind11::none(), pybind11::arg("lora_a") = pybind11::none(),

@@ -1,0 +1,60 @@
+"""Global gradient norm and clipping over many tensors, for training the
+quaternion components or the LoRA factors of a model (hundreds of small
+tensors a step): two kernel launches for all of them, nothing read back to the
+host."""
+
+from __future__ import annotations
+
+from collections.abc import Iterable
+
+import torch
+
+from .mx import _ext
+
+__all__ = ["clip_grad_norm"]
+
+
+def clip_grad_norm(parameters, max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale the gradients of ``parameters`` in place so that their global
+    2-norm is at most ``max_norm``; return the norm before that (a float32
+    scalar on their device).
+
+    ``g <- g * min(1, max_norm / (norm + 1e-6))``.  ``parameters`` is a tensor
+    or an iterable of tensors on one CUDA device; those without a gradient
+    are skipped, one that comes up twice counts once.  Gradients may be
+    float32, bfloat16 and float16 side by side; sums are kept in 64 bits in a
+    fixed order.  An infinite ``max_norm`` gives the norm and leaves the
+    gradients; with a NaN norm every gradient becomes NaN otherwise;
+    ``error_if_nonfinite`` raises ``RuntimeError`` instead (the host then waits
+    for the norm; the gradients are unchanged).  Gradients of different
+    parameters must not overlap in memory.
+    """
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    if not isinstance(parameters, Iterable):
+        raise TypeError(f"parameters must be a tensor or an iterable of tensors, got {type(parameters).__name__}")
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be at least 0, got {max_norm}")
+    grads = {}
+    for p in parameters:
+        if p.grad is not None:
+            grads[id(p.grad)] = p.grad
+    grads = list(grads.values())
+    if not grads:
+        return torch.tensor(0.0)
+    for g in grads:
+        if g.layout != torch.strided:
+            raise RuntimeError("sparse gradients are not supported")
+    with torch.no_grad():
+        # a gradient with gaps in memory goes through a dense copy
+        dense = _ext().dense_grads(grads)
+        norm = _ext().grad_clip(dense, float("inf") if error_if_nonfinite else max_norm)
+        if error_if_nonfinite:
+            if not bool(torch.isfinite(norm)):
+                raise RuntimeError(f"the global norm of the gradients is {float(norm)}; they are not clipped")
+            norm = _ext().grad_clip(dense, max_norm)
+        for g, d in zip(grads, dense):
+            if d is not g:
+                g.copy_(d)
+    return norm

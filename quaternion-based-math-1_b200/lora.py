@@ -11,6 +11,9 @@ device call: the kernel adds ``scale * (x A^T) B^T`` in fp32 before the single
 output rounding.  With dropout active (training, ``p > 0``) the residual's
 input differs from the base's, so the base runs fused with its bias and the
 residual is added from the dropped-out input.
+
+The base may be a ``QuaternionLinear`` or one frozen in 4 bits
+(``MXQuaternionLinear``); the factors have the base's type either way.
 """
 
 from __future__ import annotations
@@ -21,6 +24,7 @@ import torch
 import torch.nn as nn
 
 from .linear import QuaternionLinear, fused_quaternion_linear
+from .mx import MXQuaternionLinear, mx_quaternion_linear
 
 __all__ = [
     "LoRAQuaternionLinear",
@@ -32,10 +36,11 @@ __all__ = [
 
 
 class LoRAQuaternionLinear(nn.Module):
-    """A ``QuaternionLinear`` whose weights stay fixed, with a learnable rank-r
-    residual ``scale * B (A x)`` added on the same fused device call."""
+    """A ``QuaternionLinear`` or ``MXQuaternionLinear`` whose weights stay fixed,
+    with a learnable rank-r residual ``scale * B (A x)`` added on the same fused
+    device call."""
 
-    def __init__(self, base: QuaternionLinear, rank: int = 8, alpha: float | None = None,
+    def __init__(self, base: QuaternionLinear | MXQuaternionLinear, rank: int = 8, alpha: float | None = None,
                  dropout: float = 0.0):
         super().__init__()
         if rank <= 0:
@@ -48,7 +53,7 @@ class LoRAQuaternionLinear(nn.Module):
         self.rank = rank
         self.alpha = alpha if alpha is not None else 2 * rank
         self.scale = self.alpha / rank
-        ref = next(base.parameters())
+        ref = base.type_of if isinstance(base, MXQuaternionLinear) else next(base.parameters())
         self.lora_A = nn.Parameter(torch.empty(rank, self.in_features, device=ref.device,
                                                dtype=ref.dtype))
         self.lora_B = nn.Parameter(torch.zeros(self.out_features, rank, device=ref.device,
@@ -62,10 +67,13 @@ class LoRAQuaternionLinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         b = self.base
+        mx = isinstance(b, MXQuaternionLinear)
         if isinstance(self.lora_dropout, nn.Dropout) and self.training:
-            out = fused_quaternion_linear(x, b.wr, b.wi, b.wj, b.wk, b.bias)
+            out = b(x) if mx else fused_quaternion_linear(x, b.wr, b.wi, b.wj, b.wk, b.bias)
             lora = (self.lora_dropout(x) @ self.lora_A.t()) @ self.lora_B.t()
             return out + self.scale * lora
+        if mx:
+            return mx_quaternion_linear(x, b.weights, b.bias, self.lora_A, self.lora_B, self.scale)
         return fused_quaternion_linear(x, b.wr, b.wi, b.wj, b.wk, b.bias, self.lora_A, self.lora_B,
                                        self.scale, static_weights=b.static_weights,
                                        packed=b._packed_for_call(x, self.lora_A, self.lora_B))
@@ -76,8 +84,9 @@ class LoRAQuaternionLinear(nn.Module):
 
 
 def inject_lora(model: nn.Module, rank: int = 8, alpha: float | None = None, dropout: float = 0.0):
-    """Wrap every ``QuaternionLinear`` of ``model`` in place; return the wrapped names."""
-    targets = [(n, m) for n, m in model.named_modules() if isinstance(m, QuaternionLinear)]
+    """Wrap every ``QuaternionLinear`` and ``MXQuaternionLinear`` of ``model`` in
+    place; return the wrapped names."""
+    targets = [(n, m) for n, m in model.named_modules() if isinstance(m, (QuaternionLinear, MXQuaternionLinear))]
     wrapped = []
     for name, mod in targets:
         parent_name, _, leaf = name.rpartition(".")
