@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <cstring>
 
@@ -13,6 +14,7 @@
 #include "qlin_clip.cuh"
 #include "qlin_host.h"
 #include "qlin_mx.cuh"
+#include "qlin_mx_few.cuh"
 #include "qlin_mx_lora.cuh"
 
 namespace {
@@ -62,16 +64,41 @@ struct Carve {
   }
 };
 
+// 16-bit inputs of up to this many tokens take the streaming kernels
+// (qlin_mx_few.cuh), more the dequantised path; fp32 always streams.
+constexpr int64_t kFewTokens = 64;
+
+bool streams(int dtype, int64_t M) { return dtype == QLIN_F32 || M <= kFewTokens; }
+
+// Tokens of a tile of the streaming kernels (one or two tokens apart): the
+// smallest tile that holds them all, at most 32.
+int few_tile(int64_t M) { return M <= 8 ? 8 : (M <= 16 ? 16 : 32); }
+
+// One or two tokens whose B words fit beside the ring.
+constexpr size_t kOneMaxX = 128 * 1024;
+bool is_one(int dtype, int64_t M, int64_t K_g) {
+  const int64_t kb = ceil_div(K_g, kMxBlock);
+  return M <= 2 && (size_t)kb * 512 * (dtype == QLIN_F32 ? 3 : 1) <= kOneMaxX;
+}
+
 struct ForwardWs {
-  size_t planes = 0, inner = 0, inner_bytes = 0, total = 0;
+  size_t arranged = 0, t = 0, planes = 0, inner = 0, inner_bytes = 0, total = 0;
 };
 
 ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   ForwardWs w;
   Carve c;
-  w.planes = c.take(4 * K_g * N_g * elem(dtype));
-  qlin_workspace_size(dtype, M, K_g, N_g, rank, &w.inner_bytes);
-  w.inner = c.take((int64_t)w.inner_bytes);
+  if (streams(dtype, M)) {
+    if (!is_one(dtype, M, K_g)) {
+      const int64_t C = few_tile(M);
+      w.arranged = c.take(ceil_div(M, C) * ceil_div(K_g, kMxBlock) * (dtype == QLIN_F32 ? 3 : 1) * 4 * C * 64);
+    }
+    w.t = c.take(M * rank * 4);
+  } else {
+    w.planes = c.take(4 * K_g * N_g * elem(dtype));
+    qlin_workspace_size(dtype, M, K_g, N_g, rank, &w.inner_bytes);
+    w.inner = c.take((int64_t)w.inner_bytes);
+  }
   w.total = c.at;
   return w;
 }
@@ -115,6 +142,115 @@ void launch_dequantize(const void* mx, const MxPlanes<T>& dst, int64_t ld, int64
   for (int c = 0; c < 4; ++c) vec = vec && aligned(dst.w[c], 16);
   qlin_mx_dequantize_kernel<T><<<record_ctas(K_g, N_g, sms), 256, 0, s>>>(static_cast<const uint8_t*>(mx), dst, ld,
                                                                          (int)K_g, (int)N_g, vec);
+}
+
+// Launch as a programmatic dependent of the stream's previous kernel.
+template <typename... KArgs, typename... Args>
+int launch_dependent(void (*kernel)(KArgs...), unsigned ctas, unsigned threads, size_t smem, cudaStream_t s,
+                     Args... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
+}
+
+constexpr size_t kMostSmem = 227 * 1024;
+
+// Raises a kernel's shared-memory limit once per device.
+template <typename K>
+int allow_smem(K kernel, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QLIN_ERR_LAUNCH;
+  if (done.load(std::memory_order_acquire) >> dev & 1) return QLIN_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem) != cudaSuccess)
+    return QLIN_ERR_LAUNCH;
+  done.fetch_or(1ull << dev, std::memory_order_release);
+  return QLIN_OK;
+}
+
+// Stages of a ring: what fits `budget` beside `fixed` bytes, at least 2, at
+// most what a CTA uses.
+int ring_stages(size_t budget, size_t fixed, size_t stage, int64_t uses) {
+  const int64_t fit = budget > fixed ? (int64_t)((budget - fixed) / stage) : 0;
+  return (int)std::max<int64_t>(2, std::min(fit, uses));
+}
+
+template <typename T>
+int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  if (allow_smem(qlin_mx_one_kernel<T>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+  MxFewParams<T> prm = base;
+  const int per_sm = prm.tiles > sms ? 2 : 1;
+  const int ctas = std::min(prm.tiles, per_sm * sms);
+  const int64_t uses = ceil_div(prm.kb, kMxWarps) * ceil_div(prm.tiles, ctas);
+  prm.ring = ring_stages(kMostSmem / per_sm - 1024, mx_one_smem<T>(prm.kb, 0, prm.rank), kMxOneStage + 16, uses);
+  const size_t smem = mx_one_smem<T>(prm.kb, prm.ring, prm.rank);
+  if (smem > kMostSmem) return QLIN_ERR_SHAPE;
+  return launch_dependent(qlin_mx_one_kernel<T>, ctas, kMxThreads, smem, s, prm);
+}
+
+template <typename T, int NT, int WO>
+int launch_many(const MxFewParams<T>& base, int sms, cudaStream_t s) {
+  using Cfg = MxManyCfg<T, NT, WO>;
+  static std::atomic<uint64_t> done{0};
+  if (allow_smem(qlin_mx_many_kernel<T, NT, WO>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+  MxFewParams<T> prm = base;
+  const int64_t total = ceil_div(prm.tiles, WO) * ceil_div(prm.M, Cfg::kC);
+  const int ctas = (int)std::min<int64_t>(total, sms);
+  const int64_t uses = ceil_div(prm.kb, Cfg::kWK) * ceil_div(total, ctas);
+  prm.ring = ring_stages(kMostSmem, mx_many_smem<T, NT, WO>(0, prm.rank), Cfg::kStage + 16, uses);
+  const size_t smem = mx_many_smem<T, NT, WO>(prm.ring, prm.rank);
+  if (smem > kMostSmem) return QLIN_ERR_SHAPE;
+  return launch_dependent(qlin_mx_many_kernel<T, NT, WO>, ctas, kMxThreads, smem, s, prm);
+}
+
+// The streaming kernels: a prologue where there are B words to arrange or an
+// adapter, then the product.
+template <typename T>
+int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, const T* a, const T* b, int rank,
+            float scale, T* y, int64_t ld_y, int64_t M, int64_t K_g, int64_t N_g, uint8_t* ws, const ForwardWs& w,
+            int sms, cudaStream_t s) {
+  MxFewParams<T> prm{};
+  prm.x = x;
+  prm.ld_x = ld_x;
+  prm.mx = static_cast<const uint8_t*>(mx);
+  prm.arranged = ws + w.arranged;
+  prm.bias = bias;
+  prm.lora_b = b;
+  prm.t = reinterpret_cast<const float*>(ws + w.t);
+  prm.y = y;
+  prm.ld_y = ld_y;
+  prm.M = (int)M;
+  prm.K_g = (int)K_g;
+  prm.N_g = (int)N_g;
+  prm.rank = rank;
+  prm.kb = (int)ceil_div(K_g, kMxBlock);
+  prm.tiles = (int)ceil_div(N_g, kMxRows);
+  prm.vec = aligned(x, 4 * sizeof(T)) && ld_x % 4 == 0;
+  const bool one = is_one(dtype, M, K_g);
+  const int C = few_tile(M);
+  const int64_t octets = one ? 0 : ceil_div(M, C) * C * 4 * prm.kb;
+  const int64_t blocks = ceil_div(octets, 256), down = rank * ceil_div(M, kMxDownTokens);
+  if (blocks + down > INT32_MAX) return QLIN_ERR_SHAPE;
+  prm.after_prologue = blocks + down > 0;
+  if (prm.after_prologue) {
+    const int st = launch_dependent(qlin_mx_prologue_kernel<T>, (unsigned)(blocks + down), 256, 0, s, x, ld_x, (int)M,
+                                    (int)K_g, prm.kb, C, prm.vec, ws + w.arranged, (int)blocks, octets, a,
+                                    (int)aligned(a, 4 * sizeof(T)), rank, scale,
+                                    reinterpret_cast<float*>(ws + w.t));
+    if (st != QLIN_OK) return st;
+  }
+  if (one) return launch_one<T>(prm, sms, s);
+  if (C == 8) return launch_many<T, 1, 1>(prm, sms, s);
+  if (C == 16) return launch_many<T, 2, 2>(prm, sms, s);
+  return launch_many<T, 4, 4>(prm, sms, s);
 }
 
 template <typename TP, typename TQ, typename TC>
@@ -257,6 +393,10 @@ int qlin_mx_forward(int dtype, const void* x, int64_t ld_x, const void* mx, cons
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   return by_type(dtype, [&](auto v) {
     using T = decltype(v);
+    if (streams(dtype, M))
+      return run_few<T>(dtype, static_cast<const T*>(x), ld_x, mx, static_cast<const T*>(bias),
+                        static_cast<const T*>(lora_a), static_cast<const T*>(lora_b), rank, lora_scale,
+                        static_cast<T*>(y), ld_y, M, K_g, N_g, ws, w, sms, static_cast<cudaStream_t>(stream));
     const MxPlanes<T> p = planes_at<T>(ws + w.planes, K_g, N_g);
     launch_dequantize<T>(mx, p, K_g, K_g, N_g, sms, static_cast<cudaStream_t>(stream));
     if (launched() != QLIN_OK) return (int)QLIN_ERR_LAUNCH;

@@ -1,0 +1,649 @@
+// The layer with 4-bit weights for few tokens (decode, small batches; fp32 at
+// any size): a stream of the codes through shared memory into warp-level
+// tensor-core products (mma m16n8k16, fp32 accumulators).
+//
+//     y_a[o] = sum_i sum_p s(a, p) W_p[o, i] x_{a^p}[i]
+//
+// The weights are the A operand in their stored form: 16 output quaternions x
+// 16 input quaternions of one component W_p, expanded from codes in registers
+// (no 4x real matrix), so a code is expanded once for all four output
+// components and all tokens.  A lane's 16-byte piece of a record holds eight
+// input quaternions of a row for all p: the k slots of the operand are
+// numbered so that lane t of a group owns input quaternions 8t .. 8t+7 of the
+// block in both operands, in the pairs (k, k + 4) that two shifts and masks
+// take out of a code word.
+//
+//   one or two tokens: the eight columns of B are (a, token), column (a, m)
+//     holding s(a, p) x_{a^p}[m]: four products of K = 32 give everything.
+//   more: the columns are eight tokens of a component plane x_q, sixteen
+//     products (a, p) per eight tokens with the sign on A.
+//
+// Expansion of a pair of codes: sign and magnitude bits are moved to the sign
+// and to the lowest exponent and highest mantissa bits of two 16-bit floats
+// (value 2^-126 or 2^-14 times the code's), then one packed multiplication by
+// 2^(126 or 14) * scale * 2^-c gives the weights, exactly: c = max(0, E0 - 128)
+// for bf16, with E0 the layer's largest scale (c = 0 unless weights reach 16),
+// E0 - 128 for fp16, which keeps scales down to 2^-38 of the largest exact.
+// The accumulated sums are multiplied by 2^c.
+//
+// fp32 inputs are split into three bf16 parts of 8 bits each (x = x1 + x2 + x3
+// exactly, down to bf16's smallest number); their products go to the same
+// accumulator, which starts from zero for every block of 32 input quaternions
+// and is added to the fp32 sum outside the tensor core, whose own additions
+// truncate.
+//
+// Bound by the codes' bytes for one token of a wide layer, by latency for
+// narrow layers, by the expansion and the tensor pipe from about 8 tokens on.
+#pragma once
+
+#include <type_traits>
+
+#include "qlin_common.cuh"
+#include "qlin_mx.cuh"
+
+namespace qlin {
+
+constexpr int kMxWarps = 8;                       // consumer warps of a CTA
+constexpr int kMxThreads = 32 * (kMxWarps + 1);   // and the warp that issues the copies
+constexpr int kMxRedRow = 65;                     // floats of a reduction row: 64 outputs, padded
+constexpr int kMxSmemRank = 256;                  // adapters of up to this rank keep t in shared memory
+constexpr int kMxFewBar = 1;                      // named barrier of the consumer warps
+
+__host__ __device__ constexpr int mx_t_rank(int rank) { return rank <= kMxSmemRank ? rank : 0; }
+
+// Sign of component a's product with W_p: bit p of the mask set where it is negative.
+__device__ __forceinline__ uint32_t mx_negative(int a) {
+  return a == 0 ? 0xEu : (a == 1 ? 0x8u : (a == 2 ? 0x2u : 0x4u));
+}
+
+template <typename T>
+struct MxOperand {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr int kParts = std::is_same<T, float>::value ? 3 : 1;
+};
+
+// c of the layer whose largest scale is e0.
+template <bool HALF>
+__device__ __forceinline__ int mx_shift(uint32_t e0) {
+  return HALF ? (int)e0 - 128 : max(0, (int)e0 - 128);
+}
+
+// The packed multiplier of codes with scale e.  bf16: exponent field
+// E - 127 - c + 126 + 127; a NaN scale saturates at infinity, which makes NaNs
+// of the block's zero codes.
+template <bool HALF>
+__device__ __forceinline__ uint32_t mx_multiplier(uint32_t e, int c) {
+  if constexpr (HALF) {
+    const int f = min((int)e - 98 - c, 31);  // E - 127 - c + 14 + 15
+    return (f > 0 ? (uint32_t)f << 10 : (f >= -9 ? 1u << (f + 9) : 0u)) * 0x00010001u;
+  } else {
+    return (uint32_t)min((int)e + 126 - c, 255) * 0x00800080u;
+  }
+}
+
+template <bool HALF>
+__device__ __forceinline__ uint32_t mx_mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (HALF) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Eight codes -> pairs (k, k + 4), k = 0..3, times the multiplier.
+template <bool HALF>
+__device__ __forceinline__ void mx_expand(uint32_t w, uint32_t mult, uint32_t (&r)[4]) {
+  constexpr uint32_t kMag = HALF ? 0x0E000E00u : 0x01C001C0u;
+  constexpr int kAt = HALF ? 9 : 6;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t sign = (w << (12 - 4 * k)) & 0x80008000u;
+    const uint32_t mag = (kAt >= 4 * k ? w << (kAt - 4 * k) : w >> (4 * k - kAt)) & kMag;
+    r[k] = mx_mul2<HALF>(sign | mag, mult);
+  }
+}
+
+template <bool HALF>
+__device__ __forceinline__ void mx_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                       uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+// A lane's share of a record: the A operands of the block's two k16 steps for
+// all four components.
+template <bool HALF>
+__device__ __forceinline__ void mx_load_a(uint32_t rec, int g, int t, int c, uint32_t (&lo)[4][4],
+                                          uint32_t (&hi)[4][4]) {
+  const uint4 wl = lds128(rec + g * 64 + t * 16), wh = lds128(rec + (g + 8) * 64 + t * 16);
+  const uint32_t sl = lds32(rec + kMxCodeBytes + g * 4), sh = lds32(rec + kMxCodeBytes + (g + 8) * 4);
+  const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w};
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    mx_expand<HALF>(l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, c), lo[p]);
+    mx_expand<HALF>(h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, c), hi[p]);
+  }
+}
+
+// The three bf16 parts of an fp32 value by truncation; a value that is not
+// finite is its own first part.
+__device__ __forceinline__ void mx_parts(float v, uint32_t (&p)[3]) {
+  const uint32_t u = __float_as_uint(v);
+  p[1] = p[2] = 0u;
+  if ((u & 0x7F800000u) == 0x7F800000u) {
+    p[0] = (u >> 16) | ((u & 0x007FFFFFu) ? 0x40u : 0u);
+    return;
+  }
+  p[0] = u >> 16;
+  const float r = v - __uint_as_float(u & 0xFFFF0000u);
+  const uint32_t ur = __float_as_uint(r);
+  p[1] = ur >> 16;
+  p[2] = __float_as_uint(r - __uint_as_float(ur & 0xFFFF0000u)) >> 16;
+}
+
+// Eight input quaternions 8 oct .. 8 oct + 7 of a row as B words: out[part][q][k]
+// holds component q of quaternions k and k + 4; zero past the layer's.
+template <typename T>
+__device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool vec,
+                                           uint32_t (&out)[MxOperand<T>::kParts][4][4]) {
+  const int left = K_g - 8 * oct;
+  const T* at = row + 32 * (int64_t)oct;
+  if constexpr (sizeof(T) == 2) {
+    uint32_t w[8][2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[j][0] = w[j][1] = 0u;
+      if (j < left) {
+        if (vec) {
+          asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(w[j][0]), "=r"(w[j][1]) : "l"(at + 4 * j) : "memory");
+        } else {
+          const unsigned short* e = reinterpret_cast<const unsigned short*>(at + 4 * j);
+          w[j][0] = e[0] | (uint32_t)e[1] << 16;
+          w[j][1] = e[2] | (uint32_t)e[3] << 16;
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        out[0][q][k] = __byte_perm(w[k][q >> 1], w[k + 4][q >> 1], (q & 1) ? 0x7632 : 0x5410);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float v[2][4] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = k + 4 * h;
+        if (j < left) {
+          if (vec) {
+            const float4 f = ld_cg_f4(at + 4 * j);
+            v[h][0] = f.x; v[h][1] = f.y; v[h][2] = f.z; v[h][3] = f.w;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[h][q] = at[4 * j + q];
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t a[3], b[3];
+        mx_parts(v[0][q], a);
+        mx_parts(v[1][q], b);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) out[s][q][k] = a[s] | b[s] << 16;
+      }
+    }
+  }
+}
+
+template <typename T>
+struct MxFewParams {
+  const T* x;
+  int64_t ld_x;
+  const uint8_t* mx;
+  const uint8_t* arranged;  // B words of all tokens (more than two tokens)
+  const T* bias;
+  const T* lora_b;          // [4 N_g, rank]
+  const float* t;           // [M, rank] scaled down projection
+  T* y;
+  int64_t ld_y;
+  int M, K_g, N_g, rank;
+  int kb;                   // blocks of a row
+  int tiles;                // tiles of 16 output quaternions
+  int ring;                 // stages of the ring
+  int vec;                  // whole quaternions of x are aligned
+  int after_prologue;       // t comes from the previous kernel, which waited for everything before it
+};
+
+// Sums the K split of a tile's outputs (o of 16, a) for `toks` tokens from the
+// reduction rows, adds adapter and bias, and stores.  `warps` rows of partial
+// sums per token starting at red (rows of kMxRedRow floats, token-major).
+template <typename T>
+__device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float* red, int warps, int warp_stride,
+                                          int tok_local, int col, int64_t m, int64_t n0, float factor,
+                                          const float* ts) {
+  const int64_t n = n0 + col;
+  if (m >= prm.M || n >= 4 * (int64_t)prm.N_g) return;
+  float v = 0.f;
+  for (int w = 0; w < warps; ++w) v += red[w * warp_stride + tok_local * kMxRedRow + col];
+  v *= factor;
+  if (prm.rank > 0) {
+    const T* b = prm.lora_b + n * prm.rank;
+    float l = 0.f;
+    int r = 0;
+    if (sizeof(T) == 2 && prm.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(prm.lora_b) & 15) == 0) {
+      for (; r < prm.rank; r += 8) {
+        const uint4 q = ld_cg_v4(b + r);
+        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) l = fmaf(ts[r + j], to_f32(e[j]), l);
+      }
+    } else {
+      for (; r < prm.rank; ++r) l = fmaf(ts[r], to_f32(b[r]), l);
+    }
+    v += l;
+  }
+  if (prm.bias) v += to_f32(prm.bias[n]);
+  prm.y[m * prm.ld_y + n] = from_f32<T>(v);
+}
+
+// ---------------------------------------------------------------------------
+// one or two tokens
+// ---------------------------------------------------------------------------
+constexpr int kMxOneStage = kMxWarps * kMxRecord;  // a record per warp
+
+template <typename T>
+__host__ __device__ constexpr size_t mx_one_x_bytes(int kb) { return (size_t)kb * MxOperand<T>::kParts * 512; }
+
+// Shared memory: ring, x (B words [block][part][q][token][t]), reduction rows
+// (two buffers), t, barriers.
+template <typename T>
+constexpr size_t mx_one_smem(int kb, int ring, int rank) {
+  return (size_t)ring * kMxOneStage + mx_one_x_bytes<T>(kb) + 2 * kMxWarps * 2 * kMxRedRow * 4 +
+         2 * mx_t_rank(rank) * 4 +         16 * ring + 64;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMxThreads)
+qlin_mx_one_kernel(const MxFewParams<T> prm) {
+  constexpr bool HALF = MxOperand<T>::kHalf;
+  constexpr int P = MxOperand<T>::kParts;
+  extern __shared__ __align__(128) uint8_t mx_smem[];
+  const int S = prm.ring, kb = prm.kb;
+  uint8_t* xs = mx_smem + S * kMxOneStage;
+  float* red = reinterpret_cast<float*>(xs + mx_one_x_bytes<T>(kb));
+  float* ts = red + 2 * kMxWarps * 2 * kMxRedRow;
+  uint64_t* full = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + 2 * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
+  uint64_t* empty = full + S;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nst = (kb + kMxWarps - 1) / kMxWarps;
+  const int my_tiles = (int)blockIdx.x < prm.tiles ? (prm.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kMxWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (!prm.after_prologue) pdl_wait_prior();
+  __syncthreads();
+
+  if (warp == kMxWarps) {
+    if (lane == 0) {
+      int it = 0;
+      for (int j = 0; j < my_tiles && !*abort_flag; ++j) {
+        const int64_t tile = blockIdx.x + (int64_t)j * gridDim.x;
+        const uint8_t* src = prm.mx + kMxHeader + tile * kb * kMxRecord;
+        for (int st = 0; st < nst; ++st, ++it) {
+          const int s = it % S, u = it / S;
+          if (u > 0 && !mbar_wait(&empty[s], (u - 1) & 1)) {
+            *abort_flag = 1;
+            break;
+          }
+          const uint32_t bytes = min(kMxWarps, kb - st * kMxWarps) * kMxRecord;
+          mbar_arrive_expect_tx(&full[s], bytes);
+          bulk_load(mx_smem + s * kMxOneStage, src + (int64_t)st * kMxOneStage, bytes, &full[s]);
+        }
+      }
+      // issued copies have landed before the shared memory goes away
+      for (int k = max(0, it - S); k < it; ++k) mbar_wait(&full[k % S], (k / S) & 1);
+    }
+    return;
+  }
+
+  // x: a thread takes eight input quaternions of a token
+  for (int idx = threadIdx.x; idx < 2 * 4 * kb; idx += 32 * kMxWarps) {
+    const int tok = idx >= 4 * kb ? 1 : 0, oct = idx - tok * 4 * kb;
+    uint32_t w[P][4][4] = {};
+    if (tok < prm.M) mx_arrange<T>(prm.x + tok * prm.ld_x, oct, prm.K_g, prm.vec, w);
+#pragma unroll
+    for (int s = 0; s < P; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(xs + (((oct >> 2) * P + s) * 8 + q * 2 + tok) * 64 + (oct & 3) * 16) =
+            make_uint4(w[s][q][0], w[s][q][1], w[s][q][2], w[s][q][3]);
+  }
+  uint32_t e0;
+  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(e0) : "l"(prm.mx) : "memory");
+  const int c = mx_shift<HALF>(e0);
+  const float factor = scalbnf(1.f, c);
+  const int g = lane >> 2, t = lane & 3;
+  const int a_of = g >> 1, tok_of = g & 1;  // this lane's B column
+  uint32_t flip[4], from[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    flip[p] = (mx_negative(a_of) >> p & 1) ? 0x80008000u : 0u;
+    from[p] = smem_u32(xs) + ((a_of ^ p) * 2 + tok_of) * 64 + t * 16;
+  }
+  asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+
+  int it = 0;
+  for (int j = 0; j < my_tiles; ++j) {
+    const int64_t tile = blockIdx.x + (int64_t)j * gridDim.x;
+    float acc[2][4] = {};
+    for (int st = 0; st < nst; ++st, ++it) {
+      const int s = it % S, b = st * kMxWarps + warp;
+      if (!*abort_flag && !mbar_wait(&full[s], (it / S) & 1)) *abort_flag = 1;
+      if (b < kb) {
+        uint32_t lo[4][4], hi[4][4];
+        mx_load_a<HALF>(smem_u32(mx_smem) + s * kMxOneStage + warp * kMxRecord, g, t, c, lo, hi);
+        float d[2][4] = {};
+#pragma unroll
+        for (int s3 = 0; s3 < P; ++s3)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint4 w = lds128(from[p] + (b * P + s3) * 512);
+            float(&to)[4] = P > 1 ? d[p & 1] : acc[p & 1];
+            mx_mma<HALF>(to, lo[p][0], hi[p][0], lo[p][1], hi[p][1], w.x ^ flip[p], w.y ^ flip[p]);
+            mx_mma<HALF>(to, lo[p][2], hi[p][2], lo[p][3], hi[p][3], w.z ^ flip[p], w.w ^ flip[p]);
+          }
+        if constexpr (P > 1)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[0][k] += d[0][k] + d[1][k];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+    // lane (g, t): rows g and g + 8, columns (a = t, token 0), (a = t, token 1)
+    float* mine = red + ((j & 1) * kMxWarps + warp) * 2 * kMxRedRow;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      mine[(k & 1) * kMxRedRow + 4 * (g + 8 * (k >> 1)) + t] = acc[0][k] + acc[1][k];
+    if (j == 0 && prm.rank > 0) {
+      if (prm.after_prologue) pdl_wait_prior();
+      for (int k = threadIdx.x; k < prm.M * mx_t_rank(prm.rank); k += 32 * kMxWarps) ts[k] = __ldcg(prm.t + k);
+    }
+    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+    if (threadIdx.x < 128) {
+      const int tok = threadIdx.x >> 6, col = threadIdx.x & 63;
+      mx_finish<T>(prm, red + (j & 1) * kMxWarps * 2 * kMxRedRow, kMxWarps, 2 * kMxRedRow, tok, col, tok,
+                   tile * 4 * kMxRows, factor, (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// B words of many tokens, and the down projection of few
+// ---------------------------------------------------------------------------
+// arranged[token tile of C][block][part][q][token][t]: C * 4 * parts * 64 bytes a block.
+template <typename T>
+__device__ __forceinline__ void mx_arrange_one(const T* x, int64_t ld_x, int M, int K_g, int kb, int C, bool vec,
+                                               uint8_t* __restrict__ out, int64_t idx) {
+  constexpr int P = MxOperand<T>::kParts;
+  // consecutive threads: consecutive octets of a token
+  const int64_t m = idx / (4 * kb);
+  const int oct = (int)(idx - m * 4 * kb);
+  const int64_t vt = m / C;
+  const int tok = (int)(m - vt * C);
+  uint32_t w[P][4][4] = {};
+  if (m < M) mx_arrange<T>(x + m * ld_x, oct, K_g, vec, w);
+  uint8_t* at = out + ((vt * kb + (oct >> 2)) * P * 4 * C + tok) * 64 + (oct & 3) * 16;
+#pragma unroll
+  for (int s = 0; s < P; ++s)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint4*>(at + (int64_t)(s * 4 + q) * C * 64) =
+          make_uint4(w[s][q][0], w[s][q][1], w[s][q][2], w[s][q][3]);
+}
+
+constexpr int kMxDownTokens = 4;  // tokens of a down-projection CTA
+
+// Four consecutive elements.
+template <typename T>
+__device__ __forceinline__ float4 mx_load4(const T* at, bool vec) {
+  if (!vec) return make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
+  if constexpr (sizeof(T) == 4) {
+    return ld_cg_f4(at);
+  } else {
+    uint2 q;
+    asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(q.x), "=r"(q.y) : "l"(at) : "memory");
+    const T* e = reinterpret_cast<const T*>(&q);
+    return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
+  }
+}
+
+// Blocks [0, arrange_blocks): the B words.  The rest: t[m, r] = scale x A^T,
+// one rank and kMxDownTokens tokens per block, the row of A read once.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_prologue_kernel(const T* __restrict__ x, int64_t ld_x, int M, int K_g, int kb, int C, int vec,
+                        uint8_t* __restrict__ arranged, int arrange_blocks, int64_t octets,
+                        const T* __restrict__ lora_a, int vec_a, int rank, float scale, float* __restrict__ t) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  if ((int)blockIdx.x < arrange_blocks) {
+    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (idx < octets) mx_arrange_one<T>(x, ld_x, M, K_g, kb, C, vec, arranged, idx);
+    return;
+  }
+  __shared__ float part[8][kMxDownTokens];
+  const int b = (int)blockIdx.x - arrange_blocks;
+  const int r = b % rank, m0 = b / rank * kMxDownTokens;
+  const T* a = lora_a + (int64_t)r * 4 * K_g;
+  float s[kMxDownTokens] = {};
+  for (int i = threadIdx.x; i < K_g; i += 256) {
+    const float4 av = mx_load4(a + 4 * (int64_t)i, vec_a);
+#pragma unroll
+    for (int u = 0; u < kMxDownTokens; ++u) {
+      if (m0 + u >= M) break;
+      const float4 xv = mx_load4(x + (int64_t)(m0 + u) * ld_x + 4 * (int64_t)i, vec);
+      s[u] = fmaf(av.x, xv.x, fmaf(av.y, xv.y, fmaf(av.z, xv.z, fmaf(av.w, xv.w, s[u]))));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kMxDownTokens; ++u)
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int u = 0; u < kMxDownTokens; ++u) part[threadIdx.x >> 5][u] = s[u];
+  __syncthreads();
+  if (threadIdx.x < kMxDownTokens && m0 + (int)threadIdx.x < M) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += part[w][threadIdx.x];
+    t[(int64_t)(m0 + threadIdx.x) * rank + r] = scale * v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// more tokens: NT groups of eight per tile, WO tiles of output quaternions per
+// CTA (WO warps side by side, kMxWarps / WO along the blocks)
+// ---------------------------------------------------------------------------
+template <typename T, int NT, int WO>
+struct MxManyCfg {
+  static constexpr int kP = MxOperand<T>::kParts;
+  static constexpr int kC = 8 * NT;                      // tokens of a tile
+  static constexpr int kWK = kMxWarps / WO;              // blocks of a stage
+  static constexpr int kXBlock = kP * 4 * kC * 64;       // B words of a block
+  static constexpr int kStage = kWK * (WO * kMxRecord + kXBlock);
+  static constexpr int kRed = kMxWarps * 8 * kMxRedRow * 4;  // partial sums of eight tokens
+  static constexpr int kFixed = 2 * kRed + 64;
+  static_assert(kStage % 16 == 0, "copies of whole 16-byte pieces");
+};
+
+template <typename T, int NT, int WO>
+constexpr size_t mx_many_smem(int ring, int rank) {
+  using Cfg = MxManyCfg<T, NT, WO>;
+  return (size_t)ring * (Cfg::kStage + 16) + Cfg::kFixed + (size_t)Cfg::kC * mx_t_rank(rank) * 4;
+}
+
+template <typename T, int NT, int WO>
+__global__ void __launch_bounds__(kMxThreads, NT == 1 ? 2 : 1)
+qlin_mx_many_kernel(const MxFewParams<T> prm) {
+  using Cfg = MxManyCfg<T, NT, WO>;
+  constexpr bool HALF = MxOperand<T>::kHalf;
+  constexpr int P = Cfg::kP, C = Cfg::kC, WK = Cfg::kWK;
+  extern __shared__ __align__(128) uint8_t mx_smem[];
+  const int S = prm.ring, kb = prm.kb;
+  float* red = reinterpret_cast<float*>(mx_smem + S * Cfg::kStage);
+  float* ts = red + 2 * kMxWarps * 8 * kMxRedRow;
+  uint64_t* full = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + C * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
+  uint64_t* empty = full + S;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nst = (kb + WK - 1) / WK;
+  const int groups = (prm.tiles + WO - 1) / WO;           // CTA tiles along the outputs
+  const int total = groups * ((prm.M + C - 1) / C);
+  const int my_tiles = (int)blockIdx.x < total ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kMxWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  pdl_wait_prior();  // the B words and t
+  __syncthreads();
+
+  if (warp == kMxWarps) {
+    if (lane == 0) {
+      int it = 0;
+      for (int j = 0; j < my_tiles && !*abort_flag; ++j) {
+        const int id = (int)blockIdx.x + j * (int)gridDim.x;
+        const int64_t vt = id / groups, tile0 = (int64_t)(id - (int)vt * groups) * WO;
+        for (int st = 0; st < nst; ++st, ++it) {
+          const int s = it % S, u = it / S;
+          if (u > 0 && !mbar_wait(&empty[s], (u - 1) & 1)) {
+            *abort_flag = 1;
+            break;
+          }
+          const int b0 = st * WK, nb = min(WK, kb - b0);
+          const int rows = min(WO, prm.tiles - (int)tile0);
+          uint8_t* dst = mx_smem + s * Cfg::kStage;
+          mbar_arrive_expect_tx(&full[s], nb * (rows * kMxRecord + Cfg::kXBlock));
+          for (int w = 0; w < rows; ++w)
+            bulk_load(dst + w * WK * kMxRecord, prm.mx + kMxHeader + ((tile0 + w) * kb + b0) * kMxRecord,
+                      nb * kMxRecord, &full[s]);
+          bulk_load(dst + WO * WK * kMxRecord, prm.arranged + (vt * kb + b0) * Cfg::kXBlock, nb * Cfg::kXBlock,
+                    &full[s]);
+        }
+      }
+      for (int k = max(0, it - S); k < it; ++k) mbar_wait(&full[k % S], (k / S) & 1);
+    }
+    return;
+  }
+
+  uint32_t e0;
+  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(e0) : "l"(prm.mx) : "memory");
+  const int c = mx_shift<HALF>(e0);
+  const float factor = scalbnf(1.f, c);
+  const int g = lane >> 2, t = lane & 3;
+  const int wo = warp / WK, wk = warp - wo * WK;
+  int it = 0, round = 0;
+  for (int j = 0; j < my_tiles; ++j) {
+    const int id = (int)blockIdx.x + j * (int)gridDim.x;
+    const int64_t vt = id / groups, tile0 = (int64_t)(id - (int)vt * groups) * WO;
+    float acc[NT][4][4] = {};
+    for (int st = 0; st < nst; ++st, ++it) {
+      const int s = it % S;
+      if (!*abort_flag && !mbar_wait(&full[s], (it / S) & 1)) *abort_flag = 1;
+      if (st * WK + wk < kb && tile0 + wo < prm.tiles) {
+        const uint32_t base = smem_u32(mx_smem) + s * Cfg::kStage;
+        uint32_t lo[4][4], hi[4][4];
+        mx_load_a<HALF>(base + (wo * WK + wk) * kMxRecord, g, t, c, lo, hi);
+        const uint32_t xb = base + WO * WK * kMxRecord + wk * Cfg::kXBlock + g * 64 + t * 16;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float d[4][4] = {};
+#pragma unroll
+          for (int s3 = 0; s3 < P; ++s3)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 w = lds128(xb + ((s3 * 4 + q) * C + nt * 8) * 64);
+#pragma unroll
+              for (int a = 0; a < 4; ++a) {
+                const int p = a ^ q;
+                const bool neg = (a == 0 && p != 0) || (a == 1 && p == 3) || (a == 2 && p == 1) || (a == 3 && p == 2);
+                const uint32_t f = neg ? 0x80008000u : 0u;
+                float(&to)[4] = P > 1 ? d[a] : acc[nt][a];
+                mx_mma<HALF>(to, lo[p][0] ^ f, hi[p][0] ^ f, lo[p][1] ^ f, hi[p][1] ^ f, w.x, w.y);
+                mx_mma<HALF>(to, lo[p][2] ^ f, hi[p][2] ^ f, lo[p][3] ^ f, hi[p][3] ^ f, w.z, w.w);
+              }
+            }
+          if constexpr (P > 1)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) acc[nt][a][k] += d[a][k];
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+    if (mx_t_rank(prm.rank) > 0 && (j == 0 || id / groups != (id - (int)gridDim.x) / groups)) {
+      // t of this token tile (the barrier below orders it before its readers;
+      // the readers of the tile before have passed theirs)
+      asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+      const int64_t first = vt * C * prm.rank, count = min((int64_t)C, prm.M - vt * C) * prm.rank;
+      for (int64_t k = threadIdx.x; k < count; k += 32 * kMxWarps) ts[k] = __ldcg(prm.t + first + k);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt, ++round) {
+      // eight tokens at a time through one of two buffers
+      float* buf = red + (round & 1) * kMxWarps * 8 * kMxRedRow;
+      float* mine = buf + warp * 8 * kMxRedRow;
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mine[(2 * t + (k & 1)) * kMxRedRow + 4 * (g + 8 * (k >> 1)) + a] = acc[nt][a][k];
+      asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+      for (int k = threadIdx.x; k < 8 * 64 * WO; k += 32 * kMxWarps) {
+        const int col = k & 63, w = (k >> 6) % WO, tok = (k >> 6) / WO;
+        const int64_t m = vt * C + nt * 8 + tok;
+        mx_finish<T>(prm, buf + w * WK * 8 * kMxRedRow, WK, 8 * kMxRedRow, tok, col, m,
+                     (tile0 + w) * 4 * kMxRows, factor,
+                     (prm.rank <= kMxSmemRank ? ts : prm.t + vt * C * prm.rank) + (nt * 8 + tok) * prm.rank);
+      }
+    }
+  }
+}
+
+}  // namespace qlin

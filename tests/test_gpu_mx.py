@@ -108,7 +108,7 @@ def test_forward_over_odd_sizes(qb, cuda, dtype, fin, fout, M):
     check_forward(qb, ref.draw(dtype, M, fin, fout, bias=True, rank=5, seed=fin + fout + M, device=cuda), dtype, 2)
 
 
-@pytest.mark.parametrize("rank", [1, 4, 7, 16, 32, 33, 64, 65, 100, 130])
+@pytest.mark.parametrize("rank", [1, 4, 7, 16, 32, 33, 64, 65, 100, 130, 300])
 @pytest.mark.parametrize("M", [1, 12, 150])
 def test_forward_over_ranks(qb, cuda, rank, M):
     check_forward(qb, ref.draw("bf16", M, 256, 192, rank=rank, seed=rank, device=cuda), "bf16", 2)
