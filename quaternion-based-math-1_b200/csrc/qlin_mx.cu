@@ -78,7 +78,7 @@ int few_tile(int64_t M) { return M <= 8 ? 8 : (M <= 16 ? 16 : 32); }
 constexpr size_t kOneMaxX = 128 * 1024;
 bool is_one(int dtype, int64_t M, int64_t K_g) {
   const int64_t kb = ceil_div(K_g, kMxBlock);
-  return M <= 2 && (size_t)kb * 512 * (dtype == QLIN_F32 ? 3 : 1) <= kOneMaxX;
+  return M <= 2 && (size_t)kb * 1024 * (dtype == QLIN_F32 ? 3 : 1) + M * 4 * K_g * elem(dtype) <= kOneMaxX;
 }
 
 struct ForwardWs {
@@ -161,7 +161,7 @@ int launch_dependent(void (*kernel)(KArgs...), unsigned ctas, unsigned threads, 
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
 }
 
-constexpr size_t kMostSmem = 227 * 1024;
+constexpr size_t kMostSmem = 226 * 1024;  // 1 KB of the 227 for static shared memory
 
 // Raises a kernel's shared-memory limit once per device.
 template <typename K>
@@ -182,18 +182,17 @@ int ring_stages(size_t budget, size_t fixed, size_t stage, int64_t uses) {
   return (int)std::max<int64_t>(2, std::min(fit, uses));
 }
 
-template <typename T>
-int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
+template <typename T, int W>
+int launch_one(const MxFewParams<T>& base, int per_sm, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (allow_smem(qlin_mx_one_kernel<T>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+  if (allow_smem(qlin_mx_one_kernel<T, W>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
   MxFewParams<T> prm = base;
-  const int per_sm = prm.tiles > sms ? 2 : 1;
   const int ctas = std::min(prm.tiles, per_sm * sms);
-  const int64_t uses = ceil_div(prm.kb, kMxWarps) * ceil_div(prm.tiles, ctas);
-  prm.ring = ring_stages(kMostSmem / per_sm - 1024, mx_one_smem<T>(prm.kb, 0, prm.rank), kMxOneStage + 16, uses);
-  const size_t smem = mx_one_smem<T>(prm.kb, prm.ring, prm.rank);
+  const int64_t uses = ceil_div(prm.kb, W) * ceil_div(prm.tiles, ctas);
+  prm.ring = ring_stages(kMostSmem / per_sm - 1024, mx_one_smem<T, W>(prm.M, prm.K_g, 0, prm.rank), W * kMxRecord + 16, uses);
+  const size_t smem = mx_one_smem<T, W>(prm.M, prm.K_g, prm.ring, prm.rank);
   if (smem > kMostSmem) return QLIN_ERR_SHAPE;
-  return launch_dependent(qlin_mx_one_kernel<T>, ctas, kMxThreads, smem, s, prm);
+  return launch_dependent(qlin_mx_one_kernel<T, W>, ctas, 32 * (W + 1), smem, s, prm);
 }
 
 template <typename T, int NT, int WO>
@@ -247,7 +246,12 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
                                     reinterpret_cast<float*>(ws + w.t));
     if (st != QLIN_OK) return st;
   }
-  if (one) return launch_one<T>(prm, sms, s);
+  if (one) {
+    prm.vec = aligned(x, 16) && (4 * K_g * sizeof(T)) % 16 == 0 && (M == 1 || (ld_x * sizeof(T)) % 16 == 0);
+    // at most a tile per SM: 16 warps share its K; more tiles: two CTAs of 8 warps per SM
+    if (prm.tiles <= sms) return launch_one<T, 16>(prm, 1, sms, s);
+    return launch_one<T, 8>(prm, 2, sms, s);
+  }
   if (C == 8) return launch_many<T, 1, 1>(prm, sms, s);
   if (C == 16) return launch_many<T, 2, 2>(prm, sms, s);
   return launch_many<T, 4, 4>(prm, sms, s);

@@ -10,21 +10,32 @@
 // rounded to nearest, ties to the even code, saturating at 6 (the quotient is
 // below 8).  The power-of-two quotient is exact, so the codes are those of the
 // real-number definition.  E is clamped to [0, 254] (a block of zeros has
-// E = 0); a block that holds an infinity or a NaN gets E = 255 and zero codes
-// and stands for NaNs.
+// E = 0); a block that holds an infinity or a NaN gets zero codes and stands
+// for NaNs.
 //
-// Buffer: a header of kMxHeader bytes (word 0: the largest E below 255 of the
-// layer), then one record per 16 output quaternions (tile) and 32 input
+// Buffer: a header of kMxHeader bytes (word 0: the largest F of the layer's
+// finite blocks), then one record per 16 output quaternions (tile) and 32 input
 // quaternions (block), tile-major, blocks of one tile contiguous:
 //
 //     record (1088 bytes) = codes [16 rows][4 octets t][4 components p] words,
-//                           then scales [16 rows][4 components p] bytes
+//                           then F [16 rows][4 components p] bytes
 //
-// Word (row, t, p) holds the codes of input quaternions 32 b + 8 t + j
-// (j = 0..7) of component p in nibble j.  So one 16-byte piece holds all four
-// components of eight input quaternions of a row, and the pieces that the 32
-// lanes of an m16 tensor-core operand need are two runs of 512 bytes.  Rows and
-// input quaternions past the layer's are zero codes with E = 0.
+// F = E + 1, or 255 for NaNs, so that the fp32 number with exponent field F is
+// normal (twice the scale) or infinite.  Rows and input quaternions past the
+// layer's are zero codes with F = 1.
+//
+// Word (row, t, p) holds the codes of input quaternions 32 b + 8 t + j (j =
+// 0..7) of component p, quaternions k and k + 4 (a pair) in its low and high
+// half.  The four bits of a code lie where shifts by 0, 3 and 6 and one mask
+// bring three of the four pairs to sign and magnitude bits of two bf16 values
+// (bit of a half: 8 7 6 magnitude, 15 sign):
+//
+//     pair 0: 8 7 6, 15    pair 1: 5 4 3, 12    pair 2: 2 1 0, 9
+//     pair 3: the rest: 11 10 13, 14
+//
+// One 16-byte piece holds all four components of eight input quaternions of a
+// row, and the pieces that the 32 lanes of an m16 tensor-core operand need are
+// two runs of 512 bytes.
 #pragma once
 
 #include <type_traits>
@@ -39,17 +50,50 @@ constexpr int kMxCodeBytes = kMxRows * kMxBlock * 4 / 2;
 constexpr int kMxRecord = kMxCodeBytes + kMxRows * 4;
 constexpr int kMxHeader = 128;
 
-// 2^(E - 127) as fp32 (E = 0: the subnormal 2^-127; E = 255: NaN).
-__device__ __forceinline__ float mx_scale(uint32_t e) {
-  return __uint_as_float(e == 255u ? 0x7FC00000u : (e == 0u ? 0x00400000u : e << 23));
+// The scale 2^(F - 128) as fp32 (F = 1: the subnormal 2^-127).
+__device__ __forceinline__ float mx_scale(uint32_t f) {
+  return __uint_as_float(f == 255u ? 0x7FC00000u : (f == 1u ? 0x00400000u : (f - 1u) << 23));
 }
 
-// e2m1 value of the low four bits of c.
-__device__ __forceinline__ float mx_value(uint32_t c) {
-  const uint32_t m = c & 7u;
-  // exponent field 0: 0 or 0.5; else 2^(e - 1) (1 + m / 2)
-  const uint32_t bits = m < 2u ? m * 0x3F000000u : ((126u + (m >> 1)) << 23 | (m & 1u) << 22);
-  return __uint_as_float(bits | (c & 8u) << 28);
+// Bits of a code (sign, magnitude of 3 bits) of element j of a word.
+__device__ __forceinline__ uint32_t mx_place(uint32_t sign, uint32_t mag, int j) {
+  const int k = j & 3;
+  const uint32_t bits = k < 3 ? mag << (6 - 3 * k) | sign << (15 - 3 * k)
+                              : (mag >> 1) << 10 | (mag & 1u) << 13 | sign << 14;
+  return bits << (16 * (j >> 2));
+}
+
+// Eight codes of a word as pairs (k, k + 4) of 16-bit floats: bf16 with the
+// code's value times 2^-126, or f16 with its value times 2^-14 (both exact;
+// the codes of +-0.5 are subnormal there).
+template <bool HALF>
+__device__ __forceinline__ void mx_expand(uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t w3 = w << 3, w6 = w << 6;
+  if constexpr (HALF) {
+    constexpr uint32_t kS = 0x80008000u, kM = 0x0E000E00u;
+    r[0] = (w & kS) | (w3 & kM);
+    r[1] = (w3 & kS) | (w6 & kM);
+    r[2] = (w6 & kS) | ((w << 9) & kM);
+    r[3] = ((w << 1) & kS) | ((w >> 4) & 0x02000200u) | (w & 0x0C000C00u);
+  } else {
+    constexpr uint32_t kSM = 0x81C081C0u;
+    r[0] = w & kSM;
+    r[1] = w3 & kSM;
+    r[2] = w6 & kSM;
+    r[3] = ((w << 1) & 0x80008000u) | ((w >> 7) & 0x00400040u) | ((w >> 3) & 0x01800180u);
+  }
+}
+
+// The values of a word's codes, in order.
+__device__ __forceinline__ void mx_values(uint32_t w, float (&v)[8]) {
+  uint32_t r[4];
+  mx_expand<true>(w, r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&r[k]);
+    v[k] = __low2float(h) * 16384.f;
+    v[k + 4] = __high2float(h) * 16384.f;
+  }
 }
 
 // E of a block whose largest magnitude is amax (finite).
@@ -125,19 +169,19 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       const bool bad = m >= 0x7F800000u;
-      const uint32_t e = bad ? 255u : mx_exponent(__uint_as_float(m));
+      const uint32_t e = mx_exponent(__uint_as_float(m));
       uint32_t word = 0;
       if (!bad) {
-        top = max(top, e);
+        top = max(top, e + 1u);
         const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - E): E is at most 252
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t sign = __float_as_uint(v[j]) >> 31;
-          word |= (mx_code(fabsf(v[j]) * inv) | sign << 3) << (4 * j);
+          word |= mx_place(sign, mx_code(fabsf(v[j]) * inv), j);
         }
       }
       *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = word;
-      if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)e;
+      if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
     }
   }
   __shared__ uint32_t tops[8];
@@ -174,9 +218,11 @@ qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst,
       const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4);
       const float s = mx_scale(in[kMxCodeBytes + row * 4 + p]);
       T* at = dst.w[p] + o * ld + i;
+      float c[8];
+      mx_values(word, c);
       T v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(mx_value(word >> (4 * j)) * s);
+      for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(c[j] * s);
       if (vec && left >= 8) {
 #pragma unroll
         for (int c = 0; c < (int)sizeof(T) / 2; ++c)
@@ -210,8 +256,10 @@ qlin_mx_adjoint_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, in
       const uint8_t* in = mx + kMxHeader + (tile * kb + b) * kMxRecord;
       const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4);
       const float s = mx_scale(in[kMxCodeBytes + row * 4 + p]) * (p == 0 ? 1.f : -1.f);
+      float c[8];
+      mx_values(word, c);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) turn[p][8 * t + j][16 * u + row] = from_f32<T>(mx_value(word >> (4 * j)) * s);
+      for (int j = 0; j < 8; ++j) turn[p][8 * t + j][16 * u + row] = from_f32<T>(c[j] * s);
     }
     __syncthreads();
     const int64_t o0 = 64 * g;

@@ -18,13 +18,17 @@
 //   more: the columns are eight tokens of a component plane x_q, sixteen
 //     products (a, p) per eight tokens with the sign on A.
 //
-// Expansion of a pair of codes: sign and magnitude bits are moved to the sign
-// and to the lowest exponent and highest mantissa bits of two 16-bit floats
-// (value 2^-126 or 2^-14 times the code's), then one packed multiplication by
-// 2^(126 or 14) * scale * 2^-c gives the weights, exactly: c = max(0, E0 - 128)
-// for bf16, with E0 the layer's largest scale (c = 0 unless weights reach 16),
-// E0 - 128 for fp16, which keeps scales down to 2^-38 of the largest exact.
-// The accumulated sums are multiplied by 2^c.
+// Codes expand exactly to bf16 values times 2^-126 (f16: 2^-14), see mx_expand.
+//   one or two tokens: those are the operand.  x (bf16) is multiplied by 2^k
+//     beforehand, k = 126 minus the exponent of the token's largest value, so
+//     that neither overflows nor underflows (a scaling up is exact); the
+//     product of a block and component starts from zero and joins the fp32 sum
+//     with its scale in one multiply-add per value.
+//   more: a packed multiplication by 2^(126 or 14) * scale * 2^-c makes the
+//     weights, exactly: c = max(0, F0 - 129) for bf16, with F0 the layer's
+//     largest F (c = 0 unless weights reach 16), F0 - 129 for f16, which keeps
+//     scales down to 2^-38 of the largest exact.  The sums are multiplied by
+//     2^c at the end.
 //
 // fp32 inputs are split into three bf16 parts of 8 bits each (x = x1 + x2 + x3
 // exactly, down to bf16's smallest number); their products go to the same
@@ -62,22 +66,22 @@ struct MxOperand {
   static constexpr int kParts = std::is_same<T, float>::value ? 3 : 1;
 };
 
-// c of the layer whose largest scale is e0.
+// c of the layer whose largest F is f0.
 template <bool HALF>
-__device__ __forceinline__ int mx_shift(uint32_t e0) {
-  return HALF ? (int)e0 - 128 : max(0, (int)e0 - 128);
+__device__ __forceinline__ int mx_shift(uint32_t f0) {
+  return HALF ? (int)f0 - 129 : max(0, (int)f0 - 129);
 }
 
-// The packed multiplier of codes with scale e.  bf16: exponent field
-// E - 127 - c + 126 + 127; a NaN scale saturates at infinity, which makes NaNs
-// of the block's zero codes.
+// The packed multiplier of codes with scale F.  bf16: exponent field
+// F - 128 - c + 126 + 127; a NaN block's F saturates at infinity, which makes
+// NaNs of its zero codes.
 template <bool HALF>
-__device__ __forceinline__ uint32_t mx_multiplier(uint32_t e, int c) {
+__device__ __forceinline__ uint32_t mx_multiplier(uint32_t f, int c) {
   if constexpr (HALF) {
-    const int f = min((int)e - 98 - c, 31);  // E - 127 - c + 14 + 15
-    return (f > 0 ? (uint32_t)f << 10 : (f >= -9 ? 1u << (f + 9) : 0u)) * 0x00010001u;
+    const int e = min((int)f - 99 - c, 31);  // F - 128 - c + 14 + 15
+    return (e > 0 ? (uint32_t)e << 10 : (e >= -9 ? 1u << (e + 9) : 0u)) * 0x00010001u;
   } else {
-    return (uint32_t)min((int)e + 126 - c, 255) * 0x00800080u;
+    return (uint32_t)min((int)f + 125 - c, 255) * 0x00800080u;
   }
 }
 
@@ -89,17 +93,11 @@ __device__ __forceinline__ uint32_t mx_mul2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Eight codes -> pairs (k, k + 4), k = 0..3, times the multiplier.
 template <bool HALF>
-__device__ __forceinline__ void mx_expand(uint32_t w, uint32_t mult, uint32_t (&r)[4]) {
-  constexpr uint32_t kMag = HALF ? 0x0E000E00u : 0x01C001C0u;
-  constexpr int kAt = HALF ? 9 : 6;
+__device__ __forceinline__ void mx_expand_scaled(uint32_t w, uint32_t mult, uint32_t (&r)[4]) {
+  mx_expand<HALF>(w, r);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t sign = (w << (12 - 4 * k)) & 0x80008000u;
-    const uint32_t mag = (kAt >= 4 * k ? w << (kAt - 4 * k) : w >> (4 * k - kAt)) & kMag;
-    r[k] = mx_mul2<HALF>(sign | mag, mult);
-  }
+  for (int k = 0; k < 4; ++k) r[k] = mx_mul2<HALF>(r[k], mult);
 }
 
 template <bool HALF>
@@ -126,8 +124,8 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   return v;
 }
 
-// A lane's share of a record: the A operands of the block's two k16 steps for
-// all four components.
+// A lane's share of a record: the A operands (weights) of the block's two k16
+// steps for all four components.
 template <bool HALF>
 __device__ __forceinline__ void mx_load_a(uint32_t rec, int g, int t, int c, uint32_t (&lo)[4][4],
                                           uint32_t (&hi)[4][4]) {
@@ -136,8 +134,8 @@ __device__ __forceinline__ void mx_load_a(uint32_t rec, int g, int t, int c, uin
   const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    mx_expand<HALF>(l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, c), lo[p]);
-    mx_expand<HALF>(h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, c), hi[p]);
+    mx_expand_scaled<HALF>(l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, c), lo[p]);
+    mx_expand_scaled<HALF>(h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, c), hi[p]);
   }
 }
 
@@ -157,9 +155,10 @@ __device__ __forceinline__ void mx_parts(float v, uint32_t (&p)[3]) {
   p[2] = __float_as_uint(r - __uint_as_float(ur & 0xFFFF0000u)) >> 16;
 }
 
-// Eight input quaternions 8 oct .. 8 oct + 7 of a row as B words: out[part][q][k]
-// holds component q of quaternions k and k + 4; zero past the layer's.
-template <typename T>
+// Eight input quaternions 8 oct .. 8 oct + 7 of a row (in global or, SHARED, in
+// shared memory) as B words: out[part][q][k] holds component q of quaternions k
+// and k + 4; zero past the layer's.
+template <typename T, bool SHARED = false>
 __device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool vec,
                                            uint32_t (&out)[MxOperand<T>::kParts][4][4]) {
   const int left = K_g - 8 * oct;
@@ -170,7 +169,11 @@ __device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool 
     for (int j = 0; j < 8; ++j) {
       w[j][0] = w[j][1] = 0u;
       if (j < left) {
-        if (vec) {
+        if (SHARED) {
+          const uint2 v = *reinterpret_cast<const uint2*>(at + 4 * j);
+          w[j][0] = v.x;
+          w[j][1] = v.y;
+        } else if (vec) {
           asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(w[j][0]), "=r"(w[j][1]) : "l"(at + 4 * j) : "memory");
         } else {
           const unsigned short* e = reinterpret_cast<const unsigned short*>(at + 4 * j);
@@ -193,7 +196,7 @@ __device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool 
         const int j = k + 4 * h;
         if (j < left) {
           if (vec) {
-            const float4 f = ld_cg_f4(at + 4 * j);
+            const float4 f = SHARED ? *reinterpret_cast<const float4*>(at + 4 * j) : ld_cg_f4(at + 4 * j);
             v[h][0] = f.x; v[h][1] = f.y; v[h][2] = f.z; v[h][3] = f.w;
           } else {
 #pragma unroll
@@ -228,7 +231,7 @@ struct MxFewParams {
   int kb;                   // blocks of a row
   int tiles;                // tiles of 16 output quaternions
   int ring;                 // stages of the ring
-  int vec;                  // whole quaternions of x are aligned
+  int vec;                  // whole quaternions of x are aligned (one or two tokens: x takes bulk copies)
   int after_prologue;       // t comes from the previous kernel, which waited for everything before it
 };
 
@@ -267,51 +270,66 @@ __device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float
 // ---------------------------------------------------------------------------
 // one or two tokens
 // ---------------------------------------------------------------------------
-constexpr int kMxOneStage = kMxWarps * kMxRecord;  // a record per warp
-
 template <typename T>
-__host__ __device__ constexpr size_t mx_one_x_bytes(int kb) { return (size_t)kb * MxOperand<T>::kParts * 512; }
+__host__ __device__ constexpr size_t mx_one_x_bytes(int kb) { return (size_t)kb * MxOperand<T>::kParts * 1024; }
 
-// Shared memory: ring, x (B words [block][part][q][token][t]), reduction rows
-// (two buffers), t, barriers.
+// Shared memory: ring, x as B words [block][part][sign][q][token][t] (both
+// signs, so that no lane flips its operand), x as it came, reduction rows (two
+// buffers), t, barriers.
 template <typename T>
-constexpr size_t mx_one_smem(int kb, int ring, int rank) {
-  return (size_t)ring * kMxOneStage + mx_one_x_bytes<T>(kb) + 2 * kMxWarps * 2 * kMxRedRow * 4 +
-         2 * mx_t_rank(rank) * 4 +         16 * ring + 64;
+__host__ __device__ constexpr size_t mx_one_raw_bytes(int K_g) { return ((size_t)K_g * 4 * sizeof(T) + 15) / 16 * 16; }
+template <typename T, int W>
+constexpr size_t mx_one_smem(int M, int K_g, int ring, int rank) {
+  return (size_t)ring * (W * kMxRecord) + mx_one_x_bytes<T>((K_g + kMxBlock - 1) / kMxBlock) +
+         M * mx_one_raw_bytes<T>(K_g) + 2 * W * 2 * kMxRedRow * 4 +
+         2 * mx_t_rank(rank) * 4 + 16 * ring + 64;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kMxThreads)
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * (W + 1))
 qlin_mx_one_kernel(const MxFewParams<T> prm) {
   constexpr bool HALF = MxOperand<T>::kHalf;
   constexpr int P = MxOperand<T>::kParts;
+  constexpr int kStage = W * kMxRecord;  // a record per warp
+  using E = typename std::conditional<sizeof(T) == 2, unsigned short, uint32_t>::type;
   extern __shared__ __align__(128) uint8_t mx_smem[];
   const int S = prm.ring, kb = prm.kb;
-  uint8_t* xs = mx_smem + S * kMxOneStage;
-  float* red = reinterpret_cast<float*>(xs + mx_one_x_bytes<T>(kb));
-  float* ts = red + 2 * kMxWarps * 2 * kMxRedRow;
+  uint8_t* xs = mx_smem + S * kStage;
+  uint8_t* raw = xs + mx_one_x_bytes<T>(kb);
+  const size_t raw_row = mx_one_raw_bytes<T>(prm.K_g);
+  float* red = reinterpret_cast<float*>(raw + prm.M * raw_row);
+  float* ts = red + 2 * W * 2 * kMxRedRow;
   uint64_t* full = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + 2 * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
   uint64_t* empty = full + S;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S);
+  uint64_t* x_full = empty + S;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(x_full + 1);
+  uint32_t* largest = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag + 1));  // [2], of the tokens, as bits
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nst = (kb + kMxWarps - 1) / kMxWarps;
+  const int nst = (kb + W - 1) / W;
   const int my_tiles = (int)blockIdx.x < prm.tiles ? (prm.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kMxWarps);
+      mbar_init(&empty[s], W);
     }
+    mbar_init(x_full, 1);
     *abort_flag = 0;
+    largest[0] = largest[1] = 0u;
     fence_mbar_init();
   }
   if (!prm.after_prologue) pdl_wait_prior();
   __syncthreads();
 
-  if (warp == kMxWarps) {
+  if (warp == W) {
     if (lane == 0) {
+      if (prm.vec) {  // ahead of the codes: behind them x would be the last to arrive
+        const uint32_t row = (uint32_t)prm.K_g * 4 * sizeof(T);
+        mbar_arrive_expect_tx(x_full, prm.M * row);
+        for (int m = 0; m < prm.M; ++m) bulk_load(raw + m * raw_row, prm.x + m * prm.ld_x, row, x_full);
+      }
       int it = 0;
       for (int j = 0; j < my_tiles && !*abort_flag; ++j) {
         const int64_t tile = blockIdx.x + (int64_t)j * gridDim.x;
@@ -322,84 +340,141 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
             *abort_flag = 1;
             break;
           }
-          const uint32_t bytes = min(kMxWarps, kb - st * kMxWarps) * kMxRecord;
+          const uint32_t bytes = min(W, kb - st * W) * kMxRecord;
           mbar_arrive_expect_tx(&full[s], bytes);
-          bulk_load(mx_smem + s * kMxOneStage, src + (int64_t)st * kMxOneStage, bytes, &full[s]);
+          bulk_load(mx_smem + s * kStage, src + (int64_t)st * kStage, bytes, &full[s]);
         }
       }
       // issued copies have landed before the shared memory goes away
+      if (prm.vec) mbar_wait(x_full, 0);
       for (int k = max(0, it - S); k < it; ++k) mbar_wait(&full[k % S], (k / S) & 1);
     }
     return;
   }
 
-  // x: a thread takes eight input quaternions of a token
-  for (int idx = threadIdx.x; idx < 2 * 4 * kb; idx += 32 * kMxWarps) {
-    const int tok = idx >= 4 * kb ? 1 : 0, oct = idx - tok * 4 * kb;
+  if (prm.vec) {
+    if (!mbar_wait(x_full, 0)) *abort_flag = 1;
+  } else {  // rows that no bulk copy takes
+    for (int m = 0; m < prm.M; ++m)
+      for (int k = threadIdx.x; k < 4 * prm.K_g; k += 32 * W)
+        reinterpret_cast<E*>(raw + m * raw_row)[k] = *reinterpret_cast<const volatile E*>(prm.x + m * prm.ld_x + k);
+    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
+  }
+  // true = sum * factor: F's exponent field makes twice the scale, the codes
+  // carry 2^-14 (f16) or, with x's 2^k, 2^(k - 126)
+  const int octets = 4 * kb;
+  float factor[2] = {8192.f, 8192.f};
+  uint32_t up[2] = {0u, 0u};  // 2^k, packed
+  if constexpr (!HALF) {
+    // k from the largest finite magnitude of a token
+#pragma unroll
+    for (int tok = 0; tok < 2; ++tok) {
+      if (tok >= prm.M) break;
+      uint32_t m = 0;
+      for (int k = threadIdx.x; k < prm.K_g; k += 32 * W) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 v = reinterpret_cast<const uint2*>(raw + tok * raw_row)[k];
+          const uint32_t e[4] = {v.x << 16, v.x & 0xFFFF0000u, v.y << 16, v.y & 0xFFFF0000u};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) m = max(m, (e[q] & 0x7F800000u) == 0x7F800000u ? 0u : e[q] & 0x7F800000u);
+        } else {
+          const uint4 v = reinterpret_cast<const uint4*>(raw + tok * raw_row)[k];
+          const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) m = max(m, (e[q] & 0x7F800000u) == 0x7F800000u ? 0u : e[q] & 0x7F800000u);
+        }
+      }
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (lane == 0 && m > 0u) atomicMax(&largest[tok], m);
+    }
+    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
+#pragma unroll
+    for (int tok = 0; tok < 2; ++tok) {
+      const int k = min(127, 253 - (int)(largest[tok] >> 23));
+      factor[tok] = scalbnf(1.f, 125 - k);
+      up[tok] = (uint32_t)(127 + k) * 0x00800080u;
+    }
+  }
+  // a thread takes eight input quaternions of a token
+  for (int idx = threadIdx.x; idx < 2 * octets; idx += 32 * W) {
+    const int tok = idx >= octets ? 1 : 0, oct = idx - tok * octets;
     uint32_t w[P][4][4] = {};
-    if (tok < prm.M) mx_arrange<T>(prm.x + tok * prm.ld_x, oct, prm.K_g, prm.vec, w);
+    if (tok < prm.M) {
+      mx_arrange<T, true>(reinterpret_cast<const T*>(raw + tok * raw_row), oct, prm.K_g, true, w);
+      if constexpr (!HALF)
+#pragma unroll
+        for (int s = 0; s < P; ++s)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[s][q][k] = mx_mul2<false>(w[s][q][k], tok ? up[1] : up[0]);
+    }
 #pragma unroll
     for (int s = 0; s < P; ++s)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(xs + (((oct >> 2) * P + s) * 8 + q * 2 + tok) * 64 + (oct & 3) * 16) =
-            make_uint4(w[s][q][0], w[s][q][1], w[s][q][2], w[s][q][3]);
+      for (int q = 0; q < 4; ++q) {
+        uint4* at = reinterpret_cast<uint4*>(xs + (((oct >> 2) * P + s) * 16 + q * 2 + tok) * 64 + (oct & 3) * 16);
+        at[0] = make_uint4(w[s][q][0], w[s][q][1], w[s][q][2], w[s][q][3]);
+        at[32] = make_uint4(w[s][q][0] ^ 0x80008000u, w[s][q][1] ^ 0x80008000u, w[s][q][2] ^ 0x80008000u,
+                            w[s][q][3] ^ 0x80008000u);
+      }
   }
-  uint32_t e0;
-  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(e0) : "l"(prm.mx) : "memory");
-  const int c = mx_shift<HALF>(e0);
-  const float factor = scalbnf(1.f, c);
+  asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
   const int g = lane >> 2, t = lane & 3;
   const int a_of = g >> 1, tok_of = g & 1;  // this lane's B column
-  uint32_t flip[4], from[4];
+  uint32_t from[4];
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    flip[p] = (mx_negative(a_of) >> p & 1) ? 0x80008000u : 0u;
-    from[p] = smem_u32(xs) + ((a_of ^ p) * 2 + tok_of) * 64 + t * 16;
-  }
-  asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+  for (int p = 0; p < 4; ++p)
+    from[p] = smem_u32(xs) + ((mx_negative(a_of) >> p & 1) * 8 + (a_of ^ p) * 2 + tok_of) * 64 + t * 16;
 
   int it = 0;
   for (int j = 0; j < my_tiles; ++j) {
     const int64_t tile = blockIdx.x + (int64_t)j * gridDim.x;
-    float acc[2][4] = {};
+    float acc[4] = {};
     for (int st = 0; st < nst; ++st, ++it) {
-      const int s = it % S, b = st * kMxWarps + warp;
+      const int s = it % S, b = st * W + warp;
       if (!*abort_flag && !mbar_wait(&full[s], (it / S) & 1)) *abort_flag = 1;
       if (b < kb) {
-        uint32_t lo[4][4], hi[4][4];
-        mx_load_a<HALF>(smem_u32(mx_smem) + s * kMxOneStage + warp * kMxRecord, g, t, c, lo, hi);
-        float d[2][4] = {};
+        const uint32_t rec = smem_u32(mx_smem) + s * kStage + warp * kMxRecord;
+        const uint4 wl = lds128(rec + g * 64 + t * 16), wh = lds128(rec + (g + 8) * 64 + t * 16);
+        const uint32_t sl = lds32(rec + kMxCodeBytes + g * 4), sh = lds32(rec + kMxCodeBytes + (g + 8) * 4);
+        const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
-        for (int s3 = 0; s3 < P; ++s3)
+        for (int p = 0; p < 4; ++p) {
+          uint32_t lo[4], hi[4];
+          mx_expand<HALF>(l[p], lo);
+          mx_expand<HALF>(h[p], hi);
+          float d[4] = {};
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const uint4 w = lds128(from[p] + (b * P + s3) * 512);
-            float(&to)[4] = P > 1 ? d[p & 1] : acc[p & 1];
-            mx_mma<HALF>(to, lo[p][0], hi[p][0], lo[p][1], hi[p][1], w.x ^ flip[p], w.y ^ flip[p]);
-            mx_mma<HALF>(to, lo[p][2], hi[p][2], lo[p][3], hi[p][3], w.z ^ flip[p], w.w ^ flip[p]);
+          for (int s3 = 0; s3 < P; ++s3) {
+            const uint4 w = lds128(from[p] + (b * P + s3) * 1024);
+            mx_mma<HALF>(d, lo[0], hi[0], lo[1], hi[1], w.x, w.y);
+            mx_mma<HALF>(d, lo[2], hi[2], lo[3], hi[3], w.z, w.w);
           }
-        if constexpr (P > 1)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[0][k] += d[0][k] + d[1][k];
+          const uint32_t fl = p < 3 ? sl << (23 - 8 * p) : sl >> 1, fh = p < 3 ? sh << (23 - 8 * p) : sh >> 1;
+          const float ml = __uint_as_float(fl & 0x7F800000u), mh = __uint_as_float(fh & 0x7F800000u);
+          acc[0] = fmaf(d[0], ml, acc[0]);
+          acc[1] = fmaf(d[1], ml, acc[1]);
+          acc[2] = fmaf(d[2], mh, acc[2]);
+          acc[3] = fmaf(d[3], mh, acc[3]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
     }
     // lane (g, t): rows g and g + 8, columns (a = t, token 0), (a = t, token 1)
-    float* mine = red + ((j & 1) * kMxWarps + warp) * 2 * kMxRedRow;
+    float* mine = red + ((j & 1) * W + warp) * 2 * kMxRedRow;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      mine[(k & 1) * kMxRedRow + 4 * (g + 8 * (k >> 1)) + t] = acc[0][k] + acc[1][k];
+    for (int k = 0; k < 4; ++k) mine[(k & 1) * kMxRedRow + 4 * (g + 8 * (k >> 1)) + t] = acc[k];
     if (j == 0 && prm.rank > 0) {
       if (prm.after_prologue) pdl_wait_prior();
-      for (int k = threadIdx.x; k < prm.M * mx_t_rank(prm.rank); k += 32 * kMxWarps) ts[k] = __ldcg(prm.t + k);
+      for (int k = threadIdx.x; k < prm.M * mx_t_rank(prm.rank); k += 32 * W) ts[k] = __ldcg(prm.t + k);
     }
-    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
     if (threadIdx.x < 128) {
       const int tok = threadIdx.x >> 6, col = threadIdx.x & 63;
-      mx_finish<T>(prm, red + (j & 1) * kMxWarps * 2 * kMxRedRow, kMxWarps, 2 * kMxRedRow, tok, col, tok,
-                   tile * 4 * kMxRows, factor, (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank);
+      mx_finish<T>(prm, red + (j & 1) * W * 2 * kMxRedRow, W, 2 * kMxRedRow, tok, col, tok,
+                   tile * 4 * kMxRows, tok ? factor[1] : factor[0], (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank);
     }
   }
 }
@@ -570,9 +645,9 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
     return;
   }
 
-  uint32_t e0;
-  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(e0) : "l"(prm.mx) : "memory");
-  const int c = mx_shift<HALF>(e0);
+  uint32_t f0;
+  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(prm.mx) : "memory");
+  const int c = mx_shift<HALF>(f0);
   const float factor = scalbnf(1.f, c);
   const int g = lane >> 2, t = lane & 3;
   const int wo = warp / WK, wk = warp - wo * WK;
