@@ -75,7 +75,7 @@ bool streams(int dtype, int64_t M) { return dtype == QLIN_F32 || M <= kFewTokens
 int few_tile(int64_t M) { return M <= 8 ? 8 : (M <= 16 ? 16 : 32); }
 
 // One or two tokens whose B words fit beside the ring.
-constexpr size_t kOneMaxX = 128 * 1024;
+constexpr size_t kOneMaxX = 150 * 1024;
 bool is_one(int dtype, int64_t M, int64_t K_g) {
   const int64_t kb = ceil_div(K_g, kMxBlock);
   return M <= 2 && (size_t)kb * 1024 * (dtype == QLIN_F32 ? 3 : 1) + M * 4 * K_g * elem(dtype) <= kOneMaxX;
@@ -182,17 +182,18 @@ int ring_stages(size_t budget, size_t fixed, size_t stage, int64_t uses) {
   return (int)std::max<int64_t>(2, std::min(fit, uses));
 }
 
-template <typename T, int W>
-int launch_one(const MxFewParams<T>& base, int per_sm, int sms, cudaStream_t s) {
+// W warps per tile, G tiles of a CTA at a time; QLIN_ERR_SHAPE where that does not fit.
+template <typename T, int W, int G>
+int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (allow_smem(qlin_mx_one_kernel<T, W>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
   MxFewParams<T> prm = base;
-  const int ctas = std::min(prm.tiles, per_sm * sms);
-  const int64_t uses = ceil_div(prm.kb, W) * ceil_div(prm.tiles, ctas);
-  prm.ring = ring_stages(kMostSmem / per_sm - 1024, mx_one_smem<T, W>(prm.M, prm.K_g, 0, prm.rank), W * kMxRecord + 16, uses);
-  const size_t smem = mx_one_smem<T, W>(prm.M, prm.K_g, prm.ring, prm.rank);
+  const int ctas = (int)std::min<int64_t>(prm.tiles, sms);
+  const int64_t uses = ceil_div(prm.kb, W) * ceil_div(prm.tiles, (int64_t)ctas * G);
+  prm.ring = ring_stages(kMostSmem, mx_one_smem<T, W, G>(prm.M, prm.K_g, 0, prm.rank), G * (W * kMxRecord + 16), uses);
+  const size_t smem = mx_one_smem<T, W, G>(prm.M, prm.K_g, prm.ring, prm.rank);
   if (smem > kMostSmem) return QLIN_ERR_SHAPE;
-  return launch_dependent(qlin_mx_one_kernel<T, W>, ctas, 32 * (W + 1), smem, s, prm);
+  if (allow_smem(qlin_mx_one_kernel<T, W, G>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+  return launch_dependent(qlin_mx_one_kernel<T, W, G>, ctas, 32 * (W + 1) * G, smem, s, prm);
 }
 
 template <typename T, int NT, int WO>
@@ -248,9 +249,13 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
   }
   if (one) {
     prm.vec = aligned(x, 16) && (4 * K_g * sizeof(T)) % 16 == 0 && (M == 1 || (ld_x * sizeof(T)) % 16 == 0);
-    // at most a tile per SM: 16 warps share its K; more tiles: two CTAs of 8 warps per SM
-    if (prm.tiles <= sms) return launch_one<T, 16>(prm, 1, sms, s);
-    return launch_one<T, 8>(prm, 2, sms, s);
+    // at most a tile per SM, or x too long for three rings: 16 warps share the
+    // tile's K; more tiles: three groups of 8 warps
+    if (prm.tiles > sms) {
+      const int st = launch_one<T, 8, 3>(prm, sms, s);
+      if (st != QLIN_ERR_SHAPE) return st;
+    }
+    return launch_one<T, 16, 1>(prm, sms, s);
   }
   if (C == 8) return launch_many<T, 1, 1>(prm, sms, s);
   if (C == 16) return launch_many<T, 2, 2>(prm, sms, s);

@@ -63,31 +63,43 @@ __device__ __forceinline__ uint32_t mx_place(uint32_t sign, uint32_t mag, int j)
   return bits << (16 * (j >> 2));
 }
 
+// Powers of two that the compiler cannot see: left shifts written as products
+// with them go to the multiply-add pipe, beside the masks on the integer pipe
+// (which alone would bound the expansion).
+struct MxPowers {
+  uint32_t p1, p3, p6;
+  __device__ __forceinline__ MxPowers() {
+    asm volatile("mov.u32 %0, 2;" : "=r"(p1));
+    asm volatile("mov.u32 %0, 8;" : "=r"(p3));
+    asm volatile("mov.u32 %0, 64;" : "=r"(p6));
+  }
+};
+
 // Eight codes of a word as pairs (k, k + 4) of 16-bit floats: bf16 with the
 // code's value times 2^-126, or f16 with its value times 2^-14 (both exact;
 // the codes of +-0.5 are subnormal there).
 template <bool HALF>
-__device__ __forceinline__ void mx_expand(uint32_t w, uint32_t (&r)[4]) {
-  const uint32_t w3 = w << 3, w6 = w << 6;
+__device__ __forceinline__ void mx_expand(const MxPowers& c, uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t w1 = w * c.p1, w3 = w * c.p3, w6 = w * c.p6;
   if constexpr (HALF) {
     constexpr uint32_t kS = 0x80008000u, kM = 0x0E000E00u;
     r[0] = (w & kS) | (w3 & kM);
     r[1] = (w3 & kS) | (w6 & kM);
-    r[2] = (w6 & kS) | ((w << 9) & kM);
-    r[3] = ((w << 1) & kS) | ((w >> 4) & 0x02000200u) | (w & 0x0C000C00u);
+    r[2] = (w6 & kS) | ((w6 * c.p3) & kM);
+    r[3] = (w1 & kS) | ((w >> 4) & 0x02000200u) | (w & 0x0C000C00u);
   } else {
     constexpr uint32_t kSM = 0x81C081C0u;
     r[0] = w & kSM;
     r[1] = w3 & kSM;
     r[2] = w6 & kSM;
-    r[3] = ((w << 1) & 0x80008000u) | ((w >> 7) & 0x00400040u) | ((w >> 3) & 0x01800180u);
+    r[3] = (w1 & 0x80008000u) | ((w >> 7) & 0x00400040u) | ((w >> 3) & 0x01800180u);
   }
 }
 
 // The values of a word's codes, in order.
 __device__ __forceinline__ void mx_values(uint32_t w, float (&v)[8]) {
   uint32_t r[4];
-  mx_expand<true>(w, r);
+  mx_expand<true>(MxPowers(), w, r);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const __half2 h = *reinterpret_cast<const __half2*>(&r[k]);

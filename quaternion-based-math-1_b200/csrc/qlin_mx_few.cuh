@@ -94,8 +94,8 @@ __device__ __forceinline__ uint32_t mx_mul2(uint32_t a, uint32_t b) {
 }
 
 template <bool HALF>
-__device__ __forceinline__ void mx_expand_scaled(uint32_t w, uint32_t mult, uint32_t (&r)[4]) {
-  mx_expand<HALF>(w, r);
+__device__ __forceinline__ void mx_expand_scaled(const MxPowers& c, uint32_t w, uint32_t mult, uint32_t (&r)[4]) {
+  mx_expand<HALF>(c, w, r);
 #pragma unroll
   for (int k = 0; k < 4; ++k) r[k] = mx_mul2<HALF>(r[k], mult);
 }
@@ -127,15 +127,15 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 // A lane's share of a record: the A operands (weights) of the block's two k16
 // steps for all four components.
 template <bool HALF>
-__device__ __forceinline__ void mx_load_a(uint32_t rec, int g, int t, int c, uint32_t (&lo)[4][4],
+__device__ __forceinline__ void mx_load_a(const MxPowers& pw, uint32_t rec, int g, int t, int c, uint32_t (&lo)[4][4],
                                           uint32_t (&hi)[4][4]) {
   const uint4 wl = lds128(rec + g * 64 + t * 16), wh = lds128(rec + (g + 8) * 64 + t * 16);
   const uint32_t sl = lds32(rec + kMxCodeBytes + g * 4), sh = lds32(rec + kMxCodeBytes + (g + 8) * 4);
   const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    mx_expand_scaled<HALF>(l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, c), lo[p]);
-    mx_expand_scaled<HALF>(h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, c), hi[p]);
+    mx_expand_scaled<HALF>(pw, l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, c), lo[p]);
+    mx_expand_scaled<HALF>(pw, h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, c), hi[p]);
   }
 }
 
@@ -155,10 +155,51 @@ __device__ __forceinline__ void mx_parts(float v, uint32_t (&p)[3]) {
   p[2] = __float_as_uint(r - __uint_as_float(ur & 0xFFFF0000u)) >> 16;
 }
 
-// Eight input quaternions 8 oct .. 8 oct + 7 of a row (in global or, SHARED, in
-// shared memory) as B words: out[part][q][k] holds component q of quaternions k
-// and k + 4; zero past the layer's.
-template <typename T, bool SHARED = false>
+// Four consecutive elements.
+template <typename T>
+__device__ __forceinline__ float4 mx_load4(const T* at, bool vec) {
+  if (!vec) return make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
+  if constexpr (sizeof(T) == 4) {
+    return ld_cg_f4(at);
+  } else {
+    uint2 q;
+    asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(q.x), "=r"(q.y) : "l"(at) : "memory");
+    const T* e = reinterpret_cast<const T*>(&q);
+    return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
+  }
+}
+
+// Input quaternions i and i + 4 of a row in shared memory as B words: out[part][q]
+// holds their components q; zero past the layer's.
+template <typename T>
+__device__ __forceinline__ void mx_arrange_pair(const T* row, int i, int K_g,
+                                                uint32_t (&out)[MxOperand<T>::kParts][4]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2* at = reinterpret_cast<const uint2*>(row);
+    const uint2 a = i < K_g ? at[i] : make_uint2(0u, 0u), b = i + 4 < K_g ? at[i + 4] : make_uint2(0u, 0u);
+    out[0][0] = __byte_perm(a.x, b.x, 0x5410);
+    out[0][1] = __byte_perm(a.x, b.x, 0x7632);
+    out[0][2] = __byte_perm(a.y, b.y, 0x5410);
+    out[0][3] = __byte_perm(a.y, b.y, 0x7632);
+  } else {
+    const float4* at = reinterpret_cast<const float4*>(row);
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 a = i < K_g ? at[i] : zero, b = i + 4 < K_g ? at[i + 4] : zero;
+    const float va[4] = {a.x, a.y, a.z, a.w}, vb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t pa[3], pb[3];
+      mx_parts(va[q], pa);
+      mx_parts(vb[q], pb);
+#pragma unroll
+      for (int s = 0; s < 3; ++s) out[s][q] = pa[s] | pb[s] << 16;
+    }
+  }
+}
+
+// Eight input quaternions 8 oct .. 8 oct + 7 of a row in global memory as B
+// words: out[part][q][k] holds component q of quaternions k and k + 4.
+template <typename T>
 __device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool vec,
                                            uint32_t (&out)[MxOperand<T>::kParts][4][4]) {
   const int left = K_g - 8 * oct;
@@ -169,11 +210,7 @@ __device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool 
     for (int j = 0; j < 8; ++j) {
       w[j][0] = w[j][1] = 0u;
       if (j < left) {
-        if (SHARED) {
-          const uint2 v = *reinterpret_cast<const uint2*>(at + 4 * j);
-          w[j][0] = v.x;
-          w[j][1] = v.y;
-        } else if (vec) {
+        if (vec) {
           asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(w[j][0]), "=r"(w[j][1]) : "l"(at + 4 * j) : "memory");
         } else {
           const unsigned short* e = reinterpret_cast<const unsigned short*>(at + 4 * j);
@@ -195,13 +232,8 @@ __device__ __forceinline__ void mx_arrange(const T* row, int oct, int K_g, bool 
       for (int h = 0; h < 2; ++h) {
         const int j = k + 4 * h;
         if (j < left) {
-          if (vec) {
-            const float4 f = SHARED ? *reinterpret_cast<const float4*>(at + 4 * j) : ld_cg_f4(at + 4 * j);
-            v[h][0] = f.x; v[h][1] = f.y; v[h][2] = f.z; v[h][3] = f.w;
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[h][q] = at[4 * j + q];
-          }
+          const float4 f = mx_load4(at + 4 * j, vec);
+          v[h][0] = f.x; v[h][1] = f.y; v[h][2] = f.z; v[h][3] = f.w;
         }
       }
 #pragma unroll
@@ -235,17 +267,17 @@ struct MxFewParams {
   int after_prologue;       // t comes from the previous kernel, which waited for everything before it
 };
 
-// Sums the K split of a tile's outputs (o of 16, a) for `toks` tokens from the
-// reduction rows, adds adapter and bias, and stores.  `warps` rows of partial
+// Sums the K split of a tile's outputs (o of 16, a) for a token from the
+// reduction rows, adds adapter and bias, and stores.  WARPS rows of partial
 // sums per token starting at red (rows of kMxRedRow floats, token-major).
-template <typename T>
-__device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float* red, int warps, int warp_stride,
-                                          int tok_local, int col, int64_t m, int64_t n0, float factor,
+template <int WARPS, typename T>
+__device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float* red, int warp_stride, int tok_local, int col, int64_t m, int64_t n0, float factor,
                                           const float* ts) {
   const int64_t n = n0 + col;
   if (m >= prm.M || n >= 4 * (int64_t)prm.N_g) return;
   float v = 0.f;
-  for (int w = 0; w < warps; ++w) v += red[w * warp_stride + tok_local * kMxRedRow + col];
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) v += red[w * warp_stride + tok_local * kMxRedRow + col];
   v *= factor;
   if (prm.rank > 0) {
     const T* b = prm.lora_b + n * prm.rank;
@@ -270,95 +302,121 @@ __device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float
 // ---------------------------------------------------------------------------
 // one or two tokens
 // ---------------------------------------------------------------------------
+
+// G groups of W consumer warps and one copying warp; a group takes a tile at a
+// time, its warps every W-th block of it.  The groups share x: with more tiles
+// than SMs, three groups keep three tiles of an SM in flight on one staged x
+// (two CTAs of one group each staged it twice and left 16 warps per SM: 15.4
+// against XX us for 5120 -> 27648).
+//
+// Shared memory: a ring per group, x as B words [block][part][sign][q][token][t]
+// (both signs, so that no lane flips its operand), x as it came, reduction rows
+// (two buffers per group), t, barriers.
+template <typename T>
+__host__ __device__ constexpr size_t mx_one_raw_bytes(int K_g) { return ((size_t)K_g * 4 * sizeof(T) + 15) / 16 * 16; }
 template <typename T>
 __host__ __device__ constexpr size_t mx_one_x_bytes(int kb) { return (size_t)kb * MxOperand<T>::kParts * 1024; }
 
-// Shared memory: ring, x as B words [block][part][sign][q][token][t] (both
-// signs, so that no lane flips its operand), x as it came, reduction rows (two
-// buffers), t, barriers.
-template <typename T>
-__host__ __device__ constexpr size_t mx_one_raw_bytes(int K_g) { return ((size_t)K_g * 4 * sizeof(T) + 15) / 16 * 16; }
-template <typename T, int W>
+template <typename T, int W, int G>
 constexpr size_t mx_one_smem(int M, int K_g, int ring, int rank) {
-  return (size_t)ring * (W * kMxRecord) + mx_one_x_bytes<T>((K_g + kMxBlock - 1) / kMxBlock) +
-         M * mx_one_raw_bytes<T>(K_g) + 2 * W * 2 * kMxRedRow * 4 +
-         2 * mx_t_rank(rank) * 4 + 16 * ring + 64;
+  return (size_t)G * ring * (W * kMxRecord + 16) + mx_one_x_bytes<T>((K_g + kMxBlock - 1) / kMxBlock) +
+         M * mx_one_raw_bytes<T>(K_g) + G * 2 * W * 2 * kMxRedRow * 4 + 2 * mx_t_rank(rank) * 4 + 64;
 }
 
-template <typename T, int W>
-__global__ void __launch_bounds__(32 * (W + 1))
+// Position in a ring of `stages` stages.
+struct MxRing {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++at == stages) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+template <typename T, int W, int G>
+__global__ void __launch_bounds__(32 * (W + 1) * G)
 qlin_mx_one_kernel(const MxFewParams<T> prm) {
   constexpr bool HALF = MxOperand<T>::kHalf;
   constexpr int P = MxOperand<T>::kParts;
   constexpr int kStage = W * kMxRecord;  // a record per warp
+  constexpr int kWorkers = 32 * W * G;   // threads that stage x
+  constexpr int kAllBar = G + 1;         // named barrier of all consumer warps; group g has 1 + g
   using E = typename std::conditional<sizeof(T) == 2, unsigned short, uint32_t>::type;
   extern __shared__ __align__(128) uint8_t mx_smem[];
   const int S = prm.ring, kb = prm.kb;
-  uint8_t* xs = mx_smem + S * kStage;
+  uint8_t* xs = mx_smem + G * S * kStage;
   uint8_t* raw = xs + mx_one_x_bytes<T>(kb);
   const size_t raw_row = mx_one_raw_bytes<T>(prm.K_g);
-  float* red = reinterpret_cast<float*>(raw + prm.M * raw_row);
-  float* ts = red + 2 * W * 2 * kMxRedRow;
-  uint64_t* full = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + 2 * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
-  uint64_t* empty = full + S;
-  uint64_t* x_full = empty + S;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(x_full + 1);
-  uint32_t* largest = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag + 1));  // [2], of the tokens, as bits
+  float* red_all = reinterpret_cast<float*>(raw + prm.M * raw_row);
+  float* ts = red_all + G * 2 * W * 2 * kMxRedRow;
+  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + 2 * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
+  uint64_t* x_full = bars + 2 * G * S;
+  uint32_t* largest = reinterpret_cast<uint32_t*>(x_full + 1);  // [2], of the tokens, as bits
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool copies = warp >= W * G;
+  const int grp = copies ? warp - W * G : warp / W;
+  uint8_t* ring = mx_smem + grp * S * kStage;
+  uint64_t* full = bars + 2 * grp * S;
+  uint64_t* empty = full + S;
   const int nst = (kb + W - 1) / W;
-  const int my_tiles = (int)blockIdx.x < prm.tiles ? (prm.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  // tile = id, id + stride, ...; a CTA's groups are far apart, so that few tiles spread over the SMs
+  const int id = (int)blockIdx.x + grp * (int)gridDim.x, stride = G * (int)gridDim.x;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], W);
+    for (int s = 0; s < G * S; ++s) {
+      mbar_init(&bars[2 * (s / S) * S + s % S], 1);
+      mbar_init(&bars[(2 * (s / S) + 1) * S + s % S], W);
     }
     mbar_init(x_full, 1);
-    *abort_flag = 0;
     largest[0] = largest[1] = 0u;
     fence_mbar_init();
   }
   if (!prm.after_prologue) pdl_wait_prior();
   __syncthreads();
 
-  if (warp == W) {
+  if (copies) {
     if (lane == 0) {
-      if (prm.vec) {  // ahead of the codes: behind them x would be the last to arrive
+      if (grp == 0 && prm.vec) {  // ahead of the codes: behind them x would be the last to arrive
         const uint32_t row = (uint32_t)prm.K_g * 4 * sizeof(T);
         mbar_arrive_expect_tx(x_full, prm.M * row);
         for (int m = 0; m < prm.M; ++m) bulk_load(raw + m * raw_row, prm.x + m * prm.ld_x, row, x_full);
       }
-      int it = 0;
-      for (int j = 0; j < my_tiles && !*abort_flag; ++j) {
-        const int64_t tile = blockIdx.x + (int64_t)j * gridDim.x;
-        const uint8_t* src = prm.mx + kMxHeader + tile * kb * kMxRecord;
-        for (int st = 0; st < nst; ++st, ++it) {
-          const int s = it % S, u = it / S;
-          if (u > 0 && !mbar_wait(&empty[s], (u - 1) & 1)) {
-            *abort_flag = 1;
+      MxRing r;
+      int issued = 0;
+      bool ok = true;
+      for (int tile = id; tile < prm.tiles && ok; tile += stride) {
+        const uint8_t* src = prm.mx + kMxHeader + (int64_t)tile * kb * kMxRecord;
+        for (int st = 0; st < nst; ++st) {
+          if (issued >= S && !mbar_wait(&empty[r.at], r.phase ^ 1u)) {
+            ok = false;
             break;
           }
           const uint32_t bytes = min(W, kb - st * W) * kMxRecord;
-          mbar_arrive_expect_tx(&full[s], bytes);
-          bulk_load(mx_smem + s * kStage, src + (int64_t)st * kStage, bytes, &full[s]);
+          mbar_arrive_expect_tx(&full[r.at], bytes);
+          bulk_load(ring + r.at * kStage, src + (int64_t)st * kStage, bytes, &full[r.at]);
+          r.next(S);
+          ++issued;
         }
       }
       // issued copies have landed before the shared memory goes away
-      if (prm.vec) mbar_wait(x_full, 0);
-      for (int k = max(0, it - S); k < it; ++k) mbar_wait(&full[k % S], (k / S) & 1);
+      if (grp == 0 && prm.vec) mbar_wait(x_full, 0);
+      for (int k = max(0, issued - S); k < issued; ++k) mbar_wait(&full[k % S], (k / S) & 1);
     }
     return;
   }
 
+  bool ok = true;  // a wait that ran out has recorded its error: on without waiting
   if (prm.vec) {
-    if (!mbar_wait(x_full, 0)) *abort_flag = 1;
+    ok = mbar_wait(x_full, 0);
   } else {  // rows that no bulk copy takes
     for (int m = 0; m < prm.M; ++m)
-      for (int k = threadIdx.x; k < 4 * prm.K_g; k += 32 * W)
+      for (int k = threadIdx.x; k < 4 * prm.K_g; k += kWorkers)
         reinterpret_cast<E*>(raw + m * raw_row)[k] = *reinterpret_cast<const volatile E*>(prm.x + m * prm.ld_x + k);
-    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"n"(kAllBar), "n"(kWorkers) : "memory");
   }
   // true = sum * factor: F's exponent field makes twice the scale, the codes
   // carry 2^-14 (f16) or, with x's 2^k, 2^(k - 126)
@@ -371,7 +429,7 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
     for (int tok = 0; tok < 2; ++tok) {
       if (tok >= prm.M) break;
       uint32_t m = 0;
-      for (int k = threadIdx.x; k < prm.K_g; k += 32 * W) {
+      for (int k = threadIdx.x; k < prm.K_g; k += kWorkers) {
         if constexpr (sizeof(T) == 2) {
           const uint2 v = reinterpret_cast<const uint2*>(raw + tok * raw_row)[k];
           const uint32_t e[4] = {v.x << 16, v.x & 0xFFFF0000u, v.y << 16, v.y & 0xFFFF0000u};
@@ -387,7 +445,7 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
       m = __reduce_max_sync(0xffffffffu, m);
       if (lane == 0 && m > 0u) atomicMax(&largest[tok], m);
     }
-    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"n"(kAllBar), "n"(kWorkers) : "memory");
 #pragma unroll
     for (int tok = 0; tok < 2; ++tok) {
       const int k = min(127, 253 - (int)(largest[tok] >> 23));
@@ -395,31 +453,25 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
       up[tok] = (uint32_t)(127 + k) * 0x00800080u;
     }
   }
-  // a thread takes eight input quaternions of a token
-  for (int idx = threadIdx.x; idx < 2 * octets; idx += 32 * W) {
-    const int tok = idx >= octets ? 1 : 0, oct = idx - tok * octets;
-    uint32_t w[P][4][4] = {};
-    if (tok < prm.M) {
-      mx_arrange<T, true>(reinterpret_cast<const T*>(raw + tok * raw_row), oct, prm.K_g, true, w);
-      if constexpr (!HALF)
-#pragma unroll
-        for (int s = 0; s < P; ++s)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[s][q][k] = mx_mul2<false>(w[s][q][k], tok ? up[1] : up[0]);
-    }
+  // a thread takes a pair of input quaternions (k, k + 4 of an octet) of a token
+  // (with one token the second's columns hold whatever the memory held: no
+  // other column sees them)
+  for (int idx = threadIdx.x; idx < prm.M * octets * 4; idx += kWorkers) {
+    const int tok = idx >= octets * 4 ? 1 : 0, pair = idx - tok * octets * 4, oct = pair >> 2, k = pair & 3;
+    uint32_t w[P][4];
+    mx_arrange_pair<T>(reinterpret_cast<const T*>(raw + tok * raw_row), 8 * oct + k, prm.K_g, w);
+    uint32_t* at = reinterpret_cast<uint32_t*>(xs + ((oct >> 2) * P * 16 + tok) * 64 + (oct & 3) * 16) + k;
 #pragma unroll
     for (int s = 0; s < P; ++s)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint4* at = reinterpret_cast<uint4*>(xs + (((oct >> 2) * P + s) * 16 + q * 2 + tok) * 64 + (oct & 3) * 16);
-        at[0] = make_uint4(w[s][q][0], w[s][q][1], w[s][q][2], w[s][q][3]);
-        at[32] = make_uint4(w[s][q][0] ^ 0x80008000u, w[s][q][1] ^ 0x80008000u, w[s][q][2] ^ 0x80008000u,
-                            w[s][q][3] ^ 0x80008000u);
+        uint32_t v = w[s][q];
+        if constexpr (!HALF) v = mx_mul2<false>(v, tok ? up[1] : up[0]);
+        at[(s * 16 + q * 2) * 16] = v;
+        at[(s * 16 + 8 + q * 2) * 16] = v ^ 0x80008000u;
       }
   }
-  asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"n"(kAllBar), "n"(kWorkers) : "memory");
   const int g = lane >> 2, t = lane & 3;
   const int a_of = g >> 1, tok_of = g & 1;  // this lane's B column
   uint32_t from[4];
@@ -427,23 +479,29 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
   for (int p = 0; p < 4; ++p)
     from[p] = smem_u32(xs) + ((mx_negative(a_of) >> p & 1) * 8 + (a_of ^ p) * 2 + tok_of) * 64 + t * 16;
 
-  int it = 0;
-  for (int j = 0; j < my_tiles; ++j) {
-    const int64_t tile = blockIdx.x + (int64_t)j * gridDim.x;
+  float* red = red_all + grp * 2 * W * 2 * kMxRedRow;
+  const int gwarp = warp - grp * W, gthread = (int)threadIdx.x - grp * W * 32;
+  const MxPowers pw;
+  uint32_t byte_up[3];  // F byte p to the exponent field
+  asm volatile("mov.u32 %0, 0x00800000;" : "=r"(byte_up[0]));
+  asm volatile("mov.u32 %0, 0x00008000;" : "=r"(byte_up[1]));
+  asm volatile("mov.u32 %0, 0x00000080;" : "=r"(byte_up[2]));
+  MxRing r;
+  int buffer = 0;
+  for (int tile = id; tile < prm.tiles; tile += stride) {
     float acc[4] = {};
-    for (int st = 0; st < nst; ++st, ++it) {
-      const int s = it % S, b = st * W + warp;
-      if (!*abort_flag && !mbar_wait(&full[s], (it / S) & 1)) *abort_flag = 1;
+    for (int b = gwarp; b < nst * W; b += W) {
+      if (ok) ok = mbar_wait(&full[r.at], r.phase);
       if (b < kb) {
-        const uint32_t rec = smem_u32(mx_smem) + s * kStage + warp * kMxRecord;
+        const uint32_t rec = smem_u32(ring) + r.at * kStage + gwarp * kMxRecord;
         const uint4 wl = lds128(rec + g * 64 + t * 16), wh = lds128(rec + (g + 8) * 64 + t * 16);
         const uint32_t sl = lds32(rec + kMxCodeBytes + g * 4), sh = lds32(rec + kMxCodeBytes + (g + 8) * 4);
         const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           uint32_t lo[4], hi[4];
-          mx_expand<HALF>(l[p], lo);
-          mx_expand<HALF>(h[p], hi);
+          mx_expand<HALF>(pw, l[p], lo);
+          mx_expand<HALF>(pw, h[p], hi);
           float d[4] = {};
 #pragma unroll
           for (int s3 = 0; s3 < P; ++s3) {
@@ -451,7 +509,7 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
             mx_mma<HALF>(d, lo[0], hi[0], lo[1], hi[1], w.x, w.y);
             mx_mma<HALF>(d, lo[2], hi[2], lo[3], hi[3], w.z, w.w);
           }
-          const uint32_t fl = p < 3 ? sl << (23 - 8 * p) : sl >> 1, fh = p < 3 ? sh << (23 - 8 * p) : sh >> 1;
+          const uint32_t fl = p < 3 ? sl * byte_up[p] : sl >> 1, fh = p < 3 ? sh * byte_up[p] : sh >> 1;
           const float ml = __uint_as_float(fl & 0x7F800000u), mh = __uint_as_float(fh & 0x7F800000u);
           acc[0] = fmaf(d[0], ml, acc[0]);
           acc[1] = fmaf(d[1], ml, acc[1]);
@@ -460,22 +518,26 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      if (lane == 0) mbar_arrive(&empty[r.at]);
+      r.next(S);
     }
     // lane (g, t): rows g and g + 8, columns (a = t, token 0), (a = t, token 1)
-    float* mine = red + ((j & 1) * W + warp) * 2 * kMxRedRow;
+    float* rows = red + buffer * W * 2 * kMxRedRow;
+    float* mine = rows + gwarp * 2 * kMxRedRow;
 #pragma unroll
     for (int k = 0; k < 4; ++k) mine[(k & 1) * kMxRedRow + 4 * (g + 8 * (k >> 1)) + t] = acc[k];
-    if (j == 0 && prm.rank > 0) {
+    if (tile == id && prm.rank > 0) {
       if (prm.after_prologue) pdl_wait_prior();
-      for (int k = threadIdx.x; k < prm.M * mx_t_rank(prm.rank); k += 32 * W) ts[k] = __ldcg(prm.t + k);
+      // (every group writes the same values)
+      for (int k = gthread; k < prm.M * mx_t_rank(prm.rank); k += 32 * W) ts[k] = __ldcg(prm.t + k);
     }
-    asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * W) : "memory");
-    if (threadIdx.x < 128) {
-      const int tok = threadIdx.x >> 6, col = threadIdx.x & 63;
-      mx_finish<T>(prm, red + (j & 1) * W * 2 * kMxRedRow, W, 2 * kMxRedRow, tok, col, tok,
-                   tile * 4 * kMxRows, tok ? factor[1] : factor[0], (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank);
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(32 * W) : "memory");
+    if (gthread < 64 * prm.M) {
+      const int tok = gthread >> 6, col = gthread & 63;
+      mx_finish<W>(prm, rows, 2 * kMxRedRow, tok, col, tok, (int64_t)tile * 4 * kMxRows,
+                   tok ? factor[1] : factor[0], (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank);
     }
+    buffer ^= 1;
   }
 }
 
@@ -504,20 +566,6 @@ __device__ __forceinline__ void mx_arrange_one(const T* x, int64_t ld_x, int M, 
 }
 
 constexpr int kMxDownTokens = 4;  // tokens of a down-projection CTA
-
-// Four consecutive elements.
-template <typename T>
-__device__ __forceinline__ float4 mx_load4(const T* at, bool vec) {
-  if (!vec) return make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
-  if constexpr (sizeof(T) == 4) {
-    return ld_cg_f4(at);
-  } else {
-    uint2 q;
-    asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(q.x), "=r"(q.y) : "l"(at) : "memory");
-    const T* e = reinterpret_cast<const T*>(&q);
-    return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
-  }
-}
 
 // Blocks [0, arrange_blocks): the B words.  The rest: t[m, r] = scale x A^T,
 // one rank and kMxDownTokens tokens per block, the row of A read once.
@@ -597,7 +645,6 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
   float* ts = red + 2 * kMxWarps * 8 * kMxRedRow;
   uint64_t* full = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + C * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
   uint64_t* empty = full + S;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + S);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nst = (kb + WK - 1) / WK;
@@ -611,7 +658,6 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kMxWarps);
     }
-    *abort_flag = 0;
     fence_mbar_init();
   }
   pdl_wait_prior();  // the B words and t
@@ -619,14 +665,16 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
 
   if (warp == kMxWarps) {
     if (lane == 0) {
-      int it = 0;
-      for (int j = 0; j < my_tiles && !*abort_flag; ++j) {
+      MxRing r;
+      int issued = 0;
+      bool ok = true;
+      for (int j = 0; j < my_tiles && ok; ++j) {
         const int id = (int)blockIdx.x + j * (int)gridDim.x;
         const int64_t vt = id / groups, tile0 = (int64_t)(id - (int)vt * groups) * WO;
-        for (int st = 0; st < nst; ++st, ++it) {
-          const int s = it % S, u = it / S;
-          if (u > 0 && !mbar_wait(&empty[s], (u - 1) & 1)) {
-            *abort_flag = 1;
+        for (int st = 0; st < nst; ++st) {
+          const int s = r.at;
+          if (issued >= S && !mbar_wait(&empty[s], r.phase ^ 1u)) {
+            ok = false;
             break;
           }
           const int b0 = st * WK, nb = min(WK, kb - b0);
@@ -638,9 +686,11 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
                       nb * kMxRecord, &full[s]);
           bulk_load(dst + WO * WK * kMxRecord, prm.arranged + (vt * kb + b0) * Cfg::kXBlock, nb * Cfg::kXBlock,
                     &full[s]);
+          r.next(S);
+          ++issued;
         }
       }
-      for (int k = max(0, it - S); k < it; ++k) mbar_wait(&full[k % S], (k / S) & 1);
+      for (int k = max(0, issued - S); k < issued; ++k) mbar_wait(&full[k % S], (k / S) & 1);
     }
     return;
   }
@@ -651,18 +701,21 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
   const float factor = scalbnf(1.f, c);
   const int g = lane >> 2, t = lane & 3;
   const int wo = warp / WK, wk = warp - wo * WK;
-  int it = 0, round = 0;
+  const MxPowers pw;
+  MxRing r;
+  int round = 0;
+  bool ok = true;
   for (int j = 0; j < my_tiles; ++j) {
     const int id = (int)blockIdx.x + j * (int)gridDim.x;
     const int64_t vt = id / groups, tile0 = (int64_t)(id - (int)vt * groups) * WO;
     float acc[NT][4][4] = {};
-    for (int st = 0; st < nst; ++st, ++it) {
-      const int s = it % S;
-      if (!*abort_flag && !mbar_wait(&full[s], (it / S) & 1)) *abort_flag = 1;
+    for (int st = 0; st < nst; ++st) {
+      const int s = r.at;
+      if (ok) ok = mbar_wait(&full[s], r.phase);
       if (st * WK + wk < kb && tile0 + wo < prm.tiles) {
         const uint32_t base = smem_u32(mx_smem) + s * Cfg::kStage;
         uint32_t lo[4][4], hi[4][4];
-        mx_load_a<HALF>(base + (wo * WK + wk) * kMxRecord, g, t, c, lo, hi);
+        mx_load_a<HALF>(pw, base + (wo * WK + wk) * kMxRecord, g, t, c, lo, hi);
         const uint32_t xb = base + WO * WK * kMxRecord + wk * Cfg::kXBlock + g * 64 + t * 16;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -691,6 +744,7 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
+      r.next(S);
     }
     if (mx_t_rank(prm.rank) > 0 && (j == 0 || id / groups != (id - (int)gridDim.x) / groups)) {
       // t of this token tile (the barrier below orders it before its readers;
@@ -713,7 +767,7 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
       for (int k = threadIdx.x; k < 8 * 64 * WO; k += 32 * kMxWarps) {
         const int col = k & 63, w = (k >> 6) % WO, tok = (k >> 6) / WO;
         const int64_t m = vt * C + nt * 8 + tok;
-        mx_finish<T>(prm, buf + w * WK * 8 * kMxRedRow, WK, 8 * kMxRedRow, tok, col, m,
+        mx_finish<WK>(prm, buf + w * WK * 8 * kMxRedRow, 8 * kMxRedRow, tok, col, m,
                      (tile0 + w) * 4 * kMxRows, factor,
                      (prm.rank <= kMxSmemRank ? ts : prm.t + vt * C * prm.rank) + (nt * 8 + tok) * prm.rank);
       }
