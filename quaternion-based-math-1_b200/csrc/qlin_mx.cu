@@ -9,6 +9,8 @@
 #include <atomic>
 #include <cstdint>
 #include <cstring>
+#include <mutex>
+#include <type_traits>
 
 #include "../../include/qlin_b200.h"
 #include "qlin_clip.cuh"
@@ -16,6 +18,7 @@
 #include "qlin_mx.cuh"
 #include "qlin_mx_few.cuh"
 #include "qlin_mx_lora.cuh"
+#include "qlin_mx_pair.cuh"
 
 namespace {
 
@@ -81,10 +84,15 @@ bool is_one(int dtype, int64_t M, int64_t K_g) {
   return M <= 2 && (size_t)kb * 1024 * (dtype == QLIN_F32 ? 3 : 1) + M * 4 * K_g * elem(dtype) <= kOneMaxX;
 }
 
+// Rows of 16-bit elements that TMA takes: 16-byte aligned start and row stride.
+bool tma_rows(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0; }
+
 struct ForwardWs {
-  size_t arranged = 0, t = 0, planes = 0, inner = 0, inner_bytes = 0, total = 0;
+  size_t arranged = 0, t = 0, x = 0, total = 0;
+  int64_t ld_parts = 0;  // columns of t's high (and low) parts
 };
 
+// Sized for the worst alignment of x: the pieces do not depend on pointers.
 ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   ForwardWs w;
   Carve c;
@@ -95,28 +103,64 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
     }
     w.t = c.take(M * rank * 4);
   } else {
-    w.planes = c.take(4 * K_g * N_g * elem(dtype));
-    qlin_workspace_size(dtype, M, K_g, N_g, rank, &w.inner_bytes);
-    w.inner = c.take((int64_t)w.inner_bytes);
+    w.ld_parts = round_up(rank, 64);
+    w.x = c.take(M * round_up(4 * K_g, 8) * 2);
+    w.t = c.take(M * 2 * w.ld_parts * 2);
   }
   w.total = c.at;
   return w;
 }
 
 struct BackwardWs {
-  size_t planes = 0, at = 0, bt = 0, t = 0, up = 0, inner = 0, inner_bytes = 0, total = 0;
+  // 16-bit
+  size_t gy = 0, x = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0;
+  int64_t M_pad = 0, ld_parts = 0, ld_planes = 0;
+  int rows0 = 0, rows1 = 0, splits0 = 0, splits1 = 0;
+  // fp32
+  size_t inner = 0, inner_bytes = 0;
+  size_t total = 0;
 };
+
+// Splits of the tokens of a gradient product: about four CTAs per SM, at least
+// four steps of 32 tokens each.
+int outer_splits(int64_t M_pad, int64_t cols, int rows) {
+  const int64_t tiles = ceil_div(cols, kMxOuterCols) * ceil_div(rows, kMxOuterRows);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 600 / std::max<int64_t>(1, tiles)));
+}
 
 BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   BackwardWs w;
   Carve c;
-  w.planes = c.take(4 * K_g * N_g * elem(dtype));
-  w.at = c.take(4 * K_g * rank * elem(dtype));
-  w.bt = c.take(4 * N_g * rank * elem(dtype));
-  w.t = c.take(M * rank * 4);
-  w.up = c.take(M * rank * 4);
-  qlin_workspace_size(dtype, M, N_g, K_g, rank, &w.inner_bytes);
-  w.inner = c.take((int64_t)w.inner_bytes);
+  if (dtype == QLIN_F32) {
+    w.planes = c.take(4 * K_g * N_g * 4);
+    w.at = c.take(4 * K_g * rank * 4);
+    w.bt = c.take(4 * N_g * rank * 4);
+    w.t = c.take(M * rank * 4);
+    w.up = c.take(M * rank * 4);
+    qlin_workspace_size(dtype, M, N_g, K_g, rank, &w.inner_bytes);
+    w.inner = c.take((int64_t)w.inner_bytes);
+  } else {
+    const int64_t K = 4 * K_g, N = 4 * N_g;
+    w.M_pad = round_up(M, kMxOuterTokens);
+    w.ld_parts = round_up(rank, 64);
+    w.ld_planes = round_up(N_g, 8);
+    w.rows0 = (int)round_up(rank, 16);
+    w.rows1 = (int)round_up(rank + 1, 16);
+    w.splits0 = outer_splits(w.M_pad, K, w.rows0);
+    w.splits1 = outer_splits(w.M_pad, N, w.rows1);
+    w.gy = c.take(M * round_up(N, 8) * 2);
+    w.x = c.take(rank > 0 ? M * round_up(K, 8) * 2 : 0);
+    w.planes = c.take(4 * K_g * w.ld_planes * 2);
+    if (rank > 0) {
+      w.at = c.take(K * rank * 2);
+      w.bt = c.take(N * rank * 2);
+      w.parts = c.take(M * 2 * w.ld_parts * 2);
+      w.up = c.take(2 * w.rows0 * w.M_pad * 2);
+      w.t = c.take(2 * w.rows1 * w.M_pad * 2);
+      w.partial0 = c.take((int64_t)w.splits0 * w.rows0 * K * 4);
+      w.partial1 = c.take((int64_t)w.splits1 * w.rows1 * N * 4);
+    }
+  }
   w.total = c.at;
   return w;
 }
@@ -260,6 +304,251 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
   if (C == 8) return launch_many<T, 1, 1>(prm, sms, s);
   if (C == 16) return launch_many<T, 2, 2>(prm, sms, s);
   return launch_many<T, 4, 4>(prm, sms, s);
+}
+
+// ---------------------------------------------------------------------------
+// many tokens, 16 bits
+// ---------------------------------------------------------------------------
+int encode_2d(CUtensorMap* map, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld, uint32_t box_cols,
+              uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  const auto encode = qlin_host_encoder();
+  if (!encode) return QLIN_ERR_LAUNCH;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? QLIN_OK
+             : QLIN_ERR_ALIGN;
+}
+
+// How many CTA pairs of a kernel the device holds at once (0: not known).
+template <typename T, int NTOK, bool MX>
+int pair_capacity() {
+  auto kernel = qlin_mx_pair_kernel<T, NTOK, MX>;
+  constexpr size_t smem = kPairSmemBytes;
+  static std::mutex mutex;
+  static int capacity[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (capacity[dev] == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2, 1, 1);
+    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = 2;
+    a.val.clusterDim.y = 1;
+    a.val.clusterDim.z = 1;
+    cfg.attrs = &a;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return 0;
+    }
+    capacity[dev] = n;
+  }
+  return capacity[dev];
+}
+
+// y = x W^T (+ bias) (+ parts B^T) on the CTA-pair kernel: W from codes (mx) or
+// from component planes.  x rows satisfy tma_rows; y 8-byte aligned, ld_y a
+// multiple of 4.
+template <typename T, int NTOK, bool MX>
+int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& planes, int64_t ld_w, const T* bias,
+                const T* parts, int64_t ld_parts, const T* lora_b, int rank, T* y, int64_t ld_y, int64_t M,
+                int64_t K_g, int64_t N_g, cudaStream_t s) {
+  using Cfg = MxPairStage<NTOK, MX>;
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  auto kernel = qlin_mx_pair_kernel<T, NTOK, MX>;
+  const int cap = pair_capacity<T, NTOK, MX>();
+  if (cap == 0) return QLIN_ERR_LAUNCH;
+  CUtensorMap map_x, map_t, map_w[4];
+  std::memset(&map_t, 0, sizeof(map_t));
+  std::memset(map_w, 0, sizeof(map_w));
+  int st = encode_2d(&map_x, bf16, x, 4 * K_g, M, ld_x, 64, Cfg::kHalf, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st == QLIN_OK && rank > 0)
+    st = encode_2d(&map_t, bf16, parts, 2 * ld_parts, M, 2 * ld_parts, 64, Cfg::kHalf, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!MX)
+    for (int p = 0; p < 4 && st == QLIN_OK; ++p)
+      st = encode_2d(&map_w[p], bf16, planes.w[p], K_g, N_g, ld_w, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+  if (st != QLIN_OK) return st;
+  MxPairParams prm{};
+  prm.mx = static_cast<const uint8_t*>(mx);
+  prm.bias = bias;
+  prm.lora_b = lora_b;
+  prm.y = y;
+  prm.ld_y = ld_y;
+  prm.M = (int)M;
+  prm.N_g = (int)N_g;
+  prm.K_g = (int)K_g;
+  prm.rank = rank;
+  prm.kb = (int)ceil_div(K_g, kMxBlock);
+  prm.w_tiles = (int)ceil_div(N_g, kMxRows);
+  prm.stages = (int)ceil_div(K_g, 32);
+  prm.lora_stages = (int)ceil_div(rank, 64);
+  prm.lo_col = (int)ld_parts;
+  prm.nb_tiles = (int)ceil_div(4 * N_g, 256);
+  const int64_t tiles = prm.nb_tiles * ceil_div(M, NTOK);
+  if (tiles * (prm.stages + prm.lora_stages) > INT32_MAX) return QLIN_ERR_SHAPE;
+  prm.tiles = (int)tiles;
+  prm.wide = aligned(y, 16) && ld_y % 8 == 0 && N_g % 2 == 0;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = 2;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, cap)), 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmemBytes;
+  cfg.stream = s;
+  cfg.attrs = attrs;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, map_x, map_t, map_w[0], map_w[1], map_w[2], map_w[3], prm) == cudaSuccess
+             ? QLIN_OK
+             : QLIN_ERR_LAUNCH;
+}
+
+// 256 tokens a tile above 128 tokens.
+template <typename T, bool MX, typename... Args>
+int run_pair(int64_t M, Args... args) {
+  return M > 128 ? launch_pair<T, 256, MX>(args...) : launch_pair<T, 128, MX>(args...);
+}
+
+// Rows that TMA takes: x itself, or a copy in the workspace.
+template <typename T>
+int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t cols, cudaStream_t s) {
+  if (tma_rows(*x, *ld)) return QLIN_OK;
+  const int64_t ld_c = round_up(cols, 8), blocks = ceil_div(rows * ld_c, 256);
+  if (blocks > INT32_MAX) return QLIN_ERR_SHAPE;
+  const int st = launch_dependent(qlin_mx_repack_kernel<T>, (unsigned)blocks, 256, 0, s, *x, *ld, static_cast<T*>(copy),
+                                  ld_c, rows, cols);
+  *x = static_cast<const T*>(copy);
+  *ld = ld_c;
+  return st;
+}
+
+template <typename T>
+MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t K, float scale, int rank, T* parts,
+                      int64_t ld_parts, T* turned, int rows, int ones, int64_t tokens) {
+  MxDownJob<T> j{};
+  j.x = x;
+  j.ld_x = ld_x;
+  j.a = a;
+  j.K = K;
+  j.scale = scale;
+  j.rank = rank;
+  j.parts = parts;
+  j.ld_parts = parts ? (int)ld_parts : 0;
+  j.turned = turned;
+  j.rows = turned ? rows : 0;
+  j.vec = K % 8 == 0 && aligned(a, 16);
+  j.ones = ones;
+  j.rank_tiles = (int)ceil_div(std::max(j.ld_parts, j.rows), kMxDownRanks);
+  j.blocks = (int)(ceil_div(tokens, kMxDownRows) * j.rank_tiles);
+  return j;
+}
+
+template <typename T>
+int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T* a, const T* b, int rank, float scale,
+                T* y, int64_t ld_y, int64_t M, int64_t K_g, int64_t N_g, uint8_t* ws, const ForwardWs& w,
+                cudaStream_t s) {
+  if (!aligned(y, 8) || ld_y % 4 != 0) return QLIN_ERR_ALIGN;
+  int st = rows_for_tma(&x, &ld_x, ws + w.x, M, 4 * K_g, s);
+  if (st != QLIN_OK) return st;
+  T* parts = reinterpret_cast<T*>(ws + w.t);
+  if (rank > 0) {
+    const MxDownJob<T> job = down_job<T>(x, ld_x, a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, 0, -1, M);
+    st = launch_dependent(qlin_mx_down_kernel<T>, job.blocks, 256, 0, s, job, MxDownJob<T>{}, (int)M, (int)M);
+    if (st != QLIN_OK) return st;
+  }
+  return run_pair<T, true>(M, x, ld_x, mx, MxPlanes<T>{}, (int64_t)0, bias, (const T*)parts, w.ld_parts, b, rank, y,
+                           ld_y, M, K_g, N_g, s);
+}
+
+// Gradients, 16 bits.
+template <typename T>
+int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void* mx, const T* a, const T* b, int rank,
+                 float scale, T* dx, int64_t ld_dx, T* da, T* db, T* dbias, int64_t M, int64_t K_g, int64_t N_g,
+                 uint8_t* ws, const BackwardWs& w, int sms, cudaStream_t s) {
+  const int64_t K = 4 * K_g, N = 4 * N_g;
+  if (dx && (!aligned(dx, 8) || ld_dx % 4 != 0)) return QLIN_ERR_ALIGN;
+  T* at = reinterpret_cast<T*>(ws + w.at);
+  T* bt = reinterpret_cast<T*>(ws + w.bt);
+  T* parts = reinterpret_cast<T*>(ws + w.parts);
+  T* up = reinterpret_cast<T*>(ws + w.up);
+  T* t = reinterpret_cast<T*>(ws + w.t);
+  int st = QLIN_OK;
+  if (dx || da || db) st = rows_for_tma(&g, &ld_g, ws + w.gy, M, N, s);
+  if (st == QLIN_OK && (da || db)) st = rows_for_tma(&x, &ld_x, ws + w.x, M, K, s);
+  if (st != QLIN_OK) return st;
+  const bool need_up = rank > 0 && (dx || da);
+  if (rank > 0 && (need_up || db)) {
+    if (need_up) {
+      const int64_t a_blocks = dx ? ceil_div(rank * K, 256) : 0, b_blocks = ceil_div(rank * N, 256);
+      st = launch_dependent(qlin_mx_turn_kernel<T>, (unsigned)(a_blocks + b_blocks), 256, 0, s, a, at, (int64_t)rank, K,
+                            b, bt, N, (int64_t)rank, a_blocks);
+      if (st != QLIN_OK) return st;
+    }
+    MxDownJob<T> j0{}, j1{};
+    if (need_up)
+      j0 = down_job<T>(g, ld_g, bt, N, scale, rank, dx ? parts : nullptr, w.ld_parts, da ? up : nullptr, w.rows0, -1,
+                       w.M_pad);
+    if (db)
+      j1 = down_job<T>(x, ld_x, a, K, scale, rank, nullptr, 0, t, w.rows1, dbias ? rank : -1, w.M_pad);
+    st = launch_dependent(qlin_mx_down_kernel<T>, (unsigned)(j0.blocks + j1.blocks), 256, 0, s, j0, j1, (int)M,
+                          (int)w.M_pad);
+    if (st != QLIN_OK) return st;
+  }
+  if (dx) {
+    MxPlanes<T> p;
+    for (int c = 0; c < 4; ++c) p.w[c] = reinterpret_cast<T*>(ws + w.planes) + c * K_g * w.ld_planes;
+    const int64_t steps = ceil_div(N_g, 64) * ceil_div(K_g, kMxBlock);
+    st = launch_dependent(qlin_mx_adjoint_kernel<T>, (unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s,
+                          static_cast<const uint8_t*>(mx), p, w.ld_planes, (int)K_g, (int)N_g);
+    if (st != QLIN_OK) return st;
+    st = run_pair<T, false>(M, g, ld_g, mx, p, w.ld_planes, (const T*)nullptr, (const T*)parts, w.ld_parts,
+                            (const T*)at, rank, dx, ld_dx, M, N_g, K_g, s);
+    if (st != QLIN_OK) return st;
+  }
+  const bool sum_with_db = db && dbias;
+  if (da || db) {
+    MxOuterJob<T> o0{}, o1{};
+    auto job = [&](MxOuterJob<T>& o, const T* turned, const T* X, int64_t ld, int64_t cols, int rows, int splits,
+                   size_t partial) {
+      o.turned = turned;
+      o.X = X;
+      o.ld = ld;
+      o.cols = (int)cols;
+      o.rows = rows;
+      o.col_tiles = (int)ceil_div(cols, kMxOuterCols);
+      o.row_tiles = (int)ceil_div(rows, kMxOuterRows);
+      o.splits = splits;
+      o.blocks = o.col_tiles * o.row_tiles * splits;
+      o.partial = reinterpret_cast<float*>(ws + partial);
+    };
+    if (da) job(o0, up, x, ld_x, K, w.rows0, w.splits0, w.partial0);
+    if (db) job(o1, t, g, ld_g, N, w.rows1, w.splits1, w.partial1);
+    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 128, 0, s, o0, o1, (int)M,
+                          (int)w.M_pad);
+    if (st != QLIN_OK) return st;
+    const int64_t blocks0 = da ? ceil_div(rank * K, 256) : 0;
+    const int64_t blocks1 = db ? ceil_div((rank + (sum_with_db ? 1 : 0)) * N, 256) : 0;
+    st = launch_dependent(qlin_mx_outer_finish_kernel<T>, (unsigned)(blocks0 + blocks1), 256, 0, s, o0, o1, rank, da,
+                          db, sum_with_db ? dbias : nullptr, blocks0);
+    if (st != QLIN_OK) return st;
+  }
+  if (dbias && !sum_with_db)
+    qlin_mx_column_sum_kernel<T><<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(g, ld_g, dbias, M, N);
+  return launched();
 }
 
 template <typename TP, typename TQ, typename TC>
@@ -406,11 +695,11 @@ int qlin_mx_forward(int dtype, const void* x, int64_t ld_x, const void* mx, cons
       return run_few<T>(dtype, static_cast<const T*>(x), ld_x, mx, static_cast<const T*>(bias),
                         static_cast<const T*>(lora_a), static_cast<const T*>(lora_b), rank, lora_scale,
                         static_cast<T*>(y), ld_y, M, K_g, N_g, ws, w, sms, static_cast<cudaStream_t>(stream));
-    const MxPlanes<T> p = planes_at<T>(ws + w.planes, K_g, N_g);
-    launch_dequantize<T>(mx, p, K_g, K_g, N_g, sms, static_cast<cudaStream_t>(stream));
-    if (launched() != QLIN_OK) return (int)QLIN_ERR_LAUNCH;
-    return qlin_forward_ex(dtype, x, ld_x, p.w[0], p.w[1], p.w[2], p.w[3], K_g, bias, lora_a, lora_b, rank,
-                           lora_scale, y, ld_y, M, K_g, N_g, ws + w.inner, w.inner_bytes, QLIN_ALGO_AUTO, 0, stream);
+    if constexpr (sizeof(T) == 2)
+      return run_prefill<T>(static_cast<const T*>(x), ld_x, mx, static_cast<const T*>(bias),
+                            static_cast<const T*>(lora_a), static_cast<const T*>(lora_b), rank, lora_scale,
+                            static_cast<T*>(y), ld_y, M, K_g, N_g, ws, w, static_cast<cudaStream_t>(stream));
+    return (int)QLIN_ERR_DTYPE;  // (fp32 always streams)
   });
 }
 
@@ -453,6 +742,11 @@ int qlin_mx_backward(int dtype, const void* gy, int64_t ld_g, const void* x, int
     const T* xt = static_cast<const T*>(x);
     const T* a = static_cast<const T*>(lora_a);
     const T* b = static_cast<const T*>(lora_b);
+    if constexpr (sizeof(T) == 2)
+      return run_backward<T>(g, ld_g, xt, ld_x, mx, a, b, rank, lora_scale, static_cast<T*>(dx), ld_dx,
+                             static_cast<T*>(da), static_cast<T*>(db), static_cast<T*>(dbias), M, K_g, N_g, ws, w, sms,
+                             s);
+    else {
     T* at = reinterpret_cast<T*>(ws + w.at);
     T* bt = reinterpret_cast<T*>(ws + w.bt);
     if (dx) {
@@ -461,8 +755,10 @@ int qlin_mx_backward(int dtype, const void* gy, int64_t ld_g, const void* x, int
       qlin_mx_adjoint_kernel<T><<<(unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s>>>(
           static_cast<const uint8_t*>(mx), p, N_g, (int)K_g, (int)N_g);
       if (rank > 0) {
-        qlin_mx_turn_kernel<T><<<(unsigned)ceil_div(rank * K, 256), 256, 0, s>>>(a, at, rank, K);
-        qlin_mx_turn_kernel<T><<<(unsigned)ceil_div(rank * N, 256), 256, 0, s>>>(b, bt, N, rank);
+        const int64_t a_blocks = ceil_div(rank * K, 256);
+        const int e = launch_dependent(qlin_mx_turn_kernel<T>, (unsigned)(a_blocks + ceil_div(rank * N, 256)), 256, 0,
+                                       s, a, at, (int64_t)rank, K, b, bt, N, (int64_t)rank, a_blocks);
+        if (e != QLIN_OK) return e;
       }
       if (launched() != QLIN_OK) return (int)QLIN_ERR_LAUNCH;
       const int e = qlin_forward_ex(dtype, gy, ld_g, p.w[0], p.w[1], p.w[2], p.w[3], N_g, nullptr, bt, at, rank,
@@ -483,6 +779,7 @@ int qlin_mx_backward(int dtype, const void* gy, int64_t ld_g, const void* x, int
     if (dbias)
       qlin_mx_column_sum_kernel<T><<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(g, ld_g, static_cast<T*>(dbias), M, N);
     return launched();
+    }
   });
 }
 

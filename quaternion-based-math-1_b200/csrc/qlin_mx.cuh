@@ -255,6 +255,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_adjoint_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g) {
   __shared__ T turn[4][kMxBlock][66];
+  pdl_wait_prior();
+  pdl_launch_dependents();
   const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
   const int64_t groups = (tiles + 3) / 4;
   const int t = threadIdx.x & 3, p = (threadIdx.x >> 2) & 3, row = threadIdx.x >> 4;

@@ -1,17 +1,25 @@
-// The adapter's products in the backward pass of a layer with 4-bit weights.
+// The adapter's products around a layer with 4-bit weights.
 //
-//     t  = s x A^T          [M, r]      t' = s gy B           [M, r]
-//     dA = t'^T x           [r, K]      dB = gy^T t           [N, r]
+//     t  = s x A^T          [M, r]      u  = s gy B           [M, r]
+//     dA = u^T x            [r, K]      dB = gy^T t           [N, r]
 //     dbias = sum_m gy[m]   [N]
 //
-// t and t' stay in fp32: rounded to 16 bits they would add an error of the
-// size of the gradients' own rounding.
+// t and u are kept as two 16-bit parts (or in fp32): rounded to one they would
+// add an error of the size of the gradients' own rounding.  x and gy are read
+// once for t and u and once for the gradients, which bounds these kernels; the
+// products are warp-level tensor-core ones (m16n8k16) whose k slots are numbered
+// so that a lane reads eight consecutive elements of a row in one 16-byte piece
+// for both operands.
 #pragma once
 
 #include "qlin_common.cuh"
+#include "qlin_mx_few.cuh"
 
 namespace qlin {
 
+// ---------------------------------------------------------------------------
+// fp32: plain products
+// ---------------------------------------------------------------------------
 // C[i, j] = alpha * sum_l P[i pi + l pl] * Q[j qj + l ql], fp32 sums; C is
 // row-major with leading dimension ld_c.  32 x 32 tile, 32 terms per step.
 template <typename TP, typename TQ, typename TC>
@@ -68,12 +76,274 @@ qlin_mx_column_sum_kernel(const T* __restrict__ g, int64_t ld_g, T* __restrict__
   }
 }
 
-// dst[c][r] = src[r][c]
+// dst[c][r] = src[r][c] for two matrices.
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_turn_kernel(const T* __restrict__ src, T* __restrict__ dst, int64_t rows, int64_t cols) {
+qlin_mx_turn_kernel(const T* __restrict__ a, T* __restrict__ at, int64_t a_rows, int64_t a_cols,
+                    const T* __restrict__ b, T* __restrict__ bt, int64_t b_rows, int64_t b_cols, int64_t a_blocks) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const bool first = (int64_t)blockIdx.x < a_blocks;
+  const int64_t k = ((int64_t)blockIdx.x - (first ? 0 : a_blocks)) * 256 + threadIdx.x;
+  const int64_t rows = first ? a_rows : b_rows, cols = first ? a_cols : b_cols;
+  // consecutive threads write consecutive elements
+  if (k < rows * cols) (first ? at : bt)[k] = (first ? a : b)[(k % rows) * cols + k / rows];
+}
+
+// dst rows of ld_d elements (ld_d >= cols), zero past cols: rows that no TMA map takes.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_repack_kernel(const T* __restrict__ src, int64_t ld_s, T* __restrict__ dst, int64_t ld_d, int64_t rows,
+                      int64_t cols) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
   const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (k < rows * cols) dst[(k % cols) * rows + k / cols] = src[k];
+  if (k >= rows * ld_d) return;
+  const int64_t r = k / ld_d, c = k - r * ld_d;
+  dst[k] = c < cols ? src[r * ld_s + c] : from_f32<T>(0.f);
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit down projections: t = scale x A^T
+// ---------------------------------------------------------------------------
+constexpr int kMxDownRows = 16;   // tokens of a CTA
+constexpr int kMxDownRanks = 32;  // ranks of a CTA
+
+template <typename T>
+struct MxDownJob {
+  const T* x;      // [M, ld_x], 16-byte aligned rows
+  int64_t ld_x;
+  const T* a;      // [rank, K]
+  int64_t K;
+  float scale;
+  T* parts;        // [M, 2 * ld_parts]: hi, then lo, zero from rank to ld_parts; or null
+  T* turned;       // [2][rows][M_pad]: hi, then lo, transposed; or null
+  int rank, ld_parts, rows, vec;  // vec: rows of A are 16-byte aligned
+  int ones;        // row of `turned` that holds ones (-1: none)
+  int rank_tiles;  // ceil(max(ld_parts, rows) / 32)
+  int blocks;
+};
+
+// Eight elements of a row of K, zero past its end.
+template <typename T>
+__device__ __forceinline__ uint4 mx_load_row8(const T* row, int64_t k, int64_t K, bool vec) {
+  if (vec && k + 8 <= K) return ld_cg_v4(row + k);
+  unsigned short h[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    h[j] = k + j < K ? *reinterpret_cast<const volatile unsigned short*>(row + k + j) : (unsigned short)0;
+  return make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                    h[6] | (uint32_t)h[7] << 16);
+}
+
+// A CTA: 16 tokens x 32 ranks, its eight warps every eighth piece of 32 terms.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_constant__ MxDownJob<T> job1, int M, int M_pad) {
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  __shared__ float red[8][kMxDownRows][kMxDownRanks + 1];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const bool first = (int)blockIdx.x < job0.blocks;
+  const MxDownJob<T>& job = first ? job0 : job1;
+  const int id = (int)blockIdx.x - (first ? 0 : job0.blocks);
+  const int m0 = id / job.rank_tiles * kMxDownRows, r0 = id % job.rank_tiles * kMxDownRanks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float acc[4][4] = {};
+  const T* xl = job.x + (int64_t)(m0 + g) * job.ld_x;
+  const T* xh = xl + 8 * job.ld_x;
+  const bool has_l = m0 + g < M, has_h = m0 + g + 8 < M;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  if (r0 < job.rank) {
+#pragma unroll 2
+    for (int64_t k0 = 32 * warp; k0 < job.K; k0 += 32 * 8) {
+      const int64_t k = k0 + 8 * t;
+      const uint4 lo = has_l ? mx_load_row8(xl, k, job.K, true) : zero;
+      const uint4 hi = has_h ? mx_load_row8(xh, k, job.K, true) : zero;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int r = r0 + 8 * n + g;
+        const uint4 b = r < job.rank ? mx_load_row8(job.a + (int64_t)r * job.K, k, job.K, job.vec) : zero;
+        mx_mma<HALF>(acc[n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+        mx_mma<HALF>(acc[n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) red[warp][g + 8 * (q >> 1)][8 * n + 2 * t + (q & 1)] = acc[n][q];
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    // hi and lo of (token, rank); ranks fastest for `parts`, tokens fastest for `turned`
+#pragma unroll
+    for (int way = 0; way < 2; ++way) {
+      if (way == 0 ? !job.parts : !job.turned) continue;
+      const int k = threadIdx.x + 256 * u;
+      const int m = way == 0 ? k >> 5 : k & 15, r = way == 0 ? k & 31 : k >> 4;
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) v += red[w][m][r];
+      v *= job.scale;
+      if (r0 + r == job.ones && m0 + m < M) v = 1.f;
+      const T hi = from_f32<T>(v);
+      const float rest = v - to_f32(hi);
+      const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
+      if (way == 0) {
+        if (m0 + m < M && r0 + r < job.ld_parts) {
+          T* at = job.parts + (int64_t)(m0 + m) * 2 * job.ld_parts + r0 + r;
+          at[0] = hi;
+          at[job.ld_parts] = lo;
+        }
+      } else if (r0 + r < job.rows) {
+        T* at = job.turned + (int64_t)(r0 + r) * M_pad + m0 + m;
+        at[0] = hi;
+        at[(int64_t)job.rows * M_pad] = lo;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit gradients: out = (hi + lo) X, sums over the tokens
+// ---------------------------------------------------------------------------
+constexpr int kMxOuterCols = 64;    // columns of X of a CTA
+constexpr int kMxOuterTokens = 32;  // tokens of a step
+constexpr int kMxOuterRows = 64;    // rows of the result of a CTA (groups of 16)
+constexpr int kMxOuterStages = 4;
+
+template <typename T>
+struct MxOuterJob {
+  const T* turned;  // [2][rows][M_pad]
+  const T* X;       // [M, ld], 16-byte aligned rows
+  int64_t ld;
+  int cols, rows;   // rows: a multiple of 16
+  int col_tiles, row_tiles, splits;
+  int blocks;
+  float* partial;   // [splits][rows][cols]
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Four warps: 16 columns each, all rows.  X comes through a ring of shared
+// memory steps (32 tokens x 64 columns, 16-byte chunks permuted within a row so
+// that the transposing loads of eight tokens two apart are free of conflicts).
+template <typename T>
+__global__ void __launch_bounds__(128)
+qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int M, int M_pad) {
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  __shared__ __align__(128) uint8_t ring[kMxOuterStages][kMxOuterTokens * kMxOuterCols * 2];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const bool first = (int)blockIdx.x < job0.blocks;
+  const MxOuterJob<T>& job = first ? job0 : job1;
+  int id = (int)blockIdx.x - (first ? 0 : job0.blocks);
+  const int ct = id % job.col_tiles;
+  id /= job.col_tiles;
+  const int rt = id % job.row_tiles, split = id / job.row_tiles;
+  const int steps = M_pad / kMxOuterTokens;
+  const int s0 = (int)((int64_t)steps * split / job.splits), s1 = (int)((int64_t)steps * (split + 1) / job.splits);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int c0 = ct * kMxOuterCols, row0 = rt * kMxOuterRows;
+  const int groups = min(kMxOuterRows, job.rows - row0) / 16;
+
+  auto fetch = [&](int step) {
+    if (step < s1) {
+      const uint32_t base = smem_u32(ring[step % kMxOuterStages]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k = threadIdx.x + 128 * u, tok = k >> 3, chunk = k & 7;
+        const int m = step * kMxOuterTokens + tok, c = c0 + 8 * chunk;
+        const int left = m < M ? min(8, job.cols - c) : 0;  // elements of the chunk inside
+        const int f = (tok & 1) | ((tok >> 3) & 3) << 1;
+        cp_async16(base + tok * 128 + ((chunk ^ f) << 4), left > 0 ? job.X + (int64_t)m * job.ld + c : job.X,
+                   left > 0 ? 2 * left : 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int k = 0; k < kMxOuterStages - 1; ++k) fetch(s0 + k);
+
+  float acc[4][2][4] = {};  // [row group][8 columns][fragment]
+  const T* hi_rows = job.turned + (int64_t)(row0 + g) * M_pad;
+  const int64_t lo_off = (int64_t)job.rows * M_pad;
+  // this lane's row of the transposing loads: matrix lane / 8 (pair j), row lane % 8
+  const int mtok = 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
+  const int mf = (mtok & 1) | ((mtok >> 3) & 3) << 1;
+  for (int step = s0; step < s1; ++step) {
+    uint4 a[4][2][2];  // [row group][part][row g, g + 8]
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < groups)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            a[r][part][h] = ld_cg_v4(hi_rows + part * lo_off + (int64_t)(16 * r + 8 * h) * M_pad +
+                                     step * kMxOuterTokens + 8 * t);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kMxOuterStages - 2) : "memory");
+    __syncthreads();
+    fetch(step + kMxOuterStages - 1);  // the stage of step - 1: every warp is past it
+    const uint32_t base = smem_u32(ring[step % kMxOuterStages]) + mtok * 128;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      uint32_t b[4];
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
+                   : "r"(base + (((2 * warp + n) ^ mf) << 4))
+                   : "memory");
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < groups)
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const uint4 l = a[r][part][0], h = a[r][part][1];
+            mx_mma<HALF>(acc[r][n], l.x, h.x, l.y, h.y, b[0], b[1]);
+            mx_mma<HALF>(acc[r][n], l.z, h.z, l.w, h.w, b[2], b[3]);
+          }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r < groups)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = row0 + 16 * r + g + 8 * (q >> 1), c = c0 + 16 * warp + 8 * n + 2 * t + (q & 1);
+          if (c < job.cols) job.partial[((int64_t)split * job.rows + row) * job.cols + c] = acc[r][n][q];
+        }
+}
+
+// Adds the splits up: da [rank, cols] from job0's; db [cols, rank] and dbias
+// [cols] (row `rank`) from job1's.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_outer_finish_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int rank, T* __restrict__ da,
+                            T* __restrict__ db, T* __restrict__ dbias, int64_t blocks0) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const bool first = (int64_t)blockIdx.x < blocks0;
+  const MxOuterJob<T>& job = first ? job0 : job1;
+  const int64_t k = ((int64_t)blockIdx.x - (first ? 0 : blocks0)) * 256 + threadIdx.x;
+  const int rows = first ? rank : rank + (dbias ? 1 : 0);
+  if (k >= (int64_t)rows * job.cols) return;
+  // consecutive threads: consecutive columns of a row
+  const int64_t r = k / job.cols, c = k - r * job.cols;
+  float v = 0.f;
+  for (int s = 0; s < job.splits; ++s)
+    v += __ldcg(job.partial + ((int64_t)s * job.rows + r) * job.cols + c);
+  if (first) da[k] = from_f32<T>(v);
+  else if (r < rank) {
+    if (db) db[c * rank + r] = from_f32<T>(v);
+  } else {
+    dbias[c] = from_f32<T>(v);
+  }
 }
 
 }  // namespace qlin

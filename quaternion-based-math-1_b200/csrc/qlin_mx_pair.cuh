@@ -1,0 +1,443 @@
+// Many tokens through a layer with 4-bit weights, and the input gradient: the
+// persistent CTA-pair kernel of qlin_pair.cuh (2-SM tcgen05 UMMA, the weight
+// operand expanded into tensor memory, x straight from TMA) with two changes.
+//
+// Weights from codes (MX): a stage's 32 output x 32 input quaternions come as two
+// records of 1088 bytes by bulk copy.  A builder lane (output quaternion o,
+// component a) reads all four components of eight input quaternions in one
+// 16-byte piece, expands them (mx_expand), multiplies by scale and sign of
+// s(a, a^q) in one packed multiplication and pairs the components up: the
+// expansion costs the integer pipe about 450 cycles of the 1024 that the eight
+// UMMAs of a stage take at 256 tokens, and a quarter of a 16-bit layer's bytes.
+// Without MX the weights are 16-bit component planes (the adjoint of the codes).
+//
+// Adapter: y += t B^T with t = s x A^T as two 16-bit parts (t = hi + lo to about
+// twice the type's precision): ceil(r / 64) more stages whose x tile is 64
+// ranks of hi and of lo and whose weight rows are the same 64 ranks of B twice.
+//
+// The accumulator holds y 2^-c (mx_shift); B is built with the same factor, and
+// the epilogue multiplies by 2^c before the bias and the one rounding.  fp16
+// bounds c from below with an adapter, so that B 2^-c stays in range for |B| up
+// to 1000.
+#pragma once
+
+#include "qlin_mx.cuh"
+#include "qlin_mx_few.cuh"
+#include "qlin_pair.cuh"
+
+namespace qlin {
+
+template <int NTOK, bool MX>
+struct MxPairStage {
+  static constexpr int kHalf = NTOK / 2;
+  static constexpr int kXAtomBytes = kHalf * 128;
+  static constexpr int kXBytes = 2 * kXAtomBytes;
+  static constexpr int kWBytes = MX ? 3072 : 4 * kPairWTileBytes;  // (two records, rounded up to whole KB)
+  static constexpr int kStageBytes = kXBytes + kWBytes;
+  static constexpr int kStages = NTOK == 256 ? (MX ? 5 : 4) : 8;
+  static constexpr int kDBufs = NTOK == 256 ? 1 : 2;
+  static constexpr int kAColBase = kDBufs * NTOK;
+  static constexpr int kEpiOffset = kStages * kStageBytes;
+  static constexpr int kBarOffset = kEpiOffset + 2 * kPairEpiBufBytes;
+  static_assert(kBarOffset + 512 + 1024 <= kPairSmemBytes, "shared memory");
+  static_assert(kStageBytes % 1024 == 0, "swizzled x tiles start on 1 KB");
+  static_assert(2 * kMxRecord <= 3072, "two records");
+  static_assert(kAColBase + kPairAStages * kPairACols <= 512, "tensor memory");
+};
+
+struct MxPairParams {
+  const uint8_t* mx;    // codes (MX)
+  const void* bias;
+  const void* lora_b;   // [4 N_g, rank] or null
+  void* y;
+  int64_t ld_y;
+  int M, N_g, K_g, rank;
+  int kb, w_tiles;      // blocks of a row; 16-row tiles of the codes
+  int stages;           // weight stages of a tile
+  int lora_stages;      // ceil(rank / 64)
+  int lo_col;           // column of t's low parts
+  int nb_tiles, tiles;
+  int wide;             // 16-byte output pieces are aligned
+};
+
+template <typename T, int NTOK, bool MX>
+__global__ void __launch_bounds__(kPairThreads, 1)
+qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_t,
+                    const __grid_constant__ CUtensorMap map_wr, const __grid_constant__ CUtensorMap map_wi,
+                    const __grid_constant__ CUtensorMap map_wj, const __grid_constant__ CUtensorMap map_wk,
+                    const MxPairParams prm) {
+  using Cfg = MxPairStage<NTOK, MX>;
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  constexpr uint32_t kIdesc = make_idesc_f16(256, NTOK, HALF ? 0u : 1u, false);
+  constexpr int S = Cfg::kStages, SA = kPairAStages, NB = Cfg::kDBufs;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);  // [S] x and W of this CTA landed
+  uint64_t* empty = full + S;     // [S] the UMMAs of the stage completed (both CTAs)
+  uint64_t* afull = empty + S;    // [SA] even CTA: both CTAs' builders wrote the A stage
+  uint64_t* aempty = afull + SA;  // [SA] the UMMAs reading the A stage completed (both CTAs)
+  uint64_t* dfull = aempty + SA;  // [NB]
+  uint64_t* dempty = dfull + NB;  // [NB], even CTA: both CTAs' epilogues drained the accumulator
+  uint64_t* drain = dempty + NB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* issued = const_cast<int*>(abort_flag) + 1;  // producer: ring stages issued
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();     // 0: issues the UMMAs
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int my_tiles = pair < prm.tiles ? (prm.tiles - 1 - pair) / pairs + 1 : 0;
+  const int nk = prm.stages + prm.lora_stages;
+  const int total = my_tiles * nk;  // ring items of this pair
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < SA; ++s) {
+      mbar_init(&afull[s], 8);
+      mbar_init(&aempty[s], 1);
+    }
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(&dfull[b], 1);
+      mbar_init(&dempty[b], 8);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *issued = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_x);
+    if (prm.lora_stages) tma_prefetch_desc(&map_t);
+    if constexpr (!MX) {
+      tma_prefetch_desc(&map_wr);
+      tma_prefetch_desc(&map_wi);
+      tma_prefetch_desc(&map_wj);
+      tma_prefetch_desc(&map_wk);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers initialised, tensor memory allocated
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // Everything below reads what earlier kernels of the stream wrote, or writes
+  // what they may read.
+  pdl_wait_prior();
+
+  auto tile_coords = [&](int t, int& n0, int& m0) {
+    const int nb = t % prm.nb_tiles, tb = t / prm.nb_tiles;
+    n0 = nb * 256 + (int)cta * kPairRows;  // this CTA's first real output
+    m0 = tb * NTOK;                        // the pair's first token
+  };
+  int c = 0;  // the accumulator holds y 2^-c
+  if constexpr (MX) {
+    uint32_t f0;
+    asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(prm.mx) : "memory");
+    c = mx_shift<HALF>(f0);
+    if (HALF && prm.rank > 0) c = max(c, -6);
+  }
+
+  if (warp == 0) {
+    // ---------------- copies of this CTA's x half-tile and weights ----------------
+    if (lane == 0) {
+      const CUtensorMap* wmap[4] = {&map_wr, &map_wi, &map_wj, &map_wk};
+      int g = 0;
+      for (int j = 0; j < my_tiles && !*abort_flag; ++j) {
+        int n0, m0;
+        tile_coords(pair + j * pairs, n0, m0);
+        const int mrow = m0 + (int)cta * Cfg::kHalf;
+        const int tile0 = n0 / (4 * kMxRows), have = max(0, min(2, prm.w_tiles - tile0));
+        for (int k = 0; k < nk; ++k, ++g) {
+          const int s = g % S, n = g / S;
+          if (n > 0 && !mbar_wait(&empty[s], (n - 1) & 1)) {
+            *abort_flag = 1;
+            break;
+          }
+          uint8_t* dst = smem + s * Cfg::kStageBytes;
+          if (k >= prm.stages) {
+            const int r = 64 * (k - prm.stages);
+            mbar_arrive_expect_tx(&full[s], Cfg::kXBytes);
+            tma_load_2d(dst, &map_t, &full[s], r, mrow);
+            tma_load_2d(dst + Cfg::kXAtomBytes, &map_t, &full[s], prm.lo_col + r, mrow);
+          } else {
+            mbar_arrive_expect_tx(&full[s], Cfg::kXBytes + (MX ? have * kMxRecord : 4 * kPairWTileBytes));
+            tma_load_2d(dst, &map_x, &full[s], k * kPairStageK, mrow);
+            tma_load_2d(dst + Cfg::kXAtomBytes, &map_x, &full[s], k * kPairStageK + 64, mrow);
+            if constexpr (MX) {
+              for (int h = 0; h < have; ++h)
+                bulk_load(dst + Cfg::kXBytes + h * kMxRecord,
+                          prm.mx + kMxHeader + ((int64_t)(tile0 + h) * prm.kb + k) * kMxRecord, kMxRecord, &full[s]);
+            } else {
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                tma_load_2d(dst + Cfg::kXBytes + p * kPairWTileBytes, wmap[p], &full[s], k * (kPairStageK / 4),
+                            n0 / 4);
+            }
+          }
+          *issued = g + 1;
+        }
+        if (*abort_flag) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && cta == 0) {
+      // ---------------- UMMA issuer (even CTA) ----------------
+      bool ok = true;
+      int g = 0;
+      for (int j = 0; j < my_tiles && ok; ++j) {
+        const int b = j % NB, u = j / NB;
+        if (u > 0 && !mbar_wait(&dempty[b], (u - 1) & 1)) ok = false;
+        tc_fence_after();
+        for (int k = 0; k < nk && ok; ++k, ++g) {
+          const int s = g % S, sa = g % SA, na = g / SA;
+          // both CTAs' builders arrive only after their own CTA's x and W of
+          // this stage landed: this one wait covers the B operand too
+          if (!mbar_wait(&afull[sa], na & 1) || *abort_flag) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t bdesc0 = smem_desc_sw128(smem + s * Cfg::kStageBytes);
+#pragma unroll
+          for (int kk = 0; kk < kPairStageK / 16; ++kk) {
+            const uint64_t bdesc = bdesc0 + (uint64_t)((kk >> 2) * (Cfg::kXAtomBytes >> 4)) + 2 * (kk & 3);
+            umma_pair_ts(tmem + b * NTOK, tmem + Cfg::kAColBase + sa * kPairACols + 8 * kk, bdesc, kIdesc,
+                         (k > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit_pair(&empty[s], 0x3);
+          umma_commit_pair(&aempty[sa], 0x3);
+        }
+        if (ok) umma_commit_pair(&dfull[b], 0x3);
+      }
+      if (!ok) *abort_flag = 1;
+      // every UMMA issued above has completed before the teardown
+      umma_commit_pair(drain, 0x1);
+      mbar_wait(drain, 0, 50000000ull);
+    }
+  } else if (warp < 6) {
+    // ---------------- builders: expanded weight rows into tensor memory ----------------
+    // Lane l of builder warp w writes tensor-memory lane 32 q + l (q = w % 4):
+    // output quaternion n0/4 + 8 q + l % 8, component a = l / 8.
+    const int quarter = warp & 3;
+    const int a = lane >> 3;
+    const int row = 8 * quarter + (lane & 7);  // of the CTA's 32 output quaternions
+    uint32_t sign[4];                          // of s(a, a^q), on both halves
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sign[q] = (mx_negative(a) >> (a ^ q) & 1) ? 0x80008000u : 0u;
+    const uint32_t tm_lane = (uint32_t)(32 * quarter) << 16;
+    const MxPowers pw;
+    const float down = scalbnf(1.f, -c);
+    int k = 0, j = 0;
+    for (int g = 0; g < total; ++g) {
+      const int s = g % S, n = g / S, sa = g % SA, na = g / SA;
+      bool ok = !*abort_flag && mbar_wait(&full[s], n & 1);
+      if (ok && na > 0) ok = mbar_wait(&aempty[sa], (na - 1) & 1);
+      if (!ok) *abort_flag = 1;
+      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + sa * kPairACols;
+      if (!*abort_flag && k >= prm.stages) {
+        // 64 ranks of this row of B, twice
+        int n0, m0;
+        tile_coords(pair + j * pairs, n0, m0);
+        const int64_t n_out = n0 + 4 * row + a;
+        const int r0 = 64 * (k - prm.stages);
+        const T* b = reinterpret_cast<const T*>(prm.lora_b) + n_out * prm.rank + r0;
+        const int left = n_out < 4 * (int64_t)prm.N_g ? min(64, prm.rank - r0) : 0;
+        const bool vec = prm.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(prm.lora_b) & 15) == 0;
+        uint32_t r[32];
+        const uint32_t mult = pack2<T>(down, down);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (vec) {
+            if (8 * e < left) v = ld_cg_v4(b + 8 * e);
+          } else {
+            unsigned short h[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              h[u] = 8 * e + u < left ? *reinterpret_cast<const volatile unsigned short*>(b + 8 * e + u) : (unsigned short)0;
+            v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                           h[6] | (uint32_t)h[7] << 16);
+          }
+          r[4 * e + 0] = c ? mx_mul2<HALF>(v.x, mult) : v.x;
+          r[4 * e + 1] = c ? mx_mul2<HALF>(v.y, mult) : v.y;
+          r[4 * e + 2] = c ? mx_mul2<HALF>(v.z, mult) : v.z;
+          r[4 * e + 3] = c ? mx_mul2<HALF>(v.w, mult) : v.w;
+        }
+        __syncwarp();
+        tmem_st32(col, r);
+        tmem_st32(col + 32, r);
+        tmem_st_wait();
+      } else if (!*abort_flag && MX) {
+        const uint32_t rec = smem_u32(smem + s * Cfg::kStageBytes + Cfg::kXBytes) + (quarter >> 1) * kMxRecord;
+        const int r16 = row & 15;
+        const uint32_t scales = lds32(rec + kMxCodeBytes + r16 * 4);
+        uint32_t mult[4];  // of component a^q, with its sign
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mult[q] = mx_multiplier<HALF>((scales >> (8 * (a ^ q))) & 255u, c) ^ sign[q];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {  // octet 2h + o: columns 16 of 32
+            const uint4 w4 = lds128(rec + r16 * 64 + (2 * h + o) * 16);
+            uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            if (a & 1) {
+              uint32_t x = w[0]; w[0] = w[1]; w[1] = x;
+              x = w[2]; w[2] = w[3]; w[3] = x;
+            }
+            if (a & 2) {
+              uint32_t x = w[0]; w[0] = w[2]; w[2] = x;
+              x = w[1]; w[1] = w[3]; w[3] = x;
+            }
+            uint32_t e[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mx_expand_scaled<HALF>(pw, w[q], mult[q], e[q]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              r[16 * o + 2 * i] = __byte_perm(e[0][i], e[1][i], 0x5410);
+              r[16 * o + 2 * i + 1] = __byte_perm(e[2][i], e[3][i], 0x5410);
+              r[16 * o + 8 + 2 * i] = __byte_perm(e[0][i], e[1][i], 0x7632);
+              r[16 * o + 8 + 2 * i + 1] = __byte_perm(e[2][i], e[3][i], 0x7632);
+            }
+          }
+          __syncwarp();
+          tmem_st32(col + 32 * h, r);
+        }
+        tmem_st_wait();
+      } else if (!*abort_flag) {
+        // W_a[o, 32 inputs]: 64 bytes, chunk u at chunk u ^ ((row >> 1) & 3) (64-byte swizzle);
+        // W_{a^q'} from lanes l ^ 8 q' (same o)
+        const uint32_t wrow =
+            smem_u32(smem + s * Cfg::kStageBytes + Cfg::kXBytes + a * kPairWTileBytes + row * 64);
+        uint32_t w0[16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint4 v = lds128(wrow + ((u ^ ((row >> 1) & 3)) << 4));
+          w0[4 * u] = v.x; w0[4 * u + 1] = v.y; w0[4 * u + 2] = v.z; w0[4 * u + 3] = v.w;
+        }
+        const uint32_t sg01 = (sign[0] & 0x8000u) | (sign[1] & 0x80000000u);
+        const uint32_t sg23 = (sign[2] & 0x8000u) | (sign[3] & 0x80000000u);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+#pragma unroll
+          for (int e8 = 0; e8 < 8; ++e8) {
+            const uint32_t v0 = w0[8 * h + e8];
+            const uint32_t v1 = __shfl_xor_sync(0xffffffffu, v0, 8);
+            const uint32_t v2 = __shfl_xor_sync(0xffffffffu, v0, 16);
+            const uint32_t v3 = __shfl_xor_sync(0xffffffffu, v0, 24);
+            r[4 * e8 + 0] = __byte_perm(v0, v1, 0x5410) ^ sg01;
+            r[4 * e8 + 1] = __byte_perm(v2, v3, 0x5410) ^ sg23;
+            r[4 * e8 + 2] = __byte_perm(v0, v1, 0x7632) ^ sg01;
+            r[4 * e8 + 3] = __byte_perm(v2, v3, 0x7632) ^ sg23;
+          }
+          tmem_st32(col + 32 * h, r);
+        }
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cta(&afull[sa], 0);
+      if (++k == nk) {
+        k = 0;
+        ++j;
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    // Drain the accumulator into registers (scaled, bias added, rounded, two
+    // tokens per word), release it to the UMMA issuer, then store through a
+    // shared-memory transpose.
+    const int quarter = warp & 3;
+    const int et = threadIdx.x - 192;  // 0..127
+    const int n_local = 32 * quarter + 4 * (lane & 7) + (lane >> 3);
+    const float factor = scalbnf(1.f, c);
+    T* __restrict__ y = reinterpret_cast<T*>(prm.y);
+    const T* __restrict__ bias = reinterpret_cast<const T*>(prm.bias);
+    for (int j = 0; j < my_tiles; ++j) {
+      const int b = j % NB, u = j / NB;
+      int n0, m0;
+      tile_coords(pair + j * pairs, n0, m0);
+      const bool got = !*abort_flag && mbar_wait(&dfull[b], u & 1);
+      if (!got) *abort_flag = 1;
+      tc_fence_after();
+      const int n = n0 + n_local;
+      const float bv = (bias && n < 4 * prm.N_g) ? to_f32(bias[n]) : 0.f;
+      uint32_t packed[NTOK / 2];
+#pragma unroll
+      for (int q = 0; q < NTOK / 32; ++q) {
+        uint32_t v[32];
+        if (got) {
+          __syncwarp();
+          tmem_ld32(tmem + ((uint32_t)(32 * quarter) << 16) + b * NTOK + 32 * q, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int t = 0; t < 32; ++t) v[t] = 0u;
+        }
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+          packed[16 * q + t] = pack2<T>(fmaf(__uint_as_float(v[2 * t]), factor, bv),
+                                        fmaf(__uint_as_float(v[2 * t + 1]), factor, bv));
+      }
+      // this warp has read its lanes of the accumulator: the even CTA may reuse it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cta(&dempty[b], 0);
+#pragma unroll
+      for (int grp = 0; grp < NTOK / kPairEpiTokens; ++grp) {
+        T* stage = reinterpret_cast<T*>(smem + Cfg::kEpiOffset + (grp & 1) * kPairEpiBufBytes);
+        unsigned short* st16 = reinterpret_cast<unsigned short*>(stage);
+#pragma unroll
+        for (int t2 = 0; t2 < kPairEpiTokens / 2; ++t2) {
+          const uint32_t wv = packed[(kPairEpiTokens / 2) * grp + t2];
+          st16[(2 * t2) * kPairRows + n_local] = (unsigned short)(wv & 0xffffu);
+          st16[(2 * t2 + 1) * kPairRows + n_local] = (unsigned short)(wv >> 16);
+        }
+        asm volatile("bar.sync %0, %1;" ::"n"(kPairEpiBar), "n"(128) : "memory");
+        if (got) {
+          // 16 tokens x 128 outputs = 256 pieces of 16 bytes, two per thread
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = et + 128 * h, t = at >> 4, cc = at & 15;
+            const int m = m0 + kPairEpiTokens * grp + t, nn = n0 + 8 * cc;
+            if (m < prm.M && nn < 4 * prm.N_g) {
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + t * kPairRows + 8 * cc);
+              T* out = y + (int64_t)m * prm.ld_y + nn;
+              if (prm.wide) {
+                *reinterpret_cast<uint4*>(out) = v;
+              } else {  // an odd number of output quaternions: 8-byte pieces
+                *reinterpret_cast<uint2*>(out) = make_uint2(v.x, v.y);
+                if (nn + 4 < 4 * prm.N_g) *reinterpret_cast<uint2*>(out + 4) = make_uint2(v.z, v.w);
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---------------- teardown ----------------
+  __syncwarp();
+  if (threadIdx.x == 0 && *abort_flag) {
+    // let issued copies land before the shared memory goes away
+    const int g1 = *issued;
+    for (int g = g1 - S > 0 ? g1 - S : 0; g < g1; ++g) mbar_wait(&full[g % S], (g / S) & 1, 50000000ull);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while the other may still use its memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+}  // namespace qlin
