@@ -89,7 +89,7 @@ bool tma_rows(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0;
 
 struct ForwardWs {
   size_t arranged = 0, t = 0, x = 0, total = 0;
-  int64_t ld_parts = 0;  // columns of t's high (and low) parts
+  int64_t ld_parts = 0;  // ranks of t's rows, in whole 16-byte pieces
 };
 
 // Sized for the worst alignment of x: the pieces do not depend on pointers.
@@ -103,7 +103,7 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
     }
     w.t = c.take(M * rank * 4);
   } else {
-    w.ld_parts = round_up(rank, 64);
+    w.ld_parts = round_up(rank, 8);
     w.x = c.take(M * round_up(4 * K_g, 8) * 2);
     w.t = c.take(M * 2 * w.ld_parts * 2);
   }
@@ -113,19 +113,19 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
 
 struct BackwardWs {
   // 16-bit
-  size_t gy = 0, x = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0;
+  size_t gy = 0, x = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0, sums = 0;
   int64_t M_pad = 0, ld_parts = 0, ld_planes = 0;
-  int rows0 = 0, rows1 = 0, splits0 = 0, splits1 = 0;
+  int rows = 0, splits0 = 0, splits1 = 0;
   // fp32
   size_t inner = 0, inner_bytes = 0;
   size_t total = 0;
 };
 
-// Splits of the tokens of a gradient product: about four CTAs per SM, at least
-// four steps of 32 tokens each.
+// Splits of the tokens of a gradient product: about one CTA per SM for each of the
+// two, at least four steps of 32 tokens each.
 int outer_splits(int64_t M_pad, int64_t cols, int rows) {
   const int64_t tiles = ceil_div(cols, kMxOuterCols) * ceil_div(rows, kMxOuterRows);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 600 / std::max<int64_t>(1, tiles)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 148 / std::max<int64_t>(1, tiles)));
 }
 
 BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
@@ -142,12 +142,11 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
   } else {
     const int64_t K = 4 * K_g, N = 4 * N_g;
     w.M_pad = round_up(M, kMxOuterTokens);
-    w.ld_parts = round_up(rank, 64);
+    w.ld_parts = round_up(rank, 8);
     w.ld_planes = round_up(N_g, 8);
-    w.rows0 = (int)round_up(rank, 16);
-    w.rows1 = (int)round_up(rank + 1, 16);
-    w.splits0 = outer_splits(w.M_pad, K, w.rows0);
-    w.splits1 = outer_splits(w.M_pad, N, w.rows1);
+    w.rows = (int)round_up(rank, 16);
+    w.splits0 = outer_splits(w.M_pad, K, w.rows);
+    w.splits1 = outer_splits(w.M_pad, N, w.rows);
     w.gy = c.take(M * round_up(N, 8) * 2);
     w.x = c.take(rank > 0 ? M * round_up(K, 8) * 2 : 0);
     w.planes = c.take(4 * K_g * w.ld_planes * 2);
@@ -155,10 +154,11 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
       w.at = c.take(K * rank * 2);
       w.bt = c.take(N * rank * 2);
       w.parts = c.take(M * 2 * w.ld_parts * 2);
-      w.up = c.take(2 * w.rows0 * w.M_pad * 2);
-      w.t = c.take(2 * w.rows1 * w.M_pad * 2);
-      w.partial0 = c.take((int64_t)w.splits0 * w.rows0 * K * 4);
-      w.partial1 = c.take((int64_t)w.splits1 * w.rows1 * N * 4);
+      w.up = c.take(2 * w.rows * w.M_pad * 2);
+      w.t = c.take(2 * w.rows * w.M_pad * 2);
+      w.partial0 = c.take((int64_t)w.splits0 * w.rows * K * 4);
+      w.partial1 = c.take((int64_t)w.splits1 * w.rows * N * 4);
+      w.sums = c.take((int64_t)w.splits1 * N * 4);
     }
   }
   w.total = c.at;
@@ -309,15 +309,16 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
 // ---------------------------------------------------------------------------
 // many tokens, 16 bits
 // ---------------------------------------------------------------------------
-int encode_2d(CUtensorMap* map, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld, uint32_t box_cols,
-              uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+// A TMA map of `dims` (innermost first; `strides` in elements from the second on).
+int encode_map(CUtensorMap* map, bool bf16, const void* base, int rank, const int64_t (&dims)[3],
+               const int64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
   const auto encode = qlin_host_encoder();
   if (!encode) return QLIN_ERR_LAUNCH;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
-  const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
-  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+  const cuuint64_t d[3] = {(cuuint64_t)dims[0], (cuuint64_t)dims[1], (cuuint64_t)dims[2]};
+  const cuuint64_t st[2] = {(cuuint64_t)(strides[0] * 2), (cuuint64_t)(strides[1] * 2)};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+                const_cast<void*>(base), d, st, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? QLIN_OK
              : QLIN_ERR_ALIGN;
@@ -371,12 +372,13 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
   CUtensorMap map_x, map_t, map_w[4];
   std::memset(&map_t, 0, sizeof(map_t));
   std::memset(map_w, 0, sizeof(map_w));
-  int st = encode_2d(&map_x, bf16, x, 4 * K_g, M, ld_x, 64, Cfg::kHalf, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (st == QLIN_OK && rank > 0)
-    st = encode_2d(&map_t, bf16, parts, 2 * ld_parts, M, 2 * ld_parts, 64, Cfg::kHalf, CU_TENSOR_MAP_SWIZZLE_128B);
+  int st = encode_map(&map_x, bf16, x, 2, {4 * K_g, M, 1}, {ld_x, 0}, {64, Cfg::kHalf, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st == QLIN_OK && rank > 0)  // [part][token][rank]: ranks past ld_parts read as zero
+    st = encode_map(&map_t, bf16, parts, 3, {ld_parts, M, 2}, {2 * ld_parts, ld_parts}, {64, Cfg::kHalf, 1},
+                    CU_TENSOR_MAP_SWIZZLE_128B);
   if (!MX)
     for (int p = 0; p < 4 && st == QLIN_OK; ++p)
-      st = encode_2d(&map_w[p], bf16, planes.w[p], K_g, N_g, ld_w, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+      st = encode_map(&map_w[p], bf16, planes.w[p], 2, {K_g, N_g, 1}, {ld_w, 0}, {32, 32, 1}, CU_TENSOR_MAP_SWIZZLE_64B);
   if (st != QLIN_OK) return st;
   MxPairParams prm{};
   prm.mx = static_cast<const uint8_t*>(mx);
@@ -392,7 +394,6 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
   prm.w_tiles = (int)ceil_div(N_g, kMxRows);
   prm.stages = (int)ceil_div(K_g, 32);
   prm.lora_stages = (int)ceil_div(rank, 64);
-  prm.lo_col = (int)ld_parts;
   prm.nb_tiles = (int)ceil_div(4 * N_g, 256);
   const int64_t tiles = prm.nb_tiles * ceil_div(M, NTOK);
   if (tiles * (prm.stages + prm.lora_stages) > INT32_MAX) return QLIN_ERR_SHAPE;
@@ -438,7 +439,7 @@ int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t col
 
 template <typename T>
 MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t K, float scale, int rank, T* parts,
-                      int64_t ld_parts, T* turned, int rows, int ones, int64_t tokens) {
+                      int64_t ld_parts, T* turned, int rows, int64_t tokens) {
   MxDownJob<T> j{};
   j.x = x;
   j.ld_x = ld_x;
@@ -451,7 +452,6 @@ MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t K, float sca
   j.turned = turned;
   j.rows = turned ? rows : 0;
   j.vec = K % 8 == 0 && aligned(a, 16);
-  j.ones = ones;
   j.rank_tiles = (int)ceil_div(std::max(j.ld_parts, j.rows), kMxDownRanks);
   j.blocks = (int)(ceil_div(tokens, kMxDownRows) * j.rank_tiles);
   return j;
@@ -466,7 +466,7 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
   if (st != QLIN_OK) return st;
   T* parts = reinterpret_cast<T*>(ws + w.t);
   if (rank > 0) {
-    const MxDownJob<T> job = down_job<T>(x, ld_x, a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, 0, -1, M);
+    const MxDownJob<T> job = down_job<T>(x, ld_x, a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, 0, M);
     st = launch_dependent(qlin_mx_down_kernel<T>, job.blocks, 256, 0, s, job, MxDownJob<T>{}, (int)M, (int)M);
     if (st != QLIN_OK) return st;
   }
@@ -478,7 +478,7 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
 template <typename T>
 int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void* mx, const T* a, const T* b, int rank,
                  float scale, T* dx, int64_t ld_dx, T* da, T* db, T* dbias, int64_t M, int64_t K_g, int64_t N_g,
-                 uint8_t* ws, const BackwardWs& w, int sms, cudaStream_t s) {
+                 uint8_t* ws, const BackwardWs& w, cudaStream_t s) {
   const int64_t K = 4 * K_g, N = 4 * N_g;
   if (dx && (!aligned(dx, 8) || ld_dx % 4 != 0)) return QLIN_ERR_ALIGN;
   T* at = reinterpret_cast<T*>(ws + w.at);
@@ -491,30 +491,29 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
   if (st == QLIN_OK && (da || db)) st = rows_for_tma(&x, &ld_x, ws + w.x, M, K, s);
   if (st != QLIN_OK) return st;
   const bool need_up = rank > 0 && (dx || da);
+  MxPlanes<T> p{};
+  if (dx || need_up) {
+    // conj(W)^T, A^T and B^T
+    for (int c = 0; c < 4; ++c) p.w[c] = reinterpret_cast<T*>(ws + w.planes) + c * K_g * w.ld_planes;
+    const int64_t steps = dx ? ceil_div(N_g, kMxTurnRows) * ceil_div(K_g, kMxBlock) : 0;
+    const int64_t a_blocks = dx ? ceil_div(rank * K, 256) : 0, b_blocks = need_up ? ceil_div(rank * N, 256) : 0;
+    if (steps + a_blocks + b_blocks > INT32_MAX) return QLIN_ERR_SHAPE;
+    st = launch_dependent(qlin_mx_turn_all_kernel<T>, (unsigned)(steps + a_blocks + b_blocks), 256, 0, s,
+                          static_cast<const uint8_t*>(mx), p, w.ld_planes, (int)K_g, (int)N_g, steps, a, at,
+                          (int64_t)rank, K, b, bt, N, (int64_t)rank, a_blocks);
+    if (st != QLIN_OK) return st;
+  }
   if (rank > 0 && (need_up || db)) {
-    if (need_up) {
-      const int64_t a_blocks = dx ? ceil_div(rank * K, 256) : 0, b_blocks = ceil_div(rank * N, 256);
-      st = launch_dependent(qlin_mx_turn_kernel<T>, (unsigned)(a_blocks + b_blocks), 256, 0, s, a, at, (int64_t)rank, K,
-                            b, bt, N, (int64_t)rank, a_blocks);
-      if (st != QLIN_OK) return st;
-    }
     MxDownJob<T> j0{}, j1{};
     if (need_up)
-      j0 = down_job<T>(g, ld_g, bt, N, scale, rank, dx ? parts : nullptr, w.ld_parts, da ? up : nullptr, w.rows0, -1,
-                       w.M_pad);
+      j0 = down_job<T>(g, ld_g, bt, N, scale, rank, dx ? parts : nullptr, w.ld_parts, da ? up : nullptr, w.rows, w.M_pad);
     if (db)
-      j1 = down_job<T>(x, ld_x, a, K, scale, rank, nullptr, 0, t, w.rows1, dbias ? rank : -1, w.M_pad);
+      j1 = down_job<T>(x, ld_x, a, K, scale, rank, nullptr, 0, t, w.rows, w.M_pad);
     st = launch_dependent(qlin_mx_down_kernel<T>, (unsigned)(j0.blocks + j1.blocks), 256, 0, s, j0, j1, (int)M,
                           (int)w.M_pad);
     if (st != QLIN_OK) return st;
   }
   if (dx) {
-    MxPlanes<T> p;
-    for (int c = 0; c < 4; ++c) p.w[c] = reinterpret_cast<T*>(ws + w.planes) + c * K_g * w.ld_planes;
-    const int64_t steps = ceil_div(N_g, 64) * ceil_div(K_g, kMxBlock);
-    st = launch_dependent(qlin_mx_adjoint_kernel<T>, (unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s,
-                          static_cast<const uint8_t*>(mx), p, w.ld_planes, (int)K_g, (int)N_g);
-    if (st != QLIN_OK) return st;
     st = run_pair<T, false>(M, g, ld_g, mx, p, w.ld_planes, (const T*)nullptr, (const T*)parts, w.ld_parts,
                             (const T*)at, rank, dx, ld_dx, M, N_g, K_g, s);
     if (st != QLIN_OK) return st;
@@ -535,10 +534,13 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
       o.blocks = o.col_tiles * o.row_tiles * splits;
       o.partial = reinterpret_cast<float*>(ws + partial);
     };
-    if (da) job(o0, up, x, ld_x, K, w.rows0, w.splits0, w.partial0);
-    if (db) job(o1, t, g, ld_g, N, w.rows1, w.splits1, w.partial1);
-    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 128, 0, s, o0, o1, (int)M,
-                          (int)w.M_pad);
+    if (da) job(o0, up, x, ld_x, K, w.rows, w.splits0, w.partial0);
+    if (db) job(o1, t, g, ld_g, N, w.rows, w.splits1, w.partial1);
+    static std::atomic<uint64_t> done{0};
+    if (allow_smem(qlin_mx_outer_kernel<T>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+    if (sum_with_db) o1.sums = reinterpret_cast<float*>(ws + w.sums);
+    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 256, kMxOuterSmem, s, o0, o1,
+                          (int)M, (int)w.M_pad);
     if (st != QLIN_OK) return st;
     const int64_t blocks0 = da ? ceil_div(rank * K, 256) : 0;
     const int64_t blocks1 = db ? ceil_div((rank + (sum_with_db ? 1 : 0)) * N, 256) : 0;
@@ -744,8 +746,7 @@ int qlin_mx_backward(int dtype, const void* gy, int64_t ld_g, const void* x, int
     const T* b = static_cast<const T*>(lora_b);
     if constexpr (sizeof(T) == 2)
       return run_backward<T>(g, ld_g, xt, ld_x, mx, a, b, rank, lora_scale, static_cast<T*>(dx), ld_dx,
-                             static_cast<T*>(da), static_cast<T*>(db), static_cast<T*>(dbias), M, K_g, N_g, ws, w, sms,
-                             s);
+                             static_cast<T*>(da), static_cast<T*>(db), static_cast<T*>(dbias), M, K_g, N_g, ws, w, s);
     else {
     T* at = reinterpret_cast<T*>(ws + w.at);
     T* bt = reinterpret_cast<T*>(ws + w.bt);

@@ -248,7 +248,7 @@ qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst,
   }
 }
 
-// The weights of the adjoint layer, conj(W)^T, as four component rows
+// The weights of the adjoint layer, conj(W)^T, in fp32 as four component rows
 // [K_g, N_g]: 64 output quaternions x 32 input quaternions of one component
 // per CTA step, turned through shared memory.
 template <typename T>

@@ -66,10 +66,12 @@ struct MxOperand {
   static constexpr int kParts = std::is_same<T, float>::value ? 3 : 1;
 };
 
-// c of the layer whose largest F is f0.
+// c of the layer whose largest F is f0.  With an adapter of some rank that goes
+// through the same accumulator, fp16 keeps B 2^-c in range for |B| up to 1000.
 template <bool HALF>
-__device__ __forceinline__ int mx_shift(uint32_t f0) {
-  return HALF ? (int)f0 - 129 : max(0, (int)f0 - 129);
+__device__ __forceinline__ int mx_shift(uint32_t f0, int rank = 0) {
+  const int c = (int)f0 - 129;
+  return HALF ? (rank > 0 ? max(c, -6) : c) : max(0, c);
 }
 
 // The packed multiplier of codes with scale F.  bf16: exponent field

@@ -90,6 +90,77 @@ qlin_mx_turn_kernel(const T* __restrict__ a, T* __restrict__ at, int64_t a_rows,
   if (k < rows * cols) (first ? at : bt)[k] = (first ? a : b)[(k % rows) * cols + k / rows];
 }
 
+constexpr int kMxTurnRows = 64;  // output quaternions of a step
+
+// What the 16-bit gradients need turned, in one launch: blocks [0, steps) make
+// the components of conj(W)^T 2^-c (rows of ld elements), the next a_blocks A^T,
+// the rest B^T.  A step is 64 output x 32 input quaternions; a thread takes two
+// neighbouring output quaternions, eight input quaternions and two components,
+// so that the turned pairs go to shared memory as words, a warp's in a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
+                        int64_t steps, const T* __restrict__ a, T* __restrict__ at, int64_t a_rows, int64_t a_cols,
+                        const T* __restrict__ b, T* __restrict__ bt, int64_t b_rows, int64_t b_cols,
+                        int64_t a_blocks) {
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  __shared__ __align__(16) uint32_t turned[4 * kMxBlock][36];  // [component, input quaternion][pair of outputs]
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  if ((int64_t)blockIdx.x >= steps) {
+    const bool first = (int64_t)blockIdx.x < steps + a_blocks;
+    const int64_t k = ((int64_t)blockIdx.x - steps - (first ? 0 : a_blocks)) * 256 + threadIdx.x;
+    const int64_t rows = first ? a_rows : b_rows, cols = first ? a_cols : b_cols;
+    // consecutive threads write consecutive elements
+    if (k < rows * cols) (first ? at : bt)[k] = (first ? a : b)[(k % rows) * cols + k / rows];
+    return;
+  }
+  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
+  const int64_t og = blockIdx.x / kb, blk = blockIdx.x - og * kb;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = warp & 3, ph = warp >> 2;
+  uint32_t f0;
+  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(mx) : "memory");
+  const int c = mx_shift<HALF>(f0, a_rows > 0 ? 1 : 0);
+  const int row = 2 * lane;  // of 64
+  const int64_t tile = 4 * og + row / kMxRows;
+  uint2 w[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+  uint32_t f[2] = {0u, 0u};
+  if (tile < tiles) {
+    const uint8_t* rec = mx + kMxHeader + (tile * kb + blk) * kMxRecord;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = row % kMxRows + u;
+      w[u] = *reinterpret_cast<const uint2*>(rec + r * 64 + t * 16 + ph * 8);
+      f[u] = *reinterpret_cast<const uint16_t*>(rec + kMxCodeBytes + r * 4 + ph * 2);
+    }
+  }
+  const MxPowers pw;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int p = 2 * ph + h;
+    uint32_t e[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      mx_expand_scaled<HALF>(pw, h ? w[u].y : w[u].x,
+                             mx_multiplier<HALF>((f[u] >> (8 * h)) & 255u, c) ^ (p ? 0x80008000u : 0u), e[u]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      turned[p * kMxBlock + 8 * t + k][lane] = __byte_perm(e[0][k], e[1][k], 0x5410);
+      turned[p * kMxBlock + 8 * t + k + 4][lane] = __byte_perm(e[0][k], e[1][k], 0x7632);
+    }
+  }
+  __syncthreads();
+  // 16-byte pieces: eight output quaternions of a row (rows of ld, a multiple of 8)
+#pragma unroll
+  for (int k = threadIdx.x; k < 4 * kMxBlock * 8; k += 256) {
+    const int piece = k & 7, i = (k >> 3) & 31, p = k >> 8;
+    const int64_t o = og * kMxTurnRows + 8 * piece, in = blk * kMxBlock + i;
+    if (o < ld && in < K_g)
+      *reinterpret_cast<uint4*>(dst.w[p] + in * ld + o) =
+          *reinterpret_cast<const uint4*>(&turned[p * kMxBlock + i][4 * piece]);
+  }
+}
+
 // dst rows of ld_d elements (ld_d >= cols), zero past cols: rows that no TMA map takes.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -116,10 +187,9 @@ struct MxDownJob {
   const T* a;      // [rank, K]
   int64_t K;
   float scale;
-  T* parts;        // [M, 2 * ld_parts]: hi, then lo, zero from rank to ld_parts; or null
+  T* parts;        // [M, 2, ld_parts]: hi and lo, zero from rank to ld_parts; or null
   T* turned;       // [2][rows][M_pad]: hi, then lo, transposed; or null
   int rank, ld_parts, rows, vec;  // vec: rows of A are 16-byte aligned
-  int ones;        // row of `turned` that holds ones (-1: none)
   int rank_tiles;  // ceil(max(ld_parts, rows) / 32)
   int blocks;
 };
@@ -154,20 +224,28 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
   const T* xh = xl + 8 * job.ld_x;
   const bool has_l = m0 + g < M, has_h = m0 + g + 8 < M;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  if (r0 < job.rank) {
-#pragma unroll 2
-    for (int64_t k0 = 32 * warp; k0 < job.K; k0 += 32 * 8) {
-      const int64_t k = k0 + 8 * t;
-      const uint4 lo = has_l ? mx_load_row8(xl, k, job.K, true) : zero;
-      const uint4 hi = has_h ? mx_load_row8(xh, k, job.K, true) : zero;
+  // four pieces at a time: 24 loads of 16 bytes in flight per lane
+  for (int64_t k0 = 32 * warp; k0 < job.K && r0 < job.rank; k0 += 4 * 32 * 8) {
+    uint4 lo[4], hi[4], b[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t k = k0 + u * 32 * 8 + 8 * t;
+      const bool in = k < job.K;
+      lo[u] = in && has_l ? mx_load_row8(xl, k, job.K, true) : zero;
+      hi[u] = in && has_h ? mx_load_row8(xh, k, job.K, true) : zero;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int r = r0 + 8 * n + g;
-        const uint4 b = r < job.rank ? mx_load_row8(job.a + (int64_t)r * job.K, k, job.K, job.vec) : zero;
-        mx_mma<HALF>(acc[n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-        mx_mma<HALF>(acc[n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+        b[u][n] = in && r < job.rank ? mx_load_row8(job.a + (int64_t)r * job.K, k, job.K, job.vec) : zero;
       }
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        mx_mma<HALF>(acc[n], lo[u].x, hi[u].x, lo[u].y, hi[u].y, b[u][n].x, b[u][n].y);
+        mx_mma<HALF>(acc[n], lo[u].z, hi[u].z, lo[u].w, hi[u].w, b[u][n].z, b[u][n].w);
+      }
   }
 #pragma unroll
   for (int n = 0; n < 4; ++n)
@@ -186,7 +264,6 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
 #pragma unroll
       for (int w = 0; w < 8; ++w) v += red[w][m][r];
       v *= job.scale;
-      if (r0 + r == job.ones && m0 + m < M) v = 1.f;
       const T hi = from_f32<T>(v);
       const float rest = v - to_f32(hi);
       const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
@@ -208,10 +285,13 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
 // ---------------------------------------------------------------------------
 // 16-bit gradients: out = (hi + lo) X, sums over the tokens
 // ---------------------------------------------------------------------------
-constexpr int kMxOuterCols = 64;    // columns of X of a CTA
+constexpr int kMxOuterCols = 128;   // columns of X of a CTA, 16 per warp
 constexpr int kMxOuterTokens = 32;  // tokens of a step
 constexpr int kMxOuterRows = 64;    // rows of the result of a CTA (groups of 16)
 constexpr int kMxOuterStages = 4;
+constexpr int kMxOuterXBytes = kMxOuterTokens * kMxOuterCols * 2;
+constexpr int kMxOuterStage = kMxOuterXBytes + 2 * kMxOuterRows * kMxOuterTokens * 2;
+constexpr int kMxOuterSmem = kMxOuterStages * kMxOuterStage;
 
 template <typename T>
 struct MxOuterJob {
@@ -222,20 +302,23 @@ struct MxOuterJob {
   int col_tiles, row_tiles, splits;
   int blocks;
   float* partial;   // [splits][rows][cols]
+  float* sums;      // [splits][cols] column sums of X, or null
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Four warps: 16 columns each, all rows.  X comes through a ring of shared
-// memory steps (32 tokens x 64 columns, 16-byte chunks permuted within a row so
-// that the transposing loads of eight tokens two apart are free of conflicts).
+// Eight warps: 16 columns each, all rows.  X and the rows of (hi, lo) come through
+// a ring of shared memory steps (32 tokens x 128 columns; 16-byte chunks permuted
+// within a row of X so that the transposing loads of eight tokens two apart are
+// free of conflicts).
 template <typename T>
-__global__ void __launch_bounds__(128)
-qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int M, int M_pad) {
+__global__ void __launch_bounds__(256)
+qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int M,
+                     int M_pad) {
   constexpr bool HALF = std::is_same<T, __half>::value;
-  __shared__ __align__(128) uint8_t ring[kMxOuterStages][kMxOuterTokens * kMxOuterCols * 2];
+  extern __shared__ __align__(128) uint8_t mx_smem[];
   pdl_wait_prior();
   pdl_launch_dependents();
   const bool first = (int)blockIdx.x < job0.blocks;
@@ -248,19 +331,26 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   const int s0 = (int)((int64_t)steps * split / job.splits), s1 = (int)((int64_t)steps * (split + 1) / job.splits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int c0 = ct * kMxOuterCols, row0 = rt * kMxOuterRows;
-  const int groups = min(kMxOuterRows, job.rows - row0) / 16;
+  const int rows = min(kMxOuterRows, job.rows - row0), groups = rows / 16;
+  const T* turned = job.turned + (int64_t)row0 * M_pad;
+  const int64_t lo_off = (int64_t)job.rows * M_pad;
 
   auto fetch = [&](int step) {
     if (step < s1) {
-      const uint32_t base = smem_u32(ring[step % kMxOuterStages]);
+      const uint32_t base = smem_u32(mx_smem) + (step % kMxOuterStages) * kMxOuterStage;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int k = threadIdx.x + 128 * u, tok = k >> 3, chunk = k & 7;
+        const int k = threadIdx.x + 256 * u, tok = k >> 4, chunk = k & 15;
         const int m = step * kMxOuterTokens + tok, c = c0 + 8 * chunk;
         const int left = m < M ? min(8, job.cols - c) : 0;  // elements of the chunk inside
         const int f = (tok & 1) | ((tok >> 3) & 3) << 1;
-        cp_async16(base + tok * 128 + ((chunk ^ f) << 4), left > 0 ? job.X + (int64_t)m * job.ld + c : job.X,
+        cp_async16(base + tok * 256 + ((chunk ^ f) << 4), left > 0 ? job.X + (int64_t)m * job.ld + c : job.X,
                    left > 0 ? 2 * left : 0);
+      }
+      for (int k = threadIdx.x; k < 8 * rows; k += 256) {  // [part][row][4 chunks]
+        const int part = k >= 4 * rows ? 1 : 0, r = (k - part * 4 * rows) >> 2, chunk = k & 3;
+        cp_async16(base + kMxOuterXBytes + (part * kMxOuterRows + r) * 64 + (chunk << 4),
+                   turned + part * lo_off + (int64_t)r * M_pad + step * kMxOuterTokens + 8 * chunk, 16);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -269,43 +359,45 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   for (int k = 0; k < kMxOuterStages - 1; ++k) fetch(s0 + k);
 
   float acc[4][2][4] = {};  // [row group][8 columns][fragment]
-  const T* hi_rows = job.turned + (int64_t)(row0 + g) * M_pad;
-  const int64_t lo_off = (int64_t)job.rows * M_pad;
+  float sum[2] = {0.f, 0.f};
+  const bool sums = job.sums && rt == 0;
   // this lane's row of the transposing loads: matrix lane / 8 (pair j), row lane % 8
   const int mtok = 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
   const int mf = (mtok & 1) | ((mtok >> 3) & 3) << 1;
   for (int step = s0; step < s1; ++step) {
-    uint4 a[4][2][2];  // [row group][part][row g, g + 8]
+    asm volatile("cp.async.wait_group %0;" ::"n"(kMxOuterStages - 2) : "memory");
+    __syncthreads();
+    fetch(step + kMxOuterStages - 1);  // into the stage of step - 1: every warp is past it
+    const uint32_t base = smem_u32(mx_smem) + (step % kMxOuterStages) * kMxOuterStage;
+    uint32_t b[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
+                   : "r"(base + mtok * 256 + (((2 * warp + n) ^ mf) << 4))
+                   : "memory");
+    if (sums) {  // the lane holds eight tokens of column g
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const T* e = reinterpret_cast<const T*>(&b[n][j]);
+          sum[n] += to_f32(e[0]) + to_f32(e[1]);
+        }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (r < groups)
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+        for (int part = 0; part < 2; ++part) {
+          const uint32_t at = base + kMxOuterXBytes + (part * kMxOuterRows + 16 * r + g) * 64 + t * 16;
+          const uint4 l = lds128(at), h = lds128(at + 8 * 64);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            a[r][part][h] = ld_cg_v4(hi_rows + part * lo_off + (int64_t)(16 * r + 8 * h) * M_pad +
-                                     step * kMxOuterTokens + 8 * t);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kMxOuterStages - 2) : "memory");
-    __syncthreads();
-    fetch(step + kMxOuterStages - 1);  // the stage of step - 1: every warp is past it
-    const uint32_t base = smem_u32(ring[step % kMxOuterStages]) + mtok * 128;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      uint32_t b[4];
-      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
-                   : "r"(base + (((2 * warp + n) ^ mf) << 4))
-                   : "memory");
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < groups)
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            const uint4 l = a[r][part][0], h = a[r][part][1];
-            mx_mma<HALF>(acc[r][n], l.x, h.x, l.y, h.y, b[0], b[1]);
-            mx_mma<HALF>(acc[r][n], l.z, h.z, l.w, h.w, b[2], b[3]);
+          for (int n = 0; n < 2; ++n) {
+            mx_mma<HALF>(acc[r][n], l.x, h.x, l.y, h.y, b[n][0], b[n][1]);
+            mx_mma<HALF>(acc[r][n], l.z, h.z, l.w, h.w, b[n][2], b[n][3]);
           }
-    }
+        }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
@@ -318,10 +410,19 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
           const int row = row0 + 16 * r + g + 8 * (q >> 1), c = c0 + 16 * warp + 8 * n + 2 * t + (q & 1);
           if (c < job.cols) job.partial[((int64_t)split * job.rows + row) * job.cols + c] = acc[r][n][q];
         }
+  if (sums)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      float v = sum[n];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      const int c = c0 + 16 * warp + 8 * n + g;
+      if (t == 0 && c < job.cols) job.sums[(int64_t)split * job.cols + c] = v;
+    }
 }
 
 // Adds the splits up: da [rank, cols] from job0's; db [cols, rank] and dbias
-// [cols] (row `rank`) from job1's.
+// [cols] from job1's.
 template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_outer_finish_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int rank, T* __restrict__ da,
@@ -335,15 +436,14 @@ qlin_mx_outer_finish_kernel(const __grid_constant__ MxOuterJob<T> job0, const __
   if (k >= (int64_t)rows * job.cols) return;
   // consecutive threads: consecutive columns of a row
   const int64_t r = k / job.cols, c = k - r * job.cols;
+  const bool bias = r == rank;
+  const float* at = bias ? job.sums + c : job.partial + r * job.cols + c;
+  const int64_t step = bias ? job.cols : (int64_t)job.rows * job.cols;
   float v = 0.f;
-  for (int s = 0; s < job.splits; ++s)
-    v += __ldcg(job.partial + ((int64_t)s * job.rows + r) * job.cols + c);
+  for (int s = 0; s < job.splits; ++s) v += __ldcg(at + s * step);
   if (first) da[k] = from_f32<T>(v);
-  else if (r < rank) {
-    if (db) db[c * rank + r] = from_f32<T>(v);
-  } else {
-    dbias[c] = from_f32<T>(v);
-  }
+  else if (bias) dbias[c] = from_f32<T>(v);
+  else db[c * rank + r] = from_f32<T>(v);
 }
 
 }  // namespace qlin

@@ -9,7 +9,8 @@
 // s(a, a^q) in one packed multiplication and pairs the components up: the
 // expansion costs the integer pipe about 450 cycles of the 1024 that the eight
 // UMMAs of a stage take at 256 tokens, and a quarter of a 16-bit layer's bytes.
-// Without MX the weights are 16-bit component planes (the adjoint of the codes).
+// Without MX the weights are 16-bit component planes: the adjoint of the codes,
+// times 2^-c.
 //
 // Adapter: y += t B^T with t = s x A^T as two 16-bit parts (t = hi + lo to about
 // twice the type's precision): ceil(r / 64) more stages whose x tile is 64
@@ -46,7 +47,7 @@ struct MxPairStage {
 };
 
 struct MxPairParams {
-  const uint8_t* mx;    // codes (MX)
+  const uint8_t* mx;    // codes
   const void* bias;
   const void* lora_b;   // [4 N_g, rank] or null
   void* y;
@@ -55,7 +56,6 @@ struct MxPairParams {
   int kb, w_tiles;      // blocks of a row; 16-row tiles of the codes
   int stages;           // weight stages of a tile
   int lora_stages;      // ceil(rank / 64)
-  int lo_col;           // column of t's low parts
   int nb_tiles, tiles;
   int wide;             // 16-byte output pieces are aligned
 };
@@ -136,13 +136,9 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     n0 = nb * 256 + (int)cta * kPairRows;  // this CTA's first real output
     m0 = tb * NTOK;                        // the pair's first token
   };
-  int c = 0;  // the accumulator holds y 2^-c
-  if constexpr (MX) {
-    uint32_t f0;
-    asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(prm.mx) : "memory");
-    c = mx_shift<HALF>(f0);
-    if (HALF && prm.rank > 0) c = max(c, -6);
-  }
+  uint32_t f0;
+  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(prm.mx) : "memory");
+  const int c = mx_shift<HALF>(f0, prm.rank);  // the accumulator holds y 2^-c
 
   if (warp == 0) {
     // ---------------- copies of this CTA's x half-tile and weights ----------------
@@ -164,8 +160,8 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           if (k >= prm.stages) {
             const int r = 64 * (k - prm.stages);
             mbar_arrive_expect_tx(&full[s], Cfg::kXBytes);
-            tma_load_2d(dst, &map_t, &full[s], r, mrow);
-            tma_load_2d(dst + Cfg::kXAtomBytes, &map_t, &full[s], prm.lo_col + r, mrow);
+            tma_load_3d(dst, &map_t, &full[s], r, mrow, 0);
+            tma_load_3d(dst + Cfg::kXAtomBytes, &map_t, &full[s], r, mrow, 1);
           } else {
             mbar_arrive_expect_tx(&full[s], Cfg::kXBytes + (MX ? have * kMxRecord : 4 * kPairWTileBytes));
             tma_load_2d(dst, &map_x, &full[s], k * kPairStageK, mrow);
