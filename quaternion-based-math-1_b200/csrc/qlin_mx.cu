@@ -88,7 +88,7 @@ bool is_one(int dtype, int64_t M, int64_t K_g) {
 bool tma_rows(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0; }
 
 struct ForwardWs {
-  size_t arranged = 0, t = 0, x = 0, total = 0;
+  size_t arranged = 0, t = 0, x = 0, a = 0, total = 0;
   int64_t ld_parts = 0;  // ranks of t's rows, in whole 16-byte pieces
 };
 
@@ -106,6 +106,7 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
     w.ld_parts = round_up(rank, 8);
     w.x = c.take(M * round_up(4 * K_g, 8) * 2);
     w.t = c.take(M * 2 * w.ld_parts * 2);
+    w.a = c.take(rank * round_up(4 * K_g, 8) * 2);
   }
   w.total = c.at;
   return w;
@@ -113,7 +114,7 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
 
 struct BackwardWs {
   // 16-bit
-  size_t gy = 0, x = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0, sums = 0;
+  size_t gy = 0, x = 0, a = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0, sums = 0;
   int64_t M_pad = 0, ld_parts = 0, ld_planes = 0;
   int rows = 0, splits0 = 0, splits1 = 0;
   // fp32
@@ -121,11 +122,11 @@ struct BackwardWs {
   size_t total = 0;
 };
 
-// Splits of the tokens of a gradient product: about one CTA per SM for each of the
-// two, at least four steps of 32 tokens each.
+// Splits of the tokens of a gradient product: about 1.5 CTAs per SM for each of the
+// two (three fit an SM), at least four steps of 32 tokens each.
 int outer_splits(int64_t M_pad, int64_t cols, int rows) {
   const int64_t tiles = ceil_div(cols, kMxOuterCols) * ceil_div(rows, kMxOuterRows);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 148 / std::max<int64_t>(1, tiles)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 222 / std::max<int64_t>(1, tiles)));
 }
 
 BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
@@ -152,7 +153,8 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
     w.planes = c.take(4 * K_g * w.ld_planes * 2);
     if (rank > 0) {
       w.at = c.take(K * rank * 2);
-      w.bt = c.take(N * rank * 2);
+      w.bt = c.take(round_up(N, 8) * rank * 2);
+      w.a = c.take(rank * round_up(K, 8) * 2);
       w.parts = c.take(M * 2 * w.ld_parts * 2);
       w.up = c.take(2 * w.rows * w.M_pad * 2);
       w.t = c.take(2 * w.rows * w.M_pad * 2);
@@ -205,15 +207,15 @@ int launch_dependent(void (*kernel)(KArgs...), unsigned ctas, unsigned threads, 
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
 }
 
-constexpr size_t kMostSmem = 226 * 1024;  // 1 KB of the 227 for static shared memory
+constexpr size_t kMostSmem = 226 * 1024;  // 1 KB of the 227 left for static shared memory
 
 // Raises a kernel's shared-memory limit once per device.
 template <typename K>
-int allow_smem(K kernel, std::atomic<uint64_t>& done) {
+int allow_smem(K kernel, std::atomic<uint64_t>& done, size_t bytes = kMostSmem) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return QLIN_ERR_LAUNCH;
   if (done.load(std::memory_order_acquire) >> dev & 1) return QLIN_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem) != cudaSuccess)
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
     return QLIN_ERR_LAUNCH;
   done.fetch_or(1ull << dev, std::memory_order_release);
   return QLIN_OK;
@@ -424,10 +426,11 @@ int run_pair(int64_t M, Args... args) {
   return M > 128 ? launch_pair<T, 256, MX>(args...) : launch_pair<T, 128, MX>(args...);
 }
 
-// Rows that TMA takes: x itself, or a copy in the workspace.
+// Rows that TMA takes (whole: and that are whole 16-byte pieces): x itself, or a
+// copy in the workspace with zeros up to the next 16 bytes.
 template <typename T>
-int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t cols, cudaStream_t s) {
-  if (tma_rows(*x, *ld)) return QLIN_OK;
+int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t cols, bool whole, cudaStream_t s) {
+  if (tma_rows(*x, *ld) && !(whole && cols % 8 != 0)) return QLIN_OK;
   const int64_t ld_c = round_up(cols, 8), blocks = ceil_div(rows * ld_c, 256);
   if (blocks > INT32_MAX) return QLIN_ERR_SHAPE;
   const int st = launch_dependent(qlin_mx_repack_kernel<T>, (unsigned)blocks, 256, 0, s, *x, *ld, static_cast<T*>(copy),
@@ -438,23 +441,31 @@ int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t col
 }
 
 template <typename T>
-MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t K, float scale, int rank, T* parts,
+MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t ld_a, int64_t K, float scale, int rank, T* parts,
                       int64_t ld_parts, T* turned, int rows, int64_t tokens) {
   MxDownJob<T> j{};
   j.x = x;
   j.ld_x = ld_x;
   j.a = a;
-  j.K = K;
+  j.ld_a = ld_a;
+  j.K = (int)round_up(K, 8);
   j.scale = scale;
   j.rank = rank;
   j.parts = parts;
   j.ld_parts = parts ? (int)ld_parts : 0;
   j.turned = turned;
   j.rows = turned ? rows : 0;
-  j.vec = K % 8 == 0 && aligned(a, 16);
   j.rank_tiles = (int)ceil_div(std::max(j.ld_parts, j.rows), kMxDownRanks);
   j.blocks = (int)(ceil_div(tokens, kMxDownRows) * j.rank_tiles);
   return j;
+}
+
+template <typename T>
+int launch_down(const MxDownJob<T>& j0, const MxDownJob<T>& j1, int64_t M, int64_t M_pad, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  if (allow_smem(qlin_mx_down_kernel<T>, done, kMxDownSmem) != QLIN_OK) return QLIN_ERR_LAUNCH;
+  return launch_dependent(qlin_mx_down_kernel<T>, (unsigned)(j0.blocks + j1.blocks), 256, kMxDownSmem, s, j0, j1,
+                          (int)M, (int)M_pad);
 }
 
 template <typename T>
@@ -462,12 +473,15 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
                 T* y, int64_t ld_y, int64_t M, int64_t K_g, int64_t N_g, uint8_t* ws, const ForwardWs& w,
                 cudaStream_t s) {
   if (!aligned(y, 8) || ld_y % 4 != 0) return QLIN_ERR_ALIGN;
-  int st = rows_for_tma(&x, &ld_x, ws + w.x, M, 4 * K_g, s);
+  int st = rows_for_tma(&x, &ld_x, ws + w.x, M, 4 * K_g, rank > 0, s);
   if (st != QLIN_OK) return st;
   T* parts = reinterpret_cast<T*>(ws + w.t);
   if (rank > 0) {
-    const MxDownJob<T> job = down_job<T>(x, ld_x, a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, 0, M);
-    st = launch_dependent(qlin_mx_down_kernel<T>, job.blocks, 256, 0, s, job, MxDownJob<T>{}, (int)M, (int)M);
+    int64_t ld_a = 4 * K_g;
+    st = rows_for_tma(&a, &ld_a, ws + w.a, rank, 4 * K_g, true, s);
+    if (st != QLIN_OK) return st;
+    const MxDownJob<T> job = down_job<T>(x, ld_x, a, ld_a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, 0, M);
+    st = launch_down<T>(job, MxDownJob<T>{}, M, M, s);
     if (st != QLIN_OK) return st;
   }
   return run_pair<T, true>(M, x, ld_x, mx, MxPlanes<T>{}, (int64_t)0, bias, (const T*)parts, w.ld_parts, b, rank, y,
@@ -487,8 +501,11 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
   T* up = reinterpret_cast<T*>(ws + w.up);
   T* t = reinterpret_cast<T*>(ws + w.t);
   int st = QLIN_OK;
-  if (dx || da || db) st = rows_for_tma(&g, &ld_g, ws + w.gy, M, N, s);
-  if (st == QLIN_OK && (da || db)) st = rows_for_tma(&x, &ld_x, ws + w.x, M, K, s);
+  if (dx || da || db) st = rows_for_tma(&g, &ld_g, ws + w.gy, M, N, rank > 0, s);
+  if (st == QLIN_OK && (da || db)) st = rows_for_tma(&x, &ld_x, ws + w.x, M, K, true, s);
+  const T* a8 = a;  // A's rows, in whole 16-byte pieces
+  int64_t ld_a = K;
+  if (st == QLIN_OK && db) st = rows_for_tma(&a8, &ld_a, ws + w.a, rank, K, true, s);
   if (st != QLIN_OK) return st;
   const bool need_up = rank > 0 && (dx || da);
   MxPlanes<T> p{};
@@ -496,21 +513,20 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     // conj(W)^T, A^T and B^T
     for (int c = 0; c < 4; ++c) p.w[c] = reinterpret_cast<T*>(ws + w.planes) + c * K_g * w.ld_planes;
     const int64_t steps = dx ? ceil_div(N_g, kMxTurnRows) * ceil_div(K_g, kMxBlock) : 0;
-    const int64_t a_blocks = dx ? ceil_div(rank * K, 256) : 0, b_blocks = need_up ? ceil_div(rank * N, 256) : 0;
+    const int64_t a_blocks = dx ? ceil_div(rank * K, 256) : 0, b_blocks = need_up ? ceil_div(rank * round_up(N, 8), 256) : 0;
     if (steps + a_blocks + b_blocks > INT32_MAX) return QLIN_ERR_SHAPE;
     st = launch_dependent(qlin_mx_turn_all_kernel<T>, (unsigned)(steps + a_blocks + b_blocks), 256, 0, s,
                           static_cast<const uint8_t*>(mx), p, w.ld_planes, (int)K_g, (int)N_g, steps, a, at,
-                          (int64_t)rank, K, b, bt, N, (int64_t)rank, a_blocks);
+                          (int64_t)rank, K, b, bt, N, (int64_t)rank, round_up(N, 8), a_blocks);
     if (st != QLIN_OK) return st;
   }
   if (rank > 0 && (need_up || db)) {
     MxDownJob<T> j0{}, j1{};
     if (need_up)
-      j0 = down_job<T>(g, ld_g, bt, N, scale, rank, dx ? parts : nullptr, w.ld_parts, da ? up : nullptr, w.rows, w.M_pad);
+      j0 = down_job<T>(g, ld_g, bt, round_up(N, 8), N, scale, rank, dx ? parts : nullptr, w.ld_parts, da ? up : nullptr, w.rows, w.M_pad);
     if (db)
-      j1 = down_job<T>(x, ld_x, a, K, scale, rank, nullptr, 0, t, w.rows, w.M_pad);
-    st = launch_dependent(qlin_mx_down_kernel<T>, (unsigned)(j0.blocks + j1.blocks), 256, 0, s, j0, j1, (int)M,
-                          (int)w.M_pad);
+      j1 = down_job<T>(x, ld_x, a8, ld_a, K, scale, rank, nullptr, 0, t, w.rows, w.M_pad);
+    st = launch_down<T>(j0, j1, M, w.M_pad, s);
     if (st != QLIN_OK) return st;
   }
   if (dx) {
@@ -537,9 +553,9 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     if (da) job(o0, up, x, ld_x, K, w.rows, w.splits0, w.partial0);
     if (db) job(o1, t, g, ld_g, N, w.rows, w.splits1, w.partial1);
     static std::atomic<uint64_t> done{0};
-    if (allow_smem(qlin_mx_outer_kernel<T>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+    if (allow_smem(qlin_mx_outer_kernel<T>, done, kMxOuterSmem) != QLIN_OK) return QLIN_ERR_LAUNCH;
     if (sum_with_db) o1.sums = reinterpret_cast<float*>(ws + w.sums);
-    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 256, kMxOuterSmem, s, o0, o1,
+    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 128, kMxOuterSmem, s, o0, o1,
                           (int)M, (int)w.M_pad);
     if (st != QLIN_OK) return st;
     const int64_t blocks0 = da ? ceil_div(rank * K, 256) : 0;

@@ -102,6 +102,7 @@ __device__ __forceinline__ void mx_expand_scaled(const MxPowers& c, uint32_t w, 
   for (int k = 0; k < 4; ++k) r[k] = mx_mul2<HALF>(r[k], mult);
 }
 
+// d += A B
 template <bool HALF>
 __device__ __forceinline__ void mx_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                        uint32_t b0, uint32_t b1) {
@@ -112,6 +113,22 @@ __device__ __forceinline__ void mx_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// d = A B
+template <bool HALF>
+__device__ __forceinline__ void mx_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm("{\n\t.reg .f32 z;\n\tmov.f32 z, 0f00000000;\n\t"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {z,z,z,z};\n\t}"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("{\n\t.reg .f32 z;\n\tmov.f32 z, 0f00000000;\n\t"
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {z,z,z,z};\n\t}"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -504,11 +521,12 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
           uint32_t lo[4], hi[4];
           mx_expand<HALF>(pw, l[p], lo);
           mx_expand<HALF>(pw, h[p], hi);
-          float d[4] = {};
+          float d[4];
 #pragma unroll
           for (int s3 = 0; s3 < P; ++s3) {
             const uint4 w = lds128(from[p] + (b * P + s3) * 1024);
-            mx_mma<HALF>(d, lo[0], hi[0], lo[1], hi[1], w.x, w.y);
+            if (s3 == 0) mx_mma_first<HALF>(d, lo[0], hi[0], lo[1], hi[1], w.x, w.y);
+            else mx_mma<HALF>(d, lo[0], hi[0], lo[1], hi[1], w.x, w.y);
             mx_mma<HALF>(d, lo[2], hi[2], lo[3], hi[3], w.z, w.w);
           }
           const uint32_t fl = p < 3 ? sl * byte_up[p] : sl >> 1, fh = p < 3 ? sh * byte_up[p] : sh >> 1;

@@ -94,14 +94,14 @@ constexpr int kMxTurnRows = 64;  // output quaternions of a step
 
 // What the 16-bit gradients need turned, in one launch: blocks [0, steps) make
 // the components of conj(W)^T 2^-c (rows of ld elements), the next a_blocks A^T,
-// the rest B^T.  A step is 64 output x 32 input quaternions; a thread takes two
+// the rest B^T (rows of ld_bt elements, zero past B's rows).  A step is 64 output x 32 input quaternions; a thread takes two
 // neighbouring output quaternions, eight input quaternions and two components,
 // so that the turned pairs go to shared memory as words, a warp's in a row.
 template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
                         int64_t steps, const T* __restrict__ a, T* __restrict__ at, int64_t a_rows, int64_t a_cols,
-                        const T* __restrict__ b, T* __restrict__ bt, int64_t b_rows, int64_t b_cols,
+                        const T* __restrict__ b, T* __restrict__ bt, int64_t b_rows, int64_t b_cols, int64_t ld_bt,
                         int64_t a_blocks) {
   constexpr bool HALF = std::is_same<T, __half>::value;
   __shared__ __align__(16) uint32_t turned[4 * kMxBlock][36];  // [component, input quaternion][pair of outputs]
@@ -110,9 +110,13 @@ qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, i
   if ((int64_t)blockIdx.x >= steps) {
     const bool first = (int64_t)blockIdx.x < steps + a_blocks;
     const int64_t k = ((int64_t)blockIdx.x - steps - (first ? 0 : a_blocks)) * 256 + threadIdx.x;
-    const int64_t rows = first ? a_rows : b_rows, cols = first ? a_cols : b_cols;
     // consecutive threads write consecutive elements
-    if (k < rows * cols) (first ? at : bt)[k] = (first ? a : b)[(k % rows) * cols + k / rows];
+    if (first) {
+      if (k < a_rows * a_cols) at[k] = a[(k % a_rows) * a_cols + k / a_rows];
+    } else if (k < ld_bt * b_cols) {
+      const int64_t r = k % ld_bt;
+      bt[k] = r < b_rows ? b[r * b_cols + k / ld_bt] : from_f32<T>(0.f);
+    }
     return;
   }
   const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
@@ -161,7 +165,8 @@ qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, i
   }
 }
 
-// dst rows of ld_d elements (ld_d >= cols), zero past cols: rows that no TMA map takes.
+// dst rows of ld_d elements (ld_d >= cols), zero past cols: rows that no 16-byte
+// load takes.
 template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_repack_kernel(const T* __restrict__ src, int64_t ld_s, T* __restrict__ dst, int64_t ld_d, int64_t rows,
@@ -182,35 +187,38 @@ constexpr int kMxDownRanks = 32;  // ranks of a CTA
 
 template <typename T>
 struct MxDownJob {
-  const T* x;      // [M, ld_x], 16-byte aligned rows
+  const T* x;      // [M, ld_x]
   int64_t ld_x;
-  const T* a;      // [rank, K]
-  int64_t K;
+  const T* a;      // [rank, ld_a]
+  int64_t ld_a;    // (both: 16-byte aligned rows of K elements)
+  int K;           // a multiple of 8: zero past the product's terms
   float scale;
   T* parts;        // [M, 2, ld_parts]: hi and lo, zero from rank to ld_parts; or null
   T* turned;       // [2][rows][M_pad]: hi, then lo, transposed; or null
-  int rank, ld_parts, rows, vec;  // vec: rows of A are 16-byte aligned
+  int rank, ld_parts, rows;
   int rank_tiles;  // ceil(max(ld_parts, rows) / 32)
   int blocks;
 };
 
-// Eight elements of a row of K, zero past its end.
-template <typename T>
-__device__ __forceinline__ uint4 mx_load_row8(const T* row, int64_t k, int64_t K, bool vec) {
-  if (vec && k + 8 <= K) return ld_cg_v4(row + k);
-  unsigned short h[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    h[j] = k + j < K ? *reinterpret_cast<const volatile unsigned short*>(row + k + j) : (unsigned short)0;
-  return make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                    h[6] | (uint32_t)h[7] << 16);
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+constexpr int kMxDownStages = 4;
+constexpr int kMxDownPieces = 6;  // 16-byte pieces of a lane and stage: two tokens, four ranks
+constexpr int kMxDownSmem = kMxDownStages * kMxDownPieces * 256 * 16;
+
 // A CTA: 16 tokens x 32 ranks, its eight warps every eighth piece of 32 terms.
+// Tokens and ranks past the last read the last one's row; what comes of them is
+// replaced by zeros.  A lane fetches what it will multiply itself, asynchronously
+// and up to three pieces ahead, into slots of its own: no barrier in the loop, and
+// 24 loads in flight however the compiler spends its registers.
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_constant__ MxDownJob<T> job1, int M, int M_pad) {
+qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_constant__ MxDownJob<T> job1, int M,
+                    int M_pad) {
   constexpr bool HALF = std::is_same<T, __half>::value;
+  extern __shared__ __align__(128) uint8_t mx_smem[];
   __shared__ float red[8][kMxDownRows][kMxDownRanks + 1];
   pdl_wait_prior();
   pdl_launch_dependents();
@@ -220,32 +228,44 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
   const int m0 = id / job.rank_tiles * kMxDownRows, r0 = id % job.rank_tiles * kMxDownRanks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float acc[4][4] = {};
-  const T* xl = job.x + (int64_t)(m0 + g) * job.ld_x;
-  const T* xh = xl + 8 * job.ld_x;
-  const bool has_l = m0 + g < M, has_h = m0 + g + 8 < M;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  // four pieces at a time: 24 loads of 16 bytes in flight per lane
-  for (int64_t k0 = 32 * warp; k0 < job.K && r0 < job.rank; k0 += 4 * 32 * 8) {
-    uint4 lo[4], hi[4], b[4][4];
+  if (r0 < job.rank && m0 < M) {
+    const T* xl = job.x + (int64_t)min(m0 + g, M - 1) * job.ld_x;
+    const T* xh = job.x + (int64_t)min(m0 + g + 8, M - 1) * job.ld_x;
+    const T* ar[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t k = k0 + u * 32 * 8 + 8 * t;
-      const bool in = k < job.K;
-      lo[u] = in && has_l ? mx_load_row8(xl, k, job.K, true) : zero;
-      hi[u] = in && has_h ? mx_load_row8(xh, k, job.K, true) : zero;
+    for (int n = 0; n < 4; ++n) ar[n] = job.a + (int64_t)min(r0 + 8 * n + g, job.rank - 1) * job.ld_a;
+    constexpr int kStep = 32 * 8;
+    const uint32_t slots = smem_u32(mx_smem) + threadIdx.x * 16;
+    int k = 32 * warp + 8 * t;   // next to fetch
+    MxRing in, out;
+    auto fetch = [&]() {
+      const uint32_t at = slots + in.at * kMxDownPieces * 256 * 16;
+      const int bytes = k < job.K ? 16 : 0, from = k < job.K ? k : 0;
+      // (the slot's values were consumed by products issued before: their registers are read)
+      cp_async16(at, xl + from, bytes);
+      cp_async16(at + 256 * 16, xh + from, bytes);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) cp_async16(at + (2 + n) * 256 * 16, ar[n] + from, bytes);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      k += kStep;
+      in.next(kMxDownStages);
+    };
+#pragma unroll
+    for (int u = 0; u < kMxDownStages - 1; ++u) fetch();
+    for (int done = 32 * warp; done < job.K; done += kStep) {
+      fetch();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kMxDownStages - 1) : "memory");
+      const uint32_t at = slots + out.at * kMxDownPieces * 256 * 16;
+      out.next(kMxDownStages);
+      const uint4 lo = lds128(at), hi = lds128(at + 256 * 16);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const int r = r0 + 8 * n + g;
-        b[u][n] = in && r < job.rank ? mx_load_row8(job.a + (int64_t)r * job.K, k, job.K, job.vec) : zero;
+        const uint4 b = lds128(at + (2 + n) * 256 * 16);
+        mx_mma<HALF>(acc[n], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+        mx_mma<HALF>(acc[n], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
       }
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        mx_mma<HALF>(acc[n], lo[u].x, hi[u].x, lo[u].y, hi[u].y, b[u][n].x, b[u][n].y);
-        mx_mma<HALF>(acc[n], lo[u].z, hi[u].z, lo[u].w, hi[u].w, b[u][n].z, b[u][n].w);
-      }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
 #pragma unroll
   for (int n = 0; n < 4; ++n)
@@ -263,7 +283,7 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) v += red[w][m][r];
-      v *= job.scale;
+      v = m0 + m < M && r0 + r < job.rank ? v * job.scale : 0.f;
       const T hi = from_f32<T>(v);
       const float rest = v - to_f32(hi);
       const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
@@ -285,7 +305,7 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
 // ---------------------------------------------------------------------------
 // 16-bit gradients: out = (hi + lo) X, sums over the tokens
 // ---------------------------------------------------------------------------
-constexpr int kMxOuterCols = 128;   // columns of X of a CTA, 16 per warp
+constexpr int kMxOuterCols = 128;   // columns of X of a CTA, 32 per warp
 constexpr int kMxOuterTokens = 32;  // tokens of a step
 constexpr int kMxOuterRows = 64;    // rows of the result of a CTA (groups of 16)
 constexpr int kMxOuterStages = 4;
@@ -305,16 +325,12 @@ struct MxOuterJob {
   float* sums;      // [splits][cols] column sums of X, or null
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
-// Eight warps: 16 columns each, all rows.  X and the rows of (hi, lo) come through
+// Four warps: 32 columns each, all rows.  X and the rows of (hi, lo) come through
 // a ring of shared memory steps (32 tokens x 128 columns; 16-byte chunks permuted
 // within a row of X so that the transposing loads of eight tokens two apart are
 // free of conflicts).
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int M,
                      int M_pad) {
   constexpr bool HALF = std::is_same<T, __half>::value;
@@ -332,34 +348,52 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int c0 = ct * kMxOuterCols, row0 = rt * kMxOuterRows;
   const int rows = min(kMxOuterRows, job.rows - row0), groups = rows / 16;
-  const T* turned = job.turned + (int64_t)row0 * M_pad;
-  const int64_t lo_off = (int64_t)job.rows * M_pad;
-
-  auto fetch = [&](int step) {
-    if (step < s1) {
-      const uint32_t base = smem_u32(mx_smem) + (step % kMxOuterStages) * kMxOuterStage;
+  // what this thread fetches of a step: a chunk of X of four tokens, and a chunk of
+  // up to two rows of both parts
+  const int tok = threadIdx.x >> 4, chunk = threadIdx.x & 15;  // tokens tok + 8 u
+  const int left = min(8, job.cols - (c0 + 8 * chunk));        // elements of the chunk inside
+  const int bytes = left > 0 ? 2 * left : 0;
+  const T* xp = job.X + (int64_t)(s0 * kMxOuterTokens + tok) * job.ld + (left > 0 ? c0 + 8 * chunk : 0);
+  const int64_t x_eight = 8 * job.ld;
+  uint32_t x_at[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = threadIdx.x + 256 * u, tok = k >> 4, chunk = k & 15;
-        const int m = step * kMxOuterTokens + tok, c = c0 + 8 * chunk;
-        const int left = m < M ? min(8, job.cols - c) : 0;  // elements of the chunk inside
-        const int f = (tok & 1) | ((tok >> 3) & 3) << 1;
-        cp_async16(base + tok * 256 + ((chunk ^ f) << 4), left > 0 ? job.X + (int64_t)m * job.ld + c : job.X,
-                   left > 0 ? 2 * left : 0);
+  for (int u = 0; u < 4; ++u) x_at[u] = (tok + 8 * u) * 256 + ((chunk ^ ((tok & 1) | u << 1)) << 4);
+  const int ar = threadIdx.x >> 2;  // rows ar and ar + 32
+  const T* ap = job.turned + (int64_t)(row0 + min(ar, rows - 1)) * M_pad + s0 * kMxOuterTokens + 8 * (threadIdx.x & 3);
+  const int64_t lo_off = (int64_t)job.rows * M_pad, row32 = 32 * (int64_t)M_pad;
+  const uint32_t a_at = kMxOuterXBytes + ar * 64 + ((threadIdx.x & 3) << 4);
+  int m_next = s0 * kMxOuterTokens + tok;
+  const int m_end = s1 * kMxOuterTokens;  // (tok < 8: a step begins before it or not at all)
+  MxRing in, out;
+  auto fetch = [&]() {
+    if (m_next < m_end) {
+      const uint32_t base = smem_u32(mx_smem) + in.at * kMxOuterStage;
+      const T* x = xp;
+#pragma unroll
+      for (int u = 0; u < 4; ++u, x += x_eight) {
+        const bool here = m_next + 8 * u < M;
+        cp_async16(base + x_at[u], here ? x : job.X, here ? bytes : 0);
       }
-      for (int k = threadIdx.x; k < 8 * rows; k += 256) {  // [part][row][4 chunks]
-        const int part = k >= 4 * rows ? 1 : 0, r = (k - part * 4 * rows) >> 2, chunk = k & 3;
-        cp_async16(base + kMxOuterXBytes + (part * kMxOuterRows + r) * 64 + (chunk << 4),
-                   turned + part * lo_off + (int64_t)r * M_pad + step * kMxOuterTokens + 8 * chunk, 16);
+      if (ar < rows) {
+        cp_async16(base + a_at, ap, 16);
+        cp_async16(base + a_at + kMxOuterRows * 64, ap + lo_off, 16);
       }
+      if (ar + 32 < rows) {
+        cp_async16(base + a_at + 32 * 64, ap + row32, 16);
+        cp_async16(base + a_at + (kMxOuterRows + 32) * 64, ap + row32 + lo_off, 16);
+      }
+      xp += 4 * x_eight;
+      ap += kMxOuterTokens;
+      m_next += kMxOuterTokens;
+      in.next(kMxOuterStages);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int k = 0; k < kMxOuterStages - 1; ++k) fetch(s0 + k);
+  for (int k = 0; k < kMxOuterStages - 1; ++k) fetch();
 
-  float acc[4][2][4] = {};  // [row group][8 columns][fragment]
-  float sum[2] = {0.f, 0.f};
+  float acc[4][4][4] = {};  // [row group][8 columns][fragment]
+  float sum[4] = {};
   const bool sums = job.sums && rt == 0;
   // this lane's row of the transposing loads: matrix lane / 8 (pair j), row lane % 8
   const int mtok = 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
@@ -367,22 +401,24 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   for (int step = s0; step < s1; ++step) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kMxOuterStages - 2) : "memory");
     __syncthreads();
-    fetch(step + kMxOuterStages - 1);  // into the stage of step - 1: every warp is past it
-    const uint32_t base = smem_u32(mx_smem) + (step % kMxOuterStages) * kMxOuterStage;
-    uint32_t b[2][4];
+    fetch();  // into the stage of the step before: every warp is past it
+    const uint32_t base = smem_u32(mx_smem) + out.at * kMxOuterStage;
+    out.next(kMxOuterStages);
+    uint32_t b[4][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 4; ++n)
       asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                    : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
-                   : "r"(base + mtok * 256 + (((2 * warp + n) ^ mf) << 4))
+                   : "r"(base + mtok * 256 + (((4 * warp + n) ^ mf) << 4))
                    : "memory");
     if (sums) {  // the lane holds eight tokens of column g
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const T* e = reinterpret_cast<const T*>(&b[n][j]);
-          sum[n] += to_f32(e[0]) + to_f32(e[1]);
+          sum[n] += HALF ? __low2float(*reinterpret_cast<const __half2*>(&b[n][j])) +
+                               __high2float(*reinterpret_cast<const __half2*>(&b[n][j]))
+                         : __uint_as_float(b[n][j] << 16) + __uint_as_float(b[n][j] & 0xFFFF0000u);
         }
     }
 #pragma unroll
@@ -393,7 +429,7 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
           const uint32_t at = base + kMxOuterXBytes + (part * kMxOuterRows + 16 * r + g) * 64 + t * 16;
           const uint4 l = lds128(at), h = lds128(at + 8 * 64);
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
+          for (int n = 0; n < 4; ++n) {
             mx_mma<HALF>(acc[r][n], l.x, h.x, l.y, h.y, b[n][0], b[n][1]);
             mx_mma<HALF>(acc[r][n], l.z, h.z, l.w, h.w, b[n][2], b[n][3]);
           }
@@ -404,19 +440,19 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   for (int r = 0; r < 4; ++r)
     if (r < groups)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int row = row0 + 16 * r + g + 8 * (q >> 1), c = c0 + 16 * warp + 8 * n + 2 * t + (q & 1);
+          const int row = row0 + 16 * r + g + 8 * (q >> 1), c = c0 + 32 * warp + 8 * n + 2 * t + (q & 1);
           if (c < job.cols) job.partial[((int64_t)split * job.rows + row) * job.cols + c] = acc[r][n][q];
         }
   if (sums)
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < 4; ++n) {
       float v = sum[n];
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       v += __shfl_xor_sync(0xffffffffu, v, 2);
-      const int c = c0 + 16 * warp + 8 * n + g;
+      const int c = c0 + 32 * warp + 8 * n + g;
       if (t == 0 && c < job.cols) job.sums[(int64_t)split * job.cols + c] = v;
     }
 }
