@@ -228,6 +228,13 @@ int ring_stages(size_t budget, size_t fixed, size_t stage, int64_t uses) {
   return (int)std::max<int64_t>(2, std::min(fit, uses));
 }
 
+// Whether a CTA keeps the rows of lora_b of a tile of 64 `wo` outputs in shared memory.
+template <typename T>
+bool stages_b(const MxFewParams<T>& prm, int wo) {
+  return prm.rank > 0 && prm.rank <= kMxSmemRank && prm.rank * sizeof(T) % 16 == 0 && aligned(prm.lora_b, 16) &&
+         mx_b_bytes<T>(prm.rank, wo) <= kMxMostB;
+}
+
 // W warps per tile, G tiles of a CTA at a time; QLIN_ERR_SHAPE where that does not fit.
 template <typename T, int W, int G>
 int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
@@ -235,8 +242,11 @@ int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   MxFewParams<T> prm = base;
   const int ctas = (int)std::min<int64_t>(prm.tiles, sms);
   const int64_t uses = ceil_div(prm.kb, W) * ceil_div(prm.tiles, (int64_t)ctas * G);
-  prm.ring = ring_stages(kMostSmem, mx_one_smem<T, W, G>(prm.M, prm.K_g, 0, prm.rank), G * (W * kMxRecord + 16), uses);
-  const size_t smem = mx_one_smem<T, W, G>(prm.M, prm.K_g, prm.ring, prm.rank);
+  prm.stage_b = stages_b(prm, 1);
+  const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, 1) : 0;
+  prm.ring = ring_stages(kMostSmem, mx_one_smem<T, W, G>(prm.M, prm.K_g, 0, prm.rank, b), G * (W * kMxRecord + 16),
+                         uses);
+  const size_t smem = mx_one_smem<T, W, G>(prm.M, prm.K_g, prm.ring, prm.rank, b);
   if (smem > kMostSmem) return QLIN_ERR_SHAPE;
   if (allow_smem(qlin_mx_one_kernel<T, W, G>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
   return launch_dependent(qlin_mx_one_kernel<T, W, G>, ctas, 32 * (W + 1) * G, smem, s, prm);
@@ -251,8 +261,10 @@ int launch_many(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   const int64_t total = ceil_div(prm.tiles, WO) * ceil_div(prm.M, Cfg::kC);
   const int ctas = (int)std::min<int64_t>(total, sms);
   const int64_t uses = ceil_div(prm.kb, Cfg::kWK) * ceil_div(total, ctas);
-  prm.ring = ring_stages(kMostSmem, mx_many_smem<T, NT, WO>(0, prm.rank), Cfg::kStage + 16, uses);
-  const size_t smem = mx_many_smem<T, NT, WO>(prm.ring, prm.rank);
+  prm.stage_b = stages_b(prm, WO);
+  const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
+  prm.ring = ring_stages(kMostSmem, mx_many_smem<T, NT, WO>(0, prm.rank, b), Cfg::kStage + 16, uses);
+  const size_t smem = mx_many_smem<T, NT, WO>(prm.ring, prm.rank, b);
   if (smem > kMostSmem) return QLIN_ERR_SHAPE;
   return launch_dependent(qlin_mx_many_kernel<T, NT, WO>, ctas, kMxThreads, smem, s, prm);
 }
@@ -304,8 +316,12 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
     return launch_one<T, 16, 1>(prm, sms, s);
   }
   if (C == 8) return launch_many<T, 1, 1>(prm, sms, s);
-  if (C == 16) return launch_many<T, 2, 2>(prm, sms, s);
-  return launch_many<T, 4, 4>(prm, sms, s);
+  // side by side, tiles of a CTA share the B words (two or four of them); alone,
+  // there are more CTAs (fp32's B words are too long for that)
+  if constexpr (sizeof(T) == 2)
+    if (prm.tiles * ceil_div(M, C) <= 2 * sms)
+      return C == 16 ? launch_many<T, 2, 1>(prm, sms, s) : launch_many<T, 4, 1>(prm, sms, s);
+  return C == 16 ? launch_many<T, 2, 2>(prm, sms, s) : launch_many<T, 4, 4>(prm, sms, s);
 }
 
 // ---------------------------------------------------------------------------

@@ -143,6 +143,10 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 // A lane's share of a record: the A operands (weights) of the block's two k16
 // steps for all four components.
 template <bool HALF>
@@ -283,15 +287,40 @@ struct MxFewParams {
   int tiles;                // tiles of 16 output quaternions
   int ring;                 // stages of the ring
   int vec;                  // whole quaternions of x are aligned (one or two tokens: x takes bulk copies)
+  int stage_b;              // rows of lora_b come through shared memory
   int after_prologue;       // t comes from the previous kernel, which waited for everything before it
 };
 
+// Rows of lora_b in shared memory: padded by 16 bytes, so that neighbouring rows'
+// pieces lie in different banks; two buffers for a tile of 64 * WO outputs.
+template <typename T>
+__host__ __device__ constexpr int mx_b_row(int rank) { return rank * (int)sizeof(T) + 16; }
+template <typename T>
+__host__ __device__ constexpr int mx_b_bytes(int rank, int wo) { return 2 * 64 * wo * mx_b_row<T>(rank); }
+constexpr int kMxMostB = 24 * 1024;  // of the two buffers
+
+// Fetches the rows of lora_b of a tile's outputs n0 .. n0 + 64 WO - 1 (the last one's
+// again past the end), by `threads` threads.
+template <typename T>
+__device__ __forceinline__ void mx_fetch_b(const MxFewParams<T>& prm, uint8_t* dst, int64_t n0, int rows, int thread,
+                                           int threads) {
+  const int chunks = prm.rank * (int)sizeof(T) / 16;
+  for (int k = thread; k < rows * chunks; k += threads) {
+    const int row = k / chunks, c = k - row * chunks;
+    const int64_t n = min(n0 + row, 4 * (int64_t)prm.N_g - 1);
+    cp_async16(smem_u32(dst) + row * mx_b_row<T>(prm.rank) + 16 * c,
+               reinterpret_cast<const uint8_t*>(prm.lora_b + n * prm.rank) + 16 * c, 16);
+  }
+}
+
 // Sums the K split of a tile's outputs (o of 16, a) for a token from the
 // reduction rows, adds adapter and bias, and stores.  WARPS rows of partial
-// sums per token starting at red (rows of kMxRedRow floats, token-major).
+// sums per token starting at red (rows of kMxRedRow floats, token-major); `b`: the
+// output's row of lora_b in shared memory, or null.
 template <int WARPS, typename T>
-__device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float* red, int warp_stride, int tok_local, int col, int64_t m, int64_t n0, float factor,
-                                          const float* ts) {
+__device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float* red, int warp_stride, int tok_local,
+                                          int col, int64_t m, int64_t n0, float factor, const float* ts,
+                                          const uint8_t* b_row) {
   const int64_t n = n0 + col;
   if (m >= prm.M || n >= 4 * (int64_t)prm.N_g) return;
   float v = 0.f;
@@ -299,18 +328,18 @@ __device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float
   for (int w = 0; w < WARPS; ++w) v += red[w * warp_stride + tok_local * kMxRedRow + col];
   v *= factor;
   if (prm.rank > 0) {
-    const T* b = prm.lora_b + n * prm.rank;
     float l = 0.f;
-    int r = 0;
-    if (sizeof(T) == 2 && prm.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(prm.lora_b) & 15) == 0) {
-      for (; r < prm.rank; r += 8) {
-        const uint4 q = ld_cg_v4(b + r);
+    if (b_row) {
+      constexpr int V = 16 / (int)sizeof(T);
+      for (int r = 0; r < prm.rank; r += V) {
+        const uint4 q = *reinterpret_cast<const uint4*>(b_row + r * (int)sizeof(T));
         const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) l = fmaf(ts[r + j], to_f32(e[j]), l);
+        for (int j = 0; j < V; ++j) l = fmaf(ts[r + j], to_f32(e[j]), l);
       }
     } else {
-      for (; r < prm.rank; ++r) l = fmaf(ts[r], to_f32(b[r]), l);
+      const T* b = prm.lora_b + n * prm.rank;
+      for (int r = 0; r < prm.rank; ++r) l = fmaf(ts[r], to_f32(b[r]), l);
     }
     v += l;
   }
@@ -337,9 +366,9 @@ template <typename T>
 __host__ __device__ constexpr size_t mx_one_x_bytes(int kb) { return (size_t)kb * MxOperand<T>::kParts * 1024; }
 
 template <typename T, int W, int G>
-constexpr size_t mx_one_smem(int M, int K_g, int ring, int rank) {
+constexpr size_t mx_one_smem(int M, int K_g, int ring, int rank, int b_bytes) {
   return (size_t)G * ring * (W * kMxRecord + 16) + mx_one_x_bytes<T>((K_g + kMxBlock - 1) / kMxBlock) +
-         M * mx_one_raw_bytes<T>(K_g) + G * 2 * W * 2 * kMxRedRow * 4 + 2 * mx_t_rank(rank) * 4 + 64;
+         M * mx_one_raw_bytes<T>(K_g) + G * (2 * W * 2 * kMxRedRow * 4 + b_bytes) + 2 * mx_t_rank(rank) * 4 + 64;
 }
 
 // Position in a ring of `stages` stages.
@@ -368,7 +397,9 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
   uint8_t* xs = mx_smem + G * S * kStage;
   uint8_t* raw = xs + mx_one_x_bytes<T>(kb);
   const size_t raw_row = mx_one_raw_bytes<T>(prm.K_g);
-  float* red_all = reinterpret_cast<float*>(raw + prm.M * raw_row);
+  const int b_bytes = prm.stage_b ? mx_b_bytes<T>(prm.rank, 1) : 0;
+  uint8_t* bs_all = raw + prm.M * raw_row;
+  float* red_all = reinterpret_cast<float*>(bs_all + G * b_bytes);
   float* ts = red_all + G * 2 * W * 2 * kMxRedRow;
   uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + 2 * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
   uint64_t* x_full = bars + 2 * G * S;
@@ -508,6 +539,8 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
   MxRing r;
   int buffer = 0;
   for (int tile = id; tile < prm.tiles; tile += stride) {
+    uint8_t* bs = bs_all + grp * b_bytes + buffer * (b_bytes / 2);
+    if (prm.stage_b) mx_fetch_b<T>(prm, bs, (int64_t)tile * 4 * kMxRows, 64, gthread, 32 * W);
     float acc[4] = {};
     for (int b = gwarp; b < nst * W; b += W) {
       if (ok) ok = mbar_wait(&full[r.at], r.phase);
@@ -551,11 +584,13 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
       // (every group writes the same values)
       for (int k = gthread; k < prm.M * mx_t_rank(prm.rank); k += 32 * W) ts[k] = __ldcg(prm.t + k);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(32 * W) : "memory");
     if (gthread < 64 * prm.M) {
       const int tok = gthread >> 6, col = gthread & 63;
       mx_finish<W>(prm, rows, 2 * kMxRedRow, tok, col, tok, (int64_t)tile * 4 * kMxRows,
-                   tok ? factor[1] : factor[0], (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank);
+                   tok ? factor[1] : factor[0], (prm.rank <= kMxSmemRank ? ts : prm.t) + tok * prm.rank,
+                   prm.stage_b ? bs + col * mx_b_row<T>(prm.rank) : nullptr);
     }
     buffer ^= 1;
   }
@@ -643,14 +678,14 @@ struct MxManyCfg {
   static constexpr int kXBlock = kP * 4 * kC * 64;       // B words of a block
   static constexpr int kStage = kWK * (WO * kMxRecord + kXBlock);
   static constexpr int kRed = kMxWarps * 8 * kMxRedRow * 4;  // partial sums of eight tokens
-  static constexpr int kFixed = 2 * kRed + 64;
+  static constexpr int kFixed = 2 * kRed + 64;  // without t and rows of lora_b
   static_assert(kStage % 16 == 0, "copies of whole 16-byte pieces");
 };
 
 template <typename T, int NT, int WO>
-constexpr size_t mx_many_smem(int ring, int rank) {
+constexpr size_t mx_many_smem(int ring, int rank, int b_bytes) {
   using Cfg = MxManyCfg<T, NT, WO>;
-  return (size_t)ring * (Cfg::kStage + 16) + Cfg::kFixed + (size_t)Cfg::kC * mx_t_rank(rank) * 4;
+  return (size_t)ring * (Cfg::kStage + 16) + Cfg::kFixed + (size_t)Cfg::kC * mx_t_rank(rank) * 4 + b_bytes;
 }
 
 template <typename T, int NT, int WO>
@@ -661,7 +696,9 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
   constexpr int P = Cfg::kP, C = Cfg::kC, WK = Cfg::kWK;
   extern __shared__ __align__(128) uint8_t mx_smem[];
   const int S = prm.ring, kb = prm.kb;
-  float* red = reinterpret_cast<float*>(mx_smem + S * Cfg::kStage);
+  const int b_bytes = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
+  uint8_t* bs_both = mx_smem + S * Cfg::kStage;
+  float* red = reinterpret_cast<float*>(bs_both + b_bytes);
   float* ts = red + 2 * kMxWarps * 8 * kMxRedRow;
   uint64_t* full = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ts + C * mx_t_rank(prm.rank)) + 7) & ~uintptr_t(7));
   uint64_t* empty = full + S;
@@ -728,6 +765,8 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
   for (int j = 0; j < my_tiles; ++j) {
     const int id = (int)blockIdx.x + j * (int)gridDim.x;
     const int64_t vt = id / groups, tile0 = (int64_t)(id - (int)vt * groups) * WO;
+    uint8_t* bs = bs_both + (j & 1) * (b_bytes / 2);
+    if (prm.stage_b) mx_fetch_b<T>(prm, bs, tile0 * 4 * kMxRows, 64 * WO, threadIdx.x, 32 * kMxWarps);
     float acc[NT][4][4] = {};
     for (int st = 0; st < nst; ++st) {
       const int s = r.at;
@@ -783,13 +822,15 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           mine[(2 * t + (k & 1)) * kMxRedRow + 4 * (g + 8 * (k >> 1)) + a] = acc[nt][a][k];
+      asm volatile("cp.async.wait_all;" ::: "memory");
       asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
       for (int k = threadIdx.x; k < 8 * 64 * WO; k += 32 * kMxWarps) {
         const int col = k & 63, w = (k >> 6) % WO, tok = (k >> 6) / WO;
         const int64_t m = vt * C + nt * 8 + tok;
         mx_finish<WK>(prm, buf + w * WK * 8 * kMxRedRow, 8 * kMxRedRow, tok, col, m,
                      (tile0 + w) * 4 * kMxRows, factor,
-                     (prm.rank <= kMxSmemRank ? ts : prm.t + vt * C * prm.rank) + (nt * 8 + tok) * prm.rank);
+                     (prm.rank <= kMxSmemRank ? ts : prm.t + vt * C * prm.rank) + (nt * 8 + tok) * prm.rank,
+                     prm.stage_b ? bs + (64 * w + col) * mx_b_row<T>(prm.rank) : nullptr);
       }
     }
   }

@@ -200,10 +200,6 @@ struct MxDownJob {
   int blocks;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 constexpr int kMxDownStages = 4;
 constexpr int kMxDownPieces = 6;  // 16-byte pieces of a lane and stage: two tokens, four ranks
 constexpr int kMxDownSmem = kMxDownStages * kMxDownPieces * 256 * 16;
