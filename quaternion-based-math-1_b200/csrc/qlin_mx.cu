@@ -129,16 +129,28 @@ int outer_splits(int64_t M_pad, int64_t cols, int rows) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 222 / std::max<int64_t>(1, tiles)));
 }
 
+// The same for fp32: about two CTAs per SM each, at least 32 tokens.
+int outer32_splits(int64_t M, int64_t cols, int rank) {
+  const int64_t tiles = ceil_div(cols, kMxOuter32Cols) * ceil_div(rank, kMxOuter32Ranks);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(M / 32, 296 / std::max<int64_t>(1, tiles)));
+}
+
 BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   BackwardWs w;
   Carve c;
   if (dtype == QLIN_F32) {
     w.planes = c.take(4 * K_g * N_g * 4);
-    w.at = c.take(4 * K_g * rank * 4);
-    w.bt = c.take(4 * N_g * rank * 4);
-    w.t = c.take(M * rank * 4);
-    w.up = c.take(M * rank * 4);
-    qlin_workspace_size(dtype, M, N_g, K_g, rank, &w.inner_bytes);
+    if (rank > 0) {
+      w.splits0 = outer32_splits(M, 4 * K_g, rank);
+      w.splits1 = outer32_splits(M, 4 * N_g, rank);
+      w.bt = c.take(4 * N_g * rank * 4);
+      w.t = c.take(M * rank * 4);
+      w.up = c.take(M * rank * 4);
+      w.partial0 = c.take((int64_t)w.splits0 * rank * 4 * K_g * 4);
+      w.partial1 = c.take((int64_t)w.splits1 * rank * 4 * N_g * 4);
+      w.sums = c.take((int64_t)w.splits1 * 4 * N_g * 4);
+    }
+    qlin_workspace_size(dtype, M, N_g, K_g, 0, &w.inner_bytes);
     w.inner = c.take((int64_t)w.inner_bytes);
   } else {
     const int64_t K = 4 * K_g, N = 4 * N_g;
@@ -581,15 +593,80 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     if (st != QLIN_OK) return st;
   }
   if (dbias && !sum_with_db)
-    qlin_mx_column_sum_kernel<T><<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(g, ld_g, dbias, M, N);
-  return launched();
+    st = launch_dependent(qlin_mx_column_sum_kernel<T>, (unsigned)ceil_div(N, 32), 256, 0, s, g, ld_g, dbias, M, N);
+  return st != QLIN_OK ? st : launched();
 }
 
-template <typename TP, typename TQ, typename TC>
-void strided_gemm(const TP* P, int64_t pi, int64_t pl, const TQ* Q, int64_t qj, int64_t ql, TC* C, int64_t ld_c,
-                  int64_t I, int64_t J, int64_t L, float alpha, cudaStream_t s) {
-  const dim3 grid((unsigned)ceil_div(I, 32), (unsigned)ceil_div(J, 32));
-  qlin_mx_strided_gemm_kernel<TP, TQ, TC><<<grid, 256, 0, s>>>(P, pi, pl, Q, qj, ql, C, ld_c, I, J, L, alpha);
+// Gradients, fp32: the adjoint's components through qlin_forward_ex, the adapter on
+// the CUDA cores.
+int run_backward32(const float* g, int64_t ld_g, const float* x, int64_t ld_x, const void* mx, const float* a,
+                   const float* b, int rank, float scale, float* dx, int64_t ld_dx, float* da, float* db, float* dbias,
+                   int64_t M, int64_t K_g, int64_t N_g, uint8_t* ws, const BackwardWs& w, int sms, cudaStream_t s) {
+  const int64_t K = 4 * K_g, N = 4 * N_g;
+  float* bt = reinterpret_cast<float*>(ws + w.bt);
+  float* t = reinterpret_cast<float*>(ws + w.t);
+  float* up = reinterpret_cast<float*>(ws + w.up);
+  int st = QLIN_OK;
+  auto down = [&](const float* in, int64_t ld, int64_t groups, const float* rows, float* out) {
+    return launch_dependent(qlin_mx_prologue_kernel<float>, (unsigned)(rank * ceil_div(M, kMxDownTokens)), 256, 0, s,
+                            in, ld, (int)M, (int)groups, 1, 8, (int)(aligned(in, 16) && ld % 4 == 0),
+                            static_cast<uint8_t*>(nullptr), 0, (int64_t)0, rows, (int)aligned(rows, 16), rank, scale,
+                            out);
+  };
+  if (rank * ceil_div(M, kMxDownTokens) > INT32_MAX) return QLIN_ERR_SHAPE;
+  if (rank > 0 && (dx || da)) {
+    st = launch_dependent(qlin_mx_turn_kernel<float>, (unsigned)ceil_div(rank * N, 256), 256, 0, s, b, bt, N,
+                          (int64_t)rank);
+    if (st == QLIN_OK) st = down(g, ld_g, N_g, bt, up);
+  }
+  if (st == QLIN_OK && db) st = down(x, ld_x, K_g, a, t);
+  if (st != QLIN_OK) return st;
+  if (dx) {
+    const MxPlanes<float> p = planes_at<float>(ws + w.planes, K_g, N_g);
+    const int64_t steps = ceil_div(N_g, 64) * ceil_div(K_g, kMxBlock);
+    st = launch_dependent(qlin_mx_adjoint_kernel<float>, (unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s,
+                          static_cast<const uint8_t*>(mx), p, N_g, (int)K_g, (int)N_g);
+    if (st != QLIN_OK) return st;
+    st = qlin_forward_ex(QLIN_F32, g, ld_g, p.w[0], p.w[1], p.w[2], p.w[3], N_g, nullptr, nullptr, nullptr, 0, 0.f, dx,
+                         ld_dx, M, N_g, K_g, ws + w.inner, w.inner_bytes, QLIN_ALGO_AUTO, 0, s);
+    if (st != QLIN_OK) return st;
+    if (rank > 0) {
+      const dim3 grid((unsigned)ceil_div(K, 256), (unsigned)ceil_div(M, 8));
+      if (grid.y > 65535) return QLIN_ERR_SHAPE;
+      qlin_mx_add_adapter32_kernel<<<grid, 256, 0, s>>>(up, a, rank, dx, ld_dx, M, K);
+    }
+  }
+  const bool sum_with_db = db && dbias;
+  if (da || db) {
+    MxOuterJob<float> o0{}, o1{};
+    auto job = [&](MxOuterJob<float>& o, const float* rows, const float* X, int64_t ld, int64_t cols, int splits,
+                   size_t partial) {
+      o.turned = rows;
+      o.X = X;
+      o.ld = ld;
+      o.cols = (int)cols;
+      o.rows = rank;
+      o.col_tiles = (int)ceil_div(cols, kMxOuter32Cols);
+      o.row_tiles = (int)ceil_div(rank, kMxOuter32Ranks);
+      o.splits = splits;
+      o.blocks = o.col_tiles * o.row_tiles * splits;
+      o.partial = reinterpret_cast<float*>(ws + partial);
+    };
+    if (da) job(o0, up, x, ld_x, K, w.splits0, w.partial0);
+    if (db) job(o1, t, g, ld_g, N, w.splits1, w.partial1);
+    if (sum_with_db) o1.sums = reinterpret_cast<float*>(ws + w.sums);
+    st = launch_dependent(qlin_mx_outer32_kernel, (unsigned)(o0.blocks + o1.blocks), kMxOuter32Cols, 0, s, o0, o1,
+                          (int)M);
+    if (st != QLIN_OK) return st;
+    const int64_t blocks0 = da ? ceil_div(rank * K, 256) : 0;
+    const int64_t blocks1 = db ? ceil_div((rank + (sum_with_db ? 1 : 0)) * N, 256) : 0;
+    st = launch_dependent(qlin_mx_outer_finish_kernel<float>, (unsigned)(blocks0 + blocks1), 256, 0, s, o0, o1, rank,
+                          da, db, sum_with_db ? dbias : nullptr, blocks0);
+    if (st != QLIN_OK) return st;
+  }
+  if (dbias && !sum_with_db)
+    st = launch_dependent(qlin_mx_column_sum_kernel<float>, (unsigned)ceil_div(N, 32), 256, 0, s, g, ld_g, dbias, M, N);
+  return st != QLIN_OK ? st : launched();
 }
 
 template <int CAP>
@@ -779,40 +856,10 @@ int qlin_mx_backward(int dtype, const void* gy, int64_t ld_g, const void* x, int
     if constexpr (sizeof(T) == 2)
       return run_backward<T>(g, ld_g, xt, ld_x, mx, a, b, rank, lora_scale, static_cast<T*>(dx), ld_dx,
                              static_cast<T*>(da), static_cast<T*>(db), static_cast<T*>(dbias), M, K_g, N_g, ws, w, s);
-    else {
-    T* at = reinterpret_cast<T*>(ws + w.at);
-    T* bt = reinterpret_cast<T*>(ws + w.bt);
-    if (dx) {
-      const MxPlanes<T> p = planes_at<T>(ws + w.planes, K_g, N_g);
-      const int64_t steps = ceil_div(N_g, 64) * ceil_div(K_g, kMxBlock);
-      qlin_mx_adjoint_kernel<T><<<(unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s>>>(
-          static_cast<const uint8_t*>(mx), p, N_g, (int)K_g, (int)N_g);
-      if (rank > 0) {
-        const int64_t a_blocks = ceil_div(rank * K, 256);
-        const int e = launch_dependent(qlin_mx_turn_kernel<T>, (unsigned)(a_blocks + ceil_div(rank * N, 256)), 256, 0,
-                                       s, a, at, (int64_t)rank, K, b, bt, N, (int64_t)rank, a_blocks);
-        if (e != QLIN_OK) return e;
-      }
-      if (launched() != QLIN_OK) return (int)QLIN_ERR_LAUNCH;
-      const int e = qlin_forward_ex(dtype, gy, ld_g, p.w[0], p.w[1], p.w[2], p.w[3], N_g, nullptr, bt, at, rank,
-                                    lora_scale, dx, ld_dx, M, N_g, K_g, ws + w.inner, w.inner_bytes, QLIN_ALGO_AUTO,
-                                    0, stream);
-      if (e != QLIN_OK) return e;
-    }
-    float* t = reinterpret_cast<float*>(ws + w.t);
-    float* up = reinterpret_cast<float*>(ws + w.up);
-    if (da) {
-      strided_gemm<T, T, float>(g, ld_g, 1, b, 1, rank, up, rank, M, rank, N, lora_scale, s);
-      strided_gemm<float, T, T>(up, 1, rank, xt, 1, ld_x, static_cast<T*>(da), K, rank, K, M, 1.f, s);
-    }
-    if (db) {
-      strided_gemm<T, T, float>(xt, ld_x, 1, a, K, 1, t, rank, M, rank, K, lora_scale, s);
-      strided_gemm<T, float, T>(g, 1, ld_g, t, 1, rank, static_cast<T*>(db), rank, N, rank, M, 1.f, s);
-    }
-    if (dbias)
-      qlin_mx_column_sum_kernel<T><<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(g, ld_g, static_cast<T*>(dbias), M, N);
-    return launched();
-    }
+    else
+      return run_backward32(g, ld_g, xt, ld_x, mx, a, b, rank, lora_scale, static_cast<T*>(dx), ld_dx,
+                            static_cast<T*>(da), static_cast<T*>(db), static_cast<T*>(dbias), M, K_g, N_g, ws, w, sms,
+                            s);
   });
 }
 

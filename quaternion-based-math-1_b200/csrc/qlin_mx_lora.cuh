@@ -17,51 +17,13 @@
 
 namespace qlin {
 
-// ---------------------------------------------------------------------------
-// fp32: plain products
-// ---------------------------------------------------------------------------
-// C[i, j] = alpha * sum_l P[i pi + l pl] * Q[j qj + l ql], fp32 sums; C is
-// row-major with leading dimension ld_c.  32 x 32 tile, 32 terms per step.
-template <typename TP, typename TQ, typename TC>
-__global__ void __launch_bounds__(256)
-qlin_mx_strided_gemm_kernel(const TP* __restrict__ P, int64_t pi, int64_t pl, const TQ* __restrict__ Q, int64_t qj,
-                            int64_t ql, TC* __restrict__ C, int64_t ld_c, int64_t I, int64_t J, int64_t L,
-                            float alpha) {
-  __shared__ float ps[32][33], qs[32][33];
-  const int64_t i0 = (int64_t)blockIdx.x * 32, j0 = (int64_t)blockIdx.y * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  float acc[4] = {};
-  for (int64_t l0 = 0; l0 < L; l0 += 32) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      // lanes along the contiguous direction of each operand
-      const int s = ty + 8 * u;
-      const int pr = pl == 1 ? s : tx, pc = pl == 1 ? tx : s;
-      const int qr = ql == 1 ? s : tx, qc = ql == 1 ? tx : s;
-      ps[pr][pc] = i0 + pr < I && l0 + pc < L ? to_f32(P[(i0 + pr) * pi + (l0 + pc) * pl]) : 0.f;
-      qs[qr][qc] = j0 + qr < J && l0 + qc < L ? to_f32(Q[(j0 + qr) * qj + (l0 + qc) * ql]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int l = 0; l < 32; ++l) {
-      const float q = qs[tx][l];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) acc[u] = fmaf(ps[ty + 8 * u][l], q, acc[u]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = i0 + ty + 8 * u, j = j0 + tx;
-    if (i < I && j < J) C[i * ld_c + j] = from_f32<TC>(alpha * acc[u]);
-  }
-}
-
 // out[n] = sum_m g[m, n]
 template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_column_sum_kernel(const T* __restrict__ g, int64_t ld_g, T* __restrict__ out, int64_t M, int64_t N) {
   __shared__ float part[8][32];
+  pdl_wait_prior();
+  pdl_launch_dependents();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + tx;
   float s = 0.f;
@@ -76,18 +38,15 @@ qlin_mx_column_sum_kernel(const T* __restrict__ g, int64_t ld_g, T* __restrict__
   }
 }
 
-// dst[c][r] = src[r][c] for two matrices.
+// dst[c][r] = src[r][c]
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_turn_kernel(const T* __restrict__ a, T* __restrict__ at, int64_t a_rows, int64_t a_cols,
-                    const T* __restrict__ b, T* __restrict__ bt, int64_t b_rows, int64_t b_cols, int64_t a_blocks) {
+qlin_mx_turn_kernel(const T* __restrict__ src, T* __restrict__ dst, int64_t rows, int64_t cols) {
   pdl_wait_prior();
   pdl_launch_dependents();
-  const bool first = (int64_t)blockIdx.x < a_blocks;
-  const int64_t k = ((int64_t)blockIdx.x - (first ? 0 : a_blocks)) * 256 + threadIdx.x;
-  const int64_t rows = first ? a_rows : b_rows, cols = first ? a_cols : b_cols;
+  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
   // consecutive threads write consecutive elements
-  if (k < rows * cols) (first ? at : bt)[k] = (first ? a : b)[(k % rows) * cols + k / rows];
+  if (k < rows * cols) dst[k] = src[(k % rows) * cols + k / rows];
 }
 
 constexpr int kMxTurnRows = 64;  // output quaternions of a step
@@ -311,7 +270,7 @@ constexpr int kMxOuterSmem = kMxOuterStages * kMxOuterStage;
 
 template <typename T>
 struct MxOuterJob {
-  const T* turned;  // [2][rows][M_pad]
+  const T* turned;  // [2][rows][M_pad]; fp32: [M][rows]
   const T* X;       // [M, ld], 16-byte aligned rows
   int64_t ld;
   int cols, rows;   // rows: a multiple of 16
@@ -451,6 +410,89 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
       const int c = c0 + 32 * warp + 8 * n + g;
       if (t == 0 && c < job.cols) job.sums[(int64_t)split * job.cols + c] = v;
     }
+}
+
+// ---------------------------------------------------------------------------
+// fp32: on the CUDA cores
+// ---------------------------------------------------------------------------
+constexpr int kMxOuter32Cols = 128;   // columns of a CTA, one per thread
+constexpr int kMxOuter32Ranks = 32;   // ranks of a CTA, in registers
+constexpr int kMxOuter32Tokens = 32;  // tokens whose t is staged at a time
+
+// partial[split][r][c] = sum_m t[m, r] X[m, c] (and the column sums of X).
+__global__ void __launch_bounds__(kMxOuter32Cols)
+qlin_mx_outer32_kernel(const __grid_constant__ MxOuterJob<float> job0, const __grid_constant__ MxOuterJob<float> job1,
+                       int M) {
+  __shared__ float4 ts[kMxOuter32Tokens][kMxOuter32Ranks / 4];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const bool first = (int)blockIdx.x < job0.blocks;
+  const MxOuterJob<float>& job = first ? job0 : job1;
+  int id = (int)blockIdx.x - (first ? 0 : job0.blocks);
+  const int ct = id % job.col_tiles;
+  id /= job.col_tiles;
+  const int rt = id % job.row_tiles, split = id / job.row_tiles;
+  const int m0 = (int)((int64_t)M * split / job.splits), m1 = (int)((int64_t)M * (split + 1) / job.splits);
+  const int c = ct * kMxOuter32Cols + threadIdx.x, r0 = rt * kMxOuter32Ranks;
+  const bool here = c < job.cols;
+  const float* x = job.X + (here ? c : 0);
+  float4 acc[kMxOuter32Ranks / 4];
+#pragma unroll
+  for (int r = 0; r < kMxOuter32Ranks / 4; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int m = m0; m < m1; m += kMxOuter32Tokens) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < kMxOuter32Tokens * kMxOuter32Ranks; k += kMxOuter32Cols) {
+      const int tok = k / kMxOuter32Ranks, r = r0 + k % kMxOuter32Ranks;
+      reinterpret_cast<float*>(ts)[k] =
+          m + tok < m1 && r < job.rows ? __ldcg(job.turned + (int64_t)(m + tok) * job.rows + r) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u0 = 0; u0 < kMxOuter32Tokens; u0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = m + u0 + u < m1 ? __ldcg(x + (int64_t)(m + u0 + u) * job.ld) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        sum += v[u];
+#pragma unroll
+        for (int r = 0; r < kMxOuter32Ranks / 4; ++r) {
+          const float4 t = ts[u0 + u][r];
+          acc[r].x = fmaf(t.x, v[u], acc[r].x);
+          acc[r].y = fmaf(t.y, v[u], acc[r].y);
+          acc[r].z = fmaf(t.z, v[u], acc[r].z);
+          acc[r].w = fmaf(t.w, v[u], acc[r].w);
+        }
+      }
+    }
+  }
+  if (!here) return;
+#pragma unroll
+  for (int r = 0; r < kMxOuter32Ranks; ++r)
+    if (r0 + r < job.rows)
+      job.partial[((int64_t)split * job.rows + r0 + r) * job.cols + c] = reinterpret_cast<const float*>(acc)[r];
+  if (job.sums && rt == 0) job.sums[(int64_t)split * job.cols + c] = sum;
+}
+
+// dx[m, k] += sum_r up[m, r] A[r, k]
+__global__ void __launch_bounds__(256)
+qlin_mx_add_adapter32_kernel(const float* __restrict__ up, const float* __restrict__ a, int rank,
+                             float* __restrict__ dx, int64_t ld_dx, int64_t M, int64_t K) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, m0 = (int64_t)blockIdx.y * 8;
+  if (k >= K) return;
+  float v[8] = {};
+  for (int r = 0; r < rank; ++r) {
+    const float av = __ldcg(a + (int64_t)r * K + k);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (m0 + u < M) v[u] = fmaf(__ldcg(up + (m0 + u) * rank + r), av, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (m0 + u < M) dx[(m0 + u) * ld_dx + k] += v[u];
 }
 
 // Adds the splits up: da [rank, cols] from job0's; db [cols, rank] and dbias
