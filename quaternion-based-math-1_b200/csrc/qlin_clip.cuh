@@ -13,21 +13,22 @@
 // what the first has left in L2 (sets of up to about 100 MB are read from
 // HBM once).
 //
-// Squares are summed in fp32 within a piece and thread (at most 16 terms) and
-// in fp64 from there on, in an order that depends only on the sizes: the same
-// gradients give the same bits.  A thread whose fp32 sum overflows sums its
-// piece again in fp64.
+// Squares are summed in fp32 within a piece and thread (8 terms) and in fp64 from
+// there on, in an order that depends only on the sizes: the same gradients give
+// the same bits.  A thread whose fp32 sum overflows sums its piece again in fp64.
 #pragma once
 
 #include "qlin_common.cuh"
 
 namespace qlin {
 
-constexpr int kClipThreads = 512;
-constexpr int kClipPiece = kClipThreads * 16;  // elements
+constexpr int kClipThreads = 256;
+constexpr int kClipEach = 8;                          // elements of a thread
+constexpr int kClipPiece = kClipThreads * kClipEach;  // elements
+constexpr int kClipBatch = 4;                         // whole pieces of a tensor whose loads go out together
 constexpr int kClipTensors = 512;              // most table entries of a launch
 constexpr int kClipFewTensors = 64;            // entries of the small table (less to hand to a launch)
-constexpr int kClipCtasPerSm = 4;
+constexpr int kClipCtasPerSm = 8;
 
 template <int CAP>
 struct ClipTable {
@@ -38,17 +39,20 @@ struct ClipTable {
   int count;
 };
 
+// A thread's elements of a whole, aligned piece: 16-byte pieces apart by
+// kClipThreads * 16 bytes.
 template <typename T>
-__device__ __forceinline__ double clip_piece_sum(const T* at, long long left) {
-  constexpr int V = 16 / (int)sizeof(T);  // elements of a 16-byte load
-  float s = 0.f;
-  if (left >= kClipPiece && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-    uint4 q[16 / V];
+struct ClipLoad {
+  static constexpr int V = 16 / (int)sizeof(T);
+  uint4 q[kClipEach / V];
+  __device__ __forceinline__ void load(const T* piece) {
 #pragma unroll
-    for (int u = 0; u < 16 / V; ++u)
-      q[u] = ld_cg_v4(at + ((long long)u * kClipThreads + threadIdx.x) * V);
+    for (int u = 0; u < kClipEach / V; ++u) q[u] = ld_cg_v4(piece + (u * kClipThreads + threadIdx.x) * V);
+  }
+  __device__ __forceinline__ double squares() const {
+    float s = 0.f;
 #pragma unroll
-    for (int u = 0; u < 16 / V; ++u)
+    for (int u = 0; u < kClipEach / V; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float v = to_f32(reinterpret_cast<const T*>(&q[u])[j]);
@@ -57,7 +61,7 @@ __device__ __forceinline__ double clip_piece_sum(const T* at, long long left) {
     if (s <= 3.0e38f) return (double)s;
     double d = 0.0;
 #pragma unroll
-    for (int u = 0; u < 16 / V; ++u)
+    for (int u = 0; u < kClipEach / V; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const double v = (double)to_f32(reinterpret_cast<const T*>(&q[u])[j]);
@@ -65,8 +69,39 @@ __device__ __forceinline__ double clip_piece_sum(const T* at, long long left) {
       }
     return d;
   }
+  __device__ __forceinline__ void store_scaled(T* piece, float f) {
+#pragma unroll
+    for (int u = 0; u < kClipEach / V; ++u) {
+      T* e = reinterpret_cast<T*>(&q[u]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = from_f32<T>(to_f32(e[j]) * f);
+      *reinterpret_cast<uint4*>(piece + (u * kClipThreads + threadIdx.x) * V) = q[u];
+    }
+  }
+};
+
+// The sum of squares of this thread's elements of `n` consecutive pieces of a
+// tensor, of which `left` elements are there.
+template <typename T>
+__device__ __forceinline__ double clip_sum(const T* at, int n, long long left) {
   double d = 0.0;
-  for (long long k = threadIdx.x; k < min(left, (long long)kClipPiece); k += kClipThreads) {
+  if ((reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    if (n == kClipBatch && left >= (long long)kClipBatch * kClipPiece) {
+      ClipLoad<T> a[kClipBatch];
+#pragma unroll
+      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece);
+#pragma unroll
+      for (int u = 0; u < kClipBatch; ++u) d += a[u].squares();
+      return d;
+    }
+    for (; n > 0 && left >= kClipPiece; --n, left -= kClipPiece, at += kClipPiece) {
+      ClipLoad<T> a;
+      a.load(at);
+      d += a.squares();
+    }
+  }
+  const long long rest = min(left, (long long)n * kClipPiece);
+  for (long long k = threadIdx.x; k < rest; k += kClipThreads) {
     const double v = (double)to_f32(at[k]);
     d += v * v;
   }
@@ -74,24 +109,24 @@ __device__ __forceinline__ double clip_piece_sum(const T* at, long long left) {
 }
 
 template <typename T>
-__device__ __forceinline__ void clip_piece_scale(T* at, long long left, float f) {
-  constexpr int V = 16 / (int)sizeof(T);
-  if (left >= kClipPiece && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-    uint4 q[16 / V];
+__device__ __forceinline__ void clip_scale(T* at, int n, long long left, float f) {
+  if ((reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    if (n == kClipBatch && left >= (long long)kClipBatch * kClipPiece) {
+      ClipLoad<T> a[kClipBatch];
 #pragma unroll
-    for (int u = 0; u < 16 / V; ++u)
-      q[u] = ld_cg_v4(at + ((long long)u * kClipThreads + threadIdx.x) * V);
+      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece);
 #pragma unroll
-    for (int u = 0; u < 16 / V; ++u) {
-      T* e = reinterpret_cast<T*>(&q[u]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) e[j] = from_f32<T>(to_f32(e[j]) * f);
-      *reinterpret_cast<uint4*>(at + ((long long)u * kClipThreads + threadIdx.x) * V) = q[u];
+      for (int u = 0; u < kClipBatch; ++u) a[u].store_scaled(at + u * kClipPiece, f);
+      return;
     }
-    return;
+    for (; n > 0 && left >= kClipPiece; --n, left -= kClipPiece, at += kClipPiece) {
+      ClipLoad<T> a;
+      a.load(at);
+      a.store_scaled(at, f);
+    }
   }
-  for (long long k = threadIdx.x; k < min(left, (long long)kClipPiece); k += kClipThreads)
-    at[k] = from_f32<T>(to_f32(at[k]) * f);
+  const long long rest = min(left, (long long)n * kClipPiece);
+  for (long long k = threadIdx.x; k < rest; k += kClipThreads) at[k] = from_f32<T>(to_f32(at[k]) * f);
 }
 
 // The tensor that holds a piece: the last whose first piece is not past it.
@@ -106,7 +141,7 @@ __device__ __forceinline__ int clip_find(const ClipTable<CAP>& tab, long long pi
   return lo;
 }
 
-// Sum of 512 threads' values, the same in every thread (fixed order).
+// Sum of all threads' values, the same in every thread (fixed order).
 __device__ __forceinline__ double clip_block_sum(double v, double* slots) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -131,12 +166,14 @@ qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __rest
   double s = 0.0;
   if (p0 < p1) {
     int k = clip_find(tab, p0);
-    for (long long p = p0; p < p1; ++p) {
+    for (long long p = p0; p < p1;) {
       while (p >= tab.first[k + 1]) ++k;
+      const int n = (int)min((long long)kClipBatch, min(p1, tab.first[k + 1]) - p);
       const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
-      if (tab.type[k] == 0) s += clip_piece_sum(static_cast<const float*>(tab.data[k]) + at, left);
-      else if (tab.type[k] == 1) s += clip_piece_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, left);
-      else s += clip_piece_sum(static_cast<const __half*>(tab.data[k]) + at, left);
+      if (tab.type[k] == 0) s += clip_sum(static_cast<const float*>(tab.data[k]) + at, n, left);
+      else if (tab.type[k] == 1) s += clip_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, n, left);
+      else s += clip_sum(static_cast<const __half*>(tab.data[k]) + at, n, left);
+      p += n;
     }
   }
   s = clip_block_sum(s, slots);
@@ -164,12 +201,14 @@ qlin_grad_scale_kernel(const __grid_constant__ ClipTable<CAP> tab, const double*
   const long long p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
   if (p0 >= p1) return;
   int k = clip_find(tab, p1 - 1);
-  for (long long p = p1 - 1; p >= p0; --p) {
-    while (p < tab.first[k]) --k;
+  for (long long p = p1; p > p0;) {  // backwards
+    while (p - 1 < tab.first[k]) --k;
+    const int n = (int)min((long long)kClipBatch, p - max(p0, tab.first[k]));
+    p -= n;
     const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
-    if (tab.type[k] == 0) clip_piece_scale(static_cast<float*>(tab.data[k]) + at, left, f);
-    else if (tab.type[k] == 1) clip_piece_scale(static_cast<__nv_bfloat16*>(tab.data[k]) + at, left, f);
-    else clip_piece_scale(static_cast<__half*>(tab.data[k]) + at, left, f);
+    if (tab.type[k] == 0) clip_scale(static_cast<float*>(tab.data[k]) + at, n, left, f);
+    else if (tab.type[k] == 1) clip_scale(static_cast<__nv_bfloat16*>(tab.data[k]) + at, n, left, f);
+    else clip_scale(static_cast<__half*>(tab.data[k]) + at, n, left, f);
   }
 }
 

@@ -55,12 +55,24 @@ __device__ __forceinline__ float mx_scale(uint32_t f) {
   return __uint_as_float(f == 255u ? 0x7FC00000u : (f == 1u ? 0x00400000u : (f - 1u) << 23));
 }
 
-// Bits of a code (sign, magnitude of 3 bits) of element j of a word.
-__device__ __forceinline__ uint32_t mx_place(uint32_t sign, uint32_t mag, int j) {
-  const int k = j & 3;
-  const uint32_t bits = k < 3 ? mag << (6 - 3 * k) | sign << (15 - 3 * k)
-                              : (mag >> 1) << 10 | (mag & 1u) << 13 | sign << 14;
-  return bits << (16 * (j >> 2));
+// Eight quotients (below 8 in magnitude) as a code word: conversions to e2m1 (to
+// nearest, ties to the even code, saturating at 6) pack nibble j = element j,
+// whose bits then move to their places, both halves at once.
+__device__ __forceinline__ uint32_t mx_pack(const float (&q)[8]) {
+  uint32_t n;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(n)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  auto at = [&](int left, uint32_t mask) { return (left >= 0 ? n << left : n >> -left) & (mask | mask << 16); };
+  return at(6, 0x01C0u) | at(12, 0x8000u) |                   // pair 0
+         at(-1, 0x0038u) | at(5, 0x1000u) |                   // pair 1
+         at(-8, 0x0007u) | at(-2, 0x0200u) |                  // pair 2
+         at(-3, 0x0C00u) | at(1, 0x2000u) | at(-1, 0x4000u);  // pair 3
 }
 
 // Powers of two that the compiler cannot see: left shifts written as products
@@ -114,14 +126,8 @@ __device__ __forceinline__ uint32_t mx_exponent(float amax) {
   return field <= 2u ? 0u : field - 2u;
 }
 
-// Code of the magnitude a = |w| / scale, by the midpoints between neighbouring
-// values (a tie goes to the even code).
-__device__ __forceinline__ uint32_t mx_code(float a) {
-  return (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-}
-
 // Eight consecutive elements of a row from `at`, zero from `left` on (vec: the
-// row pieces are 16-byte aligned and whole).
+// row pieces are 16-byte aligned).
 template <typename T>
 __device__ __forceinline__ void mx_load8(const T* at, int64_t left, bool vec, float (&v)[8]) {
   if (vec && left >= 8) {
@@ -149,7 +155,8 @@ struct MxPlanes {
 // Quantisation: a warp makes a record at a time, two rows (four components of
 // four octets each) per step.  A lane holds eight elements of one block, the
 // four lanes of a block share its maximum.  Bound by the bytes read (2 or 4 a
-// weight) and written (0.53): one pass, everything else in registers.
+// weight) and written (0.53): one pass, the loads of four steps at a time in
+// flight, everything else in registers.
 template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_g, uint8_t* __restrict__ mx,
@@ -163,37 +170,34 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
     const int64_t tile = rec / kb, b = rec - tile * kb;
     uint8_t* out = mx + kMxHeader + rec * kMxRecord;
     const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
+    const T* row0 = src.w[p] + (tile * kMxRows + half) * ld + i;
 #pragma unroll
-    for (int step = 0; step < kMxRows / 2; ++step) {
-      const int row = 2 * step + half;
-      const int64_t o = tile * kMxRows + row;
-      float v[8];
-      if (o < N_g && left > 0) {
-        mx_load8(src.w[p] + o * ld + i, left, vec, v);
-      } else {
+    for (int s4 = 0; s4 < kMxRows / 2; s4 += 4) {
+      float v[4][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      for (int u = 0; u < 4; ++u) {
+        const int64_t o = tile * kMxRows + 2 * (s4 + u) + half;
+        mx_load8(row0 + 2 * (s4 + u) * ld, o < N_g ? left : 0, vec, v[u]);
       }
-      // magnitudes as integers: the order of finite values, infinities and NaNs above them
-      uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const bool bad = m >= 0x7F800000u;
-      const uint32_t e = mx_exponent(__uint_as_float(m));
-      uint32_t word = 0;
-      if (!bad) {
-        top = max(top, e + 1u);
+      for (int u = 0; u < 4; ++u) {
+        const int row = 2 * (s4 + u) + half;
+        // magnitudes as integers: the order of finite values, infinities and NaNs above them
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[u][j]) & 0x7FFFFFFFu);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const bool bad = m >= 0x7F800000u;
+        const uint32_t e = mx_exponent(__uint_as_float(m));
         const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - E): E is at most 252
+        float q[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t sign = __float_as_uint(v[j]) >> 31;
-          word |= mx_place(sign, mx_code(fabsf(v[j]) * inv), j);
-        }
+        for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[u][j] * inv;
+        if (!bad) top = max(top, e + 1u);
+        *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
+        if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
       }
-      *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = word;
-      if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
     }
   }
   __shared__ uint32_t tops[8];
@@ -222,23 +226,28 @@ qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst,
     const uint8_t* in = mx + kMxHeader + rec * kMxRecord;
     const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
     if (left <= 0) continue;
+    uint32_t word[kMxRows / 2], f[kMxRows / 2];
 #pragma unroll
     for (int step = 0; step < kMxRows / 2; ++step) {
       const int row = 2 * step + half;
-      const int64_t o = tile * kMxRows + row;
+      word[step] = __ldcg(reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4));
+      f[step] = __ldcg(in + kMxCodeBytes + row * 4 + p);
+    }
+#pragma unroll
+    for (int step = 0; step < kMxRows / 2; ++step) {
+      const int64_t o = tile * kMxRows + 2 * step + half;
       if (o >= N_g) continue;
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4);
-      const float s = mx_scale(in[kMxCodeBytes + row * 4 + p]);
+      const float s = mx_scale(f[step]);
       T* at = dst.w[p] + o * ld + i;
       float c[8];
-      mx_values(word, c);
-      T v[8];
+      mx_values(word[step], c);
+      __align__(16) T v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(c[j] * s);
       if (vec && left >= 8) {
 #pragma unroll
-        for (int c = 0; c < (int)sizeof(T) / 2; ++c)
-          reinterpret_cast<uint4*>(at)[c] = reinterpret_cast<const uint4*>(v)[c];
+        for (int u = 0; u < (int)sizeof(T) / 2; ++u)
+          reinterpret_cast<uint4*>(at)[u] = reinterpret_cast<const uint4*>(v)[u];
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)

@@ -8,6 +8,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
+#include <cmath>
+#include <limits>
 #include <string>
 #include <vector>
 
@@ -208,36 +211,68 @@ std::vector<at::Tensor> mx_backward(const at::Tensor& gy, const at::Tensor& x, c
   return {dx, da, db, dbias};
 }
 
-// Clips dense, non-overlapping tensors in place; returns their global norm (fp32 scalar).
-at::Tensor grad_clip(const std::vector<at::Tensor>& grads, double max_norm) {
-  TORCH_CHECK(!grads.empty(), "no gradients");
+// Clips the gradients of the parameters in place, each gradient once; returns their
+// global norm.  error_if_nonfinite: only a finite one, which the host waits for.
+at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm, bool error_if_nonfinite) {
+  TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must be at least 0, got ", max_norm);
+  std::vector<at::Tensor> grads;
+  std::vector<void*> seen;
+  for (const auto& h : parameters) {
+    TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), "parameters must be tensors, got ",
+                     std::string(pybind11::str(pybind11::type::of(h))));
+    const at::Tensor g = THPVariable_Unpack(h.ptr()).grad();
+    if (!g.defined()) continue;
+    grads.push_back(g);
+    seen.push_back(g.unsafeGetTensorImpl());
+  }
+  // a gradient that comes up twice counts once
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) {
+    std::vector<at::Tensor> once;
+    for (const at::Tensor& g : grads)
+      if (std::none_of(once.begin(), once.end(), [&](const at::Tensor& o) { return o.is_same(g); })) once.push_back(g);
+    grads.swap(once);
+  }
+  if (grads.empty()) return at::zeros({}, at::kFloat);
+  std::vector<at::Tensor> dense;
   std::vector<void*> data;
   std::vector<int64_t> sizes;
   std::vector<int> types;
+  bool copied = false;
   for (const at::Tensor& g : grads) {
+    TORCH_CHECK(g.layout() == at::kStrided, "sparse gradients are not supported");
     check_cuda(g, grads[0], false);
-    TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradients must be dense");
-    data.push_back(g.data_ptr());
-    sizes.push_back(g.numel());
     types.push_back(dtype_code(g.scalar_type()));
   }
   c10::cuda::CUDAGuard guard(grads[0].device());
+  at::NoGradGuard no_grad;
+  for (const at::Tensor& g : grads) {
+    // one with gaps in memory goes through a dense copy
+    dense.push_back(g.is_contiguous() || g.is_non_overlapping_and_dense() ? g : g.contiguous());
+    copied = copied || !dense.back().is_same(g);
+    data.push_back(dense.back().data_ptr());
+    sizes.push_back(g.numel());
+  }
   const int count = static_cast<int>(grads.size());
   size_t need = 0;
   check_status(qlin_grad_clip_workspace_size(count, &need), "qlin_grad_clip_workspace_size");
   const at::Tensor ws = bytes_on(grads[0], need);
   at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-  check_status(qlin_grad_clip(count, data.data(), sizes.data(), types.data(), static_cast<float>(max_norm),
-                              norm.data_ptr<float>(), ws.data_ptr(), need, stream_of(grads[0])),
-               "qlin_grad_clip");
+  auto run = [&](double limit) {
+    check_status(qlin_grad_clip(count, data.data(), sizes.data(), types.data(), static_cast<float>(limit),
+                                norm.data_ptr<float>(), ws.data_ptr(), need, stream_of(grads[0])),
+                 "qlin_grad_clip");
+  };
+  if (error_if_nonfinite) {
+    run(std::numeric_limits<double>::infinity());  // the norm alone
+    const float n = norm.item<float>();
+    TORCH_CHECK(std::isfinite(n), "the global norm of the gradients is ", n, "; they are not clipped");
+  }
+  run(max_norm);
+  if (copied)
+    for (size_t k = 0; k < grads.size(); ++k)
+      if (!dense[k].is_same(grads[k])) grads[k].copy_(dense[k]);
   return norm;
-}
-
-// The tensors, with a contiguous copy in the place of each that has gaps.
-std::vector<at::Tensor> dense_grads(std::vector<at::Tensor> grads) {
-  for (at::Tensor& g : grads)
-    if (!g.is_non_overlapping_and_dense()) g = g.contiguous();
-  return grads;
 }
 
 pybind11::object or_none(const at::Tensor& t) { return t.defined() ? pybind11::cast(t) : pybind11::none(); }
@@ -262,6 +297,5 @@ void register_mx(pybind11::module& m) {
           return py::make_tuple(or_none(g[0]), or_none(g[1]), or_none(g[2]), or_none(g[3]));
         },
         "gradients of mx_forward");
-  m.def("dense_grads", &dense_grads, "gradients without gaps in memory");
-  m.def("grad_clip", &grad_clip, "global norm of gradient tensors, clipped in place");
+  m.def("clip_grad_norm", &clip_grad_norm, "global norm of the parameters' gradients, clipped in place");
 }

@@ -5,8 +5,6 @@ host."""
 
 from __future__ import annotations
 
-from collections.abc import Iterable
-
 import torch
 
 from .mx import _ext
@@ -31,30 +29,4 @@ def clip_grad_norm(parameters, max_norm: float, error_if_nonfinite: bool = False
     """
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    if not isinstance(parameters, Iterable):
-        raise TypeError(f"parameters must be a tensor or an iterable of tensors, got {type(parameters).__name__}")
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must be at least 0, got {max_norm}")
-    grads = {}
-    for p in parameters:
-        if p.grad is not None:
-            grads[id(p.grad)] = p.grad
-    grads = list(grads.values())
-    if not grads:
-        return torch.tensor(0.0)
-    for g in grads:
-        if g.layout != torch.strided:
-            raise RuntimeError("sparse gradients are not supported")
-    with torch.no_grad():
-        # a gradient with gaps in memory goes through a dense copy
-        dense = _ext().dense_grads(grads)
-        norm = _ext().grad_clip(dense, float("inf") if error_if_nonfinite else max_norm)
-        if error_if_nonfinite:
-            if not bool(torch.isfinite(norm)):
-                raise RuntimeError(f"the global norm of the gradients is {float(norm)}; they are not clipped")
-            norm = _ext().grad_clip(dense, max_norm)
-        for g, d in zip(grads, dense):
-            if d is not g:
-                g.copy_(d)
-    return norm
+    return _ext().clip_grad_norm(parameters, float(max_norm), error_if_nonfinite)
