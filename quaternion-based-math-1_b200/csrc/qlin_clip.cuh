@@ -5,13 +5,15 @@
 //
 // Two launches over one table of tensors (a kernel parameter: no copy to the
 // device, so both can be captured into a graph).  The elements of all tensors
-// form one line of pieces of kClipPiece elements, no piece in two tensors;
-// every CTA takes an equal run of pieces in both launches.
+// form one line of pieces of kClipPiece elements, no piece in two tensors; the
+// CTAs take batches of kClipBatch pieces in turn, so that at any time they read
+// one stretch of the line.
 //
 // Bound by the bytes: read once for the norm, read and written once for the
-// product.  The second launch walks its run backwards, so that it begins with
-// what the first has left in L2 (sets of up to about 100 MB are read from
-// HBM once).
+// product.  The second launch walks the line backwards, so that it begins with
+// what the first has left in L2: the first reads all but the last kClipKeep bytes
+// of the set as the first to be evicted, the second reads and writes everything
+// so.
 //
 // Squares are summed in fp32 within a piece and thread (8 terms) and in fp64 from
 // there on, in an order that depends only on the sizes: the same gradients give
@@ -28,7 +30,8 @@ constexpr int kClipPiece = kClipThreads * kClipEach;  // elements
 constexpr int kClipBatch = 4;                         // whole pieces of a tensor whose loads go out together
 constexpr int kClipTensors = 512;              // most table entries of a launch
 constexpr int kClipFewTensors = 64;            // entries of the small table (less to hand to a launch)
-constexpr int kClipCtasPerSm = 8;
+constexpr int kClipCtasPerSm = 6;
+constexpr long long kClipKeep = 72ll << 20;           // of the 126 MB of L2
 
 template <int CAP>
 struct ClipTable {
@@ -39,15 +42,32 @@ struct ClipTable {
   int count;
 };
 
+// Evict-first policy of L2.
+__device__ __forceinline__ uint64_t clip_policy() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
 // A thread's elements of a whole, aligned piece: 16-byte pieces apart by
 // kClipThreads * 16 bytes.
 template <typename T>
 struct ClipLoad {
   static constexpr int V = 16 / (int)sizeof(T);
   uint4 q[kClipEach / V];
-  __device__ __forceinline__ void load(const T* piece) {
+  __device__ __forceinline__ void load(const T* piece, bool keep) {
+    const uint64_t policy = clip_policy();
 #pragma unroll
-    for (int u = 0; u < kClipEach / V; ++u) q[u] = ld_cg_v4(piece + (u * kClipThreads + threadIdx.x) * V);
+    for (int u = 0; u < kClipEach / V; ++u) {
+      const T* at = piece + (u * kClipThreads + threadIdx.x) * V;
+      if (keep)
+        q[u] = ld_cg_v4(at);
+      else
+        asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+                     : "=r"(q[u].x), "=r"(q[u].y), "=r"(q[u].z), "=r"(q[u].w)
+                     : "l"(at), "l"(policy)
+                     : "memory");
+    }
   }
   __device__ __forceinline__ double squares() const {
     float s = 0.f;
@@ -75,7 +95,10 @@ struct ClipLoad {
       T* e = reinterpret_cast<T*>(&q[u]);
 #pragma unroll
       for (int j = 0; j < V; ++j) e[j] = from_f32<T>(to_f32(e[j]) * f);
-      *reinterpret_cast<uint4*>(piece + (u * kClipThreads + threadIdx.x) * V) = q[u];
+      asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1, %2, %3, %4}, %5;"
+                   ::"l"(piece + (u * kClipThreads + threadIdx.x) * V), "r"(q[u].x), "r"(q[u].y), "r"(q[u].z),
+                     "r"(q[u].w), "l"(clip_policy())
+                   : "memory");
     }
   }
 };
@@ -83,20 +106,20 @@ struct ClipLoad {
 // The sum of squares of this thread's elements of `n` consecutive pieces of a
 // tensor, of which `left` elements are there.
 template <typename T>
-__device__ __forceinline__ double clip_sum(const T* at, int n, long long left) {
+__device__ __forceinline__ double clip_sum(const T* at, int n, long long left, bool keep) {
   double d = 0.0;
   if ((reinterpret_cast<uintptr_t>(at) & 15) == 0) {
     if (n == kClipBatch && left >= (long long)kClipBatch * kClipPiece) {
       ClipLoad<T> a[kClipBatch];
 #pragma unroll
-      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece);
+      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece, keep);
 #pragma unroll
       for (int u = 0; u < kClipBatch; ++u) d += a[u].squares();
       return d;
     }
     for (; n > 0 && left >= kClipPiece; --n, left -= kClipPiece, at += kClipPiece) {
       ClipLoad<T> a;
-      a.load(at);
+      a.load(at, keep);
       d += a.squares();
     }
   }
@@ -114,31 +137,19 @@ __device__ __forceinline__ void clip_scale(T* at, int n, long long left, float f
     if (n == kClipBatch && left >= (long long)kClipBatch * kClipPiece) {
       ClipLoad<T> a[kClipBatch];
 #pragma unroll
-      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece);
+      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece, false);
 #pragma unroll
       for (int u = 0; u < kClipBatch; ++u) a[u].store_scaled(at + u * kClipPiece, f);
       return;
     }
     for (; n > 0 && left >= kClipPiece; --n, left -= kClipPiece, at += kClipPiece) {
       ClipLoad<T> a;
-      a.load(at);
+      a.load(at, false);
       a.store_scaled(at, f);
     }
   }
   const long long rest = min(left, (long long)n * kClipPiece);
   for (long long k = threadIdx.x; k < rest; k += kClipThreads) at[k] = from_f32<T>(to_f32(at[k]) * f);
-}
-
-// The tensor that holds a piece: the last whose first piece is not past it.
-template <int CAP>
-__device__ __forceinline__ int clip_find(const ClipTable<CAP>& tab, long long piece) {
-  int lo = 0, hi = tab.count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (tab.first[mid] <= piece) lo = mid;
-    else hi = mid;
-  }
-  return lo;
 }
 
 // Sum of all threads' values, the same in every thread (fixed order).
@@ -156,23 +167,25 @@ __device__ __forceinline__ double clip_block_sum(double v, double* slots) {
 
 // partials[blockIdx.x] = this CTA's share of the sum of squares.
 template <int CAP>
-__global__ void __launch_bounds__(kClipThreads)
-qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __restrict__ partials) {
+__global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm)
+qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __restrict__ partials,
+                      float keep_share) {
   __shared__ double slots[kClipThreads / 32];
   pdl_wait_prior();
   pdl_launch_dependents();
   const long long pieces = tab.first[tab.count];
-  const long long p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
+  const long long keep_from = pieces - (long long)(keep_share * (float)pieces);
   double s = 0.0;
-  if (p0 < p1) {
-    int k = clip_find(tab, p0);
-    for (long long p = p0; p < p1;) {
+  int k = 0;
+  for (long long b = (long long)blockIdx.x * kClipBatch; b < pieces; b += (long long)gridDim.x * kClipBatch) {
+    for (long long p = b; p < min(pieces, b + kClipBatch);) {
       while (p >= tab.first[k + 1]) ++k;
-      const int n = (int)min((long long)kClipBatch, min(p1, tab.first[k + 1]) - p);
+      const int n = (int)(min(b + kClipBatch, tab.first[k + 1]) - p);
       const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
-      if (tab.type[k] == 0) s += clip_sum(static_cast<const float*>(tab.data[k]) + at, n, left);
-      else if (tab.type[k] == 1) s += clip_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, n, left);
-      else s += clip_sum(static_cast<const __half*>(tab.data[k]) + at, n, left);
+      const bool keep = p >= keep_from;
+      if (tab.type[k] == 0) s += clip_sum(static_cast<const float*>(tab.data[k]) + at, n, left, keep);
+      else if (tab.type[k] == 1) s += clip_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, n, left, keep);
+      else s += clip_sum(static_cast<const __half*>(tab.data[k]) + at, n, left, keep);
       p += n;
     }
   }
@@ -180,9 +193,9 @@ qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __rest
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-// Every CTA adds up all partial sums (in the same order) and scales its run.
+// Every CTA adds up all partial sums (in the same order) and scales its pieces.
 template <int CAP>
-__global__ void __launch_bounds__(kClipThreads)
+__global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm)
 qlin_grad_scale_kernel(const __grid_constant__ ClipTable<CAP> tab, const double* __restrict__ partials, int n_partials,
                        float max_norm, float* __restrict__ norm_out) {
   __shared__ double slots[kClipThreads / 32];
@@ -197,18 +210,18 @@ qlin_grad_scale_kernel(const __grid_constant__ ClipTable<CAP> tab, const double*
   float f = max_norm / (norm + 1e-6f);
   if (f > 1.f) f = 1.f;
   if (isinf(max_norm)) return;  // the norm alone
-  const long long pieces = tab.first[tab.count];
-  const long long p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
-  if (p0 >= p1) return;
-  int k = clip_find(tab, p1 - 1);
-  for (long long p = p1; p > p0;) {  // backwards
-    while (p - 1 < tab.first[k]) --k;
-    const int n = (int)min((long long)kClipBatch, p - max(p0, tab.first[k]));
-    p -= n;
-    const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
-    if (tab.type[k] == 0) clip_scale(static_cast<float*>(tab.data[k]) + at, n, left, f);
-    else if (tab.type[k] == 1) clip_scale(static_cast<__nv_bfloat16*>(tab.data[k]) + at, n, left, f);
-    else clip_scale(static_cast<__half*>(tab.data[k]) + at, n, left, f);
+  const long long pieces = tab.first[tab.count], batches = (pieces + kClipBatch - 1) / kClipBatch;
+  int k = tab.count - 1;
+  for (long long b = batches - 1 - blockIdx.x; b >= 0; b -= gridDim.x) {  // backwards
+    for (long long p = min(pieces, (b + 1) * kClipBatch); p > b * kClipBatch;) {
+      while (p - 1 < tab.first[k]) --k;
+      const int n = (int)(p - max(b * kClipBatch, tab.first[k]));
+      p -= n;
+      const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
+      if (tab.type[k] == 0) clip_scale(static_cast<float*>(tab.data[k]) + at, n, left, f);
+      else if (tab.type[k] == 1) clip_scale(static_cast<__nv_bfloat16*>(tab.data[k]) + at, n, left, f);
+      else clip_scale(static_cast<__half*>(tab.data[k]) + at, n, left, f);
+    }
   }
 }
 

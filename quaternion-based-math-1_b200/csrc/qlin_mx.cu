@@ -186,11 +186,11 @@ MxPlanes<T> planes_at(void* base, int64_t K_g, int64_t N_g) {
   return p;
 }
 
-// CTAs of the record kernels: eight records (one per warp) a step, at most
-// four CTAs per SM.
+// CTAs of the record kernels: a warp takes half a record, at most 64 CTAs per SM
+// (then each warp takes several).
 unsigned record_ctas(int64_t K_g, int64_t N_g, int sms) {
   const int64_t records = ceil_div(N_g, kMxRows) * ceil_div(K_g, kMxBlock);
-  return (unsigned)std::min<int64_t>(ceil_div(records, 8), 8ll * sms);
+  return (unsigned)std::min<int64_t>(ceil_div(records, 4), 64ll * sms);
 }
 
 template <typename T>
@@ -671,7 +671,7 @@ int run_backward32(const float* g, int64_t ld_g, const float* x, int64_t ld_x, c
 
 template <int CAP>
 void clip_tables(int count, void* const* grads, const int64_t* sizes, const int* dtypes, float max_norm, float* norm,
-                 double* partials, int ctas, cudaStream_t s) {
+                 double* partials, int ctas, float keep_share, cudaStream_t s) {
   const int rounds = (int)std::max<int64_t>(1, ceil_div(count, CAP));
   for (int pass = 0; pass < 2; ++pass)
     for (int r = 0; r < rounds; ++r) {
@@ -694,17 +694,17 @@ void clip_tables(int count, void* const* grads, const int64_t* sizes, const int*
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
       if (pass == 0)
-        cudaLaunchKernelEx(&cfg, qlin_grad_norm_kernel<CAP>, tab, partials + (int64_t)r * ctas);
+        cudaLaunchKernelEx(&cfg, qlin_grad_norm_kernel<CAP>, tab, partials + (int64_t)r * ctas, keep_share);
       else
         cudaLaunchKernelEx(&cfg, qlin_grad_scale_kernel<CAP>, tab, (const double*)partials, rounds * ctas, max_norm,
                            norm);
     }
 }
 
-// CTAs of the clipping kernels for a set of tensors: a run of pieces each, at
+// CTAs of the clipping kernels for a set of tensors: a batch of pieces each, at
 // most what the device holds at once.
 int clip_ctas(int64_t pieces, int sms) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(pieces, (int64_t)kClipCtasPerSm * sms));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(pieces, kClipBatch), (int64_t)kClipCtasPerSm * sms));
 }
 
 // Upper bound of the SM count, to size a workspace without a device.
@@ -874,13 +874,14 @@ int qlin_grad_clip(int count, void* const* grads, const int64_t* sizes, const in
                    float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   if (count < 0) return QLIN_ERR_SHAPE;
   if (!norm || (count > 0 && (!grads || !sizes || !dtypes)) || !(max_norm >= 0.f)) return QLIN_ERR_ARG;
-  int64_t pieces = 0;
+  int64_t pieces = 0, bytes = 0;
   for (int k = 0; k < count; ++k) {
     if (sizes[k] < 0) return QLIN_ERR_SHAPE;
     if (!known(dtypes[k])) return QLIN_ERR_DTYPE;
     if (sizes[k] > 0 && !grads[k]) return QLIN_ERR_ARG;
     if (!aligned(grads[k], (uintptr_t)elem(dtypes[k]))) return QLIN_ERR_ALIGN;
     pieces += ceil_div(sizes[k], kClipPiece);
+    bytes += sizes[k] * elem(dtypes[k]);
   }
   size_t need = 0;
   qlin_grad_clip_workspace_size(count, &need);
@@ -892,10 +893,11 @@ int qlin_grad_clip(int count, void* const* grads, const int64_t* sizes, const in
   cudaGetLastError();
   const int ctas = clip_ctas(pieces, (int)std::min<int64_t>(sms, kMostSms));
   double* partials = static_cast<double*>(workspace);
+  const float keep_share = bytes > kClipKeep ? (float)kClipKeep / (float)bytes : 1.f;
   if (count <= kClipFewTensors)
-    clip_tables<kClipFewTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, s);
+    clip_tables<kClipFewTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, keep_share, s);
   else
-    clip_tables<kClipTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, s);
+    clip_tables<kClipTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, keep_share, s);
   return launched();
 }
 

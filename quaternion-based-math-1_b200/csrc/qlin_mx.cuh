@@ -152,11 +152,11 @@ struct MxPlanes {
   T* w[4];
 };
 
-// Quantisation: a warp makes a record at a time, two rows (four components of
-// four octets each) per step.  A lane holds eight elements of one block, the
+// Quantisation: a warp makes half a record (eight rows), two rows (four components
+// of four octets each) per step.  A lane holds eight elements of one block, the
 // four lanes of a block share its maximum.  Bound by the bytes read (2 or 4 a
-// weight) and written (0.53): one pass, the loads of four steps at a time in
-// flight, everything else in registers.
+// weight) and written (0.53): one pass, all loads of a warp in flight at once,
+// everything else in registers.
 template <typename T>
 __global__ void __launch_bounds__(256)
 qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_g, uint8_t* __restrict__ mx,
@@ -166,38 +166,33 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
   const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
   const int64_t warps = (int64_t)gridDim.x * 8;
   uint32_t top = 0;
-  for (int64_t rec = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); rec < tiles * kb; rec += warps) {
-    const int64_t tile = rec / kb, b = rec - tile * kb;
+  for (int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < 2 * tiles * kb; unit += warps) {
+    const int64_t rec = unit >> 1, tile = rec / kb, b = rec - tile * kb;
+    const int first = 8 * (int)(unit & 1) + half;  // row of the first step
     uint8_t* out = mx + kMxHeader + rec * kMxRecord;
-    const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
-    const T* row0 = src.w[p] + (tile * kMxRows + half) * ld + i;
+    const int64_t i = b * kMxBlock + 8 * t, left = K_g - i, o0 = tile * kMxRows + first;
+    const T* row0 = src.w[p] + o0 * ld + i;
+    float v[4][8];
 #pragma unroll
-    for (int s4 = 0; s4 < kMxRows / 2; s4 += 4) {
-      float v[4][8];
+    for (int u = 0; u < 4; ++u) mx_load8(row0 + 2 * u * ld, o0 + 2 * u < N_g ? left : 0, vec, v[u]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t o = tile * kMxRows + 2 * (s4 + u) + half;
-        mx_load8(row0 + 2 * (s4 + u) * ld, o < N_g ? left : 0, vec, v[u]);
-      }
+    for (int u = 0; u < 4; ++u) {
+      const int row = first + 2 * u;
+      // magnitudes as integers: the order of finite values, infinities and NaNs above them
+      uint32_t m = 0;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int row = 2 * (s4 + u) + half;
-        // magnitudes as integers: the order of finite values, infinities and NaNs above them
-        uint32_t m = 0;
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[u][j]) & 0x7FFFFFFFu);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const bool bad = m >= 0x7F800000u;
+      const uint32_t e = mx_exponent(__uint_as_float(m));
+      const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - E): E is at most 252
+      float q[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[u][j]) & 0x7FFFFFFFu);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const bool bad = m >= 0x7F800000u;
-        const uint32_t e = mx_exponent(__uint_as_float(m));
-        const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - E): E is at most 252
-        float q[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[u][j] * inv;
-        if (!bad) top = max(top, e + 1u);
-        *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
-        if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
-      }
+      for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[u][j] * inv;
+      if (!bad) top = max(top, e + 1u);
+      *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
+      if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
     }
   }
   __shared__ uint32_t tops[8];
@@ -221,21 +216,22 @@ qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst,
   const int t = lane & 3, p = (lane >> 2) & 3, half = lane >> 4;
   const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
   const int64_t warps = (int64_t)gridDim.x * 8;
-  for (int64_t rec = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); rec < tiles * kb; rec += warps) {
-    const int64_t tile = rec / kb, b = rec - tile * kb;
+  for (int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < 2 * tiles * kb; unit += warps) {
+    const int64_t rec = unit >> 1, tile = rec / kb, b = rec - tile * kb;
+    const int first = 8 * (int)(unit & 1) + half;
     const uint8_t* in = mx + kMxHeader + rec * kMxRecord;
     const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
     if (left <= 0) continue;
-    uint32_t word[kMxRows / 2], f[kMxRows / 2];
+    uint32_t word[4], f[4];
 #pragma unroll
-    for (int step = 0; step < kMxRows / 2; ++step) {
-      const int row = 2 * step + half;
+    for (int step = 0; step < 4; ++step) {
+      const int row = first + 2 * step;
       word[step] = __ldcg(reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4));
       f[step] = __ldcg(in + kMxCodeBytes + row * 4 + p);
     }
 #pragma unroll
-    for (int step = 0; step < kMxRows / 2; ++step) {
-      const int64_t o = tile * kMxRows + 2 * step + half;
+    for (int step = 0; step < 4; ++step) {
+      const int64_t o = tile * kMxRows + first + 2 * step;
       if (o >= N_g) continue;
       const float s = mx_scale(f[step]);
       T* at = dst.w[p] + o * ld + i;
