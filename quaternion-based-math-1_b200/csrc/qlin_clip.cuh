@@ -11,9 +11,9 @@
 //
 // Bound by the bytes: read once for the norm, read and written once for the
 // product.  The second launch walks the line backwards, so that it begins with
-// what the first has left in L2: the first reads all but the last kClipKeep bytes
-// of the set as the first to be evicted, the second reads and writes everything
-// so.
+// what the first has left in L2; a set that L2 holds is read from HBM once.
+// (Evict-first hints for all but the last 40 or 72 MB of the first pass changed
+// nothing: 134 to 142 us for 270 MB either way, near the 124 us of three passes.)
 //
 // Squares are summed in fp32 within a piece and thread (8 terms) and in fp64 from
 // there on, in an order that depends only on the sizes: the same gradients give
@@ -31,7 +31,6 @@ constexpr int kClipBatch = 4;                         // whole pieces of a tenso
 constexpr int kClipTensors = 512;              // most table entries of a launch
 constexpr int kClipFewTensors = 64;            // entries of the small table (less to hand to a launch)
 constexpr int kClipCtasPerSm = 6;
-constexpr long long kClipKeep = 72ll << 20;           // of the 126 MB of L2
 
 template <int CAP>
 struct ClipTable {
@@ -42,32 +41,15 @@ struct ClipTable {
   int count;
 };
 
-// Evict-first policy of L2.
-__device__ __forceinline__ uint64_t clip_policy() {
-  uint64_t p;
-  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
-  return p;
-}
-
 // A thread's elements of a whole, aligned piece: 16-byte pieces apart by
 // kClipThreads * 16 bytes.
 template <typename T>
 struct ClipLoad {
   static constexpr int V = 16 / (int)sizeof(T);
   uint4 q[kClipEach / V];
-  __device__ __forceinline__ void load(const T* piece, bool keep) {
-    const uint64_t policy = clip_policy();
+  __device__ __forceinline__ void load(const T* piece) {
 #pragma unroll
-    for (int u = 0; u < kClipEach / V; ++u) {
-      const T* at = piece + (u * kClipThreads + threadIdx.x) * V;
-      if (keep)
-        q[u] = ld_cg_v4(at);
-      else
-        asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
-                     : "=r"(q[u].x), "=r"(q[u].y), "=r"(q[u].z), "=r"(q[u].w)
-                     : "l"(at), "l"(policy)
-                     : "memory");
-    }
+    for (int u = 0; u < kClipEach / V; ++u) q[u] = ld_cg_v4(piece + (u * kClipThreads + threadIdx.x) * V);
   }
   __device__ __forceinline__ double squares() const {
     float s = 0.f;
@@ -95,10 +77,7 @@ struct ClipLoad {
       T* e = reinterpret_cast<T*>(&q[u]);
 #pragma unroll
       for (int j = 0; j < V; ++j) e[j] = from_f32<T>(to_f32(e[j]) * f);
-      asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1, %2, %3, %4}, %5;"
-                   ::"l"(piece + (u * kClipThreads + threadIdx.x) * V), "r"(q[u].x), "r"(q[u].y), "r"(q[u].z),
-                     "r"(q[u].w), "l"(clip_policy())
-                   : "memory");
+      *reinterpret_cast<uint4*>(piece + (u * kClipThreads + threadIdx.x) * V) = q[u];
     }
   }
 };
@@ -106,20 +85,20 @@ struct ClipLoad {
 // The sum of squares of this thread's elements of `n` consecutive pieces of a
 // tensor, of which `left` elements are there.
 template <typename T>
-__device__ __forceinline__ double clip_sum(const T* at, int n, long long left, bool keep) {
+__device__ __forceinline__ double clip_sum(const T* at, int n, long long left) {
   double d = 0.0;
   if ((reinterpret_cast<uintptr_t>(at) & 15) == 0) {
     if (n == kClipBatch && left >= (long long)kClipBatch * kClipPiece) {
       ClipLoad<T> a[kClipBatch];
 #pragma unroll
-      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece, keep);
+      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece);
 #pragma unroll
       for (int u = 0; u < kClipBatch; ++u) d += a[u].squares();
       return d;
     }
     for (; n > 0 && left >= kClipPiece; --n, left -= kClipPiece, at += kClipPiece) {
       ClipLoad<T> a;
-      a.load(at, keep);
+      a.load(at);
       d += a.squares();
     }
   }
@@ -137,14 +116,14 @@ __device__ __forceinline__ void clip_scale(T* at, int n, long long left, float f
     if (n == kClipBatch && left >= (long long)kClipBatch * kClipPiece) {
       ClipLoad<T> a[kClipBatch];
 #pragma unroll
-      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece, false);
+      for (int u = 0; u < kClipBatch; ++u) a[u].load(at + u * kClipPiece);
 #pragma unroll
       for (int u = 0; u < kClipBatch; ++u) a[u].store_scaled(at + u * kClipPiece, f);
       return;
     }
     for (; n > 0 && left >= kClipPiece; --n, left -= kClipPiece, at += kClipPiece) {
       ClipLoad<T> a;
-      a.load(at, false);
+      a.load(at);
       a.store_scaled(at, f);
     }
   }
@@ -168,13 +147,11 @@ __device__ __forceinline__ double clip_block_sum(double v, double* slots) {
 // partials[blockIdx.x] = this CTA's share of the sum of squares.
 template <int CAP>
 __global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm)
-qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __restrict__ partials,
-                      float keep_share) {
+qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __restrict__ partials) {
   __shared__ double slots[kClipThreads / 32];
   pdl_wait_prior();
   pdl_launch_dependents();
   const long long pieces = tab.first[tab.count];
-  const long long keep_from = pieces - (long long)(keep_share * (float)pieces);
   double s = 0.0;
   int k = 0;
   for (long long b = (long long)blockIdx.x * kClipBatch; b < pieces; b += (long long)gridDim.x * kClipBatch) {
@@ -182,10 +159,9 @@ qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __rest
       while (p >= tab.first[k + 1]) ++k;
       const int n = (int)(min(b + kClipBatch, tab.first[k + 1]) - p);
       const long long at = (p - tab.first[k]) * kClipPiece, left = tab.size[k] - at;
-      const bool keep = p >= keep_from;
-      if (tab.type[k] == 0) s += clip_sum(static_cast<const float*>(tab.data[k]) + at, n, left, keep);
-      else if (tab.type[k] == 1) s += clip_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, n, left, keep);
-      else s += clip_sum(static_cast<const __half*>(tab.data[k]) + at, n, left, keep);
+      if (tab.type[k] == 0) s += clip_sum(static_cast<const float*>(tab.data[k]) + at, n, left);
+      else if (tab.type[k] == 1) s += clip_sum(static_cast<const __nv_bfloat16*>(tab.data[k]) + at, n, left);
+      else s += clip_sum(static_cast<const __half*>(tab.data[k]) + at, n, left);
       p += n;
     }
   }

@@ -671,7 +671,7 @@ int run_backward32(const float* g, int64_t ld_g, const float* x, int64_t ld_x, c
 
 template <int CAP>
 void clip_tables(int count, void* const* grads, const int64_t* sizes, const int* dtypes, float max_norm, float* norm,
-                 double* partials, int ctas, float keep_share, cudaStream_t s) {
+                 double* partials, int ctas, cudaStream_t s) {
   const int rounds = (int)std::max<int64_t>(1, ceil_div(count, CAP));
   for (int pass = 0; pass < 2; ++pass)
     for (int r = 0; r < rounds; ++r) {
@@ -694,7 +694,7 @@ void clip_tables(int count, void* const* grads, const int64_t* sizes, const int*
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
       if (pass == 0)
-        cudaLaunchKernelEx(&cfg, qlin_grad_norm_kernel<CAP>, tab, partials + (int64_t)r * ctas, keep_share);
+        cudaLaunchKernelEx(&cfg, qlin_grad_norm_kernel<CAP>, tab, partials + (int64_t)r * ctas);
       else
         cudaLaunchKernelEx(&cfg, qlin_grad_scale_kernel<CAP>, tab, (const double*)partials, rounds * ctas, max_norm,
                            norm);
@@ -874,14 +874,13 @@ int qlin_grad_clip(int count, void* const* grads, const int64_t* sizes, const in
                    float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   if (count < 0) return QLIN_ERR_SHAPE;
   if (!norm || (count > 0 && (!grads || !sizes || !dtypes)) || !(max_norm >= 0.f)) return QLIN_ERR_ARG;
-  int64_t pieces = 0, bytes = 0;
+  int64_t pieces = 0;
   for (int k = 0; k < count; ++k) {
     if (sizes[k] < 0) return QLIN_ERR_SHAPE;
     if (!known(dtypes[k])) return QLIN_ERR_DTYPE;
     if (sizes[k] > 0 && !grads[k]) return QLIN_ERR_ARG;
     if (!aligned(grads[k], (uintptr_t)elem(dtypes[k]))) return QLIN_ERR_ALIGN;
     pieces += ceil_div(sizes[k], kClipPiece);
-    bytes += sizes[k] * elem(dtypes[k]);
   }
   size_t need = 0;
   qlin_grad_clip_workspace_size(count, &need);
@@ -893,11 +892,10 @@ int qlin_grad_clip(int count, void* const* grads, const int64_t* sizes, const in
   cudaGetLastError();
   const int ctas = clip_ctas(pieces, (int)std::min<int64_t>(sms, kMostSms));
   double* partials = static_cast<double*>(workspace);
-  const float keep_share = bytes > kClipKeep ? (float)kClipKeep / (float)bytes : 1.f;
   if (count <= kClipFewTensors)
-    clip_tables<kClipFewTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, keep_share, s);
+    clip_tables<kClipFewTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, s);
   else
-    clip_tables<kClipTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, keep_share, s);
+    clip_tables<kClipTensors>(count, grads, sizes, dtypes, max_norm, norm, partials, ctas, s);
   return launched();
 }
 
