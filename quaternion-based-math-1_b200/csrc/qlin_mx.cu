@@ -368,7 +368,7 @@ int pair_capacity() {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
-    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.blockDim = dim3(kMxPairThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute a;
     a.id = cudaLaunchAttributeClusterDimension;
@@ -438,7 +438,7 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
   attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, cap)), 1, 1);
-  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.blockDim = dim3(kMxPairThreads, 1, 1);
   cfg.dynamicSmemBytes = kPairSmemBytes;
   cfg.stream = s;
   cfg.attrs = attrs;

@@ -11,6 +11,8 @@
 // UMMAs of a stage take at 256 tokens, and a quarter of a 16-bit layer's bytes.
 // Without MX the weights are 16-bit component planes: the adjoint of the codes,
 // times 2^-c.
+// One set of builder warps could not keep up with the UMMAs on codes (a 4096 layer
+// at 2048 tokens: 66 us, 57 on planes); two sets take every other stage each.
 //
 // Adapter: y += t B^T with t = s x A^T as two 16-bit parts (t = hi + lo to about
 // twice the type's precision): ceil(r / 64) more stages whose x tile is 64
@@ -28,6 +30,10 @@
 
 namespace qlin {
 
+constexpr int kMxPairBuilders = 8;  // warps 2-9: two sets of four, every other stage each
+constexpr int kMxPairEpilogue = 8;  // warps 10-17: two sets of four, half of the tokens each
+constexpr int kMxPairThreads = 32 * (2 + kMxPairBuilders + kMxPairEpilogue);
+
 template <int NTOK, bool MX>
 struct MxPairStage {
   static constexpr int kHalf = NTOK / 2;
@@ -35,11 +41,11 @@ struct MxPairStage {
   static constexpr int kXBytes = 2 * kXAtomBytes;
   static constexpr int kWBytes = MX ? 3072 : 4 * kPairWTileBytes;  // (two records, rounded up to whole KB)
   static constexpr int kStageBytes = kXBytes + kWBytes;
-  static constexpr int kStages = NTOK == 256 ? (MX ? 5 : 4) : 8;
+  static constexpr int kStages = NTOK == 256 ? (MX ? 5 : 4) : (MX ? 8 : 7);
   static constexpr int kDBufs = NTOK == 256 ? 1 : 2;
   static constexpr int kAColBase = kDBufs * NTOK;
   static constexpr int kEpiOffset = kStages * kStageBytes;
-  static constexpr int kBarOffset = kEpiOffset + 2 * kPairEpiBufBytes;
+  static constexpr int kBarOffset = kEpiOffset + 4 * kPairEpiBufBytes;  // two buffers per epilogue set
   static_assert(kBarOffset + 512 + 1024 <= kPairSmemBytes, "shared memory");
   static_assert(kStageBytes % 1024 == 0, "swizzled x tiles start on 1 KB");
   static_assert(2 * kMxRecord <= 3072, "two records");
@@ -61,7 +67,7 @@ struct MxPairParams {
 };
 
 template <typename T, int NTOK, bool MX>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kMxPairThreads, 1)
 qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_t,
                     const __grid_constant__ CUtensorMap map_wr, const __grid_constant__ CUtensorMap map_wi,
                     const __grid_constant__ CUtensorMap map_wj, const __grid_constant__ CUtensorMap map_wk,
@@ -103,7 +109,7 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(&dfull[b], 1);
-      mbar_init(&dempty[b], 8);
+      mbar_init(&dempty[b], 2 * kMxPairEpilogue);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -217,7 +223,7 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       umma_commit_pair(drain, 0x1);
       mbar_wait(drain, 0, 50000000ull);
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + kMxPairBuilders) {
     // ---------------- builders: expanded weight rows into tensor memory ----------------
     // Lane l of builder warp w writes tensor-memory lane 32 q + l (q = w % 4):
     // output quaternion n0/4 + 8 q + l % 8, component a = l / 8.
@@ -230,8 +236,13 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const uint32_t tm_lane = (uint32_t)(32 * quarter) << 16;
     const MxPowers pw;
     const float down = scalbnf(1.f, -c);
-    int k = 0, j = 0;
-    for (int g = 0; g < total; ++g) {
+    const int set = (warp - 2) >> 2;
+    int k = set, j = 0;
+    for (int g = set; g < total; g += 2, k += 2) {
+      while (k >= nk) {
+        k -= nk;
+        ++j;
+      }
       const int s = g % S, n = g / S, sa = g % SA, na = g / SA;
       bool ok = !*abort_flag && mbar_wait(&full[s], n & 1);
       if (ok && na > 0) ok = mbar_wait(&aempty[sa], (na - 1) & 1);
@@ -341,10 +352,6 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cta(&afull[sa], 0);
-      if (++k == nk) {
-        k = 0;
-        ++j;
-      }
     }
   } else {
     // ---------------- epilogue ----------------
@@ -352,7 +359,9 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     // tokens per word), release it to the UMMA issuer, then store through a
     // shared-memory transpose.
     const int quarter = warp & 3;
-    const int et = threadIdx.x - 192;  // 0..127
+    const int half = (warp - 2 - kMxPairBuilders) >> 2;  // of the tile's tokens
+    const int et = (threadIdx.x - 32 * (2 + kMxPairBuilders)) & 127;
+    constexpr int kTok = NTOK / 2;
     const int n_local = 32 * quarter + 4 * (lane & 7) + (lane >> 3);
     const float factor = scalbnf(1.f, c);
     T* __restrict__ y = reinterpret_cast<T*>(prm.y);
@@ -366,13 +375,13 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       tc_fence_after();
       const int n = n0 + n_local;
       const float bv = (bias && n < 4 * prm.N_g) ? to_f32(bias[n]) : 0.f;
-      uint32_t packed[NTOK / 2];
+      uint32_t packed[kTok / 2];
 #pragma unroll
-      for (int q = 0; q < NTOK / 32; ++q) {
+      for (int q = 0; q < kTok / 32; ++q) {
         uint32_t v[32];
         if (got) {
           __syncwarp();
-          tmem_ld32(tmem + ((uint32_t)(32 * quarter) << 16) + b * NTOK + 32 * q, v);
+          tmem_ld32(tmem + ((uint32_t)(32 * quarter) << 16) + b * NTOK + half * kTok + 32 * q, v);
           tmem_ld_wait();
         } else {
 #pragma unroll
@@ -388,8 +397,8 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive_cta(&dempty[b], 0);
 #pragma unroll
-      for (int grp = 0; grp < NTOK / kPairEpiTokens; ++grp) {
-        T* stage = reinterpret_cast<T*>(smem + Cfg::kEpiOffset + (grp & 1) * kPairEpiBufBytes);
+      for (int grp = 0; grp < kTok / kPairEpiTokens; ++grp) {
+        T* stage = reinterpret_cast<T*>(smem + Cfg::kEpiOffset + (2 * half + (grp & 1)) * kPairEpiBufBytes);
         unsigned short* st16 = reinterpret_cast<unsigned short*>(stage);
 #pragma unroll
         for (int t2 = 0; t2 < kPairEpiTokens / 2; ++t2) {
@@ -397,13 +406,13 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           st16[(2 * t2) * kPairRows + n_local] = (unsigned short)(wv & 0xffffu);
           st16[(2 * t2 + 1) * kPairRows + n_local] = (unsigned short)(wv >> 16);
         }
-        asm volatile("bar.sync %0, %1;" ::"n"(kPairEpiBar), "n"(128) : "memory");
+        asm volatile("bar.sync %0, %1;" ::"r"(kPairEpiBar + half), "n"(128) : "memory");
         if (got) {
           // 16 tokens x 128 outputs = 256 pieces of 16 bytes, two per thread
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int at = et + 128 * h, t = at >> 4, cc = at & 15;
-            const int m = m0 + kPairEpiTokens * grp + t, nn = n0 + 8 * cc;
+            const int m = m0 + half * kTok + kPairEpiTokens * grp + t, nn = n0 + 8 * cc;
             if (m < prm.M && nn < 4 * prm.N_g) {
               const uint4 v = *reinterpret_cast<const uint4*>(stage + t * kPairRows + 8 * cc);
               T* out = y + (int64_t)m * prm.ld_y + nn;
