@@ -41,7 +41,7 @@ struct MxPairStage {
   static constexpr int kXBytes = 2 * kXAtomBytes;
   static constexpr int kWBytes = MX ? 3072 : 4 * kPairWTileBytes;  // (two records, rounded up to whole KB)
   static constexpr int kStageBytes = kXBytes + kWBytes;
-  static constexpr int kStages = NTOK == 256 ? (MX ? 5 : 4) : (MX ? 8 : 7);
+  static constexpr int kStages = kPairAStages;  // x, W and the expanded rows share a ring position
   static constexpr int kDBufs = NTOK == 256 ? 1 : 2;
   static constexpr int kAColBase = kDBufs * NTOK;
   static constexpr int kEpiOffset = kStages * kStageBytes;
@@ -66,6 +66,17 @@ struct MxPairParams {
   int wide;             // 16-byte output pieces are aligned
 };
 
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 template <typename T, int NTOK, bool MX>
 __global__ void __launch_bounds__(kMxPairThreads, 1)
 qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_t,
@@ -75,15 +86,14 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   using Cfg = MxPairStage<NTOK, MX>;
   constexpr bool HALF = std::is_same<T, __half>::value;
   constexpr uint32_t kIdesc = make_idesc_f16(256, NTOK, HALF ? 0u : 1u, false);
-  constexpr int S = Cfg::kStages, SA = kPairAStages, NB = Cfg::kDBufs;
+  constexpr int S = Cfg::kStages, NB = Cfg::kDBufs;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);  // [S] x and W of this CTA landed
   uint64_t* empty = full + S;     // [S] the UMMAs of the stage completed (both CTAs)
-  uint64_t* afull = empty + S;    // [SA] even CTA: both CTAs' builders wrote the A stage
-  uint64_t* aempty = afull + SA;  // [SA] the UMMAs reading the A stage completed (both CTAs)
-  uint64_t* dfull = aempty + SA;  // [NB]
+  uint64_t* afull = empty + S;    // [S] even CTA: both CTAs' builders wrote the expanded rows
+  uint64_t* dfull = afull + S;    // [NB]
   uint64_t* dempty = dfull + NB;  // [NB], even CTA: both CTAs' epilogues drained the accumulator
   uint64_t* drain = dempty + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -102,10 +112,7 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-    }
-    for (int s = 0; s < SA; ++s) {
       mbar_init(&afull[s], 8);
-      mbar_init(&aempty[s], 1);
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(&dfull[b], 1);
@@ -189,39 +196,44 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && cta == 0) {
+    if (cta == 0) {
       // ---------------- UMMA issuer (even CTA) ----------------
+      // The whole warp walks the loop, so that everything but the issue itself is
+      // uniform; one elected lane issues.
       bool ok = true;
       int g = 0;
       for (int j = 0; j < my_tiles && ok; ++j) {
         const int b = j % NB, u = j / NB;
         if (u > 0 && !mbar_wait(&dempty[b], (u - 1) & 1)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         for (int k = 0; k < nk && ok; ++k, ++g) {
-          const int s = g % S, sa = g % SA, na = g / SA;
+          const int s = g % S, n = g / S;
           // both CTAs' builders arrive only after their own CTA's x and W of
           // this stage landed: this one wait covers the B operand too
-          if (!mbar_wait(&afull[sa], na & 1) || *abort_flag) {
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu, mbar_wait(&afull[s], n & 1) && !*abort_flag);
+          if (!ok) break;
           tc_fence_after();
           const uint64_t bdesc0 = smem_desc_sw128(smem + s * Cfg::kStageBytes);
+          const uint32_t d = tmem + b * NTOK, a0 = tmem + Cfg::kAColBase + s * kPairACols;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kPairStageK / 16; ++kk) {
-            const uint64_t bdesc = bdesc0 + (uint64_t)((kk >> 2) * (Cfg::kXAtomBytes >> 4)) + 2 * (kk & 3);
-            umma_pair_ts(tmem + b * NTOK, tmem + Cfg::kAColBase + sa * kPairACols + 8 * kk, bdesc, kIdesc,
-                         (k > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < kPairStageK / 16; ++kk)
+              umma_pair_ts(d, a0 + 8 * kk, bdesc0 + (uint64_t)((kk >> 2) * (Cfg::kXAtomBytes >> 4)) + 2 * (kk & 3),
+                           kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[s], 0x3);
+            if (k == nk - 1) umma_commit_pair(&dfull[b], 0x3);
           }
-          umma_commit_pair(&empty[s], 0x3);
-          umma_commit_pair(&aempty[sa], 0x3);
+          __syncwarp();
         }
-        if (ok) umma_commit_pair(&dfull[b], 0x3);
       }
-      if (!ok) *abort_flag = 1;
-      // every UMMA issued above has completed before the teardown
-      umma_commit_pair(drain, 0x1);
-      mbar_wait(drain, 0, 50000000ull);
+      if (elect_one()) {
+        if (!ok) *abort_flag = 1;
+        // every UMMA issued above has completed before the teardown
+        umma_commit_pair(drain, 0x1);
+        mbar_wait(drain, 0, 50000000ull);
+      }
+      __syncwarp();
     }
   } else if (warp < 2 + kMxPairBuilders) {
     // ---------------- builders: expanded weight rows into tensor memory ----------------
@@ -243,11 +255,12 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         k -= nk;
         ++j;
       }
-      const int s = g % S, n = g / S, sa = g % SA, na = g / SA;
-      bool ok = !*abort_flag && mbar_wait(&full[s], n & 1);
-      if (ok && na > 0) ok = mbar_wait(&aempty[sa], (na - 1) & 1);
+      // (x and W of a stage are fetched once its last UMMAs are done, so the rows'
+      // tensor memory is free too when they land)
+      const int s = g % S, n = g / S;
+      const bool ok = !*abort_flag && mbar_wait(&full[s], n & 1);
       if (!ok) *abort_flag = 1;
-      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + sa * kPairACols;
+      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + s * kPairACols;
       if (!*abort_flag && k >= prm.stages) {
         // 64 ranks of this row of B, twice
         int n0, m0;
@@ -351,7 +364,7 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cta(&afull[sa], 0);
+      if (lane == 0) mbar_arrive_cta(&afull[s], 0);
     }
   } else {
     // ---------------- epilogue ----------------
