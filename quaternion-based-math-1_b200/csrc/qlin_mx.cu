@@ -67,11 +67,13 @@ struct Carve {
   }
 };
 
-// 16-bit inputs of up to this many tokens take the streaming kernels
-// (qlin_mx_few.cuh), more the dequantised path; fp32 always streams.
-constexpr int64_t kFewTokens = 64;
-
-bool streams(int dtype, int64_t M) { return dtype == QLIN_F32 || M <= kFewTokens; }
+// 16-bit inputs of up to 32 tokens take the streaming kernels (qlin_mx_few.cuh), and
+// up to 64 where the layer has at most a tile of 16 output quaternions per SM (4096
+// -> 4096 at 64 tokens 14 against 22 us, 5120 -> 27648 74 against 60); more take the
+// CTA-pair kernel (qlin_mx_pair.cuh).  fp32 always streams.
+bool streams(int dtype, int64_t M, int64_t N_g) {
+  return dtype == QLIN_F32 || M <= 32 || (M <= 64 && N_g <= 148 * kMxRows);
+}
 
 // Tokens of a tile of the streaming kernels (one or two tokens apart): the
 // smallest tile that holds them all, at most 32.
@@ -96,7 +98,7 @@ struct ForwardWs {
 ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   ForwardWs w;
   Carve c;
-  if (streams(dtype, M)) {
+  if (streams(dtype, M, N_g)) {
     if (!is_one(dtype, M, K_g)) {
       const int64_t C = few_tile(M);
       w.arranged = c.take(ceil_div(M, C) * ceil_div(K_g, kMxBlock) * (dtype == QLIN_F32 ? 3 : 1) * 4 * C * 64);
@@ -448,10 +450,14 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
              : QLIN_ERR_LAUNCH;
 }
 
-// 256 tokens a tile above 128 tokens.
+// Tiles of 256 tokens, or of 128 where those end sooner: a wave of them takes about
+// 0.6 of the time (stages of 0.45 against 0.75 us), and few tokens or outputs leave
+// pairs without a tile of 256.
 template <typename T, bool MX, typename... Args>
-int run_pair(int64_t M, Args... args) {
-  return M > 128 ? launch_pair<T, 256, MX>(args...) : launch_pair<T, 128, MX>(args...);
+int run_pair(int64_t M, int64_t N_g, Args... args) {
+  const int64_t nb = ceil_div(4 * N_g, 256), cap = std::max(1, pair_capacity<T, 256, MX>());
+  const int64_t waves256 = ceil_div(nb * ceil_div(M, 256), cap), waves128 = ceil_div(nb * ceil_div(M, 128), cap);
+  return 3 * waves128 < 5 * waves256 ? launch_pair<T, 128, MX>(args...) : launch_pair<T, 256, MX>(args...);
 }
 
 // Rows that TMA takes (whole: and that are whole 16-byte pieces): x itself, or a
@@ -512,7 +518,7 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
     st = launch_down<T>(job, MxDownJob<T>{}, M, M, s);
     if (st != QLIN_OK) return st;
   }
-  return run_pair<T, true>(M, x, ld_x, mx, MxPlanes<T>{}, (int64_t)0, bias, (const T*)parts, w.ld_parts, b, rank, y,
+  return run_pair<T, true>(M, N_g, x, ld_x, mx, MxPlanes<T>{}, (int64_t)0, bias, (const T*)parts, w.ld_parts, b, rank, y,
                            ld_y, M, K_g, N_g, s);
 }
 
@@ -558,7 +564,7 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     if (st != QLIN_OK) return st;
   }
   if (dx) {
-    st = run_pair<T, false>(M, g, ld_g, mx, p, w.ld_planes, (const T*)nullptr, (const T*)parts, w.ld_parts,
+    st = run_pair<T, false>(M, K_g, g, ld_g, mx, p, w.ld_planes, (const T*)nullptr, (const T*)parts, w.ld_parts,
                             (const T*)at, rank, dx, ld_dx, M, N_g, K_g, s);
     if (st != QLIN_OK) return st;
   }
@@ -802,7 +808,7 @@ int qlin_mx_forward(int dtype, const void* x, int64_t ld_x, const void* mx, cons
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   return by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    if (streams(dtype, M))
+    if (streams(dtype, M, N_g))
       return run_few<T>(dtype, static_cast<const T*>(x), ld_x, mx, static_cast<const T*>(bias),
                         static_cast<const T*>(lora_a), static_cast<const T*>(lora_b), rank, lora_scale,
                         static_cast<T*>(y), ld_y, M, K_g, N_g, ws, w, sms, static_cast<cudaStream_t>(stream));

@@ -41,7 +41,11 @@ struct MxPairStage {
   static constexpr int kXBytes = 2 * kXAtomBytes;
   static constexpr int kWBytes = MX ? 3072 : 4 * kPairWTileBytes;  // (two records, rounded up to whole KB)
   static constexpr int kStageBytes = kXBytes + kWBytes;
-  static constexpr int kStages = kPairAStages;  // x, W and the expanded rows share a ring position
+  // At 256 tokens x, W and the expanded rows share a ring position and a barrier;
+  // at 128 the UMMAs of a stage take half as long, and x and W are fetched up to
+  // seven stages ahead to cover their latency.
+  static constexpr int kStages = NTOK == 256 ? kPairAStages : (MX ? 8 : 7);
+  static constexpr bool kSplit = kStages != kPairAStages;
   static constexpr int kDBufs = NTOK == 256 ? 1 : 2;
   static constexpr int kAColBase = kDBufs * NTOK;
   static constexpr int kEpiOffset = kStages * kStageBytes;
@@ -86,14 +90,15 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   using Cfg = MxPairStage<NTOK, MX>;
   constexpr bool HALF = std::is_same<T, __half>::value;
   constexpr uint32_t kIdesc = make_idesc_f16(256, NTOK, HALF ? 0u : 1u, false);
-  constexpr int S = Cfg::kStages, NB = Cfg::kDBufs;
+  constexpr int S = Cfg::kStages, SA = kPairAStages, NB = Cfg::kDBufs;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);  // [S] x and W of this CTA landed
   uint64_t* empty = full + S;     // [S] the UMMAs of the stage completed (both CTAs)
-  uint64_t* afull = empty + S;    // [S] even CTA: both CTAs' builders wrote the expanded rows
-  uint64_t* dfull = afull + S;    // [NB]
+  uint64_t* afull = empty + S;    // [SA] even CTA: both CTAs' builders wrote the expanded rows
+  uint64_t* aempty = afull + SA;  // [SA] (kSplit) the UMMAs reading them completed (both CTAs)
+  uint64_t* dfull = aempty + SA;  // [NB]
   uint64_t* dempty = dfull + NB;  // [NB], even CTA: both CTAs' epilogues drained the accumulator
   uint64_t* drain = dempty + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -112,7 +117,10 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < SA; ++s) {
       mbar_init(&afull[s], 8);
+      mbar_init(&aempty[s], 1);
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(&dfull[b], 1);
@@ -208,20 +216,21 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         for (int k = 0; k < nk && ok; ++k, ++g) {
-          const int s = g % S, n = g / S;
+          const int s = g % S, sa = g % SA;
           // both CTAs' builders arrive only after their own CTA's x and W of
           // this stage landed: this one wait covers the B operand too
-          ok = __all_sync(0xffffffffu, mbar_wait(&afull[s], n & 1) && !*abort_flag);
+          ok = __all_sync(0xffffffffu, mbar_wait(&afull[sa], (g / SA) & 1) && !*abort_flag);
           if (!ok) break;
           tc_fence_after();
           const uint64_t bdesc0 = smem_desc_sw128(smem + s * Cfg::kStageBytes);
-          const uint32_t d = tmem + b * NTOK, a0 = tmem + Cfg::kAColBase + s * kPairACols;
+          const uint32_t d = tmem + b * NTOK, a0 = tmem + Cfg::kAColBase + sa * kPairACols;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kPairStageK / 16; ++kk)
               umma_pair_ts(d, a0 + 8 * kk, bdesc0 + (uint64_t)((kk >> 2) * (Cfg::kXAtomBytes >> 4)) + 2 * (kk & 3),
                            kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
             umma_commit_pair(&empty[s], 0x3);
+            if constexpr (Cfg::kSplit) umma_commit_pair(&aempty[sa], 0x3);
             if (k == nk - 1) umma_commit_pair(&dfull[b], 0x3);
           }
           __syncwarp();
@@ -255,12 +264,13 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         k -= nk;
         ++j;
       }
-      // (x and W of a stage are fetched once its last UMMAs are done, so the rows'
-      // tensor memory is free too when they land)
-      const int s = g % S, n = g / S;
-      const bool ok = !*abort_flag && mbar_wait(&full[s], n & 1);
+      // (in a shared ring x and W are fetched once the position's UMMAs are done, so
+      // its tensor memory is free too when they land)
+      const int s = g % S, sa = g % SA;
+      bool ok = !*abort_flag && mbar_wait(&full[s], (g / S) & 1);
+      if (Cfg::kSplit && ok && g >= SA) ok = mbar_wait(&aempty[sa], (g / SA - 1) & 1);
       if (!ok) *abort_flag = 1;
-      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + s * kPairACols;
+      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + sa * kPairACols;
       if (!*abort_flag && k >= prm.stages) {
         // 64 ranks of this row of B, twice
         int n0, m0;
@@ -364,7 +374,7 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cta(&afull[s], 0);
+      if (lane == 0) mbar_arrive_cta(&afull[sa], 0);
     }
   } else {
     // ---------------- epilogue ----------------
