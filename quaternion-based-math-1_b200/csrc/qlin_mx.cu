@@ -391,7 +391,8 @@ int pair_capacity() {
 
 // y = x W^T (+ bias) (+ parts B^T) on the CTA-pair kernel: W from codes (mx) or
 // from component planes.  x rows satisfy tma_rows; y 8-byte aligned, ld_y a
-// multiple of 4.
+// multiple of 4.  With an adapter the launch before it is the down projection that
+// makes `parts`.
 template <typename T, int NTOK, bool MX>
 int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& planes, int64_t ld_w, const T* bias,
                 const T* parts, int64_t ld_parts, const T* lora_b, int rank, T* y, int64_t ld_y, int64_t M,

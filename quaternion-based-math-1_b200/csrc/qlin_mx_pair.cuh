@@ -70,6 +70,9 @@ struct MxPairParams {
   int wide;             // 16-byte output pieces are aligned
 };
 
+// Orders what other kernels stored before this thread's copies by the TMA unit.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
 // One lane of the (converged) warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
@@ -149,8 +152,10 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // Everything below reads what earlier kernels of the stream wrote, or writes
-  // what they may read.
-  pdl_wait_prior();
+  // what they may read.  After the down projection, which let this kernel start
+  // only when everything before it had ended, t alone is waited for, by the
+  // thread that fetches it (every output depends on it).
+  if (prm.lora_stages == 0) pdl_wait_prior();
 
   auto tile_coords = [&](int t, int& n0, int& m0) {
     const int nb = t % prm.nb_tiles, tb = t / prm.nb_tiles;
@@ -180,6 +185,10 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           uint8_t* dst = smem + s * Cfg::kStageBytes;
           if (k >= prm.stages) {
             const int r = 64 * (k - prm.stages);
+            if (j == 0 && r == 0) {
+              pdl_wait_prior();
+              fence_proxy_async();
+            }
             mbar_arrive_expect_tx(&full[s], Cfg::kXBytes);
             tma_load_3d(dst, &map_t, &full[s], r, mrow, 0);
             tma_load_3d(dst + Cfg::kXAtomBytes, &map_t, &full[s], r, mrow, 1);
