@@ -7,6 +7,8 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <cmath>
@@ -211,6 +213,68 @@ std::vector<at::Tensor> mx_backward(const at::Tensor& gy, const at::Tensor& x, c
   return {dx, da, db, dbias};
 }
 
+// The layer under autograd, in C++ (a Python function's calls from the backward
+// thread cost about 40 us a step).
+class MxLinear : public torch::autograd::Function<MxLinear> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const OptTensor& bias,
+                            const OptTensor& a, const OptTensor& b, const at::Tensor& mx, int64_t out_groups,
+                            int64_t in_groups, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({x, a.value_or(at::Tensor()), b.value_or(at::Tensor()), mx});
+    ctx->saved_data["n"] = out_groups;
+    ctx->saved_data["k"] = in_groups;
+    ctx->saved_data["s"] = scale;
+    ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+    return mx_forward(x, mx, out_groups, in_groups, bias, a, b, scale);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto opt = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    torch::autograd::variable_list out(8);
+    if (!grads[0].defined()) return out;
+    // the graph's edges are those of the tensors that were given: x, bias, A, B
+    size_t edge = 0;
+    auto wanted = [&](bool given) { return given && ctx->needs_input_grad(edge++); };
+    const bool dx = wanted(true), dbias = wanted(ctx->saved_data["bias"].toBool());
+    const bool da = wanted(saved[1].defined()), db = wanted(saved[2].defined());
+    std::vector<at::Tensor> g;
+    {
+      at::NoGradGuard no_grad;
+      g = mx_backward(grads[0], saved[0], saved[3], ctx->saved_data["n"].toInt(), ctx->saved_data["k"].toInt(),
+                      opt(saved[1]), opt(saved[2]), ctx->saved_data["s"].toDouble(), dx, da, db, dbias);
+    }
+    const int from[4] = {0, 3, 1, 2};  // x, bias, a, b of (dx, da, db, dbias)
+    for (int k = 0; k < 4; ++k) out[k] = g[from[k]];
+    if (at::GradMode::is_enabled()) {
+      // the gradients have none of their own: an error where one is asked for
+      torch::autograd::variable_list there;
+      for (auto& t : out)
+        if (t.defined()) there.push_back(t.detach().requires_grad_(true));
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "mx_quaternion_linear cannot be differentiated twice", static_cast<int64_t>(there.size()));
+      there = (*error)(std::move(there));
+      size_t at = 0;
+      for (auto& t : out)
+        if (t.defined()) t = there[at++];
+    }
+    return out;
+  }
+};
+
+// mx_forward, differentiable in x, bias, A and B.
+at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& mx, int64_t out_groups, int64_t in_groups,
+                     const OptTensor& bias, const OptTensor& a, const OptTensor& b, double scale) {
+  if (at::GradMode::is_enabled()) {
+    auto wants = [](const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); };
+    if (x.requires_grad() || wants(bias) || wants(a) || wants(b))
+      return MxLinear::apply(x, bias, a, b, mx, out_groups, in_groups, scale);
+  }
+  return mx_forward(x, mx, out_groups, in_groups, bias, a, b, scale);
+}
+
 // Clips the gradients of the parameters in place, each gradient once; returns their
 // global norm.  error_if_nonfinite: only a finite one, which the host waits for.
 at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm, bool error_if_nonfinite) {
@@ -275,8 +339,6 @@ at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm,
   return norm;
 }
 
-pybind11::object or_none(const at::Tensor& t) { return t.defined() ? pybind11::cast(t) : pybind11::none(); }
-
 }  // namespace
 
 void register_mx(pybind11::module& m) {
@@ -287,15 +349,9 @@ void register_mx(pybind11::module& m) {
           return mx_dequantize(mx, n, k, torch::python::detail::py_object_to_dtype(dtype));
         },
         "4-bit buffer -> four weight components");
-  m.def("mx_forward", &mx_forward, "quaternion linear forward on 4-bit weights (see qlin_b200.h)", py::arg("x"),
+  m.def("mx_linear", &mx_linear, "quaternion linear layer on 4-bit weights (see qlin_b200.h)", py::arg("x"),
         py::arg("mx"), py::arg("out_groups"), py::arg("in_groups"), py::arg("bias") = py::none(),
-        py::arg("lora_a") = py::none(), py::arg("lora_b") = py::none(), py::arg("lora_scale") = 0.0);
-  m.def("mx_backward",
-        [](const at::Tensor& gy, const at::Tensor& x, const at::Tensor& mx, int64_t n, int64_t k, const OptTensor& a,
-           const OptTensor& b, double scale, bool dx, bool da, bool db, bool dbias) {
-          const auto g = mx_backward(gy, x, mx, n, k, a, b, scale, dx, da, db, dbias);
-          return py::make_tuple(or_none(g[0]), or_none(g[1]), or_none(g[2]), or_none(g[3]));
-        },
-        "gradients of mx_forward");
+        py::arg("lora_a") = py::none(), py::arg("lora_b") = py::none(), py::arg("lora_scale") = 0.0,
+        py::call_guard<py::gil_scoped_release>());
   m.def("clip_grad_norm", &clip_grad_norm, "global norm of the parameters' gradients, clipped in place");
 }

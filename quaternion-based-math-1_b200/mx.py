@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .linear import QuaternionLinear
@@ -72,24 +71,6 @@ def quantize_quaternion_weights(wr, wi, wj, wk) -> MXQuaternionWeights:
     return MXQuaternionWeights(data, wr.shape[0], wr.shape[1])
 
 
-class _MXLinFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weights, bias, lora_a, lora_b, lora_scale):
-        ctx.save_for_backward(x, lora_a, lora_b, weights.data)
-        ctx.groups = (weights.out_groups, weights.in_groups)
-        ctx.lora_scale = lora_scale
-        return _ext().mx_forward(x, weights.data, *ctx.groups, bias, lora_a, lora_b, lora_scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, lora_a, lora_b, data = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, da, db, dbias = _ext().mx_backward(gy, x, data, *ctx.groups, lora_a, lora_b, ctx.lora_scale,
-                                               need[0], need[3], need[4], need[2])
-        return dx, None, dbias, da, db, None
-
-
 def mx_quaternion_linear(x, weights: MXQuaternionWeights, bias=None, lora_a=None, lora_b=None,
                          lora_scale: float = 0.0):
     """``quaternion_linear(x) + bias + lora_scale * (x A^T) B^T`` on 4-bit weights.
@@ -98,12 +79,8 @@ def mx_quaternion_linear(x, weights: MXQuaternionWeights, bias=None, lora_a=None
     ``[r, in_features]`` and B ``[out_features, r]``, all of x's dtype.
     Differentiable once in x, bias, A and B.
     """
-    if torch.is_grad_enabled():
-        for t in (x, bias, lora_a, lora_b):
-            if t is not None and t.requires_grad:
-                return _MXLinFn.apply(x, weights, bias, lora_a, lora_b, float(lora_scale))
-    return _ext().mx_forward(x, weights.data, weights.out_groups, weights.in_groups, bias, lora_a, lora_b,
-                             float(lora_scale))
+    return _ext().mx_linear(x, weights.data, weights.out_groups, weights.in_groups, bias, lora_a, lora_b,
+                            float(lora_scale))
 
 
 class MXQuaternionLinear(nn.Module):

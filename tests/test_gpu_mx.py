@@ -321,6 +321,11 @@ def test_only_wanted_gradients(qb, cuda):
         y.sum().backward()
         for k, t in leaves.items():
             assert (t.grad is not None) == (k == want)
+    # without an adapter, and without a bias
+    for drop, left in ((("a", "b"), ("x", "bias")), (("bias",), ("x", "a", "b"))):
+        leaves = {k: None if k in drop else d[k].clone().requires_grad_(True) for k in ("x", "bias", "a", "b")}
+        qb.mx_quaternion_linear(leaves["x"], q, leaves["bias"], leaves["a"], leaves["b"], 2.0).sum().backward()
+        assert all(leaves[k].grad is not None for k in left)
     # a broadcast gradient (sum) and one with a stride
     x = d["x"].clone().requires_grad_(True)
     y = qb.mx_quaternion_linear(x, q)
