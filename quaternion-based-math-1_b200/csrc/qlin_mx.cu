@@ -273,11 +273,15 @@ int launch_many(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   if (allow_smem(qlin_mx_many_kernel<T, NT, WO>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
   MxFewParams<T> prm = base;
   const int64_t total = ceil_div(prm.tiles, WO) * ceil_div(prm.M, Cfg::kC);
-  const int ctas = (int)std::min<int64_t>(total, sms);
-  const int64_t uses = ceil_div(prm.kb, Cfg::kWK) * ceil_div(total, ctas);
   prm.stage_b = stages_b(prm, WO);
   const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
-  prm.ring = ring_stages(kMostSmem, mx_many_smem<T, NT, WO>(0, prm.rank, b), Cfg::kStage + 16, uses);
+  const size_t fixed = mx_many_smem<T, NT, WO>(0, prm.rank, b), stage = Cfg::kStage + 16;
+  // two CTAs per SM where there are tiles for them and their rings fit
+  constexpr size_t kHalfSm = kMostSmem / 2 - 1024;
+  const bool two = total > sms && fixed + 2 * stage <= kHalfSm;
+  const int ctas = (int)std::min<int64_t>(total, (two ? 2 : 1) * sms);
+  const int64_t uses = ceil_div(prm.kb, Cfg::kWK) * ceil_div(total, ctas);
+  prm.ring = ring_stages(two ? kHalfSm : kMostSmem, fixed, stage, uses);
   const size_t smem = mx_many_smem<T, NT, WO>(prm.ring, prm.rank, b);
   if (smem > kMostSmem) return QLIN_ERR_SHAPE;
   return launch_dependent(qlin_mx_many_kernel<T, NT, WO>, ctas, kMxThreads, smem, s, prm);
@@ -309,11 +313,12 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
   const bool one = is_one(dtype, M, K_g);
   const int C = few_tile(M);
   const int64_t octets = one ? 0 : ceil_div(M, C) * C * 4 * prm.kb;
-  const int64_t blocks = ceil_div(octets, 256), down = rank * ceil_div(M, kMxDownTokens);
+  const int threads = mx_prologue_threads(K_g);
+  const int64_t blocks = ceil_div(octets, threads), down = rank * ceil_div(M, kMxDownTokens);
   if (blocks + down > INT32_MAX) return QLIN_ERR_SHAPE;
   prm.after_prologue = blocks + down > 0;
   if (prm.after_prologue) {
-    const int st = launch_dependent(qlin_mx_prologue_kernel<T>, (unsigned)(blocks + down), 256, 0, s, x, ld_x, (int)M,
+    const int st = launch_dependent(qlin_mx_prologue_kernel<T>, (unsigned)(blocks + down), threads, 0, s, x, ld_x, (int)M,
                                     (int)K_g, prm.kb, C, prm.vec, ws + w.arranged, (int)blocks, octets, a,
                                     (int)aligned(a, 4 * sizeof(T)), rank, scale,
                                     reinterpret_cast<float*>(ws + w.t));
@@ -615,8 +620,8 @@ int run_backward32(const float* g, int64_t ld_g, const float* x, int64_t ld_x, c
   float* up = reinterpret_cast<float*>(ws + w.up);
   int st = QLIN_OK;
   auto down = [&](const float* in, int64_t ld, int64_t groups, const float* rows, float* out) {
-    return launch_dependent(qlin_mx_prologue_kernel<float>, (unsigned)(rank * ceil_div(M, kMxDownTokens)), 256, 0, s,
-                            in, ld, (int)M, (int)groups, 1, 8, (int)(aligned(in, 16) && ld % 4 == 0),
+    return launch_dependent(qlin_mx_prologue_kernel<float>, (unsigned)(rank * ceil_div(M, kMxDownTokens)),
+                            mx_prologue_threads(groups), 0, s, in, ld, (int)M, (int)groups, 1, 8, (int)(aligned(in, 16) && ld % 4 == 0),
                             static_cast<uint8_t*>(nullptr), 0, (int64_t)0, rows, (int)aligned(rows, 16), rank, scale,
                             out);
   };

@@ -621,27 +621,32 @@ __device__ __forceinline__ void mx_arrange_one(const T* x, int64_t ld_x, int M, 
 }
 
 constexpr int kMxDownTokens = 4;  // tokens of a down-projection CTA
+// Threads of a prologue CTA: with 256, rows of 4096 took twice as many dependent
+// rounds of loads.
+constexpr int kMxPrologueMost = 512;
+inline int mx_prologue_threads(int64_t K_g) { return K_g > 512 ? kMxPrologueMost : 256; }
 
 // Blocks [0, arrange_blocks): the B words.  The rest: t[m, r] = scale x A^T,
 // one rank and kMxDownTokens tokens per block, the row of A read once.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kMxPrologueMost)
 qlin_mx_prologue_kernel(const T* __restrict__ x, int64_t ld_x, int M, int K_g, int kb, int C, int vec,
                         uint8_t* __restrict__ arranged, int arrange_blocks, int64_t octets,
                         const T* __restrict__ lora_a, int vec_a, int rank, float scale, float* __restrict__ t) {
   pdl_wait_prior();
   pdl_launch_dependents();
   if ((int)blockIdx.x < arrange_blocks) {
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (idx < octets) mx_arrange_one<T>(x, ld_x, M, K_g, kb, C, vec, arranged, idx);
     return;
   }
-  __shared__ float part[8][kMxDownTokens];
+  __shared__ float part[kMxPrologueMost / 32][kMxDownTokens];
   const int b = (int)blockIdx.x - arrange_blocks;
   const int r = b % rank, m0 = b / rank * kMxDownTokens;
   const T* a = lora_a + (int64_t)r * 4 * K_g;
   float s[kMxDownTokens] = {};
-  for (int i = threadIdx.x; i < K_g; i += 256) {
+#pragma unroll 2
+  for (int i = threadIdx.x; i < K_g; i += blockDim.x) {
     const float4 av = mx_load4(a + 4 * (int64_t)i, vec_a);
 #pragma unroll
     for (int u = 0; u < kMxDownTokens; ++u) {
@@ -660,8 +665,7 @@ qlin_mx_prologue_kernel(const T* __restrict__ x, int64_t ld_x, int M, int K_g, i
   __syncthreads();
   if (threadIdx.x < kMxDownTokens && m0 + (int)threadIdx.x < M) {
     float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) v += part[w][threadIdx.x];
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) v += part[w][threadIdx.x];
     t[(int64_t)(m0 + threadIdx.x) * rank + r] = scale * v;
   }
 }
@@ -689,7 +693,7 @@ constexpr size_t mx_many_smem(int ring, int rank, int b_bytes) {
 }
 
 template <typename T, int NT, int WO>
-__global__ void __launch_bounds__(kMxThreads, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kMxThreads, NT == 1 && sizeof(T) == 2 ? 2 : 1)
 qlin_mx_many_kernel(const MxFewParams<T> prm) {
   using Cfg = MxManyCfg<T, NT, WO>;
   constexpr bool HALF = MxOperand<T>::kHalf;
@@ -767,6 +771,15 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
     const int64_t vt = id / groups, tile0 = (int64_t)(id - (int)vt * groups) * WO;
     uint8_t* bs = bs_both + (j & 1) * (b_bytes / 2);
     if (prm.stage_b) mx_fetch_b<T>(prm, bs, tile0 * 4 * kMxRows, 64 * WO, threadIdx.x, 32 * kMxWarps);
+    if (mx_t_rank(prm.rank) > 0 && (j == 0 || id / groups != (id - (int)gridDim.x) / groups)) {
+      // t of this token tile, once every thread is past the tile before; the
+      // barrier after the products orders it before its readers
+      asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
+      const int64_t first = vt * C * prm.rank;
+      const int count = (int)min((int64_t)C, prm.M - vt * C) * prm.rank;
+      for (int k = 4 * threadIdx.x; k < count; k += 4 * 32 * kMxWarps)
+        cp_async16(smem_u32(ts + k), prm.t + first + k, 4 * min(4, count - k));
+    }
     float acc[NT][4][4] = {};
     for (int st = 0; st < nst; ++st) {
       const int s = r.at;
@@ -804,13 +817,6 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
       r.next(S);
-    }
-    if (mx_t_rank(prm.rank) > 0 && (j == 0 || id / groups != (id - (int)gridDim.x) / groups)) {
-      // t of this token tile (the barrier below orders it before its readers;
-      // the readers of the tile before have passed theirs)
-      asm volatile("bar.sync %0, %1;" ::"n"(kMxFewBar), "n"(32 * kMxWarps) : "memory");
-      const int64_t first = vt * C * prm.rank, count = min((int64_t)C, prm.M - vt * C) * prm.rank;
-      for (int64_t k = threadIdx.x; k < count; k += 32 * kMxWarps) ts[k] = __ldcg(prm.t + first + k);
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt, ++round) {
