@@ -76,8 +76,13 @@ bool streams(int dtype, int64_t M, int64_t N_g) {
 }
 
 // Tokens of a tile of the streaming kernels (one or two tokens apart): the
-// smallest tile that holds them all, at most 32.
-int few_tile(int64_t M) { return M <= 8 ? 8 : (M <= 16 ? 16 : 32); }
+// smallest tile that holds them all, at most 32; 16 where tiles of 32 (and four of
+// 16 output quaternions) would leave half of the SMs without one, in fp32, which
+// comes here with many tokens.
+int few_tile(int dtype, int64_t M, int64_t N_g) {
+  if (M <= 16) return M <= 8 ? 8 : 16;
+  return dtype == QLIN_F32 && ceil_div(N_g, 4 * kMxRows) * ceil_div(M, 32) < 74 ? 16 : 32;
+}
 
 // One or two tokens whose B words fit beside the ring.
 constexpr size_t kOneMaxX = 150 * 1024;
@@ -100,7 +105,7 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   Carve c;
   if (streams(dtype, M, N_g)) {
     if (!is_one(dtype, M, K_g)) {
-      const int64_t C = few_tile(M);
+      const int64_t C = few_tile(dtype, M, N_g);
       w.arranged = c.take(ceil_div(M, C) * ceil_div(K_g, kMxBlock) * (dtype == QLIN_F32 ? 3 : 1) * 4 * C * 64);
     }
     w.t = c.take(M * rank * 4);
@@ -115,12 +120,10 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
 }
 
 struct BackwardWs {
-  // 16-bit
+  // (fp32: planes are wide records, gy its B words)
   size_t gy = 0, x = 0, a = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0, sums = 0;
   int64_t M_pad = 0, ld_parts = 0, ld_planes = 0;
   int rows = 0, splits0 = 0, splits1 = 0;
-  // fp32
-  size_t inner = 0, inner_bytes = 0;
   size_t total = 0;
 };
 
@@ -141,8 +144,11 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
   BackwardWs w;
   Carve c;
   if (dtype == QLIN_F32) {
-    w.planes = c.take(4 * K_g * N_g * 4);
+    const int64_t C = few_tile(dtype, M, K_g);
+    w.planes = c.take(ceil_div(K_g, kMxRows) * ceil_div(N_g, kMxBlock) * kMxWideRecord);
+    w.gy = c.take(ceil_div(M, C) * ceil_div(N_g, kMxBlock) * 3 * 4 * C * 64);
     if (rank > 0) {
+      w.at = c.take(4 * K_g * rank * 4);
       w.splits0 = outer32_splits(M, 4 * K_g, rank);
       w.splits1 = outer32_splits(M, 4 * N_g, rank);
       w.bt = c.take(4 * N_g * rank * 4);
@@ -152,8 +158,6 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
       w.partial1 = c.take((int64_t)w.splits1 * rank * 4 * N_g * 4);
       w.sums = c.take((int64_t)w.splits1 * 4 * N_g * 4);
     }
-    qlin_workspace_size(dtype, M, N_g, K_g, 0, &w.inner_bytes);
-    w.inner = c.take((int64_t)w.inner_bytes);
   } else {
     const int64_t K = 4 * K_g, N = 4 * N_g;
     w.M_pad = round_up(M, kMxOuterTokens);
@@ -179,13 +183,6 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
   }
   w.total = c.at;
   return w;
-}
-
-template <typename T>
-MxPlanes<T> planes_at(void* base, int64_t K_g, int64_t N_g) {
-  MxPlanes<T> p;
-  for (int c = 0; c < 4; ++c) p.w[c] = static_cast<T*>(base) + c * K_g * N_g;
-  return p;
 }
 
 // CTAs of the record kernels: a warp takes half a record, at most 64 CTAs per SM
@@ -266,25 +263,41 @@ int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   return launch_dependent(qlin_mx_one_kernel<T, W, G>, ctas, 32 * (W + 1) * G, smem, s, prm);
 }
 
-template <typename T, int NT, int WO>
+template <typename T, int NT, int WO, bool WIDE = false>
 int launch_many(const MxFewParams<T>& base, int sms, cudaStream_t s) {
-  using Cfg = MxManyCfg<T, NT, WO>;
+  using Cfg = MxManyCfg<T, NT, WO, WIDE>;
   static std::atomic<uint64_t> done{0};
-  if (allow_smem(qlin_mx_many_kernel<T, NT, WO>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
+  if (allow_smem(qlin_mx_many_kernel<T, NT, WO, WIDE>, done) != QLIN_OK) return QLIN_ERR_LAUNCH;
   MxFewParams<T> prm = base;
   const int64_t total = ceil_div(prm.tiles, WO) * ceil_div(prm.M, Cfg::kC);
   prm.stage_b = stages_b(prm, WO);
   const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
-  const size_t fixed = mx_many_smem<T, NT, WO>(0, prm.rank, b), stage = Cfg::kStage + 16;
+  const size_t fixed = mx_many_smem<T, NT, WO, WIDE>(0, prm.rank, b), stage = Cfg::kStage + 16;
   // two CTAs per SM where there are tiles for them and their rings fit
   constexpr size_t kHalfSm = kMostSmem / 2 - 1024;
   const bool two = total > sms && fixed + 2 * stage <= kHalfSm;
   const int ctas = (int)std::min<int64_t>(total, (two ? 2 : 1) * sms);
   const int64_t uses = ceil_div(prm.kb, Cfg::kWK) * ceil_div(total, ctas);
   prm.ring = ring_stages(two ? kHalfSm : kMostSmem, fixed, stage, uses);
-  const size_t smem = mx_many_smem<T, NT, WO>(prm.ring, prm.rank, b);
+  const size_t smem = mx_many_smem<T, NT, WO, WIDE>(prm.ring, prm.rank, b);
   if (smem > kMostSmem) return QLIN_ERR_SHAPE;
-  return launch_dependent(qlin_mx_many_kernel<T, NT, WO>, ctas, kMxThreads, smem, s, prm);
+  return launch_dependent(qlin_mx_many_kernel<T, NT, WO, WIDE>, ctas, kMxThreads, smem, s, prm);
+}
+
+// The B words of x (none for `one`) and the scaled down projection, in the workspace.
+template <typename T>
+int few_prologue(const MxFewParams<T>& prm, bool one, const T* a, float scale, uint8_t* arranged, float* t,
+                 cudaStream_t s) {
+  const int C = few_tile(sizeof(T) == 4 ? QLIN_F32 : QLIN_BF16, prm.M, prm.N_g);
+  const int threads = mx_prologue_threads(prm.K_g);
+  const int64_t octets = one ? 0 : ceil_div(prm.M, C) * C * 4 * prm.kb;
+  const int64_t blocks = ceil_div(octets, threads), down = prm.rank * ceil_div(prm.M, kMxDownTokens);
+  if (blocks + down > INT32_MAX) return QLIN_ERR_SHAPE;
+  if (blocks + down == 0) return QLIN_OK;
+  const int vec = aligned(prm.x, 4 * sizeof(T)) && prm.ld_x % 4 == 0;
+  return launch_dependent(qlin_mx_prologue_kernel<T>, (unsigned)(blocks + down), threads, 0, s, prm.x, prm.ld_x, prm.M,
+                          prm.K_g, prm.kb, C, vec, arranged, (int)blocks, octets, a,
+                          (int)aligned(a, 4 * sizeof(T)), prm.rank, scale, t);
 }
 
 // The streaming kernels: a prologue where there are B words to arrange or an
@@ -297,6 +310,7 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
   prm.x = x;
   prm.ld_x = ld_x;
   prm.mx = static_cast<const uint8_t*>(mx);
+  prm.records = prm.mx + kMxHeader;
   prm.arranged = ws + w.arranged;
   prm.bias = bias;
   prm.lora_b = b;
@@ -309,28 +323,19 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
   prm.rank = rank;
   prm.kb = (int)ceil_div(K_g, kMxBlock);
   prm.tiles = (int)ceil_div(N_g, kMxRows);
-  prm.vec = aligned(x, 4 * sizeof(T)) && ld_x % 4 == 0;
   const bool one = is_one(dtype, M, K_g);
-  const int C = few_tile(M);
-  const int64_t octets = one ? 0 : ceil_div(M, C) * C * 4 * prm.kb;
-  const int threads = mx_prologue_threads(K_g);
-  const int64_t blocks = ceil_div(octets, threads), down = rank * ceil_div(M, kMxDownTokens);
-  if (blocks + down > INT32_MAX) return QLIN_ERR_SHAPE;
-  prm.after_prologue = blocks + down > 0;
-  if (prm.after_prologue) {
-    const int st = launch_dependent(qlin_mx_prologue_kernel<T>, (unsigned)(blocks + down), threads, 0, s, x, ld_x, (int)M,
-                                    (int)K_g, prm.kb, C, prm.vec, ws + w.arranged, (int)blocks, octets, a,
-                                    (int)aligned(a, 4 * sizeof(T)), rank, scale,
-                                    reinterpret_cast<float*>(ws + w.t));
-    if (st != QLIN_OK) return st;
-  }
+  const int C = few_tile(dtype, M, N_g);
+  const int st = few_prologue(prm, one, a, scale, ws + w.arranged, reinterpret_cast<float*>(ws + w.t), s);
+  if (st != QLIN_OK) return st;
   if (one) {
+    prm.after_prologue = rank > 0;
+    // x by bulk copies
     prm.vec = aligned(x, 16) && (4 * K_g * sizeof(T)) % 16 == 0 && (M == 1 || (ld_x * sizeof(T)) % 16 == 0);
     // at most a tile per SM, or x too long for three rings: 16 warps share the
     // tile's K; more tiles: three groups of 8 warps
     if (prm.tiles > sms) {
-      const int st = launch_one<T, 8, 3>(prm, sms, s);
-      if (st != QLIN_ERR_SHAPE) return st;
+      const int e = launch_one<T, 8, 3>(prm, sms, s);
+      if (e != QLIN_ERR_SHAPE) return e;
     }
     return launch_one<T, 16, 1>(prm, sms, s);
   }
@@ -609,44 +614,63 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
   return st != QLIN_OK ? st : launched();
 }
 
-// Gradients, fp32: the adjoint's components through qlin_forward_ex, the adapter on
-// the CUDA cores.
+// Gradients, fp32: dx by the streaming kernel on the adjoint's wide records, the
+// adapter's on the CUDA cores.
 int run_backward32(const float* g, int64_t ld_g, const float* x, int64_t ld_x, const void* mx, const float* a,
                    const float* b, int rank, float scale, float* dx, int64_t ld_dx, float* da, float* db, float* dbias,
                    int64_t M, int64_t K_g, int64_t N_g, uint8_t* ws, const BackwardWs& w, int sms, cudaStream_t s) {
   const int64_t K = 4 * K_g, N = 4 * N_g;
+  float* at = reinterpret_cast<float*>(ws + w.at);
   float* bt = reinterpret_cast<float*>(ws + w.bt);
   float* t = reinterpret_cast<float*>(ws + w.t);
   float* up = reinterpret_cast<float*>(ws + w.up);
+  uint8_t* arranged = ws + w.gy;
+  const bool need_up = rank > 0 && (dx || da);
   int st = QLIN_OK;
-  auto down = [&](const float* in, int64_t ld, int64_t groups, const float* rows, float* out) {
-    return launch_dependent(qlin_mx_prologue_kernel<float>, (unsigned)(rank * ceil_div(M, kMxDownTokens)),
-                            mx_prologue_threads(groups), 0, s, in, ld, (int)M, (int)groups, 1, 8, (int)(aligned(in, 16) && ld % 4 == 0),
-                            static_cast<uint8_t*>(nullptr), 0, (int64_t)0, rows, (int)aligned(rows, 16), rank, scale,
-                            out);
-  };
-  if (rank * ceil_div(M, kMxDownTokens) > INT32_MAX) return QLIN_ERR_SHAPE;
-  if (rank > 0 && (dx || da)) {
-    st = launch_dependent(qlin_mx_turn_kernel<float>, (unsigned)ceil_div(rank * N, 256), 256, 0, s, b, bt, N,
-                          (int64_t)rank);
-    if (st == QLIN_OK) st = down(g, ld_g, N_g, bt, up);
-  }
-  if (st == QLIN_OK && db) st = down(x, ld_x, K_g, a, t);
-  if (st != QLIN_OK) return st;
-  if (dx) {
-    const MxPlanes<float> p = planes_at<float>(ws + w.planes, K_g, N_g);
-    const int64_t steps = ceil_div(N_g, 64) * ceil_div(K_g, kMxBlock);
-    st = launch_dependent(qlin_mx_adjoint_kernel<float>, (unsigned)std::min<int64_t>(steps, 8ll * sms), 256, 0, s,
-                          static_cast<const uint8_t*>(mx), p, N_g, (int)K_g, (int)N_g);
+  if (dx || need_up) {
+    MxPlanes<float> records{};
+    records.w[0] = reinterpret_cast<float*>(ws + w.planes);
+    const int64_t steps = dx ? ceil_div(N_g, kMxTurnRows) * ceil_div(K_g, kMxBlock) : 0;
+    const int64_t a_blocks = dx ? ceil_div(rank * K, 256) : 0, b_blocks = need_up ? ceil_div(rank * N, 256) : 0;
+    if (steps + a_blocks + b_blocks > INT32_MAX) return QLIN_ERR_SHAPE;
+    st = launch_dependent(qlin_mx_turn_all_kernel<float>, (unsigned)(steps + a_blocks + b_blocks), 256, 0, s,
+                          static_cast<const uint8_t*>(mx), records, (int64_t)0, (int)K_g, (int)N_g, steps, a, at,
+                          (int64_t)rank, K, b, bt, N, (int64_t)rank, N, a_blocks);
     if (st != QLIN_OK) return st;
-    st = qlin_forward_ex(QLIN_F32, g, ld_g, p.w[0], p.w[1], p.w[2], p.w[3], N_g, nullptr, nullptr, nullptr, 0, 0.f, dx,
-                         ld_dx, M, N_g, K_g, ws + w.inner, w.inner_bytes, QLIN_ALGO_AUTO, 0, s);
+    MxFewParams<float> prm{};
+    prm.x = g;
+    prm.ld_x = ld_g;
+    prm.mx = static_cast<const uint8_t*>(mx);
+    prm.records = ws + w.planes;
+    prm.arranged = arranged;
+    prm.lora_b = at;
+    prm.t = up;
+    prm.y = dx;
+    prm.ld_y = ld_dx;
+    prm.M = (int)M;
+    prm.K_g = (int)N_g;
+    prm.N_g = (int)K_g;
+    prm.rank = rank;
+    prm.kb = (int)ceil_div(N_g, kMxBlock);
+    prm.tiles = (int)ceil_div(K_g, kMxRows);
+    st = few_prologue(prm, !dx, (const float*)bt, scale, arranged, up, s);
     if (st != QLIN_OK) return st;
-    if (rank > 0) {
-      const dim3 grid((unsigned)ceil_div(K, 256), (unsigned)ceil_div(M, 8));
-      if (grid.y > 65535) return QLIN_ERR_SHAPE;
-      qlin_mx_add_adapter32_kernel<<<grid, 256, 0, s>>>(up, a, rank, dx, ld_dx, M, K);
+    if (dx) {
+      const int C = few_tile(QLIN_F32, M, K_g);
+      st = C == 8 ? launch_many<float, 1, 1, true>(prm, sms, s)
+                  : (C == 16 ? launch_many<float, 2, 2, true>(prm, sms, s) : launch_many<float, 4, 4, true>(prm, sms, s));
+      if (st != QLIN_OK) return st;
     }
+  }
+  if (db) {
+    MxFewParams<float> prm{};
+    prm.x = x;
+    prm.ld_x = ld_x;
+    prm.M = (int)M;
+    prm.K_g = (int)K_g;
+    prm.rank = rank;
+    st = few_prologue(prm, true, a, scale, static_cast<uint8_t*>(nullptr), t, s);
+    if (st != QLIN_OK) return st;
   }
   const bool sum_with_db = db && dbias;
   if (da || db) {

@@ -253,40 +253,4 @@ qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst,
   }
 }
 
-// The weights of the adjoint layer, conj(W)^T, in fp32 as four component rows
-// [K_g, N_g]: 64 output quaternions x 32 input quaternions of one component
-// per CTA step, turned through shared memory.
-template <typename T>
-__global__ void __launch_bounds__(256)
-qlin_mx_adjoint_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g) {
-  __shared__ T turn[4][kMxBlock][66];
-  pdl_wait_prior();
-  pdl_launch_dependents();
-  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
-  const int64_t groups = (tiles + 3) / 4;
-  const int t = threadIdx.x & 3, p = (threadIdx.x >> 2) & 3, row = threadIdx.x >> 4;
-  for (int64_t step = blockIdx.x; step < groups * kb; step += gridDim.x) {
-    const int64_t g = step / kb, b = step - g * kb;
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t tile = 4 * g + u;
-      if (tile >= tiles) break;
-      const uint8_t* in = mx + kMxHeader + (tile * kb + b) * kMxRecord;
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4);
-      const float s = mx_scale(in[kMxCodeBytes + row * 4 + p]) * (p == 0 ? 1.f : -1.f);
-      float c[8];
-      mx_values(word, c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) turn[p][8 * t + j][16 * u + row] = from_f32<T>(c[j] * s);
-    }
-    __syncthreads();
-    const int64_t o0 = 64 * g;
-    for (int k = threadIdx.x; k < 4 * kMxBlock * 64; k += 256) {
-      const int c = k & 63, i = (k >> 6) & 31, q = k >> 11;
-      if (o0 + c < N_g && b * kMxBlock + i < K_g) dst.w[q][(b * kMxBlock + i) * ld + o0 + c] = turn[q][i][c];
-    }
-  }
-}
-
 }  // namespace qlin

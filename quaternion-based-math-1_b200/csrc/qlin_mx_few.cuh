@@ -275,7 +275,8 @@ template <typename T>
 struct MxFewParams {
   const T* x;
   int64_t ld_x;
-  const uint8_t* mx;
+  const uint8_t* records;   // [tile][block]
+  const uint8_t* mx;        // the codes' header (F0)
   const uint8_t* arranged;  // B words of all tokens (more than two tokens)
   const T* bias;
   const T* lora_b;          // [4 N_g, rank]
@@ -439,7 +440,7 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
       int issued = 0;
       bool ok = true;
       for (int tile = id; tile < prm.tiles && ok; tile += stride) {
-        const uint8_t* src = prm.mx + kMxHeader + (int64_t)tile * kb * kMxRecord;
+        const uint8_t* src = prm.records + (int64_t)tile * kb * kMxRecord;
         for (int st = 0; st < nst; ++st) {
           if (issued >= S && !mbar_wait(&empty[r.at], r.phase ^ 1u)) {
             ok = false;
@@ -674,30 +675,48 @@ qlin_mx_prologue_kernel(const T* __restrict__ x, int64_t ld_x, int M, int K_g, i
 // more tokens: NT groups of eight per tile, WO tiles of output quaternions per
 // CTA (WO warps side by side, kMxWarps / WO along the blocks)
 // ---------------------------------------------------------------------------
-template <typename T, int NT, int WO>
+// Records of the adjoint, conj(W)^T 2^-c, for fp32 gradients: the same 16 x 32
+// quaternions as bf16 pairs (k, k + 4) ready for the operand,
+// [component][16 rows][4 octets][4 words] (a code's value times its scale is exact
+// in bf16).
+constexpr int kMxWideRecord = 4 * kMxRows * 4 * 16;
+
+template <bool HALF>
+__device__ __forceinline__ void mx_load_a_wide(uint32_t rec, int g, int t, uint32_t (&lo)[4][4], uint32_t (&hi)[4][4]) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint4 l = lds128(rec + p * 1024 + (g * 4 + t) * 16), h = lds128(rec + p * 1024 + ((g + 8) * 4 + t) * 16);
+    lo[p][0] = l.x; lo[p][1] = l.y; lo[p][2] = l.z; lo[p][3] = l.w;
+    hi[p][0] = h.x; hi[p][1] = h.y; hi[p][2] = h.z; hi[p][3] = h.w;
+  }
+}
+
+// WIDE: the records are wide ones.
+template <typename T, int NT, int WO, bool WIDE>
 struct MxManyCfg {
   static constexpr int kP = MxOperand<T>::kParts;
+  static constexpr int kRecord = WIDE ? kMxWideRecord : kMxRecord;
   static constexpr int kC = 8 * NT;                      // tokens of a tile
   static constexpr int kWK = kMxWarps / WO;              // blocks of a stage
   static constexpr int kXBlock = kP * 4 * kC * 64;       // B words of a block
-  static constexpr int kStage = kWK * (WO * kMxRecord + kXBlock);
+  static constexpr int kStage = kWK * (WO * kRecord + kXBlock);
   static constexpr int kRed = kMxWarps * 8 * kMxRedRow * 4;  // partial sums of eight tokens
   static constexpr int kFixed = 2 * kRed + 64;  // without t and rows of lora_b
   static_assert(kStage % 16 == 0, "copies of whole 16-byte pieces");
 };
 
-template <typename T, int NT, int WO>
+template <typename T, int NT, int WO, bool WIDE>
 constexpr size_t mx_many_smem(int ring, int rank, int b_bytes) {
-  using Cfg = MxManyCfg<T, NT, WO>;
+  using Cfg = MxManyCfg<T, NT, WO, WIDE>;
   return (size_t)ring * (Cfg::kStage + 16) + Cfg::kFixed + (size_t)Cfg::kC * mx_t_rank(rank) * 4 + b_bytes;
 }
 
-template <typename T, int NT, int WO>
+template <typename T, int NT, int WO, bool WIDE>
 __global__ void __launch_bounds__(kMxThreads, NT == 1 && sizeof(T) == 2 ? 2 : 1)
 qlin_mx_many_kernel(const MxFewParams<T> prm) {
-  using Cfg = MxManyCfg<T, NT, WO>;
+  using Cfg = MxManyCfg<T, NT, WO, WIDE>;
   constexpr bool HALF = MxOperand<T>::kHalf;
-  constexpr int P = Cfg::kP, C = Cfg::kC, WK = Cfg::kWK;
+  constexpr int P = Cfg::kP, C = Cfg::kC, WK = Cfg::kWK, kRecord = Cfg::kRecord;
   extern __shared__ __align__(128) uint8_t mx_smem[];
   const int S = prm.ring, kb = prm.kb;
   const int b_bytes = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
@@ -741,11 +760,10 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
           const int b0 = st * WK, nb = min(WK, kb - b0);
           const int rows = min(WO, prm.tiles - (int)tile0);
           uint8_t* dst = mx_smem + s * Cfg::kStage;
-          mbar_arrive_expect_tx(&full[s], nb * (rows * kMxRecord + Cfg::kXBlock));
+          mbar_arrive_expect_tx(&full[s], nb * (rows * kRecord + Cfg::kXBlock));
           for (int w = 0; w < rows; ++w)
-            bulk_load(dst + w * WK * kMxRecord, prm.mx + kMxHeader + ((tile0 + w) * kb + b0) * kMxRecord,
-                      nb * kMxRecord, &full[s]);
-          bulk_load(dst + WO * WK * kMxRecord, prm.arranged + (vt * kb + b0) * Cfg::kXBlock, nb * Cfg::kXBlock,
+            bulk_load(dst + w * WK * kRecord, prm.records + ((tile0 + w) * kb + b0) * kRecord, nb * kRecord, &full[s]);
+          bulk_load(dst + WO * WK * kRecord, prm.arranged + (vt * kb + b0) * Cfg::kXBlock, nb * Cfg::kXBlock,
                     &full[s]);
           r.next(S);
           ++issued;
@@ -787,8 +805,9 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
       if (st * WK + wk < kb && tile0 + wo < prm.tiles) {
         const uint32_t base = smem_u32(mx_smem) + s * Cfg::kStage;
         uint32_t lo[4][4], hi[4][4];
-        mx_load_a<HALF>(pw, base + (wo * WK + wk) * kMxRecord, g, t, c, lo, hi);
-        const uint32_t xb = base + WO * WK * kMxRecord + wk * Cfg::kXBlock + g * 64 + t * 16;
+        if constexpr (WIDE) mx_load_a_wide<HALF>(base + (wo * WK + wk) * kRecord, g, t, lo, hi);
+        else mx_load_a<HALF>(pw, base + (wo * WK + wk) * kRecord, g, t, c, lo, hi);
+        const uint32_t xb = base + WO * WK * kRecord + wk * Cfg::kXBlock + g * 64 + t * 16;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float d[4][4] = {};

@@ -38,22 +38,12 @@ qlin_mx_column_sum_kernel(const T* __restrict__ g, int64_t ld_g, T* __restrict__
   }
 }
 
-// dst[c][r] = src[r][c]
-template <typename T>
-__global__ void __launch_bounds__(256)
-qlin_mx_turn_kernel(const T* __restrict__ src, T* __restrict__ dst, int64_t rows, int64_t cols) {
-  pdl_wait_prior();
-  pdl_launch_dependents();
-  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  // consecutive threads write consecutive elements
-  if (k < rows * cols) dst[k] = src[(k % rows) * cols + k / rows];
-}
-
 constexpr int kMxTurnRows = 64;  // output quaternions of a step
 
-// What the 16-bit gradients need turned, in one launch: blocks [0, steps) make
-// the components of conj(W)^T 2^-c (rows of ld elements), the next a_blocks A^T,
-// the rest B^T (rows of ld_bt elements, zero past B's rows).  A step is 64 output x 32 input quaternions; a thread takes two
+// What the gradients need turned, in one launch: blocks [0, steps) make the
+// components of conj(W)^T 2^-c (16-bit types: rows of ld elements; fp32: the wide
+// records of qlin_mx_few.cuh at dst.w[0]), the next a_blocks A^T, the rest B^T
+// (rows of ld_bt elements, zero past B's rows).  A step is 64 output x 32 input quaternions; a thread takes two
 // neighbouring output quaternions, eight input quaternions and two components,
 // so that the turned pairs go to shared memory as words, a warp's in a row.
 template <typename T>
@@ -113,14 +103,31 @@ qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, i
     }
   }
   __syncthreads();
-  // 16-byte pieces: eight output quaternions of a row (rows of ld, a multiple of 8)
+  if constexpr (sizeof(T) == 4) {
+    // words (k, k + 4) of an octet of outputs, by [input tile][output block]: two
+    // tiles of 16 input quaternions, two blocks of 32 output quaternions
+    const int64_t in_tiles = (K_g + kMxRows - 1) / kMxRows, out_blocks = (N_g + kMxBlock - 1) / kMxBlock;
+    uint8_t* records = reinterpret_cast<uint8_t*>(dst.w[0]);
+    for (int k = threadIdx.x; k < 4 * 4 * kMxRows * 16; k += 256) {
+      const int word = k & 3, t = (k >> 2) & 3, r = (k >> 4) & 15, p = (k >> 8) & 3, half = (k >> 10) & 1, bl = k >> 11;
+      const int64_t it = 2 * blk + half, ob = 2 * og + bl;
+      if (it >= in_tiles || ob >= out_blocks) continue;
+      const uint32_t* row = turned[p * kMxBlock + kMxRows * half + r];
+      const int o = 32 * bl + 8 * t + word;  // and o + 4
+      const uint32_t lo = row[o >> 1], hi = row[(o + 4) >> 1];
+      *reinterpret_cast<uint32_t*>(records + (it * out_blocks + ob) * kMxWideRecord + ((p * kMxRows + r) * 4 + t) * 16 +
+                                   word * 4) = __byte_perm(lo, hi, (o & 1) ? 0x7632 : 0x5410);
+    }
+  } else {
+    // 16-byte pieces: eight output quaternions of a row (rows of ld, a multiple of 8)
 #pragma unroll
-  for (int k = threadIdx.x; k < 4 * kMxBlock * 8; k += 256) {
-    const int piece = k & 7, i = (k >> 3) & 31, p = k >> 8;
-    const int64_t o = og * kMxTurnRows + 8 * piece, in = blk * kMxBlock + i;
-    if (o < ld && in < K_g)
-      *reinterpret_cast<uint4*>(dst.w[p] + in * ld + o) =
-          *reinterpret_cast<const uint4*>(&turned[p * kMxBlock + i][4 * piece]);
+    for (int k = threadIdx.x; k < 4 * kMxBlock * 8; k += 256) {
+      const int piece = k & 7, i = (k >> 3) & 31, p = k >> 8;
+      const int64_t o = og * kMxTurnRows + 8 * piece, in = blk * kMxBlock + i;
+      if (o < ld && in < K_g)
+        *reinterpret_cast<uint4*>(dst.w[p] + in * ld + o) =
+            *reinterpret_cast<const uint4*>(&turned[p * kMxBlock + i][4 * piece]);
+    }
   }
 }
 
@@ -473,26 +480,6 @@ qlin_mx_outer32_kernel(const __grid_constant__ MxOuterJob<float> job0, const __g
     if (r0 + r < job.rows)
       job.partial[((int64_t)split * job.rows + r0 + r) * job.cols + c] = reinterpret_cast<const float*>(acc)[r];
   if (job.sums && rt == 0) job.sums[(int64_t)split * job.cols + c] = sum;
-}
-
-// dx[m, k] += sum_r up[m, r] A[r, k]
-__global__ void __launch_bounds__(256)
-qlin_mx_add_adapter32_kernel(const float* __restrict__ up, const float* __restrict__ a, int rank,
-                             float* __restrict__ dx, int64_t ld_dx, int64_t M, int64_t K) {
-  pdl_wait_prior();
-  pdl_launch_dependents();
-  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, m0 = (int64_t)blockIdx.y * 8;
-  if (k >= K) return;
-  float v[8] = {};
-  for (int r = 0; r < rank; ++r) {
-    const float av = __ldcg(a + (int64_t)r * K + k);
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (m0 + u < M) v[u] = fmaf(__ldcg(up + (m0 + u) * rank + r), av, v[u]);
-  }
-#pragma unroll
-  for (int u = 0; u < 8; ++u)
-    if (m0 + u < M) dx[(m0 + u) * ld_dx + k] += v[u];
 }
 
 // Adds the splits up: da [rank, cols] from job0's; db [cols, rank] and dbias
