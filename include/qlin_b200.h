@@ -453,6 +453,10 @@ int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g,
  * with the weights that mx stands for.  x, bias, LoRA A/B and y share dtype;
  * accumulation is fp32, outputs are rounded once.  Arguments as qlin_forward;
  * workspace of at least qlin_mx_workspace_size() bytes, 256-byte aligned.
+ * 16-bit types with more than 32 tokens want y 8-byte aligned and ld_y a multiple
+ * of 4 (QLIN_ERR_ALIGN).  fp16 with a LoRA wants |lora_b| up to 1000 there, and
+ * fp16 values of the scaled down projection.  Waits inside the kernels are bounded
+ * (qlin_get_device_error).
  */
 int qlin_mx_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes);
 int qlin_mx_forward(int dtype,
@@ -470,7 +474,8 @@ int qlin_mx_forward(int dtype,
  *   db    [4 N_g, rank]   lora_scale * gy^T (x A^T)
  *   dbias [4 N_g]         sum over the tokens of gy
  * x is read for da and db, mx for dx (either may be NULL where it is not).
- * M = 0 leaves dx alone and zeroes the others.
+ * M = 0 leaves dx alone and zeroes the others.  dx (16-bit types): 8-byte
+ * aligned, ld_dx a multiple of 4.
  */
 int qlin_mx_backward_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes);
 int qlin_mx_backward(int dtype,

@@ -147,7 +147,7 @@ __device__ __forceinline__ double clip_block_sum(double v, double* slots) {
 // partials[blockIdx.x] = this CTA's share of the sum of squares.
 template <int CAP>
 __global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm)
-qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __restrict__ partials) {
+qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* partials) {
   __shared__ double slots[kClipThreads / 32];
   pdl_wait_prior();
   pdl_launch_dependents();
@@ -172,8 +172,8 @@ qlin_grad_norm_kernel(const __grid_constant__ ClipTable<CAP> tab, double* __rest
 // Every CTA adds up all partial sums (in the same order) and scales its pieces.
 template <int CAP>
 __global__ void __launch_bounds__(kClipThreads, kClipCtasPerSm)
-qlin_grad_scale_kernel(const __grid_constant__ ClipTable<CAP> tab, const double* __restrict__ partials, int n_partials,
-                       float max_norm, float* __restrict__ norm_out) {
+qlin_grad_scale_kernel(const __grid_constant__ ClipTable<CAP> tab, const double* partials, int n_partials,
+                       float max_norm, float* norm_out) {
   __shared__ double slots[kClipThreads / 32];
   pdl_wait_prior();
   pdl_launch_dependents();

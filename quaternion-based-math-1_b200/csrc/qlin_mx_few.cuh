@@ -603,7 +603,7 @@ qlin_mx_one_kernel(const MxFewParams<T> prm) {
 // arranged[token tile of C][block][part][q][token][t]: C * 4 * parts * 64 bytes a block.
 template <typename T>
 __device__ __forceinline__ void mx_arrange_one(const T* x, int64_t ld_x, int M, int K_g, int kb, int C, bool vec,
-                                               uint8_t* __restrict__ out, int64_t idx) {
+                                               uint8_t* out, int64_t idx) {
   constexpr int P = MxOperand<T>::kParts;
   // consecutive threads: consecutive octets of a token
   const int64_t m = idx / (4 * kb);
@@ -631,9 +631,9 @@ inline int mx_prologue_threads(int64_t K_g) { return K_g > 512 ? kMxPrologueMost
 // one rank and kMxDownTokens tokens per block, the row of A read once.
 template <typename T>
 __global__ void __launch_bounds__(kMxPrologueMost)
-qlin_mx_prologue_kernel(const T* __restrict__ x, int64_t ld_x, int M, int K_g, int kb, int C, int vec,
-                        uint8_t* __restrict__ arranged, int arrange_blocks, int64_t octets,
-                        const T* __restrict__ lora_a, int vec_a, int rank, float scale, float* __restrict__ t) {
+qlin_mx_prologue_kernel(const T* x, int64_t ld_x, int M, int K_g, int kb, int C, int vec,
+                        uint8_t* arranged, int arrange_blocks, int64_t octets,
+                        const T* lora_a, int vec_a, int rank, float scale, float* t) {
   pdl_wait_prior();
   pdl_launch_dependents();
   if ((int)blockIdx.x < arrange_blocks) {

@@ -10,6 +10,9 @@
 // products are warp-level tensor-core ones (m16n8k16) whose k slots are numbered
 // so that a lane reads eight consecutive elements of a row in one 16-byte piece
 // for both operands.
+//
+// (Inputs are not declared restrict: the compiler may read through such pointers
+// before the dependency wait.)
 #pragma once
 
 #include "qlin_common.cuh"
@@ -20,7 +23,7 @@ namespace qlin {
 // out[n] = sum_m g[m, n]
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_column_sum_kernel(const T* __restrict__ g, int64_t ld_g, T* __restrict__ out, int64_t M, int64_t N) {
+qlin_mx_column_sum_kernel(const T* g, int64_t ld_g, T* out, int64_t M, int64_t N) {
   __shared__ float part[8][32];
   pdl_wait_prior();
   pdl_launch_dependents();
@@ -48,9 +51,9 @@ constexpr int kMxTurnRows = 64;  // output quaternions of a step
 // so that the turned pairs go to shared memory as words, a warp's in a row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
-                        int64_t steps, const T* __restrict__ a, T* __restrict__ at, int64_t a_rows, int64_t a_cols,
-                        const T* __restrict__ b, T* __restrict__ bt, int64_t b_rows, int64_t b_cols, int64_t ld_bt,
+qlin_mx_turn_all_kernel(const uint8_t* mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
+                        int64_t steps, const T* a, T* at, int64_t a_rows, int64_t a_cols,
+                        const T* b, T* bt, int64_t b_rows, int64_t b_cols, int64_t ld_bt,
                         int64_t a_blocks) {
   constexpr bool HALF = std::is_same<T, __half>::value;
   __shared__ __align__(16) uint32_t turned[4 * kMxBlock][36];  // [component, input quaternion][pair of outputs]
@@ -135,7 +138,7 @@ qlin_mx_turn_all_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, i
 // load takes.
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_repack_kernel(const T* __restrict__ src, int64_t ld_s, T* __restrict__ dst, int64_t ld_d, int64_t rows,
+qlin_mx_repack_kernel(const T* src, int64_t ld_s, T* dst, int64_t ld_d, int64_t rows,
                       int64_t cols) {
   pdl_wait_prior();
   pdl_launch_dependents();
@@ -486,8 +489,8 @@ qlin_mx_outer32_kernel(const __grid_constant__ MxOuterJob<float> job0, const __g
 // [cols] from job1's.
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_outer_finish_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int rank, T* __restrict__ da,
-                            T* __restrict__ db, T* __restrict__ dbias, int64_t blocks0) {
+qlin_mx_outer_finish_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1,
+                            int rank, T* da, T* db, T* dbias, int64_t blocks0) {
   pdl_wait_prior();
   pdl_launch_dependents();
   const bool first = (int64_t)blockIdx.x < blocks0;

@@ -396,8 +396,8 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     constexpr int kTok = NTOK / 2;
     const int n_local = 32 * quarter + 4 * (lane & 7) + (lane >> 3);
     const float factor = scalbnf(1.f, c);
-    T* __restrict__ y = reinterpret_cast<T*>(prm.y);
-    const T* __restrict__ bias = reinterpret_cast<const T*>(prm.bias);
+    T* y = reinterpret_cast<T*>(prm.y);
+    const T* bias = reinterpret_cast<const T*>(prm.bias);
     for (int j = 0; j < my_tiles; ++j) {
       const int b = j % NB, u = j / NB;
       int n0, m0;

@@ -302,7 +302,6 @@ at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm,
   std::vector<void*> data;
   std::vector<int64_t> sizes;
   std::vector<int> types;
-  bool copied = false;
   for (const at::Tensor& g : grads) {
     TORCH_CHECK(g.layout() == at::kStrided, "sparse gradients are not supported");
     check_cuda(g, grads[0], false);
@@ -313,7 +312,6 @@ at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm,
   for (const at::Tensor& g : grads) {
     // one with gaps in memory goes through a dense copy
     dense.push_back(g.is_contiguous() || g.is_non_overlapping_and_dense() ? g : g.contiguous());
-    copied = copied || !dense.back().is_same(g);
     data.push_back(dense.back().data_ptr());
     sizes.push_back(g.numel());
   }
@@ -333,9 +331,10 @@ at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm,
     TORCH_CHECK(std::isfinite(n), "the global norm of the gradients is ", n, "; they are not clipped");
   }
   run(max_norm);
-  if (copied)
-    for (size_t k = 0; k < grads.size(); ++k)
-      if (!dense[k].is_same(grads[k])) grads[k].copy_(dense[k]);
+  for (size_t k = 0; k < grads.size(); ++k) {
+    if (dense[k].is_same(grads[k])) grads[k].unsafeGetTensorImpl()->bump_version();  // changed in place
+    else grads[k].copy_(dense[k]);
+  }
   return norm;
 }
 

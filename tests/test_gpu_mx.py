@@ -469,3 +469,80 @@ def test_a_training_step_on_the_frozen_base(qb, cuda):
     assert abs(after - norm / 2) <= 12 * ref.tolerance("f32", 200) * norm
     torch.optim.SGD(params, lr=0.1).step()
     assert all(m.base.weight_mx.grad is None for m in net)
+
+
+# --------------------------------------------- order, devices, repeated calls
+def test_inputs_written_right_before_a_call(qb, cuda):
+    """Dependent launches see what was queued just before them: x, the codes, bias
+    and the adapter, rows of any alignment among them."""
+    for dtype, M, fin in (("bf16", 1, 512), ("bf16", 12, 516), ("bf16", 150, 516), ("f32", 20, 512), ("f16", 150, 512)):
+        d = ref.draw(dtype, M, fin, 256, rank=5, bias=True, seed=1, device=cuda)
+        e = ref.draw(dtype, M, fin, 256, rank=5, bias=True, seed=2, device=cuda)
+
+        def call(v, q):
+            return qb.mx_quaternion_linear(v["x"], q, v["bias"], v["a"], v["b"], 2.0)
+
+        want = call(e, qb.quantize_quaternion_weights(*e["w"]))
+        q = qb.quantize_quaternion_weights(*d["w"])
+        for _ in range(5):
+            call(d, q)
+            new = qb.quantize_quaternion_weights(*e["w"])
+            q.data.copy_(new.data)
+            v = {k: t.clone() for k, t in d.items() if k in ("x", "bias", "a", "b")}
+            for k in v:
+                v[k].copy_(e[k])
+            assert torch.equal(call(v, q), want)
+            q = qb.quantize_quaternion_weights(*d["w"])
+
+
+def test_two_streams_at_once(qb, cuda):
+    d = ref.draw("bf16", 90, 512, 512, rank=8, seed=1, device=cuda)
+    q = qb.quantize_quaternion_weights(*d["w"])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    xs = [d["x"], d["x"] * 0.5]
+    want = [qb.mx_quaternion_linear(x, q, None, d["a"], d["b"], 2.0) for x in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for s, x, out in zip(streams, xs, got):
+            with torch.cuda.stream(s):
+                out.append(qb.mx_quaternion_linear(x, q, None, d["a"], d["b"], 2.0))
+    torch.cuda.synchronize()
+    for w, out in zip(want, got):
+        assert all(torch.equal(o, w) for o in out)
+
+
+def test_backward_in_a_graph_beside_an_eager_one(qb, cuda):
+    """A captured forward and backward on leaves of its own; the eager pass of other
+    leaves goes on as before."""
+    d = ref.draw("bf16", 70, 256, 128, rank=8, bias=True, seed=1, device=cuda)
+    q = qb.quantize_quaternion_weights(*d["w"])
+    gy = torch.randn(70, 128, device=cuda).bfloat16()
+
+    def step(leaves):
+        y = qb.mx_quaternion_linear(leaves[0], q, leaves[1], leaves[2], leaves[3], 2.0)
+        return torch.autograd.grad(y, leaves, gy)
+
+    def leaves():
+        return [d[k].clone().requires_grad_(True) for k in ("x", "bias", "a", "b")]
+
+    want = step(leaves())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mine = leaves()
+        step(mine)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(mine)
+    for _ in range(3):
+        graph.replay()
+        eager = step(leaves())
+        torch.cuda.synchronize()
+        for a, b, w in zip(got, eager, want):
+            assert torch.equal(a, w) and torch.equal(b, w)
+
+
+def test_no_device_errors_left(qb, cuda):
+    assert qb.device_error(cuda) == 0
