@@ -185,19 +185,18 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
   return w;
 }
 
-// CTAs of the record kernels: a warp takes half a record, at most 64 CTAs per SM
-// (then each warp takes several).
-unsigned record_ctas(int64_t K_g, int64_t N_g, int sms) {
-  const int64_t records = ceil_div(N_g, kMxRows) * ceil_div(K_g, kMxBlock);
-  return (unsigned)std::min<int64_t>(ceil_div(records, 4), 64ll * sms);
+// Grid of the record kernels: a warp takes four rows (y) of two records (x).
+dim3 record_grid(int64_t K_g, int64_t N_g) {
+  const int64_t rows = ceil_div(N_g, kMxRows) * (kMxRows / kMxUnitRows);
+  return dim3((unsigned)ceil_div(K_g, 2 * kMxBlock * 8), (unsigned)std::min<int64_t>(rows, 32768));
 }
 
 template <typename T>
-void launch_dequantize(const void* mx, const MxPlanes<T>& dst, int64_t ld, int64_t K_g, int64_t N_g, int sms,
+void launch_dequantize(const void* mx, const MxPlanes<T>& dst, int64_t ld, int64_t K_g, int64_t N_g,
                        cudaStream_t s) {
   bool vec = (ld * sizeof(T)) % 16 == 0;
   for (int c = 0; c < 4; ++c) vec = vec && aligned(dst.w[c], 16);
-  qlin_mx_dequantize_kernel<T><<<record_ctas(K_g, N_g, sms), 256, 0, s>>>(static_cast<const uint8_t*>(mx), dst, ld,
+  qlin_mx_dequantize_kernel<T><<<record_grid(K_g, N_g), 256, 0, s>>>(static_cast<const uint8_t*>(mx), dst, ld,
                                                                          (int)K_g, (int)N_g, vec);
 }
 
@@ -790,7 +789,7 @@ int qlin_mx_quantize(int dtype, const void* wr, const void* wi, const void* wj, 
       src.w[c] = static_cast<const T*>(w[c]);
       vec = vec && aligned(w[c], 16);
     }
-    qlin_mx_quantize_kernel<T><<<record_ctas(K_g, N_g, sms), 256, 0, s>>>(src, ld_w, (int)K_g, (int)N_g,
+    qlin_mx_quantize_kernel<T><<<record_grid(K_g, N_g), 256, 0, s>>>(src, ld_w, (int)K_g, (int)N_g,
                                                                          static_cast<uint8_t*>(mx), vec);
     return launched();
   });
@@ -809,7 +808,7 @@ int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g, void
   return by_type(dtype, [&](auto v) {
     using T = decltype(v);
     const MxPlanes<T> dst = {{static_cast<T*>(wr), static_cast<T*>(wi), static_cast<T*>(wj), static_cast<T*>(wk)}};
-    launch_dequantize<T>(mx, dst, ld_w, K_g, N_g, sms, static_cast<cudaStream_t>(stream));
+    launch_dequantize<T>(mx, dst, ld_w, K_g, N_g, static_cast<cudaStream_t>(stream));
     return launched();
   });
 }

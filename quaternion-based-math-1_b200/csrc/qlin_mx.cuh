@@ -129,7 +129,7 @@ __device__ __forceinline__ uint32_t mx_exponent(float amax) {
 // Eight consecutive elements of a row from `at`, zero from `left` on (vec: the
 // row pieces are 16-byte aligned).
 template <typename T>
-__device__ __forceinline__ void mx_load8(const T* at, int64_t left, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void mx_load8(const T* at, int left, bool vec, float (&v)[8]) {
   if (vec && left >= 8) {
     if constexpr (sizeof(T) == 4) {
       const float4 a = ld_cg_f4(at), b = ld_cg_f4(at + 4);
@@ -152,32 +152,33 @@ struct MxPlanes {
   T* w[4];
 };
 
-// Quantisation: a warp makes half a record (eight rows), two rows (four components
-// of four octets each) per step.  A lane holds eight elements of one block, the
-// four lanes of a block share its maximum.  Bound by the bytes read (2 or 4 a
-// weight) and written (0.53): one pass, all loads of a warp in flight at once,
-// everything else in registers.
+// Quantisation: a warp takes four rows of two neighbouring records, a row of all
+// four components per step: 128 bytes in a row of each from eight lanes.  A lane
+// holds eight elements of one block, the four lanes of a block share its maximum.
+// Bound by the bytes read (2 or 4 a weight) and written (0.53): one pass, all loads
+// of a warp in flight at once, everything else in registers.
+constexpr int kMxUnitRows = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_g, uint8_t* __restrict__ mx,
-                        bool vec) {
+qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_g, uint8_t* mx, bool vec) {
   const int lane = threadIdx.x & 31;
-  const int t = lane & 3, p = (lane >> 2) & 3, half = lane >> 4;
-  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
-  const int64_t warps = (int64_t)gridDim.x * 8;
+  const int t = lane & 3, second = (lane >> 2) & 1, p = lane >> 3;
+  const int kb = (K_g + kMxBlock - 1) / kMxBlock, row_units = (N_g + kMxRows - 1) / kMxRows * (kMxRows / kMxUnitRows);
+  const int b = 2 * ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) + second;  // this lane's block
   uint32_t top = 0;
-  for (int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < 2 * tiles * kb; unit += warps) {
-    const int64_t rec = unit >> 1, tile = rec / kb, b = rec - tile * kb;
-    const int first = 8 * (int)(unit & 1) + half;  // row of the first step
-    uint8_t* out = mx + kMxHeader + rec * kMxRecord;
-    const int64_t i = b * kMxBlock + 8 * t, left = K_g - i, o0 = tile * kMxRows + first;
-    const T* row0 = src.w[p] + o0 * ld + i;
-    float v[4][8];
+  const int i = b * kMxBlock + 8 * t, left = K_g - i;
+  for (int unit = blockIdx.y; unit < row_units; unit += gridDim.y) {
+    const int tile = unit / (kMxRows / kMxUnitRows), row0 = unit % (kMxRows / kMxUnitRows) * kMxUnitRows;
+    const int o0 = tile * kMxRows + row0;
+    uint8_t* out = mx + kMxHeader + ((int64_t)tile * kb + b) * kMxRecord;
+    const T* from = src.w[p] + (int64_t)o0 * ld + i;
+    float v[kMxUnitRows][8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) mx_load8(row0 + 2 * u * ld, o0 + 2 * u < N_g ? left : 0, vec, v[u]);
+    for (int u = 0; u < kMxUnitRows; ++u, from += ld) mx_load8(from, o0 + u < N_g ? left : 0, vec, v[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = first + 2 * u;
+    for (int u = 0; u < kMxUnitRows; ++u) {
+      const int row = row0 + u;
       // magnitudes as integers: the order of finite values, infinities and NaNs above them
       uint32_t m = 0;
 #pragma unroll
@@ -191,8 +192,10 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[u][j] * inv;
       if (!bad) top = max(top, e + 1u);
-      *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
-      if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
+      if (b < kb) {
+        *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
+        if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
+      }
     }
   }
   __shared__ uint32_t tops[8];
@@ -210,31 +213,30 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
 // One rounding (none for fp32, or for bf16 in its normal range).
 template <typename T>
 __global__ void __launch_bounds__(256)
-qlin_mx_dequantize_kernel(const uint8_t* __restrict__ mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
+qlin_mx_dequantize_kernel(const uint8_t* mx, const MxPlanes<T> dst, int64_t ld, int K_g, int N_g,
                           bool vec) {
   const int lane = threadIdx.x & 31;
-  const int t = lane & 3, p = (lane >> 2) & 3, half = lane >> 4;
-  const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
-  const int64_t warps = (int64_t)gridDim.x * 8;
-  for (int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); unit < 2 * tiles * kb; unit += warps) {
-    const int64_t rec = unit >> 1, tile = rec / kb, b = rec - tile * kb;
-    const int first = 8 * (int)(unit & 1) + half;
-    const uint8_t* in = mx + kMxHeader + rec * kMxRecord;
-    const int64_t i = b * kMxBlock + 8 * t, left = K_g - i;
-    if (left <= 0) continue;
-    uint32_t word[4], f[4];
+  const int t = lane & 3, second = (lane >> 2) & 1, p = lane >> 3;
+  const int kb = (K_g + kMxBlock - 1) / kMxBlock, row_units = (N_g + kMxRows - 1) / kMxRows * (kMxRows / kMxUnitRows);
+  const int b = 2 * ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) + second;  // this lane's block
+  const int i = b * kMxBlock + 8 * t, left = K_g - i;
+  if (left <= 0) return;  // (past the last block, too)
+  for (int unit = blockIdx.y; unit < row_units; unit += gridDim.y) {
+    const int tile = unit / (kMxRows / kMxUnitRows), row0 = unit % (kMxRows / kMxUnitRows) * kMxUnitRows;
+    const uint8_t* in = mx + kMxHeader + ((int64_t)tile * kb + b) * kMxRecord;
+    uint32_t word[kMxUnitRows], f[kMxUnitRows];
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      const int row = first + 2 * step;
+    for (int step = 0; step < kMxUnitRows; ++step) {
+      const int row = row0 + step;
       word[step] = __ldcg(reinterpret_cast<const uint32_t*>(in + row * 64 + t * 16 + p * 4));
       f[step] = __ldcg(in + kMxCodeBytes + row * 4 + p);
     }
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      const int64_t o = tile * kMxRows + first + 2 * step;
+    for (int step = 0; step < kMxUnitRows; ++step) {
+      const int o = tile * kMxRows + row0 + step;
       if (o >= N_g) continue;
       const float s = mx_scale(f[step]);
-      T* at = dst.w[p] + o * ld + i;
+      T* at = dst.w[p] + (int64_t)o * ld + i;
       float c[8];
       mx_values(word[step], c);
       __align__(16) T v[8];

@@ -66,9 +66,7 @@ def quantize_quaternion_weights(wr, wi, wj, wk) -> MXQuaternionWeights:
     even, and saturate at 6 scales.  A run that holds an infinity or a NaN
     stands for NaNs.
     """
-    with torch.no_grad():
-        data = _ext().mx_quantize(wr, wi, wj, wk)
-    return MXQuaternionWeights(data, wr.shape[0], wr.shape[1])
+    return MXQuaternionWeights(_ext().mx_quantize(wr, wi, wj, wk), wr.shape[0], wr.shape[1])
 
 
 def mx_quaternion_linear(x, weights: MXQuaternionWeights, bias=None, lora_a=None, lora_b=None,
