@@ -185,10 +185,11 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
   return w;
 }
 
-// Grid of the record kernels: a warp takes four rows (y) of two records (x).
-dim3 record_grid(int64_t K_g, int64_t N_g) {
-  const int64_t rows = ceil_div(N_g, kMxRows) * (kMxRows / kMxUnitRows);
-  return dim3((unsigned)ceil_div(K_g, 2 * kMxBlock * 8), (unsigned)std::min<int64_t>(rows, 32768));
+// Grid of the record kernels: a warp takes four rows (y) of two records (x) at a
+// time; about `ctas` CTAs.
+dim3 record_grid(int64_t K_g, int64_t N_g, int64_t ctas) {
+  const int64_t rows = ceil_div(N_g, kMxRows) * (kMxRows / kMxUnitRows), x = ceil_div(K_g, 2 * kMxBlock * 8);
+  return dim3((unsigned)x, (unsigned)std::min<int64_t>({rows, ceil_div(ctas, x), 32768}));
 }
 
 template <typename T>
@@ -196,7 +197,7 @@ void launch_dequantize(const void* mx, const MxPlanes<T>& dst, int64_t ld, int64
                        cudaStream_t s) {
   bool vec = (ld * sizeof(T)) % 16 == 0;
   for (int c = 0; c < 4; ++c) vec = vec && aligned(dst.w[c], 16);
-  qlin_mx_dequantize_kernel<T><<<record_grid(K_g, N_g), 256, 0, s>>>(static_cast<const uint8_t*>(mx), dst, ld,
+  qlin_mx_dequantize_kernel<T><<<record_grid(K_g, N_g, INT32_MAX), 256, 0, s>>>(static_cast<const uint8_t*>(mx), dst, ld,
                                                                          (int)K_g, (int)N_g, vec);
 }
 
@@ -789,7 +790,7 @@ int qlin_mx_quantize(int dtype, const void* wr, const void* wi, const void* wj, 
       src.w[c] = static_cast<const T*>(w[c]);
       vec = vec && aligned(w[c], 16);
     }
-    qlin_mx_quantize_kernel<T><<<record_grid(K_g, N_g), 256, 0, s>>>(src, ld_w, (int)K_g, (int)N_g,
+    qlin_mx_quantize_kernel<T><<<record_grid(K_g, N_g, 3ll * sms), 256, 0, s>>>(src, ld_w, (int)K_g, (int)N_g,
                                                                          static_cast<uint8_t*>(mx), vec);
     return launched();
   });

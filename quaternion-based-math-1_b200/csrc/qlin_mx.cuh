@@ -126,26 +126,23 @@ __device__ __forceinline__ uint32_t mx_exponent(float amax) {
   return field <= 2u ? 0u : field - 2u;
 }
 
-// Eight consecutive elements of a row from `at`, zero from `left` on (vec: the
-// row pieces are 16-byte aligned).
+// Eight consecutive elements of a row from `at` as they are, zero from `left` on
+// (vec: the row pieces are 16-byte aligned).
 template <typename T>
-__device__ __forceinline__ void mx_load8(const T* at, int left, bool vec, float (&v)[8]) {
-  if (vec && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = ld_cg_f4(at), b = ld_cg_f4(at + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 q = ld_cg_v4(at);
-      const T* e = reinterpret_cast<const T*>(&q);
+struct MxRaw8 {
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* at, int left, bool vec) {
+    if (vec && left >= 8) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+      for (int u = 0; u < (int)sizeof(T) / 2; ++u) q[u] = ld_cg_v4(reinterpret_cast<const uint4*>(at) + u);
+      return;
     }
-    return;
-  }
+    T* e = reinterpret_cast<T*>(q);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(at[j]) : 0.f;
-}
+    for (int j = 0; j < 8; ++j) e[j] = j < left ? at[j] : from_f32<T>(0.f);
+  }
+  __device__ __forceinline__ float get(int j) const { return to_f32(reinterpret_cast<const T*>(q)[j]); }
+};
 
 template <typename T>
 struct MxPlanes {
@@ -155,8 +152,8 @@ struct MxPlanes {
 // Quantisation: a warp takes four rows of two neighbouring records, a row of all
 // four components per step: 128 bytes in a row of each from eight lanes.  A lane
 // holds eight elements of one block, the four lanes of a block share its maximum.
-// Bound by the bytes read (2 or 4 a weight) and written (0.53): one pass, all loads
-// of a warp in flight at once, everything else in registers.
+// Bound by the bytes read (2 or 4 a weight) and written (0.53): one pass, the next
+// rows' loads in flight while a warp works on these, everything else in registers.
 constexpr int kMxUnitRows = 4;
 
 template <typename T>
@@ -168,21 +165,30 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
   const int b = 2 * ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) + second;  // this lane's block
   uint32_t top = 0;
   const int i = b * kMxBlock + 8 * t, left = K_g - i;
-  for (int unit = blockIdx.y; unit < row_units; unit += gridDim.y) {
-    const int tile = unit / (kMxRows / kMxUnitRows), row0 = unit % (kMxRows / kMxUnitRows) * kMxUnitRows;
-    const int o0 = tile * kMxRows + row0;
-    uint8_t* out = mx + kMxHeader + ((int64_t)tile * kb + b) * kMxRecord;
-    const T* from = src.w[p] + (int64_t)o0 * ld + i;
-    float v[kMxUnitRows][8];
+  const T* plane = src.w[p] + i;
+  MxRaw8<T> raw[kMxUnitRows], next[kMxUnitRows];
+  auto fetch = [&](MxRaw8<T>(&to)[kMxUnitRows], int unit) {
 #pragma unroll
-    for (int u = 0; u < kMxUnitRows; ++u, from += ld) mx_load8(from, o0 + u < N_g ? left : 0, vec, v[u]);
+    for (int u = 0; u < kMxUnitRows; ++u) {
+      const int o = unit * kMxUnitRows + u;
+      to[u].load(plane + (int64_t)o * ld, o < N_g ? left : 0, vec);
+    }
+  };
+  if ((int)blockIdx.y < row_units) fetch(raw, blockIdx.y);
+  for (int unit = blockIdx.y; unit < row_units; unit += gridDim.y) {
+    if (unit + (int)gridDim.y < row_units) fetch(next, unit + gridDim.y);
+    const int tile = unit / (kMxRows / kMxUnitRows), row0 = unit % (kMxRows / kMxUnitRows) * kMxUnitRows;
+    uint8_t* out = mx + kMxHeader + ((int64_t)tile * kb + b) * kMxRecord;
 #pragma unroll
     for (int u = 0; u < kMxUnitRows; ++u) {
       const int row = row0 + u;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = raw[u].get(j);
       // magnitudes as integers: the order of finite values, infinities and NaNs above them
       uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[u][j]) & 0x7FFFFFFFu);
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       const bool bad = m >= 0x7F800000u;
@@ -190,12 +196,13 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
       const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - E): E is at most 252
       float q[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[u][j] * inv;
+      for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[j] * inv;
       if (!bad) top = max(top, e + 1u);
       if (b < kb) {
         *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
         if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
       }
+      raw[u] = next[u];
     }
   }
   __shared__ uint32_t tops[8];
