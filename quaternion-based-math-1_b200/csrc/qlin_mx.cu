@@ -84,8 +84,13 @@ int few_tile(int dtype, int64_t M, int64_t N_g) {
   return dtype == QLIN_F32 && ceil_div(N_g, 4 * kMxRows) * ceil_div(M, 32) < 74 ? 16 : 32;
 }
 
-// One or two tokens whose B words fit beside the ring.
-constexpr size_t kOneMaxX = 150 * 1024;
+// One or two tokens whose B words fit beside a ring of two stages of 16 warps and
+// everything else that a CTA of theirs may hold.
+constexpr size_t kMostSmem = 226 * 1024;  // 1 KB of the 227 left for static shared memory
+constexpr size_t kOneMaxX = 148 * 1024;
+static_assert(kOneMaxX + 2 * (16 * kMxRecord + 16) + 2 * 16 * 2 * kMxRedRow * 4 + kMxMostB + 2 * kMxSmemRank * 4 + 64 <=
+                  kMostSmem,
+              "a layer that is_one() admits has to fit");
 bool is_one(int dtype, int64_t M, int64_t K_g) {
   const int64_t kb = ceil_div(K_g, kMxBlock);
   return M <= 2 && (size_t)kb * 1024 * (dtype == QLIN_F32 ? 3 : 1) + M * 4 * K_g * elem(dtype) <= kOneMaxX;
@@ -217,8 +222,6 @@ int launch_dependent(void (*kernel)(KArgs...), unsigned ctas, unsigned threads, 
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
 }
-
-constexpr size_t kMostSmem = 226 * 1024;  // 1 KB of the 227 left for static shared memory
 
 // Raises a kernel's shared-memory limit once per device.
 template <typename K>

@@ -1,5 +1,9 @@
 """4-bit quaternion weights on the device against the definition in 64 bits."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -546,3 +550,44 @@ def test_backward_in_a_graph_beside_an_eager_one(qb, cuda):
 
 def test_no_device_errors_left(qb, cuda):
     assert qb.device_error(cuda) == 0
+
+
+@pytest.mark.parametrize("M,fin,rank", [(1, 4 * 3840, 88), (2, 4 * 3200, 88), (1, 4 * 3830, 88), (2, 4 * 3200, 256),
+                                        (1, 4 * 3789, 8)])
+def test_one_or_two_tokens_of_the_longest_rows(qb, cuda, M, fin, rank):
+    """x, a ring, the rows of lora_b and t together at the most that shared memory holds."""
+    check_forward(qb, ref.draw("bf16", M, fin, 260, rank=rank, bias=True, seed=rank, device=cuda), "bf16", 2)
+
+
+def test_first_calls_inside_a_capture(qb, cuda):
+    """Nothing that a first call sets up breaks a capture."""
+    code = """
+import importlib, sys, torch
+sys.path.insert(0, {repo!r})
+sys.path.insert(0, {repo!r} + "/tests")
+import mx_reference as ref
+qb = importlib.import_module("quaternion-based-math-1_b200")
+for dtype, M in (("bf16", 1), ("f16", 12), ("bf16", 200), ("f32", 20)):
+    d = ref.draw(dtype, M, 512, 256, rank=8, bias=True, seed=1, device="cuda")
+    leaves = [d[k].requires_grad_(True) for k in ("x", "bias", "a", "b")]
+    gy = torch.ones(M, 256, device="cuda", dtype=d["x"].dtype)
+    def step():
+        q = qb.quantize_quaternion_weights(*d["w"])
+        y = qb.mx_quaternion_linear(leaves[0], q, leaves[1], leaves[2], leaves[3], 2.0)
+        for p, g in zip(leaves, torch.autograd.grad(y, leaves, gy)):
+            p.grad = g
+        norm = qb.clip_grad_norm(leaves, 0.5)
+        return [y, norm, *(p.grad for p in leaves), *q.dequantize(torch.float32)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+    del graph
+print("same")
+"""
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code.format(repo=repo)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "same" in res.stdout, res.stderr[-2000:]
