@@ -67,21 +67,28 @@ struct Carve {
   }
 };
 
-// 16-bit inputs of up to 32 tokens take the streaming kernels (qlin_mx_few.cuh), and
-// up to 64 where the layer has at most a tile of 16 output quaternions per SM (4096
-// -> 4096 at 64 tokens 14 against 22 us, 5120 -> 27648 74 against 60); more take the
-// CTA-pair kernel (qlin_mx_pair.cuh).  fp32 always streams.
+// 16-bit inputs of up to 32 tokens take the streaming kernels (qlin_mx_few.cuh; 5120 ->
+// 27648 at 32 tokens 39 against 47 us), and up to 64 where the layer has at most a tile
+// of 16 output quaternions per SM (4096 -> 4096 at 64 tokens 13 against 21 us, 5120 ->
+// 27648 70 against 47); more take the CTA-pair kernel (qlin_mx_pair.cuh).  fp32 always
+// streams.
 bool streams(int dtype, int64_t M, int64_t N_g) {
   return dtype == QLIN_F32 || M <= 32 || (M <= 64 && N_g <= 148 * kMxRows);
 }
 
-// Tokens of a tile of the streaming kernels (one or two tokens apart): the
-// smallest tile that holds them all, at most 32; 16 where tiles of 32 (and four of
-// 16 output quaternions) would leave half of the SMs without one, in fp32, which
-// comes here with many tokens.
+// Tokens of a tile of the streaming kernels (one or two tokens apart).  16 bits: two
+// tiles of 16 run beside each other faster than one of 32 (4096 -> 4096 at 32 tokens
+// 9.3 against 12.7 us, 11008 -> 4096 16.8 against 22.2), three or four do not (64
+// tokens 17.7 against 12.9).  fp32, which comes here with any number of tokens: 16
+// (by two tiles of output quaternions) or 32 (by four) by the waves of CTAs, of which
+// one of 32 takes as long as about 3.5 of 16 (4096 -> 11008 at 128 tokens 108 against
+// 150 us, 768 -> 2304 at 512 tokens 37 against 30).
 int few_tile(int dtype, int64_t M, int64_t N_g) {
   if (M <= 16) return M <= 8 ? 8 : 16;
-  return dtype == QLIN_F32 && ceil_div(N_g, 4 * kMxRows) * ceil_div(M, 32) < 74 ? 16 : 32;
+  if (dtype != QLIN_F32) return M <= 32 ? 16 : 32;
+  const int64_t waves16 = ceil_div(ceil_div(N_g, 2 * kMxRows) * ceil_div(M, 16), 148);
+  const int64_t waves32 = ceil_div(ceil_div(N_g, 4 * kMxRows) * ceil_div(M, 32), 148);
+  return 2 * waves16 <= 7 * waves32 ? 16 : 32;
 }
 
 // One or two tokens whose B words fit beside a ring of two stages of 16 warps and
@@ -276,9 +283,12 @@ int launch_many(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   prm.stage_b = stages_b(prm, WO);
   const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
   const size_t fixed = mx_many_smem<T, NT, WO, WIDE>(0, prm.rank, b), stage = Cfg::kStage + 16;
-  // two CTAs per SM where there are tiles for them and their rings fit
+  // two CTAs per SM (tiles of 8 tokens, whose registers allow it) where their rings fit
+  // and the last wave stays as full (8 tokens, 4096 -> 11008: 172 tiles, 10.3 against
+  // 11.8 us; 5120 -> 27648: 432 tiles, 18.3 against 17.0)
   constexpr size_t kHalfSm = kMostSmem / 2 - 1024;
-  const bool two = total > sms && fixed + 2 * stage <= kHalfSm;
+  const bool two = NT == 1 && sizeof(T) == 2 && total > sms && 2 * ceil_div(total, 2 * sms) <= ceil_div(total, sms) &&
+                   fixed + 2 * stage <= kHalfSm;
   const int ctas = (int)std::min<int64_t>(total, (two ? 2 : 1) * sms);
   const int64_t uses = ceil_div(prm.kb, Cfg::kWK) * ceil_div(total, ctas);
   prm.ring = ring_stages(two ? kHalfSm : kMostSmem, fixed, stage, uses);
@@ -335,7 +345,8 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
     // x by bulk copies
     prm.vec = aligned(x, 16) && (4 * K_g * sizeof(T)) % 16 == 0 && (M == 1 || (ld_x * sizeof(T)) % 16 == 0);
     // at most a tile per SM, or x too long for three rings: 16 warps share the
-    // tile's K; more tiles: three groups of 8 warps
+    // tile's K (4096 -> 4096: 4.2 against 4.6 us); more tiles: three groups of 8 warps
+    // (5120 -> 27648: 8.3 against 8.8 us, graph replays)
     if (prm.tiles > sms) {
       const int e = launch_one<T, 8, 3>(prm, sms, s);
       if (e != QLIN_ERR_SHAPE) return e;
@@ -343,12 +354,19 @@ int run_few(int dtype, const T* x, int64_t ld_x, const void* mx, const T* bias, 
     return launch_one<T, 16, 1>(prm, sms, s);
   }
   if (C == 8) return launch_many<T, 1, 1>(prm, sms, s);
-  // side by side, tiles of a CTA share the B words (two or four of them); alone,
-  // there are more CTAs (fp32's B words are too long for that)
-  if constexpr (sizeof(T) == 2)
-    if (prm.tiles * ceil_div(M, C) <= 2 * sms)
-      return C == 16 ? launch_many<T, 2, 1>(prm, sms, s) : launch_many<T, 4, 1>(prm, sms, s);
-  return C == 16 ? launch_many<T, 2, 2>(prm, sms, s) : launch_many<T, 4, 4>(prm, sms, s);
+  // Side by side, tiles of a CTA share the B words (two or four of them: fp32's are
+  // too long for one); alone, there are more CTAs.  16 bits at 16 tokens: a wave of two
+  // side by side takes as long as 1.4 waves of one, so side by side where that halves
+  // the waves (4096 -> 11008: 2 waves -> 1, 17.1 -> 12.8 us; 5120 -> 27648: 3 against
+  // 2, 24.7 against 29.0).  Tiles of 32 tokens come with few tiles.
+  if constexpr (sizeof(T) == 2) {
+    if (C == 32) return launch_many<T, 4, 1>(prm, sms, s);
+    const int64_t alone = ceil_div(prm.tiles * ceil_div(M, C), sms);
+    const int64_t beside = ceil_div(ceil_div(prm.tiles, 2) * ceil_div(M, C), sms);
+    return alone < 2 * beside ? launch_many<T, 2, 1>(prm, sms, s) : launch_many<T, 2, 2>(prm, sms, s);
+  } else {
+    return C == 16 ? launch_many<T, 2, 2>(prm, sms, s) : launch_many<T, 4, 4>(prm, sms, s);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -464,14 +482,16 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
              : QLIN_ERR_LAUNCH;
 }
 
-// Tiles of 256 tokens, or of 128 where those end sooner: a wave of them takes about
-// 0.6 of the time (stages of 0.45 against 0.75 us), and few tokens or outputs leave
-// pairs without a tile of 256.
+// Tiles of 256 tokens, or of 128 where those end sooner: a wave of them takes nearly
+// 0.8 of the time (stages of 0.55 us, the expansion's time, against 0.71), and few
+// tokens or outputs leave pairs without a tile of 256.  (256 -> 128: 4096 -> 4096 at
+// 256 tokens, 1 wave each, 27.4 -> 21.6 us; 4096 -> 11008 at 512 tokens, 2 against 3
+// waves, 47.8 -> 55.9.)
 template <typename T, bool MX, typename... Args>
 int run_pair(int64_t M, int64_t N_g, Args... args) {
   const int64_t nb = ceil_div(4 * N_g, 256), cap = std::max(1, pair_capacity<T, 256, MX>());
   const int64_t waves256 = ceil_div(nb * ceil_div(M, 256), cap), waves128 = ceil_div(nb * ceil_div(M, 128), cap);
-  return 3 * waves128 < 5 * waves256 ? launch_pair<T, 128, MX>(args...) : launch_pair<T, 256, MX>(args...);
+  return 9 * waves128 < 11 * waves256 ? launch_pair<T, 128, MX>(args...) : launch_pair<T, 256, MX>(args...);
 }
 
 // Rows that TMA takes (whole: and that are whole 16-byte pieces): x itself, or a

@@ -1,6 +1,9 @@
 // The layer with 4-bit weights for few tokens (decode, small batches; fp32 at
 // any size): a stream of the codes through shared memory into warp-level
-// tensor-core products (mma m16n8k16, fp32 accumulators).
+// tensor-core products (mma m16n8k16, fp32 accumulators).  These, not tcgen05: with
+// one to 32 columns of x a 128-row accumulator tile per SM would leave the codes'
+// expansion, not the product, as the work, and its hand-over through tensor memory
+// costs more than the products (32 tokens, 5120 -> 27648: 39 against 47 us).
 //
 //     y_a[o] = sum_i sum_p s(a, p) W_p[o, i] x_{a^p}[i]
 //
@@ -36,8 +39,10 @@
 // and is added to the fp32 sum outside the tensor core, whose own additions
 // truncate.
 //
-// Bound by the codes' bytes for one token of a wide layer, by latency for
-// narrow layers, by the expansion and the tensor pipe from about 8 tokens on.
+// Bound by the integer pipe and start-up for one token of a wide layer, by latency
+// for narrow ones (4096 -> 4096, one token: 4.2 us in a graph, 0.42 of which are bytes),
+// by the expansion and the warp-level tensor pipe (50 %) from about 8 tokens on (4096
+// -> 4096 at 16 tokens 9.3 us; 5120 -> 27648 at 8 and 16 tokens 17 and 25 us).
 #pragma once
 
 #include <type_traits>
@@ -355,8 +360,10 @@ __device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float
 // G groups of W consumer warps and one copying warp; a group takes a tile at a
 // time, its warps every W-th block of it.  The groups share x: with more tiles
 // than SMs, three groups keep three tiles of an SM in flight on one staged x
-// (two CTAs of one group each staged it twice and left 16 warps per SM: 15.4
-// against XX us for 5120 -> 27648).
+// (5120 -> 27648, one bf16 token: 7.9 us a call, 2.4 TB/s of codes; two CTAs per SM,
+// each with its own copy of x, 12.3).  About half of that is start, staging of x and
+// the last reduction; in the loop the integer pipe (49 % over the whole launch) and
+// issue slots (55 %) bound, not HBM.
 //
 // Shared memory: a ring per group, x as B words [block][part][sign][q][token][t]
 // (both signs, so that no lane flips its operand), x as it came, reduction rows
@@ -622,8 +629,9 @@ __device__ __forceinline__ void mx_arrange_one(const T* x, int64_t ld_x, int M, 
 }
 
 constexpr int kMxDownTokens = 4;  // tokens of a down-projection CTA
-// Threads of a prologue CTA: with 256, rows of 4096 took twice as many dependent
-// rounds of loads.
+// Threads of a prologue CTA: the down projection's rounds of dependent loads against
+// CTAs whose threads have work (rank 32, rows of 4096, 16 tokens: 13.7 us with 512,
+// 15.6 with 256; rank 16, rows of 1024: 7.4 and 6.6).
 constexpr int kMxPrologueMost = 512;
 inline int mx_prologue_threads(int64_t K_g) { return K_g > 512 ? kMxPrologueMost : 256; }
 
