@@ -139,11 +139,13 @@ struct BackwardWs {
   size_t total = 0;
 };
 
-// Splits of the tokens of a gradient product: about 1.5 CTAs per SM for each of the
-// two (three fit an SM), at least four steps of 32 tokens each.
+// Splits of the tokens of a gradient product: about two CTAs per SM for each of the
+// two (three fit an SM; short ones fill more of what the input gradient's last wave
+// leaves free: 4096 layer at 2048 tokens, forward and gradients 141 us in a graph, 143
+// with 1.5), at least four steps of 32 tokens each.
 int outer_splits(int64_t M_pad, int64_t cols, int rows) {
   const int64_t tiles = ceil_div(cols, kMxOuterCols) * ceil_div(rows, kMxOuterRows);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 222 / std::max<int64_t>(1, tiles)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(M_pad / kMxOuterTokens / 4, 320 / std::max<int64_t>(1, tiles)));
 }
 
 // The same for fp32: about two CTAs per SM each, at least 32 tokens.
@@ -624,7 +626,7 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     if (allow_smem(qlin_mx_outer_kernel<T>, done, kMxOuterSmem) != QLIN_OK) return QLIN_ERR_LAUNCH;
     if (sum_with_db) o1.sums = reinterpret_cast<float*>(ws + w.sums);
     st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 128, kMxOuterSmem, s, o0, o1,
-                          (int)M, (int)w.M_pad);
+                          (int)M, (int)w.M_pad, (int)(dx != nullptr));
     if (st != QLIN_OK) return st;
     const int64_t blocks0 = da ? ceil_div(rank * K, 256) : 0;
     const int64_t blocks1 = db ? ceil_div((rank + (sum_with_db ? 1 : 0)) * N, 256) : 0;

@@ -294,13 +294,18 @@ struct MxOuterJob {
 // a ring of shared memory steps (32 tokens x 128 columns; 16-byte chunks permuted
 // within a row of X so that the transposing loads of eight tokens two apart are
 // free of conflicts).
+//
+// beside: the launch before is the CTA-pair kernel, which needs nothing from this one
+// and lets it start only when the down projections have ended.  CTAs then take the SMs
+// that its last wave leaves free; the last CTA waits for its end, so that whatever
+// waits for this kernel has waited for that one too.
 template <typename T>
 __global__ void __launch_bounds__(128)
 qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int M,
-                     int M_pad) {
+                     int M_pad, int beside) {
   constexpr bool HALF = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) uint8_t mx_smem[];
-  pdl_wait_prior();
+  if (!beside) pdl_wait_prior();
   pdl_launch_dependents();
   const bool first = (int)blockIdx.x < job0.blocks;
   const MxOuterJob<T>& job = first ? job0 : job1;
@@ -420,6 +425,7 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
       const int c = c0 + 32 * warp + 8 * n + g;
       if (t == 0 && c < job.cols) job.sums[(int64_t)split * job.cols + c] = v;
     }
+  if (beside && blockIdx.x == gridDim.x - 1) pdl_wait_prior();
 }
 
 // ---------------------------------------------------------------------------

@@ -115,7 +115,7 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int nk = prm.stages + prm.lora_stages;
   const int total = my_tiles * nk;  // ring items of this pair
 
-  pdl_launch_dependents();
+  if (prm.lora_stages == 0) pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -187,6 +187,8 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             const int r = 64 * (k - prm.stages);
             if (j == 0 && r == 0) {
               pdl_wait_prior();
+              // a kernel that starts from here on finds the down projection's results
+              pdl_launch_dependents();
               fence_proxy_async();
             }
             mbar_arrive_expect_tx(&full[s], Cfg::kXBytes);
