@@ -7,7 +7,9 @@ K1/K2 operator entry points (``quaternion/planar.py``), the LoRA residual
 and the ``kernels/`` operator interface.  Every quaternion product runs in the
 in-tree CUDA library ``lib/libqlin_b200.so`` (C ABI in ``include/qlin_b200.h``):
 a TMA + tcgen05/TMEM tensor-core kernel for bf16/f16 and a CUDA-core kernel
-for fp32.  There is no CPU path; CPU tensors raise ``RuntimeError``.
+for fp32.  ``MXQuaternionLinear`` and ``quantize_model`` hold frozen weights in
+4 bits (MXFP4), ``clip_grad_norm`` clips the gradients of a whole model.
+There is no CPU path; CPU tensors raise ``RuntimeError``.
 
 The directory name is not a Python identifier, so import it with
 ``importlib.import_module("quaternion-based-math-1_b200")``.

@@ -251,11 +251,15 @@ int ring_stages(size_t budget, size_t fixed, size_t stage, int64_t uses) {
   return (int)std::max<int64_t>(2, std::min(fit, uses));
 }
 
-// Whether a CTA keeps the rows of lora_b of a tile of 64 `wo` outputs in shared memory.
+// Whether rows of lora_b are whole 16-byte pieces, and whether a CTA keeps those of a
+// tile of 64 `wo` outputs in shared memory.
+template <typename T>
+bool pieces_b(const MxFewParams<T>& prm) {
+  return prm.rank > 0 && prm.rank * sizeof(T) % 16 == 0 && aligned(prm.lora_b, 16);
+}
 template <typename T>
 bool stages_b(const MxFewParams<T>& prm, int wo) {
-  return prm.rank > 0 && prm.rank <= kMxSmemRank && prm.rank * sizeof(T) % 16 == 0 && aligned(prm.lora_b, 16) &&
-         mx_b_bytes<T>(prm.rank, wo) <= kMxMostB;
+  return pieces_b(prm) && prm.rank <= kMxSmemRank && mx_b_bytes<T>(prm.rank, wo) <= kMxMostB;
 }
 
 // W warps per tile, G tiles of a CTA at a time; QLIN_ERR_SHAPE where that does not fit.
@@ -266,6 +270,7 @@ int launch_one(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   const int ctas = (int)std::min<int64_t>(prm.tiles, sms);
   const int64_t uses = ceil_div(prm.kb, W) * ceil_div(prm.tiles, (int64_t)ctas * G);
   prm.stage_b = stages_b(prm, 1);
+  prm.vec_b = pieces_b(prm);
   const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, 1) : 0;
   prm.ring = ring_stages(kMostSmem, mx_one_smem<T, W, G>(prm.M, prm.K_g, 0, prm.rank, b), G * (W * kMxRecord + 16),
                          uses);
@@ -283,6 +288,7 @@ int launch_many(const MxFewParams<T>& base, int sms, cudaStream_t s) {
   MxFewParams<T> prm = base;
   const int64_t total = ceil_div(prm.tiles, WO) * ceil_div(prm.M, Cfg::kC);
   prm.stage_b = stages_b(prm, WO);
+  prm.vec_b = pieces_b(prm);
   const int b = prm.stage_b ? mx_b_bytes<T>(prm.rank, WO) : 0;
   const size_t fixed = mx_many_smem<T, NT, WO, WIDE>(0, prm.rank, b), stage = Cfg::kStage + 16;
   // two CTAs per SM (tiles of 8 tokens, whose registers allow it) where their rings fit
@@ -304,13 +310,16 @@ template <typename T>
 int few_prologue(const MxFewParams<T>& prm, bool one, const T* a, float scale, uint8_t* arranged, float* t,
                  cudaStream_t s) {
   const int C = few_tile(sizeof(T) == 4 ? QLIN_F32 : QLIN_BF16, prm.M, prm.N_g);
-  const int threads = mx_prologue_threads(prm.K_g);
+  const int64_t token_groups = ceil_div(prm.M, kMxDownTokens);
+  const bool ranks = prm.rank * token_groups >= 4 * 222;  // 1.5 CTAs of four ranks per SM
+  const int threads = ranks ? 256 : mx_prologue_threads(prm.K_g);
   const int64_t octets = one ? 0 : ceil_div(prm.M, C) * C * 4 * prm.kb;
-  const int64_t blocks = ceil_div(octets, threads), down = prm.rank * ceil_div(prm.M, kMxDownTokens);
+  const int64_t blocks = ceil_div(octets, threads), down = (ranks ? ceil_div(prm.rank, kMxDownRanksMost) : prm.rank) * token_groups;
   if (blocks + down > INT32_MAX) return QLIN_ERR_SHAPE;
   if (blocks + down == 0) return QLIN_OK;
   const int vec = aligned(prm.x, 4 * sizeof(T)) && prm.ld_x % 4 == 0;
-  return launch_dependent(qlin_mx_prologue_kernel<T>, (unsigned)(blocks + down), threads, 0, s, prm.x, prm.ld_x, prm.M,
+  return launch_dependent(ranks ? qlin_mx_prologue_kernel<T, kMxDownRanksMost> : qlin_mx_prologue_kernel<T, 1>,
+                          (unsigned)(blocks + down), threads, 0, s, prm.x, prm.ld_x, prm.M,
                           prm.K_g, prm.kb, C, vec, arranged, (int)blocks, octets, a,
                           (int)aligned(a, 4 * sizeof(T)), prm.rank, scale, t);
 }

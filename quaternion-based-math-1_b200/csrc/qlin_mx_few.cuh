@@ -294,6 +294,7 @@ struct MxFewParams {
   int ring;                 // stages of the ring
   int vec;                  // whole quaternions of x are aligned (one or two tokens: x takes bulk copies)
   int stage_b;              // rows of lora_b come through shared memory
+  int vec_b;                // rows of lora_b are whole 16-byte pieces
   int after_prologue;       // t comes from the previous kernel, which waited for everything before it
 };
 
@@ -335,18 +336,20 @@ __device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float
   v *= factor;
   if (prm.rank > 0) {
     float l = 0.f;
-    if (b_row) {
+    const T* b = prm.lora_b + n * prm.rank;
+    auto pieces = [&](const uint4* row) {
       constexpr int V = 16 / (int)sizeof(T);
       for (int r = 0; r < prm.rank; r += V) {
-        const uint4 q = *reinterpret_cast<const uint4*>(b_row + r * (int)sizeof(T));
+        const uint4 q = row[r / V];
         const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
         for (int j = 0; j < V; ++j) l = fmaf(ts[r + j], to_f32(e[j]), l);
       }
-    } else {
-      const T* b = prm.lora_b + n * prm.rank;
+    };
+    if (b_row) pieces(reinterpret_cast<const uint4*>(b_row));
+    else if (prm.vec_b) pieces(reinterpret_cast<const uint4*>(b));
+    else
       for (int r = 0; r < prm.rank; ++r) l = fmaf(ts[r], to_f32(b[r]), l);
-    }
     v += l;
   }
   if (prm.bias) v += to_f32(prm.bias[n]);
@@ -635,9 +638,16 @@ constexpr int kMxDownTokens = 4;  // tokens of a down-projection CTA
 constexpr int kMxPrologueMost = 512;
 inline int mx_prologue_threads(int64_t K_g) { return K_g > 512 ? kMxPrologueMost : 256; }
 
+// Ranks of a down-projection CTA: with four, rows of x are read a quarter as often
+// (fp32, 1024 layer, rank 32 at 128 tokens, forward and gradients 114 -> 61 us, together
+// with whole 16-byte pieces of lora_b's rows); with one, CTAs are many and short, which
+// is better until there are enough of the others (bf16, 4096 layer, rank 32 at 64
+// tokens, 128 CTAs of four: 20.9 -> 23.2 us).
+constexpr int kMxDownRanksMost = 4;
+
 // Blocks [0, arrange_blocks): the B words.  The rest: t[m, r] = scale x A^T,
-// one rank and kMxDownTokens tokens per block, the row of A read once.
-template <typename T>
+// RANKS ranks and kMxDownTokens tokens per block.
+template <typename T, int RANKS>
 __global__ void __launch_bounds__(kMxPrologueMost)
 qlin_mx_prologue_kernel(const T* x, int64_t ld_x, int M, int K_g, int kb, int C, int vec,
                         uint8_t* arranged, int arrange_blocks, int64_t octets,
@@ -649,33 +659,40 @@ qlin_mx_prologue_kernel(const T* x, int64_t ld_x, int M, int K_g, int kb, int C,
     if (idx < octets) mx_arrange_one<T>(x, ld_x, M, K_g, kb, C, vec, arranged, idx);
     return;
   }
-  __shared__ float part[kMxPrologueMost / 32][kMxDownTokens];
-  const int b = (int)blockIdx.x - arrange_blocks;
-  const int r = b % rank, m0 = b / rank * kMxDownTokens;
-  const T* a = lora_a + (int64_t)r * 4 * K_g;
-  float s[kMxDownTokens] = {};
-#pragma unroll 2
+  constexpr int kSums = RANKS * kMxDownTokens;
+  __shared__ float part[kMxPrologueMost / 32][kSums];
+  const int b = (int)blockIdx.x - arrange_blocks, groups = (rank + RANKS - 1) / RANKS;
+  const int r0 = b % groups * RANKS, m0 = b / groups * kMxDownTokens;
+  float s[RANKS][kMxDownTokens] = {};
+#pragma unroll(RANKS == 1 ? 2 : 1)
   for (int i = threadIdx.x; i < K_g; i += blockDim.x) {
-    const float4 av = mx_load4(a + 4 * (int64_t)i, vec_a);
+    float4 av[RANKS];
+#pragma unroll
+    for (int k = 0; k < RANKS; ++k)  // (past the last rank: that one's again)
+      av[k] = mx_load4(lora_a + ((int64_t)min(r0 + k, rank - 1) * K_g + i) * 4, vec_a);
 #pragma unroll
     for (int u = 0; u < kMxDownTokens; ++u) {
       if (m0 + u >= M) break;
       const float4 xv = mx_load4(x + (int64_t)(m0 + u) * ld_x + 4 * (int64_t)i, vec);
-      s[u] = fmaf(av.x, xv.x, fmaf(av.y, xv.y, fmaf(av.z, xv.z, fmaf(av.w, xv.w, s[u]))));
+#pragma unroll
+      for (int k = 0; k < RANKS; ++k)
+        s[k][u] = fmaf(av[k].x, xv.x, fmaf(av[k].y, xv.y, fmaf(av[k].z, xv.z, fmaf(av[k].w, xv.w, s[k][u]))));
     }
   }
 #pragma unroll
-  for (int u = 0; u < kMxDownTokens; ++u)
+  for (int k = 0; k < kSums; ++k)
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+    for (int d = 16; d > 0; d >>= 1) s[k / kMxDownTokens][k % kMxDownTokens] +=
+        __shfl_xor_sync(0xffffffffu, s[k / kMxDownTokens][k % kMxDownTokens], d);
   if ((threadIdx.x & 31) == 0)
 #pragma unroll
-    for (int u = 0; u < kMxDownTokens; ++u) part[threadIdx.x >> 5][u] = s[u];
+    for (int k = 0; k < kSums; ++k) part[threadIdx.x >> 5][k] = s[k / kMxDownTokens][k % kMxDownTokens];
   __syncthreads();
-  if (threadIdx.x < kMxDownTokens && m0 + (int)threadIdx.x < M) {
+  const int r = r0 + (int)threadIdx.x / kMxDownTokens, m = m0 + (int)threadIdx.x % kMxDownTokens;
+  if (threadIdx.x < kSums && r < rank && m < M) {
     float v = 0.f;
     for (int w = 0; w < (int)blockDim.x / 32; ++w) v += part[w][threadIdx.x];
-    t[(int64_t)(m0 + threadIdx.x) * rank + r] = scale * v;
+    t[(int64_t)m * rank + r] = scale * v;
   }
 }
 

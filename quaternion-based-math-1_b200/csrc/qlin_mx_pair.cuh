@@ -12,7 +12,13 @@
 // Without MX the weights are 16-bit component planes: the adjoint of the codes,
 // times 2^-c.
 // One set of builder warps could not keep up with the UMMAs on codes (a 4096 layer
-// at 2048 tokens: 66 us, 57 on planes); two sets take every other stage each.
+// at 2048 tokens: 66 us, 57 on planes); two sets take every other stage each and need
+// about 1080 cycles a stage, the integer pipe's time for it, just behind the UMMAs'
+// 1024.  Tiles of 128 tokens, whose UMMAs take 512, are bound by that.
+//
+// Bound by the tensor pipe at 256 tokens (84 % of all cycles): 4096 -> 11008 at 2048
+// bf16 tokens 113 us in a burst (1630 TFLOP/s), 134 us sustained (1380, at the power
+// limit); 5120 -> 27648 with an adapter of rank 16 368 and 421 us.
 //
 // Adapter: y += t B^T with t = s x A^T as two 16-bit parts (t = hi + lo to about
 // twice the type's precision): ceil(r / 64) more stages whose x tile is 64
