@@ -18,7 +18,7 @@
 //
 // Bound by the tensor pipe at 256 tokens (84 % of all cycles): 4096 -> 11008 at 2048
 // bf16 tokens 113 us in a burst (1630 TFLOP/s), 134 us sustained (1380, at the power
-// limit); 5120 -> 27648 with an adapter of rank 16 368 and 421 us.
+// limit); 5120 -> 27648 with an adapter of rank 32 368 and 421 us.
 //
 // Adapter: y += t B^T with t = s x A^T as two 16-bit parts (t = hi + lo to about
 // twice the type's precision): ceil(r / 64) more stages whose x tile is 64
