@@ -251,15 +251,17 @@ int ring_stages(size_t budget, size_t fixed, size_t stage, int64_t uses) {
   return (int)std::max<int64_t>(2, std::min(fit, uses));
 }
 
-// Whether rows of lora_b are whole 16-byte pieces, and whether a CTA keeps those of a
-// tile of 64 `wo` outputs in shared memory.
+// Pieces that rows of lora_b are made of (16 or 8 bytes, or 0), and whether a CTA keeps
+// those of a tile of 64 `wo` outputs in shared memory.
 template <typename T>
-bool pieces_b(const MxFewParams<T>& prm) {
-  return prm.rank > 0 && prm.rank * sizeof(T) % 16 == 0 && aligned(prm.lora_b, 16);
+int pieces_b(const MxFewParams<T>& prm) {
+  for (const int piece : {16, 8})
+    if (prm.rank > 0 && prm.rank * sizeof(T) % piece == 0 && aligned(prm.lora_b, piece)) return piece;
+  return 0;
 }
 template <typename T>
 bool stages_b(const MxFewParams<T>& prm, int wo) {
-  return pieces_b(prm) && prm.rank <= kMxSmemRank && mx_b_bytes<T>(prm.rank, wo) <= kMxMostB;
+  return pieces_b(prm) == 16 && prm.rank <= kMxSmemRank && mx_b_bytes<T>(prm.rank, wo) <= kMxMostB;
 }
 
 // W warps per tile, G tiles of a CTA at a time; QLIN_ERR_SHAPE where that does not fit.

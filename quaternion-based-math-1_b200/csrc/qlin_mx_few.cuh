@@ -294,7 +294,7 @@ struct MxFewParams {
   int ring;                 // stages of the ring
   int vec;                  // whole quaternions of x are aligned (one or two tokens: x takes bulk copies)
   int stage_b;              // rows of lora_b come through shared memory
-  int vec_b;                // rows of lora_b are whole 16-byte pieces
+  int vec_b;                // rows of lora_b are whole pieces of 16 or 8 bytes (or 0)
   int after_prologue;       // t comes from the previous kernel, which waited for everything before it
 };
 
@@ -337,17 +337,18 @@ __device__ __forceinline__ void mx_finish(const MxFewParams<T>& prm, const float
   if (prm.rank > 0) {
     float l = 0.f;
     const T* b = prm.lora_b + n * prm.rank;
-    auto pieces = [&](const uint4* row) {
-      constexpr int V = 16 / (int)sizeof(T);
+    auto pieces = [&](const auto* row) {
+      constexpr int V = (int)(sizeof(*row) / sizeof(T));
       for (int r = 0; r < prm.rank; r += V) {
-        const uint4 q = row[r / V];
+        const auto q = row[r / V];
         const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
         for (int j = 0; j < V; ++j) l = fmaf(ts[r + j], to_f32(e[j]), l);
       }
     };
     if (b_row) pieces(reinterpret_cast<const uint4*>(b_row));
-    else if (prm.vec_b) pieces(reinterpret_cast<const uint4*>(b));
+    else if (prm.vec_b == 16) pieces(reinterpret_cast<const uint4*>(b));
+    else if (prm.vec_b == 8) pieces(reinterpret_cast<const uint2*>(b));
     else
       for (int r = 0; r < prm.rank; ++r) l = fmaf(ts[r], to_f32(b[r]), l);
     v += l;
