@@ -591,3 +591,35 @@ print("same")
     repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     res = subprocess.run([sys.executable, "-c", code.format(repo=repo)], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and "same" in res.stdout, res.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype,M", [("bf16", 600), ("f16", 70), ("f32", 200)])
+def test_gradients_of_buffers_that_change_between_calls(qb, cuda, dtype, M):
+    """Every kernel of a backward pass is done with its inputs when the next work of
+    the stream starts: the same buffers, refilled right behind each call."""
+    sets = []
+    for seed in (1, 2):
+        d = ref.draw(dtype, M, 1024, 768, rank=8, bias=True, seed=seed, device=cuda)
+        d["gy"] = ref.draw(dtype, M, 768, 4, seed=seed + 5, device=cuda)["x"]
+        sets.append(d)
+    q = qb.quantize_quaternion_weights(*sets[0]["w"])
+    names = ("x", "bias", "a", "b", "gy")
+
+    def step(v):
+        leaves = [v[k].detach().requires_grad_(True) for k in names[:4]]
+        y = qb.mx_quaternion_linear(leaves[0], q, leaves[1], leaves[2], leaves[3], 2.0)
+        return torch.autograd.grad(y, leaves, v["gy"])
+
+    want = []
+    for d in sets:
+        want.append(step(d))
+        torch.cuda.synchronize()
+    v = {k: sets[0][k].detach().clone() for k in names}
+    got = []
+    for n in range(12):
+        got.append(step(v))
+        for k in names:
+            v[k].copy_(sets[(n + 1) % 2][k])
+    for n, grads in enumerate(got):
+        for a, b in zip(grads, want[n % 2]):
+            assert torch.equal(a, b)
