@@ -45,7 +45,7 @@ struct MxPairStage {
   static constexpr int kHalf = NTOK / 2;
   static constexpr int kXAtomBytes = kHalf * 128;
   static constexpr int kXBytes = 2 * kXAtomBytes;
-  static constexpr int kWBytes = MX ? 3072 : 4 * kPairWTileBytes;  // (two records, rounded up to whole KB)
+  static constexpr int kWBytes = MX ? (2 * kMxRecord + 1023) / 1024 * 1024 : 4 * kPairWTileBytes;  // (two records, in whole KB)
   static constexpr int kStageBytes = kXBytes + kWBytes;
   // At 256 tokens x, W and the expanded rows share a ring position and a barrier;
   // at 128 the UMMAs of a stage take half as long, and x and W are fetched up to
@@ -58,7 +58,6 @@ struct MxPairStage {
   static constexpr int kBarOffset = kEpiOffset + 4 * kPairEpiBufBytes;  // two buffers per epilogue set
   static_assert(kBarOffset + 512 + 1024 <= kPairSmemBytes, "shared memory");
   static_assert(kStageBytes % 1024 == 0, "swizzled x tiles start on 1 KB");
-  static_assert(2 * kMxRecord <= 3072, "two records");
   static_assert(kAColBase + kPairAStages * kPairACols <= 512, "tensor memory");
 };
 
