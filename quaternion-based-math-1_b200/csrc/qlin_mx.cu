@@ -133,7 +133,8 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
 
 struct BackwardWs {
   // (fp32: planes are wide records, gy its B words)
-  size_t gy = 0, x = 0, a = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0, sums = 0;
+  size_t gy = 0, x = 0, a = 0, at = 0, bt = 0, parts = 0, up = 0, t = 0, planes = 0, partial0 = 0, partial1 = 0, sums = 0,
+         up_tops = 0, t_tops = 0;
   int64_t M_pad = 0, ld_parts = 0, ld_planes = 0;
   int rows = 0, splits0 = 0, splits1 = 0;
   size_t total = 0;
@@ -190,6 +191,10 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
       w.parts = c.take(M * 2 * w.ld_parts * 2);
       w.up = c.take(2 * w.rows * w.M_pad * 2);
       w.t = c.take(2 * w.rows * w.M_pad * 2);
+      if (dtype == QLIN_F16) {
+        w.up_tops = c.take(w.M_pad / kMxDownRows * w.rows);
+        w.t_tops = c.take(w.M_pad / kMxDownRows * w.rows);
+      }
       w.partial0 = c.take((int64_t)w.splits0 * w.rows * K * 4);
       w.partial1 = c.take((int64_t)w.splits1 * w.rows * N * 4);
       w.sums = c.take((int64_t)w.splits1 * N * 4);
@@ -523,7 +528,7 @@ int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t col
 
 template <typename T>
 MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t ld_a, int64_t K, float scale, int rank, T* parts,
-                      int64_t ld_parts, T* turned, int rows, int64_t tokens) {
+                      int64_t ld_parts, T* turned, uint8_t* tops, int rows, int64_t tokens) {
   MxDownJob<T> j{};
   j.x = x;
   j.ld_x = ld_x;
@@ -535,6 +540,7 @@ MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t ld_a, int64_
   j.parts = parts;
   j.ld_parts = parts ? (int)ld_parts : 0;
   j.turned = turned;
+  j.tops = tops;
   j.rows = turned ? rows : 0;
   j.rank_tiles = (int)ceil_div(std::max(j.ld_parts, j.rows), kMxDownRanks);
   j.blocks = (int)(ceil_div(tokens, kMxDownRows) * j.rank_tiles);
@@ -561,7 +567,7 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
     int64_t ld_a = 4 * K_g;
     st = rows_for_tma(&a, &ld_a, ws + w.a, rank, 4 * K_g, true, s);
     if (st != QLIN_OK) return st;
-    const MxDownJob<T> job = down_job<T>(x, ld_x, a, ld_a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, 0, M);
+    const MxDownJob<T> job = down_job<T>(x, ld_x, a, ld_a, 4 * K_g, scale, rank, parts, w.ld_parts, nullptr, nullptr, 0, M);
     st = launch_down<T>(job, MxDownJob<T>{}, M, M, s);
     if (st != QLIN_OK) return st;
   }
@@ -604,9 +610,10 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
   if (rank > 0 && (need_up || db)) {
     MxDownJob<T> j0{}, j1{};
     if (need_up)
-      j0 = down_job<T>(g, ld_g, bt, round_up(N, 8), N, scale, rank, dx ? parts : nullptr, w.ld_parts, da ? up : nullptr, w.rows, w.M_pad);
+      j0 = down_job<T>(g, ld_g, bt, round_up(N, 8), N, scale, rank, dx ? parts : nullptr, w.ld_parts,
+                       da ? up : nullptr, ws + w.up_tops, w.rows, w.M_pad);
     if (db)
-      j1 = down_job<T>(x, ld_x, a8, ld_a, K, scale, rank, nullptr, 0, t, w.rows, w.M_pad);
+      j1 = down_job<T>(x, ld_x, a8, ld_a, K, scale, rank, nullptr, 0, t, ws + w.t_tops, w.rows, w.M_pad);
     st = launch_down<T>(j0, j1, M, w.M_pad, s);
     if (st != QLIN_OK) return st;
   }
@@ -618,9 +625,10 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
   const bool sum_with_db = db && dbias;
   if (da || db) {
     MxOuterJob<T> o0{}, o1{};
-    auto job = [&](MxOuterJob<T>& o, const T* turned, const T* X, int64_t ld, int64_t cols, int rows, int splits,
-                   size_t partial) {
+    auto job = [&](MxOuterJob<T>& o, const T* turned, size_t tops, const T* X, int64_t ld, int64_t cols, int rows,
+                   int splits, size_t partial) {
       o.turned = turned;
+      o.tops = ws + tops;
       o.X = X;
       o.ld = ld;
       o.cols = (int)cols;
@@ -631,8 +639,8 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
       o.blocks = o.col_tiles * o.row_tiles * splits;
       o.partial = reinterpret_cast<float*>(ws + partial);
     };
-    if (da) job(o0, up, x, ld_x, K, w.rows, w.splits0, w.partial0);
-    if (db) job(o1, t, g, ld_g, N, w.rows, w.splits1, w.partial1);
+    if (da) job(o0, up, w.up_tops, x, ld_x, K, w.rows, w.splits0, w.partial0);
+    if (db) job(o1, t, w.t_tops, g, ld_g, N, w.rows, w.splits1, w.partial1);
     static std::atomic<uint64_t> done{0};
     if (allow_smem(qlin_mx_outer_kernel<T>, done, kMxOuterSmem) != QLIN_OK) return QLIN_ERR_LAUNCH;
     if (sum_with_db) o1.sums = reinterpret_cast<float*>(ws + w.sums);

@@ -5,7 +5,8 @@
 //     dbias = sum_m gy[m]   [N]
 //
 // t and u are kept as two 16-bit parts (or in fp32): rounded to one they would
-// add an error of the size of the gradients' own rounding.  x and gy are read
+// add an error of the size of the gradients' own rounding.  For dA and dB f16 parts
+// carry a power of two per rank and 16 tokens (mx_top_scale).  x and gy are read
 // once for t and u and once for the gradients, which bounds these kernels; the
 // products are warp-level tensor-core ones (m16n8k16) whose k slots are numbered
 // so that a lane reads eight consecutive elements of a row in one 16-byte piece
@@ -170,10 +171,21 @@ struct MxDownJob {
   float scale;
   T* parts;        // [M, 2, ld_parts]: hi and lo, zero from rank to ld_parts; or null
   T* turned;       // [2][rows][M_pad]: hi, then lo, transposed; or null
+  uint8_t* tops;   // f16: [M_pad / 16][rows]: exponent fields of the groups of 16 tokens (see mx_top_scale)
   int rank, ld_parts, rows;
   int rank_tiles;  // ceil(max(ld_parts, rows) / 32)
   int blocks;
 };
+
+// f16 parts of a rank and 16 tokens are multiplied by the power of two that brings
+// their largest finite magnitude, of exponent field `top`, to 2^14 .. 2^15: unscaled,
+// both parts would end at 2^-24, and u is far smaller early in a training (B starts at
+// zero) or with small gradients.  `top` is at least kMxLeastTop (the factor stays an
+// fp32 number); 0: the group has no finite value but zeros.
+constexpr int kMxLeastTop = 14;
+__device__ __forceinline__ float mx_top_scale(int top) {
+  return top ? __uint_as_float((uint32_t)(268 - top) << 23) : 1.f;
+}
 
 constexpr int kMxDownStages = 4;
 constexpr int kMxDownPieces = 6;  // 16-byte pieces of a lane and stage: two tokens, four ranks
@@ -255,6 +267,15 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
 #pragma unroll
       for (int w = 0; w < 8; ++w) v += red[w][m][r];
       v = m0 + m < M && r0 + r < job.rank ? v * job.scale : 0.f;
+      if (HALF && way == 1) {  // 16 consecutive lanes: the tokens of a rank
+        const uint32_t bits = __float_as_uint(v) & 0x7FFFFFFFu;
+        uint32_t most = bits < 0x7F800000u ? bits : 0u;
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        const int top = most ? max((int)(most >> 23), kMxLeastTop) : 0;
+        if (m == 0 && r0 + r < job.rows) job.tops[(int64_t)(m0 / kMxDownRows) * job.rows + r0 + r] = (uint8_t)top;
+        v *= mx_top_scale(top);
+      }
       const T hi = from_f32<T>(v);
       const float rest = v - to_f32(hi);
       const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
@@ -281,12 +302,14 @@ constexpr int kMxOuterTokens = 32;  // tokens of a step
 constexpr int kMxOuterRows = 64;    // rows of the result of a CTA (groups of 16)
 constexpr int kMxOuterStages = 4;
 constexpr int kMxOuterXBytes = kMxOuterTokens * kMxOuterCols * 2;
-constexpr int kMxOuterStage = kMxOuterXBytes + 2 * kMxOuterRows * kMxOuterTokens * 2;
+constexpr int kMxOuterTops = 2 * kMxOuterRows;  // bytes: f16's exponents of a step's two groups of 16 tokens
+constexpr int kMxOuterStage = kMxOuterXBytes + 2 * kMxOuterRows * kMxOuterTokens * 2 + kMxOuterTops;
 constexpr int kMxOuterSmem = kMxOuterStages * kMxOuterStage;
 
 template <typename T>
 struct MxOuterJob {
   const T* turned;  // [2][rows][M_pad]; fp32: [M][rows]
+  const uint8_t* tops;  // f16: of the parts, see MxDownJob
   const T* X;       // [M, ld], 16-byte aligned rows
   int64_t ld;
   int cols, rows;   // rows: a multiple of 16
@@ -296,10 +319,21 @@ struct MxOuterJob {
   float* sums;      // [splits][cols] column sums of X, or null
 };
 
+// The packed f16 factor 2^(top - row_top) (0 below f16's numbers) that brings a group's
+// parts to their row's power of two.
+__device__ __forceinline__ uint32_t mx_top_factor(int top, int row_top) {
+  const int e = top ? 15 + top - row_top : 1;  // (a group of zeros, infinities and NaNs: any factor)
+  return (e > 0 ? (uint32_t)e << 10 : (e > -10 ? 1u << (9 + e) : 0u)) * 0x00010001u;
+}
+
 // Four warps: 32 columns each, all rows.  X and the rows of (hi, lo) come through
 // a ring of shared memory steps (32 tokens x 128 columns; 16-byte chunks permuted
 // within a row of X so that the transposing loads of eight tokens two apart are
 // free of conflicts).
+//
+// f16: a CTA brings the parts of a row to the power of two of the row's largest group
+// among its own tokens (one packed multiplication per pair; what falls below f16 is
+// 2^-39 of that largest value) and undoes it on the sums.
 //
 // beside: the launch before is the CTA-pair kernel, which needs nothing from this one
 // and lets it start only when the down projections have ended.  CTAs then take the SMs
@@ -338,6 +372,11 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   const T* ap = job.turned + (int64_t)(row0 + min(ar, rows - 1)) * M_pad + s0 * kMxOuterTokens + 8 * (threadIdx.x & 3);
   const int64_t lo_off = (int64_t)job.rows * M_pad, row32 = 32 * (int64_t)M_pad;
   const uint32_t a_at = kMxOuterXBytes + ar * 64 + ((threadIdx.x & 3) << 4);
+  // f16: 16 exponents of a group, by the first threads
+  constexpr uint32_t kTopsAt = kMxOuterStage - kMxOuterTops;
+  const bool tops = HALF && (int)threadIdx.x < 2 * groups;
+  const int tgroup = (int)threadIdx.x >= groups, tpiece = (int)threadIdx.x - (tgroup ? groups : 0);
+  const uint8_t* tp = job.tops + (int64_t)(2 * s0 + tgroup) * job.rows + row0 + 16 * tpiece;
   int m_next = s0 * kMxOuterTokens + tok;
   const int m_end = s1 * kMxOuterTokens;  // (tok < 8: a step begins before it or not at all)
   MxRing in, out;
@@ -358,8 +397,10 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
         cp_async16(base + a_at + 32 * 64, ap + row32, 16);
         cp_async16(base + a_at + (kMxOuterRows + 32) * 64, ap + row32 + lo_off, 16);
       }
+      if (tops) cp_async16(base + kTopsAt + tgroup * kMxOuterRows + 16 * tpiece, tp, 16);
       xp += 4 * x_eight;
       ap += kMxOuterTokens;
+      tp += 2 * (int64_t)job.rows;
       m_next += kMxOuterTokens;
       in.next(kMxOuterStages);
     }
@@ -367,6 +408,19 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   };
 #pragma unroll
   for (int k = 0; k < kMxOuterStages - 1; ++k) fetch();
+
+  __shared__ int row_top[HALF ? kMxOuterRows : 1];  // the rows' largest exponents among this CTA's tokens
+  if constexpr (HALF) {
+    if (threadIdx.x < kMxOuterRows) row_top[threadIdx.x] = 0;
+    __syncthreads();
+    const int row = threadIdx.x & (kMxOuterRows - 1);
+    int top = 0;
+    if (row < rows)
+      for (int k = 2 * s0 + (int)(threadIdx.x / kMxOuterRows); k < 2 * s1; k += 128 / kMxOuterRows)
+        top = max(top, (int)__ldcg(job.tops + (int64_t)k * job.rows + row0 + row));
+    atomicMax(&row_top[row], top);  // a maximum: the same in any order
+    __syncthreads();
+  }
 
   float acc[4][4][4] = {};  // [row group][8 columns][fragment]
   float sum[4] = {};
@@ -399,29 +453,51 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (r < groups)
+      if (r < groups) {
+        uint32_t fl = 0u, fh = 0u;  // f16: of rows g and g + 8, this lane's eight tokens
+        if constexpr (HALF) {
+          const uint8_t* at = mx_smem + (base - smem_u32(mx_smem)) + kTopsAt + (t >> 1) * kMxOuterRows + 16 * r + g;
+          fl = mx_top_factor(at[0], row_top[16 * r + g]);
+          fh = mx_top_factor(at[8], row_top[16 * r + g + 8]);
+        }
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           const uint32_t at = base + kMxOuterXBytes + (part * kMxOuterRows + 16 * r + g) * 64 + t * 16;
-          const uint4 l = lds128(at), h = lds128(at + 8 * 64);
+          uint4 l = lds128(at), h = lds128(at + 8 * 64);
+          if constexpr (HALF) {
+            l.x = mx_mul2<true>(l.x, fl); l.y = mx_mul2<true>(l.y, fl);
+            l.z = mx_mul2<true>(l.z, fl); l.w = mx_mul2<true>(l.w, fl);
+            h.x = mx_mul2<true>(h.x, fh); h.y = mx_mul2<true>(h.y, fh);
+            h.z = mx_mul2<true>(h.z, fh); h.w = mx_mul2<true>(h.w, fh);
+          }
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             mx_mma<HALF>(acc[r][n], l.x, h.x, l.y, h.y, b[n][0], b[n][1]);
             mx_mma<HALF>(acc[r][n], l.z, h.z, l.w, h.w, b[n][2], b[n][3]);
           }
         }
+      }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (r < groups)
+    if (r < groups) {
+      float down[2] = {1.f, 1.f};  // of rows g and g + 8
+      if constexpr (HALF) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int top = row_top[16 * r + g + 8 * h];
+          if (top) down[h] = scalbnf(1.f, top - 141);  // 1 / mx_top_scale
+        }
+      }
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int row = row0 + 16 * r + g + 8 * (q >> 1), c = c0 + 32 * warp + 8 * n + 2 * t + (q & 1);
-          if (c < job.cols) job.partial[((int64_t)split * job.rows + row) * job.cols + c] = acc[r][n][q];
+          if (c < job.cols) job.partial[((int64_t)split * job.rows + row) * job.cols + c] = acc[r][n][q] * down[q >> 1];
         }
+    }
   if (sums)
 #pragma unroll
     for (int n = 0; n < 4; ++n) {

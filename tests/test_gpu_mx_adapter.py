@@ -1,0 +1,116 @@
+"""LoRA adapters on 4-bit weights where the adapter's own products decide the
+result: one output rounding over the types' whole range."""
+
+import numpy as np
+import pytest
+import torch
+
+import mx_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def rounded(want, dtype):
+    with np.errstate(over="ignore"):
+        return ref.f64(torch.from_numpy(np.ascontiguousarray(want)).to(ref.TORCH[dtype]))
+
+
+def bound(want, dtype, terms):
+    """2-norm of an error: that of the one rounding to the type, a tenth more for values
+    that an earlier error moves to the other neighbour, and fp32 sums of `terms` terms
+    as in ref.tolerance."""
+    return 1.1 * np.linalg.norm(rounded(want, dtype) - want) + \
+        2.0 ** -23 * (2 + terms) ** 0.5 * np.linalg.norm(want)
+
+
+def one_rounding(got, want, dtype, terms, what=""):
+    want = np.asarray(want)
+    assert np.isfinite(rounded(want, dtype)).all(), "the exact result is in range"
+    got = ref.f64(got)
+    assert np.isfinite(got).all(), what
+    assert np.linalg.norm(got - want) <= bound(want, dtype, terms), what
+
+
+def zero_base(qb, fin, fout, device):
+    return qb.quantize_quaternion_weights(*(torch.zeros(fout // 4, fin // 4, device=device) for _ in range(4)))
+
+
+def values_of(q):
+    return np.stack([ref.f64(w) for w in q.dequantize(torch.float32)])
+
+
+def backward(qb, q, d, gy):
+    leaves = {k: d[k].clone().requires_grad_(True) for k in ("x", "a", "b")}
+    y = qb.mx_quaternion_linear(leaves["x"], q, None, leaves["a"], leaves["b"], d["scale"])
+    return dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), gy)))
+
+
+def expected(q, d, gy):
+    dx, da, db, _ = ref.gradients(ref.f64(gy), ref.f64(d["x"]), values_of(q), ref.f64(d["a"]), ref.f64(d["b"]),
+                                  d["scale"])
+    return {"x": dx, "a": da, "b": db}
+
+
+# ------------------------------------------------- small gradients and factors
+@pytest.mark.parametrize("gy_std", [1.0, 1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("M", [24, 500])
+def test_adapter_gradients_of_small_fp16_values(qb, cuda, gy_std, M):
+    """A LoRA factor near zero and gradients down to fp16's smallest numbers, tokens
+    of very different size among them."""
+    d = ref.draw("f16", M, 512, 1024, rank=8, seed=M, device=cuda)
+    d["b"] = (d["b"].float() * (1e-4 / 0.05)).half()
+    q = qb.quantize_quaternion_weights(*d["w"])
+    gy = ref.draw("f16", M, 1024, 4, seed=5, device=cuda)["x"].float() * gy_std
+    for far in (0, 12):
+        g = gy * torch.exp2(-(torch.arange(M, device=cuda) % (far + 1)).float())[:, None]
+        g = g.half()
+        got, want = backward(qb, q, d, g), expected(q, d, g)
+        one_rounding(got["a"], want["a"], "f16", M + 1024, "a")
+    # the other factor: a small scale makes t small
+    d["a"] = (d["a"].float() * 1e-3).half()
+    d["scale"] = 2.0 * gy_std
+    g = ref.draw("f16", M, 1024, 4, seed=5, device=cuda)["x"]
+    got, want = backward(qb, q, d, g), expected(q, d, g)
+    one_rounding(got["b"], want["b"], "f16", M + 512, "b")
+
+
+def test_adapter_gradients_of_far_apart_token_groups(qb, cuda):
+    """Whole groups of tokens zero, and others far below the rest: their ranks' sums
+    neither vanish nor spill over."""
+    M = 320
+    d = ref.draw("f16", M, 256, 256, rank=20, seed=1, device=cuda)
+    q = qb.quantize_quaternion_weights(*d["w"])
+    level = torch.tensor([0.0, 1.0, 2.0 ** -10, 2.0 ** -20, 0.0] * 4, device=cuda).repeat_interleave(16)[:, None]
+    base = ref.draw("f16", M, 256, 4, seed=2, device=cuda)["x"].float()
+    for gy in ((base * level).half(), (base * level.flip(0)).half()):
+        got, want = backward(qb, q, d, gy), expected(q, d, gy)
+        one_rounding(got["a"], want["a"], "f16", M + 256, "a")
+        one_rounding(got["b"], want["b"], "f16", M + 256, "b")
+    # only the smallest tokens
+    gy = (ref.draw("f16", M, 256, 4, seed=2, device=cuda)["x"].float() * 2.0 ** -20).half()
+    got, want = backward(qb, q, d, gy), expected(q, d, gy)
+    one_rounding(got["a"], want["a"], "f16", M + 256, "a")
+    zero = torch.zeros_like(gy)
+    got = backward(qb, q, d, zero)
+    assert not any(bool(t.any()) for t in got.values())
+
+
+def test_nonfinite_tokens_in_adapter_gradients(qb, cuda):
+    """A token with an infinity or a NaN makes the sums it is part of non-finite, no others."""
+    M = 100
+    for dtype in ("f16", "bf16"):
+        d = ref.draw(dtype, M, 128, 128, rank=8, seed=1, device=cuda)
+        q = qb.quantize_quaternion_weights(*d["w"])
+        clean = ref.draw(dtype, M, 128, 4, seed=2, device=cuda)["x"]
+        want = backward(qb, q, d, clean)
+        for bad in (float("inf"), float("nan")):
+            gy = clean.clone()
+            gy[40, 5] = bad
+            got = backward(qb, q, d, gy)
+            keep = torch.arange(M, device=cuda) != 40
+            assert torch.equal(got["x"][keep], want["x"][keep])
+            assert not bool(got["x"][40].isfinite().any())
+            assert not bool(got["a"].isfinite().any())
+            others = torch.arange(128, device=cuda) != 5
+            assert torch.equal(got["b"][others], want["b"][others])
+            assert not bool(got["b"][5].isfinite().any())
