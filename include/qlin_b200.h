@@ -454,9 +454,8 @@ int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g,
  * accumulation is fp32, outputs are rounded once.  Arguments as qlin_forward;
  * workspace of at least qlin_mx_workspace_size() bytes, 256-byte aligned.
  * 16-bit types with more than 32 tokens want y 8-byte aligned and ld_y a multiple
- * of 4 (QLIN_ERR_ALIGN).  fp16 with a LoRA wants |lora_b| up to 1000 there, and
- * fp16 values of the scaled down projection.  Waits inside the kernels are bounded
- * (qlin_get_device_error).
+ * of 4 (QLIN_ERR_ALIGN).  The down projection is kept in fp32's range and precision
+ * for every type.  Waits inside the kernels are bounded (qlin_get_device_error).
  */
 int qlin_mx_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes);
 int qlin_mx_forward(int dtype,

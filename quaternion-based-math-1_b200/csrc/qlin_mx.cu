@@ -106,6 +106,8 @@ bool is_one(int dtype, int64_t M, int64_t K_g) {
 // Rows of 16-bit elements that TMA takes: 16-byte aligned start and row stride.
 bool tma_rows(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0; }
 
+int64_t pair_parts(int dtype) { return dtype == QLIN_F16 ? kMxPairParts<__half> : kMxPairParts<__nv_bfloat16>; }
+
 struct ForwardWs {
   size_t arranged = 0, t = 0, x = 0, a = 0, total = 0;
   int64_t ld_parts = 0;  // ranks of t's rows, in whole 16-byte pieces
@@ -124,7 +126,7 @@ ForwardWs forward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   } else {
     w.ld_parts = round_up(rank, 8);
     w.x = c.take(M * round_up(4 * K_g, 8) * 2);
-    w.t = c.take(M * 2 * w.ld_parts * 2);
+    w.t = c.take(M * pair_parts(dtype) * w.ld_parts * 2);
     w.a = c.take(rank * round_up(4 * K_g, 8) * 2);
   }
   w.total = c.at;
@@ -188,7 +190,7 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
       w.at = c.take(K * rank * 2);
       w.bt = c.take(round_up(N, 8) * rank * 2);
       w.a = c.take(rank * round_up(K, 8) * 2);
-      w.parts = c.take(M * 2 * w.ld_parts * 2);
+      w.parts = c.take(M * pair_parts(dtype) * w.ld_parts * 2);
       w.up = c.take(2 * w.rows * w.M_pad * 2);
       w.t = c.take(2 * w.rows * w.M_pad * 2);
       if (dtype == QLIN_F16) {
@@ -444,7 +446,7 @@ int pair_capacity() {
 // makes `parts`.
 template <typename T, int NTOK, bool MX>
 int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& planes, int64_t ld_w, const T* bias,
-                const T* parts, int64_t ld_parts, const T* lora_b, int rank, T* y, int64_t ld_y, int64_t M,
+                const __nv_bfloat16* parts, int64_t ld_parts, const T* lora_b, int rank, T* y, int64_t ld_y, int64_t M,
                 int64_t K_g, int64_t N_g, cudaStream_t s) {
   using Cfg = MxPairStage<NTOK, MX>;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -455,9 +457,9 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
   std::memset(&map_t, 0, sizeof(map_t));
   std::memset(map_w, 0, sizeof(map_w));
   int st = encode_map(&map_x, bf16, x, 2, {4 * K_g, M, 1}, {ld_x, 0}, {64, Cfg::kHalf, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (st == QLIN_OK && rank > 0)  // [part][token][rank]: ranks past ld_parts read as zero
-    st = encode_map(&map_t, bf16, parts, 3, {ld_parts, M, 2}, {2 * ld_parts, ld_parts}, {64, Cfg::kHalf, 1},
-                    CU_TENSOR_MAP_SWIZZLE_128B);
+  const int64_t terms = kMxPairParts<T> * ld_parts;
+  if (st == QLIN_OK && rank > 0)  // [token][term]: past the last term zero
+    st = encode_map(&map_t, true, parts, 2, {terms, M, 1}, {terms, 0}, {64, Cfg::kHalf, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
   if (!MX)
     for (int p = 0; p < 4 && st == QLIN_OK; ++p)
       st = encode_map(&map_w[p], bf16, planes.w[p], 2, {K_g, N_g, 1}, {ld_w, 0}, {32, 32, 1}, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -475,7 +477,8 @@ int launch_pair(const T* x, int64_t ld_x, const void* mx, const MxPlanes<T>& pla
   prm.kb = (int)ceil_div(K_g, kMxBlock);
   prm.w_tiles = (int)ceil_div(N_g, kMxRows);
   prm.stages = (int)ceil_div(K_g, 32);
-  prm.lora_stages = (int)ceil_div(rank, 64);
+  prm.ld_parts = (int)ld_parts;
+  prm.lora_stages = rank > 0 ? (int)ceil_div(ld_parts, kMxPairRanks<T>) : 0;
   prm.nb_tiles = (int)ceil_div(4 * N_g, 256);
   const int64_t tiles = prm.nb_tiles * ceil_div(M, NTOK);
   if (tiles * (prm.stages + prm.lora_stages) > INT32_MAX) return QLIN_ERR_SHAPE;
@@ -527,8 +530,8 @@ int rows_for_tma(const T** x, int64_t* ld, void* copy, int64_t rows, int64_t col
 }
 
 template <typename T>
-MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t ld_a, int64_t K, float scale, int rank, T* parts,
-                      int64_t ld_parts, T* turned, uint8_t* tops, int rows, int64_t tokens) {
+MxDownJob<T> down_job(const T* x, int64_t ld_x, const T* a, int64_t ld_a, int64_t K, float scale, int rank,
+                      __nv_bfloat16* parts, int64_t ld_parts, T* turned, uint8_t* tops, int rows, int64_t tokens) {
   MxDownJob<T> j{};
   j.x = x;
   j.ld_x = ld_x;
@@ -562,7 +565,7 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
   if (!aligned(y, 8) || ld_y % 4 != 0) return QLIN_ERR_ALIGN;
   int st = rows_for_tma(&x, &ld_x, ws + w.x, M, 4 * K_g, rank > 0, s);
   if (st != QLIN_OK) return st;
-  T* parts = reinterpret_cast<T*>(ws + w.t);
+  __nv_bfloat16* parts = reinterpret_cast<__nv_bfloat16*>(ws + w.t);
   if (rank > 0) {
     int64_t ld_a = 4 * K_g;
     st = rows_for_tma(&a, &ld_a, ws + w.a, rank, 4 * K_g, true, s);
@@ -571,8 +574,8 @@ int run_prefill(const T* x, int64_t ld_x, const void* mx, const T* bias, const T
     st = launch_down<T>(job, MxDownJob<T>{}, M, M, s);
     if (st != QLIN_OK) return st;
   }
-  return run_pair<T, true>(M, N_g, x, ld_x, mx, MxPlanes<T>{}, (int64_t)0, bias, (const T*)parts, w.ld_parts, b, rank, y,
-                           ld_y, M, K_g, N_g, s);
+  return run_pair<T, true>(M, N_g, x, ld_x, mx, MxPlanes<T>{}, (int64_t)0, bias, (const __nv_bfloat16*)parts,
+                           w.ld_parts, b, rank, y, ld_y, M, K_g, N_g, s);
 }
 
 // Gradients, 16 bits.
@@ -584,7 +587,7 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
   if (dx && (!aligned(dx, 8) || ld_dx % 4 != 0)) return QLIN_ERR_ALIGN;
   T* at = reinterpret_cast<T*>(ws + w.at);
   T* bt = reinterpret_cast<T*>(ws + w.bt);
-  T* parts = reinterpret_cast<T*>(ws + w.parts);
+  __nv_bfloat16* parts = reinterpret_cast<__nv_bfloat16*>(ws + w.parts);
   T* up = reinterpret_cast<T*>(ws + w.up);
   T* t = reinterpret_cast<T*>(ws + w.t);
   int st = QLIN_OK;
@@ -618,8 +621,8 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     if (st != QLIN_OK) return st;
   }
   if (dx) {
-    st = run_pair<T, false>(M, K_g, g, ld_g, mx, p, w.ld_planes, (const T*)nullptr, (const T*)parts, w.ld_parts,
-                            (const T*)at, rank, dx, ld_dx, M, N_g, K_g, s);
+    st = run_pair<T, false>(M, K_g, g, ld_g, mx, p, w.ld_planes, (const T*)nullptr, (const __nv_bfloat16*)parts,
+                            w.ld_parts, (const T*)at, rank, dx, ld_dx, M, N_g, K_g, s);
     if (st != QLIN_OK) return st;
   }
   const bool sum_with_db = db && dbias;

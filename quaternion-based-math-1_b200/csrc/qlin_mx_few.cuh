@@ -71,12 +71,20 @@ struct MxOperand {
   static constexpr int kParts = std::is_same<T, float>::value ? 3 : 1;
 };
 
-// c of the layer whose largest F is f0.  With an adapter of some rank that goes
-// through the same accumulator, fp16 keeps B 2^-c in range for |B| up to 1000.
+// An adapter in the CTA-pair kernel (see there): terms of the product per rank, and
+// ranks whose terms a stage of 128 holds.
+template <typename T>
+constexpr int kMxPairParts = MxOperand<T>::kHalf ? 5 : 3;
+template <typename T>
+constexpr int kMxPairRanks = 128 / kMxPairParts<T> / 8 * 8;
+
+// c of the layer whose largest F is f0.  An adapter's products join the accumulator
+// with B 2^-c: a bound for fp16 keeps them in fp32's range (weights so small, 2^-40 of
+// fp16's steps, are lost in the rounding of y anyway).
 template <bool HALF>
 __device__ __forceinline__ int mx_shift(uint32_t f0, int rank = 0) {
   const int c = (int)f0 - 129;
-  return HALF ? (rank > 0 ? max(c, -6) : c) : max(0, c);
+  return HALF ? (rank > 0 ? max(c, -40) : c) : max(0, c);
 }
 
 // The packed multiplier of codes with scale F.  bf16: exponent field

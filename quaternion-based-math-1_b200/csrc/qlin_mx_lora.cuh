@@ -4,9 +4,10 @@
 //     dA = u^T x            [r, K]      dB = gy^T t           [N, r]
 //     dbias = sum_m gy[m]   [N]
 //
-// t and u are kept as two 16-bit parts (or in fp32): rounded to one they would
-// add an error of the size of the gradients' own rounding.  For dA and dB f16 parts
-// carry a power of two per rank and 16 tokens (mx_top_scale).  x and gy are read
+// t and u are kept as parts (or in fp32): rounded to one they would add an error of the
+// size of the results' own rounding.  The CTA-pair kernel takes them as three bf16 parts
+// (exact), dA and dB as two 16-bit ones, with a power of two per rank and 16 tokens for
+// f16 (mx_top_scale).  x and gy are read
 // once for t and u and once for the gradients, which bounds these kernels; the
 // products are warp-level tensor-core ones (m16n8k16) whose k slots are numbered
 // so that a lane reads eight consecutive elements of a row in one 16-byte piece
@@ -169,7 +170,7 @@ struct MxDownJob {
   int64_t ld_a;    // (both: 16-byte aligned rows of K elements)
   int K;           // a multiple of 8: zero past the product's terms
   float scale;
-  T* parts;        // [M, 2, ld_parts]: hi and lo, zero from rank to ld_parts; or null
+  __nv_bfloat16* parts;  // [M, kMxPairParts<T> * ld_parts], the CTA-pair kernel's terms: zero past rank; or null
   T* turned;       // [2][rows][M_pad]: hi, then lo, transposed; or null
   uint8_t* tops;   // f16: [M_pad / 16][rows]: exponent fields of the groups of 16 tokens (see mx_top_scale)
   int rank, ld_parts, rows;
@@ -257,7 +258,7 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    // hi and lo of (token, rank); ranks fastest for `parts`, tokens fastest for `turned`
+    // the parts of (token, rank); ranks fastest for `parts`, tokens fastest for `turned`
 #pragma unroll
     for (int way = 0; way < 2; ++way) {
       if (way == 0 ? !job.parts : !job.turned) continue;
@@ -276,16 +277,27 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
         if (m == 0 && r0 + r < job.rows) job.tops[(int64_t)(m0 / kMxDownRows) * job.rows + r0 + r] = (uint8_t)top;
         v *= mx_top_scale(top);
       }
-      const T hi = from_f32<T>(v);
-      const float rest = v - to_f32(hi);
-      const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
       if (way == 0) {
         if (m0 + m < M && r0 + r < job.ld_parts) {
-          T* at = job.parts + (int64_t)(m0 + m) * 2 * job.ld_parts + r0 + r;
-          at[0] = hi;
-          at[job.ld_parts] = lo;
+          // (an infinite or NaN first part stands alone)
+          const __nv_bfloat16 p0 = __float2bfloat16_rn(v);
+          const float rest = isfinite(to_f32(p0)) ? v - to_f32(p0) : 0.f;
+          const __nv_bfloat16 p1 = __float2bfloat16_rn(rest), p2 = __float2bfloat16_rn(rest - to_f32(p1));
+          // [stage][part][rank of the stage]
+          const int first = (r0 + r) / kMxPairRanks<T> * kMxPairRanks<T>, ranks = min(kMxPairRanks<T>, job.ld_parts - first);
+          __nv_bfloat16* at = job.parts + ((int64_t)(m0 + m) * job.ld_parts + first) * kMxPairParts<T> + (r0 + r - first);
+          at[0] = p0;
+          at[ranks] = p1;
+          at[2 * ranks] = p2;
+          if (HALF) {
+            at[3 * ranks] = isfinite(to_f32(p0)) ? p0 : __float2bfloat16_rn(0.f);
+            at[4 * ranks] = p1;
+          }
         }
       } else if (r0 + r < job.rows) {
+        const T hi = from_f32<T>(v);
+        const float rest = v - to_f32(hi);
+        const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
         T* at = job.turned + (int64_t)(r0 + r) * M_pad + m0 + m;
         at[0] = hi;
         at[(int64_t)job.rows * M_pad] = lo;

@@ -20,14 +20,17 @@
 // bf16 tokens 113 us in a burst (1630 TFLOP/s), 134 us sustained (1380, at the power
 // limit); 5120 -> 27648 with an adapter of rank 32 368 and 421 us.
 //
-// Adapter: y += t B^T with t = s x A^T as two 16-bit parts (t = hi + lo to about
-// twice the type's precision): ceil(r / 64) more stages whose x tile is 64
-// ranks of hi and of lo and whose weight rows are the same 64 ranks of B twice.
+// Adapter: y += t B^T with t = s x A^T and B as sums of bf16 parts, for fp16 too: bf16
+// has fp32's range, so that neither a large B nor a small or large t leaves it.  t =
+// t0 + t1 + t2 exactly; B is one part (bf16) or two (fp16: 11 bits as 8 + 3):
+//     bf16  t0 B + t1 B + t2 B        fp16  t0 b0 + t1 b0 + t2 b0 + t0 b1 + t1 b1
+// (t2 b1 is below 2^-24 of t B).  A stage holds the terms of up to 40 ranks (fp16: 24),
+// part by part, and takes as many UMMAs as they need.  UMMAs with bf16 operands add to
+// an accumulator that f16 ones began.  The builders fetch their rows of B before they
+// wait for the stage.
 //
 // The accumulator holds y 2^-c (mx_shift); B is built with the same factor, and
-// the epilogue multiplies by 2^c before the bias and the one rounding.  fp16
-// bounds c from below with an adapter, so that B 2^-c stays in range for |B| up
-// to 1000.
+// the epilogue multiplies by 2^c before the bias and the one rounding.
 #pragma once
 
 #include "qlin_mx.cuh"
@@ -61,6 +64,22 @@ struct MxPairStage {
   static_assert(kAColBase + kPairAStages * kPairACols <= 512, "tensor memory");
 };
 
+// Two elements of a row of B times `down` (a power of two) as bf16, and (fp16) the rest.
+template <typename T>
+__device__ __forceinline__ void mx_adapter_parts(uint32_t w, float down, uint32_t& first, uint32_t& second) {
+  const T* e = reinterpret_cast<const T*>(&w);
+  const float v0 = to_f32(e[0]) * down, v1 = to_f32(e[1]) * down;
+  first = pack2<__nv_bfloat16>(v0, v1);
+  const float r0 = v0 - __uint_as_float(first << 16), r1 = v1 - __uint_as_float(first & 0xFFFF0000u);
+  second = pack2<__nv_bfloat16>(isfinite(r0) ? r0 : 0.f, isfinite(r1) ? r1 : 0.f);
+}
+
+// 32 lanes x 32 bit, four consecutive columns per thread.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+               ::"r"(taddr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+
 struct MxPairParams {
   const uint8_t* mx;    // codes
   const void* bias;
@@ -70,7 +89,8 @@ struct MxPairParams {
   int M, N_g, K_g, rank;
   int kb, w_tiles;      // blocks of a row; 16-row tiles of the codes
   int stages;           // weight stages of a tile
-  int lora_stages;      // ceil(rank / 64)
+  int ld_parts;         // rank in whole 16-byte pieces
+  int lora_stages;      // ceil(ld_parts / kMxPairRanks)
   int nb_tiles, tiles;
   int wide;             // 16-byte output pieces are aligned
 };
@@ -98,6 +118,8 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   using Cfg = MxPairStage<NTOK, MX>;
   constexpr bool HALF = std::is_same<T, __half>::value;
   constexpr uint32_t kIdesc = make_idesc_f16(256, NTOK, HALF ? 0u : 1u, false);
+  constexpr uint32_t kIdescAdapter = make_idesc_f16(256, NTOK, 1u, false);
+  constexpr int kParts = kMxPairParts<T>, kRanks = kMxPairRanks<T>;
   constexpr int S = Cfg::kStages, SA = kPairAStages, NB = Cfg::kDBufs;
 
   extern __shared__ uint8_t smem_raw[];
@@ -189,16 +211,16 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           }
           uint8_t* dst = smem + s * Cfg::kStageBytes;
           if (k >= prm.stages) {
-            const int r = 64 * (k - prm.stages);
-            if (j == 0 && r == 0) {
+            const int at = kRanks * kParts * (k - prm.stages);  // of the terms (zero past their end)
+            if (j == 0 && at == 0) {
               pdl_wait_prior();
               // a kernel that starts from here on finds the down projection's results
               pdl_launch_dependents();
               fence_proxy_async();
             }
             mbar_arrive_expect_tx(&full[s], Cfg::kXBytes);
-            tma_load_3d(dst, &map_t, &full[s], r, mrow, 0);
-            tma_load_3d(dst + Cfg::kXAtomBytes, &map_t, &full[s], r, mrow, 1);
+            tma_load_2d(dst, &map_t, &full[s], at, mrow);
+            tma_load_2d(dst + Cfg::kXAtomBytes, &map_t, &full[s], at + 64, mrow);
           } else {
             mbar_arrive_expect_tx(&full[s], Cfg::kXBytes + (MX ? have * kMxRecord : 4 * kPairWTileBytes));
             tma_load_2d(dst, &map_x, &full[s], k * kPairStageK, mrow);
@@ -240,11 +262,16 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           tc_fence_after();
           const uint64_t bdesc0 = smem_desc_sw128(smem + s * Cfg::kStageBytes);
           const uint32_t d = tmem + b * NTOK, a0 = tmem + Cfg::kAColBase + sa * kPairACols;
+          const bool adapter = k >= prm.stages;
+          const uint32_t idesc = adapter ? kIdescAdapter : kIdesc;
+          const int steps = adapter ? (kParts * min(kRanks, prm.ld_parts - kRanks * (k - prm.stages)) + 15) / 16
+                                    : kPairStageK / 16;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kPairStageK / 16; ++kk)
-              umma_pair_ts(d, a0 + 8 * kk, bdesc0 + (uint64_t)((kk >> 2) * (Cfg::kXAtomBytes >> 4)) + 2 * (kk & 3),
-                           kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
+              if (kk < steps)
+                umma_pair_ts(d, a0 + 8 * kk, bdesc0 + (uint64_t)((kk >> 2) * (Cfg::kXAtomBytes >> 4)) + 2 * (kk & 3),
+                             idesc, (k > 0 || kk > 0) ? 1u : 0u);
             umma_commit_pair(&empty[s], 0x3);
             if constexpr (Cfg::kSplit) umma_commit_pair(&aempty[sa], 0x3);
             if (k == nk - 1) umma_commit_pair(&dfull[b], 0x3);
@@ -283,42 +310,53 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       // (in a shared ring x and W are fetched once the position's UMMAs are done, so
       // its tensor memory is free too when they land)
       const int s = g % S, sa = g % SA;
-      bool ok = !*abort_flag && mbar_wait(&full[s], (g / S) & 1);
-      if (Cfg::kSplit && ok && g >= SA) ok = mbar_wait(&aempty[sa], (g / SA - 1) & 1);
-      if (!ok) *abort_flag = 1;
-      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + sa * kPairACols;
-      if (!*abort_flag && k >= prm.stages) {
-        // 64 ranks of this row of B, twice
+      const int r0 = kRanks * (k - prm.stages);  // (an adapter's stage: its ranks)
+      uint4 brow[kRanks / 8];
+      if (k >= prm.stages) {
         int n0, m0;
         tile_coords(pair + j * pairs, n0, m0);
         const int64_t n_out = n0 + 4 * row + a;
-        const int r0 = 64 * (k - prm.stages);
         const T* b = reinterpret_cast<const T*>(prm.lora_b) + n_out * prm.rank + r0;
-        const int left = n_out < 4 * (int64_t)prm.N_g ? min(64, prm.rank - r0) : 0;
+        const int left = n_out < 4 * (int64_t)prm.N_g ? prm.rank - r0 : 0;
         const bool vec = prm.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(prm.lora_b) & 15) == 0;
-        uint32_t r[32];
-        const uint32_t mult = pack2<T>(down, down);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        for (int e = 0; e < kRanks / 8; ++e) {
+          brow[e] = make_uint4(0u, 0u, 0u, 0u);
           if (vec) {
-            if (8 * e < left) v = ld_cg_v4(b + 8 * e);
+            if (8 * e < left) brow[e] = ld_cg_v4(b + 8 * e);
           } else {
             unsigned short h[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
               h[u] = 8 * e + u < left ? *reinterpret_cast<const volatile unsigned short*>(b + 8 * e + u) : (unsigned short)0;
-            v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                           h[6] | (uint32_t)h[7] << 16);
+            brow[e] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                                 h[6] | (uint32_t)h[7] << 16);
           }
-          r[4 * e + 0] = c ? mx_mul2<HALF>(v.x, mult) : v.x;
-          r[4 * e + 1] = c ? mx_mul2<HALF>(v.y, mult) : v.y;
-          r[4 * e + 2] = c ? mx_mul2<HALF>(v.z, mult) : v.z;
-          r[4 * e + 3] = c ? mx_mul2<HALF>(v.w, mult) : v.w;
         }
+      }
+      bool ok = !*abort_flag && mbar_wait(&full[s], (g / S) & 1);
+      if (Cfg::kSplit && ok && g >= SA) ok = mbar_wait(&aempty[sa], (g / SA - 1) & 1);
+      if (!ok) *abort_flag = 1;
+      const uint32_t col = tmem + tm_lane + Cfg::kAColBase + sa * kPairACols;
+      if (!*abort_flag && k >= prm.stages) {
+        const int ranks = min(kRanks, prm.ld_parts - r0);
         __syncwarp();
-        tmem_st32(col, r);
-        tmem_st32(col + 32, r);
+#pragma unroll
+        for (int e = 0; e < kRanks / 8; ++e) {
+          if (8 * e >= ranks) break;
+          uint32_t p0[4], p1[4];
+          const uint32_t w[4] = {brow[e].x, brow[e].y, brow[e].z, brow[e].w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx_adapter_parts<T>(w[u], down, p0[u], p1[u]);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            const uint32_t at = col + (part * ranks + 8 * e) / 2;
+            if (part < 3) tmem_st4(at, p0[0], p0[1], p0[2], p0[3]);
+            else tmem_st4(at, p1[0], p1[1], p1[2], p1[3]);
+          }
+        }
+        // (the last UMMA's second half where the terms end in its first)
+        if (kParts * ranks % 16) tmem_st4(col + kParts * ranks / 2, 0u, 0u, 0u, 0u);
         tmem_st_wait();
       } else if (!*abort_flag && MX) {
         const uint32_t rec = smem_u32(smem + s * Cfg::kStageBytes + Cfg::kXBytes) + (quarter >> 1) * kMxRecord;

@@ -114,3 +114,57 @@ def test_nonfinite_tokens_in_adapter_gradients(qb, cuda):
             others = torch.arange(128, device=cuda) != 5
             assert torch.equal(got["b"][others], want["b"][others])
             assert not bool(got["b"][5].isfinite().any())
+
+
+# ------------------------------------------------------------ range of fp16 factors
+def scaled(t, factor):
+    return (t.float() * factor).to(t.dtype)
+
+
+@pytest.mark.parametrize("M", [1, 24, 32, 33, 64, 65, 130, 300])
+def test_fp16_range_of_an_adapter_does_not_depend_on_the_tokens(qb, cuda, M):
+    """Large B, large and small down projections: y and dx are finite and right with
+    any number of tokens."""
+    d = ref.draw("f16", M, 512, 320, rank=12, seed=M, device=cuda)
+    gy = ref.draw("f16", M, 320, 4, seed=5, device=cuda)["x"]
+    a, b, x = d["a"], d["b"], d["x"]
+    for q in (qb.quantize_quaternion_weights(*d["w"]), zero_base(qb, 512, 320, cuda)):
+        v = values_of(q)
+        for fa, fb, fx, scale in ((1e-2, 40000.0, 1e-2, 2.0),    # |B| up to 8000, t about 2e-4
+                                  (200.0, 2e-3, 1.0, 1000.0),    # t about 2e5, B about 1e-4
+                                  (1.0, 400.0, 1e-3, 1e-3)):     # t about 1e-6, B about 20
+            d.update(a=scaled(a, fa), b=scaled(b, fb), x=scaled(x, fx), scale=scale)
+            y = qb.mx_quaternion_linear(d["x"], q, None, d["a"], d["b"], scale)
+            want = ref.layer(ref.f64(d["x"]), v, None, ref.f64(d["a"]), ref.f64(d["b"]), scale)
+            one_rounding(y, want, "f16", 512, (fa, fb))
+        for fa, fb, fg, scale in ((40000.0, 1e-2, 1e-2, 2.0), (2e-3, 200.0, 1.0, 1000.0), (400.0, 1.0, 1e-3, 1e-3)):
+            d.update(a=scaled(a, fa), b=scaled(b, fb), x=scaled(x, 1e-3), scale=scale)
+            g = scaled(gy, fg)
+            got, want = backward(qb, q, d, g), expected(q, d, g)
+            for k in ("x", "a", "b"):
+                if np.isfinite(rounded(want[k], "f16")).all():
+                    one_rounding(got[k], want[k], "f16", 512 + M, (k, fa, fb))
+
+
+# --------------------------------------------------- adapters that decide the result
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M,fin,fout,rank", [(70, 256, 256, 32), (130, 512, 260, 64), (300, 260, 512, 40),
+                                             (257, 128, 132, 100), (100, 256, 192, 300), (500, 64, 64, 7)])
+def test_one_rounding_where_the_adapter_decides(qb, cuda, dtype, M, fin, fout, rank):
+    """A base of zeros: the bound rejects a down projection, or B, rounded to one 16-bit part."""
+    d = ref.draw(dtype, M, fin, fout, rank=rank, seed=rank, device=cuda)
+    q = zero_base(qb, fin, fout, cuda)
+    gy = ref.draw(dtype, M, fout, 4, seed=5, device=cuda)["x"]
+    x, a, b, g = (ref.f64(t) for t in (d["x"], d["a"], d["b"], gy))
+    t, u = d["scale"] * x @ a.T, d["scale"] * g @ b
+    got = backward(qb, q, d, gy)
+    got["y"] = qb.mx_quaternion_linear(d["x"], q, None, d["a"], d["b"], d["scale"])
+    want = {"y": t @ b.T, "x": u @ a, "a": u.T @ x, "b": g.T @ t}
+    th, uh = rounded(t, dtype), rounded(u, dtype)
+    one_part = {"y": th @ b.T, "x": uh @ a, "a": uh.T @ x, "b": g.T @ th}
+    if dtype == "f16":  # what bf16 parts of the factors would lose
+        one_part.update(y=t @ rounded(b, "bf16").T, x=u @ rounded(a, "bf16"))
+    terms = {"y": fin + rank, "x": fout + rank, "a": M + fout, "b": M + fin}
+    for k, w in want.items():
+        one_rounding(got[k], w, dtype, terms[k], k)
+        assert np.linalg.norm(rounded(one_part[k], dtype) - w) > bound(w, dtype, terms[k]), k
