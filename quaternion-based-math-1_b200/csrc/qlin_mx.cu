@@ -191,8 +191,9 @@ BackwardWs backward_ws(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank)
       w.bt = c.take(round_up(N, 8) * rank * 2);
       w.a = c.take(rank * round_up(K, 8) * 2);
       w.parts = c.take(M * pair_parts(dtype) * w.ld_parts * 2);
-      w.up = c.take(2 * w.rows * w.M_pad * 2);
-      w.t = c.take(2 * w.rows * w.M_pad * 2);
+      const int64_t parts = dtype == QLIN_F16 ? kMxTurnedParts<__half> : kMxTurnedParts<__nv_bfloat16>;
+      w.up = c.take(parts * w.rows * w.M_pad * 2);
+      w.t = c.take(parts * w.rows * w.M_pad * 2);
       if (dtype == QLIN_F16) {
         w.up_tops = c.take(w.M_pad / kMxDownRows * w.rows);
         w.t_tops = c.take(w.M_pad / kMxDownRows * w.rows);
@@ -645,9 +646,11 @@ int run_backward(const T* g, int64_t ld_g, const T* x, int64_t ld_x, const void*
     if (da) job(o0, up, w.up_tops, x, ld_x, K, w.rows, w.splits0, w.partial0);
     if (db) job(o1, t, w.t_tops, g, ld_g, N, w.rows, w.splits1, w.partial1);
     static std::atomic<uint64_t> done{0};
-    if (allow_smem(qlin_mx_outer_kernel<T>, done, kMxOuterSmem) != QLIN_OK) return QLIN_ERR_LAUNCH;
+    if (allow_smem(qlin_mx_outer_kernel<T>, done, kMxOuterStages * mx_outer_stage<T>(kMxOuterRows)) != QLIN_OK)
+      return QLIN_ERR_LAUNCH;
     if (sum_with_db) o1.sums = reinterpret_cast<float*>(ws + w.sums);
-    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 128, kMxOuterSmem, s, o0, o1,
+    st = launch_dependent(qlin_mx_outer_kernel<T>, (unsigned)(o0.blocks + o1.blocks), 128,
+                          kMxOuterStages * mx_outer_stage<T>(w.rows), s, o0, o1,
                           (int)M, (int)w.M_pad, (int)(dx != nullptr));
     if (st != QLIN_OK) return st;
     const int64_t blocks0 = da ? ceil_div(rank * K, 256) : 0;

@@ -6,8 +6,8 @@
 //
 // t and u are kept as parts (or in fp32): rounded to one they would add an error of the
 // size of the results' own rounding.  The CTA-pair kernel takes them as three bf16 parts
-// (exact), dA and dB as two 16-bit ones, with a power of two per rank and 16 tokens for
-// f16 (mx_top_scale).  x and gy are read
+// (exact), dA and dB as three bf16 ones or two f16 ones with a power of two per rank and
+// 16 tokens (mx_top_scale).  x and gy are read
 // once for t and u and once for the gradients, which bounds these kernels; the
 // products are warp-level tensor-core ones (m16n8k16) whose k slots are numbered
 // so that a lane reads eight consecutive elements of a row in one 16-byte piece
@@ -162,6 +162,12 @@ qlin_mx_repack_kernel(const T* src, int64_t ld_s, T* dst, int64_t ld_d, int64_t 
 constexpr int kMxDownRows = 16;   // tokens of a CTA
 constexpr int kMxDownRanks = 32;  // ranks of a CTA
 
+// Parts of t and u for dA and dB: bf16's three are exact, f16's two hold 22 bits.  (Two
+// bf16 parts, 17 bits: results off by 6e-5 of their norm more than fp32 sums leave, the
+// 4096 layer's training step at 2048 tokens 153 us in place of 155.)
+template <typename T>
+constexpr int kMxTurnedParts = std::is_same<T, __half>::value ? 2 : 3;
+
 template <typename T>
 struct MxDownJob {
   const T* x;      // [M, ld_x]
@@ -171,7 +177,7 @@ struct MxDownJob {
   int K;           // a multiple of 8: zero past the product's terms
   float scale;
   __nv_bfloat16* parts;  // [M, kMxPairParts<T> * ld_parts], the CTA-pair kernel's terms: zero past rank; or null
-  T* turned;       // [2][rows][M_pad]: hi, then lo, transposed; or null
+  T* turned;       // [kMxTurnedParts<T>][rows][M_pad]: parts, the largest first, transposed; or null
   uint8_t* tops;   // f16: [M_pad / 16][rows]: exponent fields of the groups of 16 tokens (see mx_top_scale)
   int rank, ld_parts, rows;
   int rank_tiles;  // ceil(max(ld_parts, rows) / 32)
@@ -295,19 +301,21 @@ qlin_mx_down_kernel(const __grid_constant__ MxDownJob<T> job0, const __grid_cons
           }
         }
       } else if (r0 + r < job.rows) {
-        const T hi = from_f32<T>(v);
-        const float rest = v - to_f32(hi);
-        const T lo = from_f32<T>(isfinite(rest) ? rest : 0.f);  // (hi infinite or NaN: alone)
         T* at = job.turned + (int64_t)(r0 + r) * M_pad + m0 + m;
-        at[0] = hi;
-        at[(int64_t)job.rows * M_pad] = lo;
+#pragma unroll
+        for (int part = 0; part < kMxTurnedParts<T>; ++part, at += (int64_t)job.rows * M_pad) {
+          const T p = from_f32<T>(v);
+          *at = p;
+          v -= to_f32(p);
+          if (!isfinite(v)) v = 0.f;  // (an infinite or NaN part stands alone)
+        }
       }
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// 16-bit gradients: out = (hi + lo) X, sums over the tokens
+// 16-bit gradients: out = (sum of the parts) X, sums over the tokens
 // ---------------------------------------------------------------------------
 constexpr int kMxOuterCols = 128;   // columns of X of a CTA, 32 per warp
 constexpr int kMxOuterTokens = 32;  // tokens of a step
@@ -315,12 +323,16 @@ constexpr int kMxOuterRows = 64;    // rows of the result of a CTA (groups of 16
 constexpr int kMxOuterStages = 4;
 constexpr int kMxOuterXBytes = kMxOuterTokens * kMxOuterCols * 2;
 constexpr int kMxOuterTops = 2 * kMxOuterRows;  // bytes: f16's exponents of a step's two groups of 16 tokens
-constexpr int kMxOuterStage = kMxOuterXBytes + 2 * kMxOuterRows * kMxOuterTokens * 2 + kMxOuterTops;
-constexpr int kMxOuterSmem = kMxOuterStages * kMxOuterStage;
+
+// Bytes of a stage: X, the exponents, the parts of up to kMxOuterRows rows.
+template <typename T>
+__host__ __device__ constexpr int mx_outer_stage(int rows) {
+  return kMxOuterXBytes + kMxOuterTops + kMxTurnedParts<T> * (rows < kMxOuterRows ? rows : kMxOuterRows) * kMxOuterTokens * 2;
+}
 
 template <typename T>
 struct MxOuterJob {
-  const T* turned;  // [2][rows][M_pad]; fp32: [M][rows]
+  const T* turned;  // [kMxTurnedParts<T>][rows][M_pad]; fp32: [M][rows]
   const uint8_t* tops;  // f16: of the parts, see MxDownJob
   const T* X;       // [M, ld], 16-byte aligned rows
   int64_t ld;
@@ -338,7 +350,7 @@ __device__ __forceinline__ uint32_t mx_top_factor(int top, int row_top) {
   return (e > 0 ? (uint32_t)e << 10 : (e > -10 ? 1u << (9 + e) : 0u)) * 0x00010001u;
 }
 
-// Four warps: 32 columns each, all rows.  X and the rows of (hi, lo) come through
+// Four warps: 32 columns each, all rows.  X and the rows of all parts come through
 // a ring of shared memory steps (32 tokens x 128 columns; 16-byte chunks permuted
 // within a row of X so that the transposing loads of eight tokens two apart are
 // free of conflicts).
@@ -356,6 +368,7 @@ __global__ void __launch_bounds__(128)
 qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_constant__ MxOuterJob<T> job1, int M,
                      int M_pad, int beside) {
   constexpr bool HALF = std::is_same<T, __half>::value;
+  constexpr int kParts = kMxTurnedParts<T>;
   extern __shared__ __align__(128) uint8_t mx_smem[];
   if (!beside) pdl_wait_prior();
   pdl_launch_dependents();
@@ -371,7 +384,7 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   const int c0 = ct * kMxOuterCols, row0 = rt * kMxOuterRows;
   const int rows = min(kMxOuterRows, job.rows - row0), groups = rows / 16;
   // what this thread fetches of a step: a chunk of X of four tokens, and a chunk of
-  // up to two rows of both parts
+  // up to two rows of every part
   const int tok = threadIdx.x >> 4, chunk = threadIdx.x & 15;  // tokens tok + 8 u
   const int left = min(8, job.cols - (c0 + 8 * chunk));        // elements of the chunk inside
   const int bytes = left > 0 ? 2 * left : 0;
@@ -382,10 +395,11 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   for (int u = 0; u < 4; ++u) x_at[u] = (tok + 8 * u) * 256 + ((chunk ^ ((tok & 1) | u << 1)) << 4);
   const int ar = threadIdx.x >> 2;  // rows ar and ar + 32
   const T* ap = job.turned + (int64_t)(row0 + min(ar, rows - 1)) * M_pad + s0 * kMxOuterTokens + 8 * (threadIdx.x & 3);
-  const int64_t lo_off = (int64_t)job.rows * M_pad, row32 = 32 * (int64_t)M_pad;
-  const uint32_t a_at = kMxOuterXBytes + ar * 64 + ((threadIdx.x & 3) << 4);
+  const int64_t part_off = (int64_t)job.rows * M_pad, row32 = 32 * (int64_t)M_pad;
+  const int stage = mx_outer_stage<T>(job.rows), part_bytes = min(kMxOuterRows, job.rows) * kMxOuterTokens * 2;
+  constexpr uint32_t kTopsAt = kMxOuterXBytes, kPartsAt = kTopsAt + kMxOuterTops;
+  const uint32_t a_at = kPartsAt + ar * 64 + ((threadIdx.x & 3) << 4);
   // f16: 16 exponents of a group, by the first threads
-  constexpr uint32_t kTopsAt = kMxOuterStage - kMxOuterTops;
   const bool tops = HALF && (int)threadIdx.x < 2 * groups;
   const int tgroup = (int)threadIdx.x >= groups, tpiece = (int)threadIdx.x - (tgroup ? groups : 0);
   const uint8_t* tp = job.tops + (int64_t)(2 * s0 + tgroup) * job.rows + row0 + 16 * tpiece;
@@ -394,20 +408,17 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
   MxRing in, out;
   auto fetch = [&]() {
     if (m_next < m_end) {
-      const uint32_t base = smem_u32(mx_smem) + in.at * kMxOuterStage;
+      const uint32_t base = smem_u32(mx_smem) + in.at * stage;
       const T* x = xp;
 #pragma unroll
       for (int u = 0; u < 4; ++u, x += x_eight) {
         const bool here = m_next + 8 * u < M;
         cp_async16(base + x_at[u], here ? x : job.X, here ? bytes : 0);
       }
-      if (ar < rows) {
-        cp_async16(base + a_at, ap, 16);
-        cp_async16(base + a_at + kMxOuterRows * 64, ap + lo_off, 16);
-      }
-      if (ar + 32 < rows) {
-        cp_async16(base + a_at + 32 * 64, ap + row32, 16);
-        cp_async16(base + a_at + (kMxOuterRows + 32) * 64, ap + row32 + lo_off, 16);
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+        if (ar < rows) cp_async16(base + a_at + part * part_bytes, ap + part * part_off, 16);
+        if (ar + 32 < rows) cp_async16(base + a_at + part * part_bytes + 32 * 64, ap + part * part_off + row32, 16);
       }
       if (tops) cp_async16(base + kTopsAt + tgroup * kMxOuterRows + 16 * tpiece, tp, 16);
       xp += 4 * x_eight;
@@ -444,7 +455,7 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
     asm volatile("cp.async.wait_group %0;" ::"n"(kMxOuterStages - 2) : "memory");
     __syncthreads();
     fetch();  // into the stage of the step before: every warp is past it
-    const uint32_t base = smem_u32(mx_smem) + out.at * kMxOuterStage;
+    const uint32_t base = smem_u32(mx_smem) + out.at * stage;
     out.next(kMxOuterStages);
     uint32_t b[4][4];
 #pragma unroll
@@ -473,8 +484,8 @@ qlin_mx_outer_kernel(const __grid_constant__ MxOuterJob<T> job0, const __grid_co
           fh = mx_top_factor(at[8], row_top[16 * r + g + 8]);
         }
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          const uint32_t at = base + kMxOuterXBytes + (part * kMxOuterRows + 16 * r + g) * 64 + t * 16;
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t at = base + kPartsAt + part * part_bytes + (16 * r + g) * 64 + t * 16;
           uint4 l = lds128(at), h = lds128(at + 8 * 64);
           if constexpr (HALF) {
             l.x = mx_mul2<true>(l.x, fl); l.y = mx_mul2<true>(l.y, fl);

@@ -168,3 +168,26 @@ def test_one_rounding_where_the_adapter_decides(qb, cuda, dtype, M, fin, fout, r
     for k, w in want.items():
         one_rounding(got[k], w, dtype, terms[k], k)
         assert np.linalg.norm(rounded(one_part[k], dtype) - w) > bound(w, dtype, terms[k]), k
+
+
+@pytest.mark.parametrize("dtype,tie,above", [("bf16", 2.0 ** -8, 2.0 ** -20), ("f16", 2.0 ** -11, 2.0 ** -22)])
+def test_every_bit_of_a_down_projection_counts(qb, cuda, dtype, tie, above):
+    """t = u = 1 + tie + above, just past the middle between two numbers of the type, by
+    sums and products that are exact: every result is the upper one."""
+    M, F, rank = 70, 64, 8
+    T = ref.TORCH[dtype]
+    rows = torch.zeros(M, F, device=cuda)
+    rows[:, 0:8], rows[:, 8:16], rows[:, 16:24] = 1.0, tie, above
+    ones = (torch.arange(F, device=cuda)[:, None] % rank == torch.arange(rank, device=cuda)).float()  # [F, rank]
+    pick = torch.eye(F, device=cuda).new_zeros(M, F)
+    pick[:F] = torch.eye(F, device=cuda)  # each column from one token
+    q = zero_base(qb, F, F, cuda)
+    upper = 1 + 2 * tie
+    d = dict(x=rows.to(T), a=ones.t().contiguous().to(T), b=ones.to(T), scale=1.0)
+    y = qb.mx_quaternion_linear(d["x"], q, None, d["a"], d["b"], 1.0)
+    assert bool((y == upper).all())
+    assert bool((backward(qb, q, d, pick.to(T))["b"] == upper).all())
+    d["x"] = pick.to(T)
+    got = backward(qb, q, d, rows.to(T))
+    assert bool((got["x"] == upper).all())
+    assert bool((got["a"] == upper).all())
