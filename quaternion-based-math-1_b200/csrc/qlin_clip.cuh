@@ -20,7 +20,8 @@
 //
 // Squares are summed in fp32 within a piece and thread (8 terms) and in fp64 from
 // there on, in an order that depends only on the sizes: the same gradients give
-// the same bits.  A thread whose fp32 sum overflows sums its piece again in fp64.
+// the same bits.  A thread whose fp32 sum overflows, or is so small that squares may
+// have been lost below fp32's numbers (2^-90, or zero), sums its piece again in fp64.
 #pragma once
 
 #include "qlin_common.cuh"
@@ -63,7 +64,7 @@ struct ClipLoad {
         const float v = to_f32(reinterpret_cast<const T*>(&q[u])[j]);
         s = fmaf(v, v, s);
       }
-    if (s <= 3.0e38f) return (double)s;
+    if (s >= 0x1p-90f && s <= 3.0e38f) return (double)s;
     double d = 0.0;
 #pragma unroll
     for (int u = 0; u < kClipEach / V; ++u)
