@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -264,9 +265,15 @@ class MxLinear : public torch::autograd::Function<MxLinear> {
   }
 };
 
-// mx_forward, differentiable in x, bias, A and B.
+// mx_forward, differentiable in x, bias, A and B (backwards; a tangent is refused, the
+// kernels would drop it).
 at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& mx, int64_t out_groups, int64_t in_groups,
                      const OptTensor& bias, const OptTensor& a, const OptTensor& b, double scale) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    auto dual = [](const OptTensor& t) { return t.has_value() && t->defined() && t->_fw_grad(0).defined(); };
+    TORCH_CHECK(!x._fw_grad(0).defined() && !dual(bias) && !dual(a) && !dual(b),
+                "mx_quaternion_linear has no forward-mode derivatives");
+  }
   if (at::GradMode::is_enabled()) {
     auto wants = [](const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); };
     if (x.requires_grad() || wants(bias) || wants(a) || wants(b))

@@ -75,7 +75,8 @@ def mx_quaternion_linear(x, weights: MXQuaternionWeights, bias=None, lora_a=None
 
     ``x``: ``[..., in_features]``; bias ``[out_features]``; LoRA A
     ``[r, in_features]`` and B ``[out_features, r]``, all of x's dtype.
-    Differentiable once in x, bias, A and B.
+    Differentiable once in x, bias, A and B, in reverse mode only (a forward-mode
+    tangent raises ``RuntimeError``).
     """
     return _ext().mx_linear(x, weights.data, weights.out_groups, weights.in_groups, bias, lora_a, lora_b,
                             float(lora_scale))
