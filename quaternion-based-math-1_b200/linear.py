@@ -27,6 +27,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as fwd
 import torch.nn as nn
 
 from . import _lib
@@ -227,7 +228,13 @@ def fused_quaternion_linear(x, wr, wi, wj, wk, bias=None, lora_a=None, lora_b=No
     ``packed``: the same weights as one ``[out_groups, in_groups, 4]`` tensor
     (:func:`pack_quaternion_weights`), read by the kernels that take it (the
     decode GEMV and the CTA-pair prefill kernel); ignored under autograd.
+    Derivatives are reverse mode only: a forward-mode tangent raises
+    ``RuntimeError`` (the kernels would drop it).
     """
+    if fwd._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in (x, wr, wi, wj, wk, bias, lora_a, lora_b):
+            if t is not None and fwd.unpack_dual(t).tangent is not None:
+                raise RuntimeError("quaternion_linear has no forward-mode derivatives")
     if torch.is_grad_enabled():
         for t in (x, wr, wi, wj, wk, bias, lora_a, lora_b):
             if t is not None and t.requires_grad:
