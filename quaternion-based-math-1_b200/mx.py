@@ -122,18 +122,37 @@ class MXQuaternionLinear(nn.Module):
                 f"bias={self.bias is not None}, weights=mxfp4")
 
 
+# what a replaced layer hands on besides its parameters: the hooks around its forward and backward
+_HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks",
+          "_forward_pre_hooks_with_kwargs", "_backward_hooks", "_backward_pre_hooks", "_is_full_backward_hook")
+
+
 def quantize_model(model: nn.Module):
     """Replace every ``QuaternionLinear`` of ``model`` (LoRA bases too) by an
     ``MXQuaternionLinear`` in place; return the replaced names.  A layer that
-    appears under several names stays shared."""
+    appears under several names stays shared; forward and backward hooks of a
+    layer go over to its replacement (hooks on its state dict do not).
+
+    Left as they are: subclasses with a ``forward`` of their own, and layers
+    that hold their weights in another form (``FactorizedQuaternionLinear``,
+    ``UnitQuaternionLinear``, ``ColumnParallelQuaternionLinear``).  A ``model``
+    that is itself a ``QuaternionLinear`` cannot be replaced in place:
+    ``ValueError`` (:meth:`MXQuaternionLinear.from_linear` makes its
+    replacement).
+    """
+    if isinstance(model, QuaternionLinear):
+        raise ValueError("the model is a QuaternionLinear itself and cannot be replaced in place; "
+                         "use MXQuaternionLinear.from_linear")
     made: dict[QuaternionLinear, MXQuaternionLinear] = {}
     replaced = []
     for name, mod in list(model.named_modules(remove_duplicate=False)):
-        if not isinstance(mod, QuaternionLinear) or not name:
+        if not isinstance(mod, QuaternionLinear) or type(mod).forward is not QuaternionLinear.forward:
             continue
         if mod not in made:
             made[mod] = MXQuaternionLinear.from_linear(mod)
             made[mod].train(mod.training)
+            for hooks in _HOOKS:
+                setattr(made[mod], hooks, getattr(mod, hooks))
             if mod.bias is not None:
                 made[mod].bias.requires_grad_(mod.bias.requires_grad)
         parent_name, _, leaf = name.rpartition(".")

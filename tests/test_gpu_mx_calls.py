@@ -38,3 +38,42 @@ def test_function_transforms_are_refused(qb, cuda):
         torch.func.vmap(f)(x)
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda v: f(v).sum())(x)
+
+
+# ------------------------------------------------------------- model conversion
+def test_quantize_model_takes_hooks_along(qb, cuda):
+    net = torch.nn.Sequential(qb.QuaternionLinear(64, 32, bias=True), torch.nn.ReLU()).to(cuda)
+    seen = []
+    handles = [net[0].register_forward_hook(lambda m, a, out: out + 1.0),
+               net[0].register_forward_pre_hook(lambda m, a: seen.append(type(m).__name__)),
+               net[0].register_full_backward_hook(lambda m, gi, go: seen.append("backward"))]
+    qb.quantize_model(net)
+    x = torch.randn(3, 64, device=cuda, requires_grad=True)
+    want = qb.mx_quaternion_linear(x, net[0].weights, net[0].bias) + 1.0
+    got = net[0](x)
+    assert torch.equal(got, want) and seen == ["MXQuaternionLinear"]
+    got.sum().backward()
+    assert seen[1:] == ["backward"]
+    for h in handles:
+        h.remove()
+    assert torch.equal(net[0](x), qb.mx_quaternion_linear(x, net[0].weights, net[0].bias))
+    assert len(seen) == 2
+
+
+def test_quantize_model_says_what_it_leaves(qb, cuda):
+    class Doubled(qb.QuaternionLinear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Named(qb.QuaternionLinear):
+        pass
+
+    net = torch.nn.ModuleDict({"own": Doubled(32, 32), "named": Named(32, 32), "plain": qb.QuaternionLinear(32, 32),
+                               "unit": qb.UnitQuaternionLinear(32, 32)}).to(cuda)
+    before = {k: net[k] for k in ("own", "unit")}
+    assert sorted(qb.quantize_model(net)) == ["named", "plain"]
+    assert all(net[k] is m for k, m in before.items())
+    alone = qb.QuaternionLinear(32, 32).to(cuda)
+    with pytest.raises(ValueError):
+        qb.quantize_model(alone)
+    assert isinstance(alone.wr, torch.nn.Parameter)
