@@ -5,8 +5,10 @@
 // on the current stream of the tensors' device.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -313,6 +315,10 @@ at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm,
     TORCH_CHECK(g.layout() == at::kStrided, "sparse gradients are not supported");
     check_cuda(g, grads[0], false);
     types.push_back(dtype_code(g.scalar_type()));
+    // nothing is written before every gradient is known to be writable
+    at::assert_no_internal_overlap(g);
+    TORCH_CHECK(!g.is_inference() || c10::InferenceMode::is_enabled(),
+                "a gradient made in inference mode cannot be clipped outside it");
   }
   c10::cuda::CUDAGuard guard(grads[0].device());
   at::NoGradGuard no_grad;
