@@ -453,6 +453,7 @@ int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g,
  * with the weights that mx stands for.  x, bias, LoRA A/B and y share dtype;
  * accumulation is fp32, outputs are rounded once.  Arguments as qlin_forward;
  * workspace of at least qlin_mx_workspace_size() bytes, 256-byte aligned.
+ * At most 2^31 - 1024 tokens and rank 2^24 (QLIN_ERR_SHAPE).
  * 16-bit types with more than 32 tokens want y 8-byte aligned and ld_y a multiple
  * of 4 (QLIN_ERR_ALIGN).  The down projection is kept in fp32's range and precision
  * for every type.  Waits inside the kernels are bounded (qlin_get_device_error).

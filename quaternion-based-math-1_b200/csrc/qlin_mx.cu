@@ -39,9 +39,13 @@ int64_t mx_bytes(int64_t K_g, int64_t N_g) {
   return kMxHeader + ceil_div(N_g, kMxRows) * ceil_div(K_g, kMxBlock) * kMxRecord;
 }
 
+// Tokens and ranks whose padded counts and tiles stay within 32 bits.
+constexpr int64_t kMostTokens = INT32_MAX - 1023;
+constexpr int kMostRanks = 1 << 24;
+
 int check_layer(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank) {
   if (!known(dtype)) return QLIN_ERR_DTYPE;
-  if (M < 0 || M > INT32_MAX || rank < 0) return QLIN_ERR_SHAPE;
+  if (M < 0 || M > kMostTokens || rank < 0 || rank > kMostRanks) return QLIN_ERR_SHAPE;
   return check_groups(K_g, N_g);
 }
 

@@ -96,6 +96,7 @@ Adapter adapter_of(const OptTensor& a, const OptTensor& b, int64_t K, int64_t N,
     shape_error("LoRA shapes must be A [r, " + std::to_string(K) + "] and B [" + std::to_string(N) + ", r]");
   check_cuda(*a, like, true);
   check_cuda(*b, like, true);
+  if (a->size(0) > std::numeric_limits<int>::max()) shape_error("LoRA rank out of range");
   out.rank = static_cast<int>(a->size(0));
   if (out.rank > 0) {
     out.a = a->contiguous();
