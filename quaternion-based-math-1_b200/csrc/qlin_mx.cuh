@@ -13,9 +13,10 @@
 // E = 0); a block that holds an infinity or a NaN gets zero codes and stands
 // for NaNs.
 //
-// Buffer: a header of kMxHeader bytes (word 0: the largest F of the layer's
-// finite blocks), then one record per 16 output quaternions (tile) and 32 input
-// quaternions (block), tile-major, blocks of one tile contiguous:
+// Buffer: a header of kMxHeader bytes (word 0: the largest F of the layer's finite
+// blocks; word 1: 255 less the smallest F of those that are not zero), then one record
+// per 16 output quaternions (tile) and 32 input quaternions (block), tile-major, blocks
+// of one tile contiguous:
 //
 //     record (1088 bytes) = codes [16 rows][4 octets t][4 components p] words,
 //                           then F [16 rows][4 components p] bytes
@@ -166,7 +167,7 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
   const int t = lane & 3, second = (lane >> 2) & 1, p = lane >> 3;
   const int kb = (K_g + kMxBlock - 1) / kMxBlock, row_units = (N_g + kMxRows - 1) / kMxRows * (kMxRows / kMxUnitRows);
   const int b = 2 * ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) + second;  // this lane's block
-  uint32_t top = 0;
+  uint32_t top = 0, low = 0;
   const int i = b * kMxBlock + 8 * t, left = K_g - i;
   const T* plane = src.w[p] + i;
   MxRaw8<T> raw[kMxUnitRows], next[kMxUnitRows];
@@ -201,6 +202,7 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[j] = bad ? 0.f : v[j] * inv;
       if (!bad) top = max(top, e + 1u);
+      if (!bad && m > 0u) low = max(low, 254u - e);
       if (b < kb) {
         *reinterpret_cast<uint32_t*>(out + row * 64 + t * 16 + p * 4) = mx_pack(q);
         if (t == 0) out[kMxCodeBytes + row * 4 + p] = (uint8_t)(bad ? 255u : e + 1u);
@@ -208,14 +210,23 @@ qlin_mx_quantize_kernel(const MxPlanes<const T> src, int64_t ld, int K_g, int N_
       raw[u] = next[u];
     }
   }
-  __shared__ uint32_t tops[8];
+  __shared__ uint32_t tops[8], lows[8];
   top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) tops[threadIdx.x >> 5] = top;
+  low = __reduce_max_sync(0xffffffffu, low);
+  if (lane == 0) {
+    tops[threadIdx.x >> 5] = top;
+    lows[threadIdx.x >> 5] = low;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int w = 1; w < 8; ++w) top = max(top, tops[w]);
-    atomicMax(reinterpret_cast<unsigned*>(mx), top);  // a maximum: the same in any order
+    for (int w = 1; w < 8; ++w) {
+      top = max(top, tops[w]);
+      low = max(low, lows[w]);
+    }
+    // maxima: the same in any order
+    atomicMax(reinterpret_cast<unsigned*>(mx), top);
+    atomicMax(reinterpret_cast<unsigned*>(mx) + 1, low);
   }
 }
 

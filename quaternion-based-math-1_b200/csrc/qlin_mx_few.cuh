@@ -27,11 +27,8 @@
 //     that neither overflows nor underflows (a scaling up is exact); the
 //     product of a block and component starts from zero and joins the fp32 sum
 //     with its scale in one multiply-add per value.
-//   more: a packed multiplication by 2^(126 or 14) * scale * 2^-c makes the
-//     weights, exactly: c = max(0, F0 - 129) for bf16, with F0 the layer's
-//     largest F (c = 0 unless weights reach 16), F0 - 129 for f16, which keeps
-//     scales down to 2^-38 of the largest exact.  The sums are multiplied by
-//     2^c at the end.
+//   more: a packed multiplication by 2^(126 or 14) * scale * 2^-c makes the weights (see
+//     MxScaling), and the sums are multiplied by 2^c at the end.
 //
 // fp32 inputs are split into three bf16 parts of 8 bits each (x = x1 + x2 + x3
 // exactly, down to bf16's smallest number); their products go to the same
@@ -78,25 +75,47 @@ constexpr int kMxPairParts = MxOperand<T>::kHalf ? 5 : 3;
 template <typename T>
 constexpr int kMxPairRanks = 128 / kMxPairParts<T> / 8 * 8;
 
-// c of the layer whose largest F is f0.  An adapter's products join the accumulator
-// with B 2^-c: a bound for fp16 keeps them in fp32's range (weights so small, 2^-40 of
-// fp16's steps, are lost in the rounding of y anyway).
+// How a layer's weights become 16-bit operands, times 2^-c.
+//   bf16: c = max(0, F0 - 129), with F0 the layer's largest F (c = 0 unless weights reach
+//     16); exact.
+//   f16: c = F0 - 129, which makes the largest weights 12; exact where no block's scale
+//     is below 2^-24 of the largest.  In other layers (`far`) c = F0 - 141, the largest
+//     become 49152, by a second multiplication (f16 has no power above 2^15), and scales
+//     down to 2^-36 of the largest are exact: all those of fp16 weights below 8192;
+//     smaller ones are rounded at 2^-37 of the largest scale.  (Without the distinction, in
+//     the CTA-pair kernel: 4096 -> 11008 at 2048 tokens 118 -> 123 us.)
+// An adapter's products join the accumulator with B 2^-c: a bound on fp16's c keeps them
+// in fp32's range (weights so small, 2^-40 of fp16's steps, are lost in the rounding of y
+// anyway).
 template <bool HALF>
-__device__ __forceinline__ int mx_shift(uint32_t f0, int rank = 0) {
-  const int c = (int)f0 - 129;
-  return HALF ? (rank > 0 ? max(c, -40) : c) : max(0, c);
-}
+struct MxScaling {
+  int c;
+  int off;   // the multiplier of F has the exponent field F - off
+  bool far;  // (f16)
+  __device__ __forceinline__ MxScaling(const uint8_t* mx, int rank) {
+    uint32_t f0, low;
+    asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(f0), "=r"(low) : "l"(mx) : "memory");
+    if constexpr (HALF) {
+      far = (int)f0 - (255 - (int)low) > 24;
+      c = max((int)f0 - (far ? 141 : 129), rank > 0 ? -40 : -140);
+      off = c + (far ? 111 : 99);  // F - 128 - c + 14 + 15, less the 12 of kMxHalfStep
+    } else {
+      far = false;
+      c = max(0, (int)f0 - 129);
+      off = c - 125;  // F - 128 - c + 126 + 127
+    }
+  }
+};
 
-// The packed multiplier of codes with scale F.  bf16: exponent field
-// F - 128 - c + 126 + 127; a NaN block's F saturates at infinity, which makes
-// NaNs of its zero codes.
+// The packed multiplier of codes with scale F; a NaN block's F saturates at infinity,
+// which makes NaNs of its zero codes.
 template <bool HALF>
-__device__ __forceinline__ uint32_t mx_multiplier(uint32_t f, int c) {
+__device__ __forceinline__ uint32_t mx_multiplier(uint32_t f, int off) {
   if constexpr (HALF) {
-    const int e = min((int)f - 99 - c, 31);  // F - 128 - c + 14 + 15
+    const int e = min((int)f - off, 31);
     return (e > 0 ? (uint32_t)e << 10 : (e >= -9 ? 1u << (e + 9) : 0u)) * 0x00010001u;
   } else {
-    return (uint32_t)min((int)f + 125 - c, 255) * 0x00800080u;
+    return (uint32_t)min((int)f - off, 255) * 0x00800080u;
   }
 }
 
@@ -108,11 +127,18 @@ __device__ __forceinline__ uint32_t mx_mul2(uint32_t a, uint32_t b) {
   return r;
 }
 
-template <bool HALF>
-__device__ __forceinline__ void mx_expand_scaled(const MxPowers& c, uint32_t w, uint32_t mult, uint32_t (&r)[4]) {
+constexpr uint32_t kMxHalfStep = (15u + 12u) * 0x04000400u;  // 2^12, packed f16
+
+// FAR: f16's two multiplications.
+template <bool HALF, bool FAR>
+__device__ __forceinline__ void mx_expand_scaled(const MxPowers& c, uint32_t w, uint32_t mult, uint32_t (&r)[4],
+                                                 uint32_t step = kMxHalfStep) {
   mx_expand<HALF>(c, w, r);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) r[k] = mx_mul2<HALF>(r[k], mult);
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (FAR) r[k] = mx_mul2<true>(r[k], step);
+    r[k] = mx_mul2<HALF>(r[k], mult);
+  }
 }
 
 // d += A B
@@ -162,16 +188,18 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
 
 // A lane's share of a record: the A operands (weights) of the block's two k16
 // steps for all four components.
+// (f16: a first multiplication by `step`, 2^12 or 1; 16 tokens, 4096 -> 4096 with rank
+// 32: 13.0 us without it, 13.2 with it, 13.5 with a branch on `far`)
 template <bool HALF>
-__device__ __forceinline__ void mx_load_a(const MxPowers& pw, uint32_t rec, int g, int t, int c, uint32_t (&lo)[4][4],
-                                          uint32_t (&hi)[4][4]) {
+__device__ __forceinline__ void mx_load_a(const MxPowers& pw, uint32_t rec, int g, int t, int off, uint32_t step,
+                                          uint32_t (&lo)[4][4], uint32_t (&hi)[4][4]) {
   const uint4 wl = lds128(rec + g * 64 + t * 16), wh = lds128(rec + (g + 8) * 64 + t * 16);
   const uint32_t sl = lds32(rec + kMxCodeBytes + g * 4), sh = lds32(rec + kMxCodeBytes + (g + 8) * 4);
   const uint32_t l[4] = {wl.x, wl.y, wl.z, wl.w}, h[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    mx_expand_scaled<HALF>(pw, l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, c), lo[p]);
-    mx_expand_scaled<HALF>(pw, h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, c), hi[p]);
+    mx_expand_scaled<HALF, HALF>(pw, l[p], mx_multiplier<HALF>((sl >> (8 * p)) & 255u, off), lo[p], step);
+    mx_expand_scaled<HALF, HALF>(pw, h[p], mx_multiplier<HALF>((sh >> (8 * p)) & 255u, off), hi[p], step);
   }
 }
 
@@ -808,10 +836,9 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
     return;
   }
 
-  uint32_t f0;
-  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(prm.mx) : "memory");
-  const int c = mx_shift<HALF>(f0);
-  const float factor = scalbnf(1.f, c);
+  const MxScaling<HALF> sc(prm.mx, 0);
+  const float factor = scalbnf(1.f, sc.c);
+  const uint32_t step = sc.far ? kMxHalfStep : 0x3C003C00u;
   const int g = lane >> 2, t = lane & 3;
   const int wo = warp / WK, wk = warp - wo * WK;
   const MxPowers pw;
@@ -840,7 +867,7 @@ qlin_mx_many_kernel(const MxFewParams<T> prm) {
         const uint32_t base = smem_u32(mx_smem) + s * Cfg::kStage;
         uint32_t lo[4][4], hi[4][4];
         if constexpr (WIDE) mx_load_a_wide<HALF>(base + (wo * WK + wk) * kRecord, g, t, lo, hi);
-        else mx_load_a<HALF>(pw, base + (wo * WK + wk) * kRecord, g, t, c, lo, hi);
+        else mx_load_a<HALF>(pw, base + (wo * WK + wk) * kRecord, g, t, sc.off, step, lo, hi);
         const uint32_t xb = base + WO * WK * kRecord + wk * Cfg::kXBlock + g * 64 + t * 16;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {

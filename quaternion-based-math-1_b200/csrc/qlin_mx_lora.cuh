@@ -82,9 +82,7 @@ qlin_mx_turn_all_kernel(const uint8_t* mx, const MxPlanes<T> dst, int64_t ld, in
   const int64_t kb = (K_g + kMxBlock - 1) / kMxBlock, tiles = (N_g + kMxRows - 1) / kMxRows;
   const int64_t og = blockIdx.x / kb, blk = blockIdx.x - og * kb;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = warp & 3, ph = warp >> 2;
-  uint32_t f0;
-  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(mx) : "memory");
-  const int c = mx_shift<HALF>(f0, a_rows > 0 ? 1 : 0);
+  const MxScaling<HALF> sc(mx, a_rows > 0 ? 1 : 0);
   const int row = 2 * lane;  // of 64
   const int64_t tile = 4 * og + row / kMxRows;
   uint2 w[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
@@ -104,9 +102,12 @@ qlin_mx_turn_all_kernel(const uint8_t* mx, const MxPlanes<T> dst, int64_t ld, in
     const int p = 2 * ph + h;
     uint32_t e[2][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      mx_expand_scaled<HALF>(pw, h ? w[u].y : w[u].x,
-                             mx_multiplier<HALF>((f[u] >> (8 * h)) & 255u, c) ^ (p ? 0x80008000u : 0u), e[u]);
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t word = h ? w[u].y : w[u].x;
+      const uint32_t mult = mx_multiplier<HALF>((f[u] >> (8 * h)) & 255u, sc.off) ^ (p ? 0x80008000u : 0u);
+      if (HALF && sc.far) mx_expand_scaled<HALF, HALF>(pw, word, mult, e[u]);
+      else mx_expand_scaled<HALF, false>(pw, word, mult, e[u]);
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       turned[p * kMxBlock + 8 * t + k][lane] = __byte_perm(e[0][k], e[1][k], 0x5410);

@@ -29,7 +29,7 @@
 // an accumulator that f16 ones began.  The builders fetch their rows of B before they
 // wait for the stage.
 //
-// The accumulator holds y 2^-c (mx_shift); B is built with the same factor, and
+// The accumulator holds y 2^-c (MxScaling); B is built with the same factor, and
 // the epilogue multiplies by 2^c before the bias and the one rounding.
 #pragma once
 
@@ -189,9 +189,8 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     n0 = nb * 256 + (int)cta * kPairRows;  // this CTA's first real output
     m0 = tb * NTOK;                        // the pair's first token
   };
-  uint32_t f0;
-  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(f0) : "l"(prm.mx) : "memory");
-  const int c = mx_shift<HALF>(f0, prm.rank);  // the accumulator holds y 2^-c
+  const MxScaling<HALF> sc(prm.mx, prm.rank);
+  const int c = sc.c;  // the accumulator holds y 2^-c
 
   if (warp == 0) {
     // ---------------- copies of this CTA's x half-tile and weights ----------------
@@ -364,36 +363,41 @@ qlin_mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         const uint32_t scales = lds32(rec + kMxCodeBytes + r16 * 4);
         uint32_t mult[4];  // of component a^q, with its sign
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mult[q] = mx_multiplier<HALF>((scales >> (8 * (a ^ q))) & 255u, c) ^ sign[q];
+        for (int q = 0; q < 4; ++q) mult[q] = mx_multiplier<HALF>((scales >> (8 * (a ^ q))) & 255u, sc.off) ^ sign[q];
+        auto expand = [&](auto far) {
+          constexpr bool FAR = decltype(far)::value;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {  // octet 2h + o: columns 16 of 32
-            const uint4 w4 = lds128(rec + r16 * 64 + (2 * h + o) * 16);
-            uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            if (a & 1) {
-              uint32_t x = w[0]; w[0] = w[1]; w[1] = x;
-              x = w[2]; w[2] = w[3]; w[3] = x;
+            for (int o = 0; o < 2; ++o) {  // octet 2h + o: columns 16 of 32
+              const uint4 w4 = lds128(rec + r16 * 64 + (2 * h + o) * 16);
+              uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+              if (a & 1) {
+                uint32_t x = w[0]; w[0] = w[1]; w[1] = x;
+                x = w[2]; w[2] = w[3]; w[3] = x;
+              }
+              if (a & 2) {
+                uint32_t x = w[0]; w[0] = w[2]; w[2] = x;
+                x = w[1]; w[1] = w[3]; w[3] = x;
+              }
+              uint32_t e[4][4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) mx_expand_scaled<HALF, FAR>(pw, w[q], mult[q], e[q]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                r[16 * o + 2 * i] = __byte_perm(e[0][i], e[1][i], 0x5410);
+                r[16 * o + 2 * i + 1] = __byte_perm(e[2][i], e[3][i], 0x5410);
+                r[16 * o + 8 + 2 * i] = __byte_perm(e[0][i], e[1][i], 0x7632);
+                r[16 * o + 8 + 2 * i + 1] = __byte_perm(e[2][i], e[3][i], 0x7632);
+              }
             }
-            if (a & 2) {
-              uint32_t x = w[0]; w[0] = w[2]; w[2] = x;
-              x = w[1]; w[1] = w[3]; w[3] = x;
-            }
-            uint32_t e[4][4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) mx_expand_scaled<HALF>(pw, w[q], mult[q], e[q]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              r[16 * o + 2 * i] = __byte_perm(e[0][i], e[1][i], 0x5410);
-              r[16 * o + 2 * i + 1] = __byte_perm(e[2][i], e[3][i], 0x5410);
-              r[16 * o + 8 + 2 * i] = __byte_perm(e[0][i], e[1][i], 0x7632);
-              r[16 * o + 8 + 2 * i + 1] = __byte_perm(e[2][i], e[3][i], 0x7632);
-            }
+            __syncwarp();
+            tmem_st32(col + 32 * h, r);
           }
-          __syncwarp();
-          tmem_st32(col + 32 * h, r);
-        }
+        };
+        if (HALF && sc.far) expand(std::integral_constant<bool, HALF>());
+        else expand(std::false_type());
         tmem_st_wait();
       } else if (!*abort_flag) {
         // W_a[o, 32 inputs]: 64 bytes, chunk u at chunk u ^ ((row >> 1) & 3) (64-byte swizzle);

@@ -77,3 +77,36 @@ def test_quantize_model_says_what_it_leaves(qb, cuda):
     with pytest.raises(ValueError):
         qb.quantize_model(alone)
     assert isinstance(alone.wr, torch.nn.Parameter)
+
+
+# ---------------------------------------------------------------- far apart scales
+@pytest.mark.parametrize("M", [1, 3, 16, 32, 64, 65, 200])
+def test_fp16_rows_far_below_the_largest_weight(qb, cuda, M):
+    """Every row of an fp16 layer counts, down to fp16's smallest weights beside ones of
+    4096, with any number of tokens and in the input gradient."""
+    N_g, K_g = 48, 96
+    g = torch.Generator().manual_seed(M)
+    levels = torch.tensor([2.0 ** -8, 2.0 ** -16, 2.0 ** -22]).repeat_interleave(16)[:, None]
+    w = [(torch.randn(N_g, K_g, generator=g) * levels).half() for _ in range(4)]
+    for t in w:
+        t[0, :32] = torch.randn(32, generator=g).half() * 2048  # x is zero there
+    q = qb.quantize_quaternion_weights(*(t.to(cuda) for t in w))
+    v = torch.stack(q.dequantize(torch.float32)).double().cpu().numpy()
+    x = torch.randn(M, 4 * K_g, generator=g) * 256
+    x[:, :128] = 0
+    x = x.half().to(cuda)
+    y = qb.mx_quaternion_linear(x, q)
+    want = ref.layer(ref.f64(x), v)
+    small = 2.0 ** -25 / 2.0 ** -12  # half of fp16's smallest step, results of at least 2^-12
+    for k in range(3):
+        rows = slice(64 * k, 64 * k + 64)
+        assert ref.rel(ref.f64(y)[:, rows], want[:, rows]) <= ref.tolerance("f16", 4 * K_g) + small, k
+    # the gradient: columns of one level at a time
+    for k in range(3):
+        gy = torch.zeros(M, 4 * N_g)
+        gy[:, 64 * k + 4:64 * k + 64] = torch.randn(M, 60, generator=g) * 256
+        gy = gy.half().to(cuda)
+        xg = x.clone().requires_grad_(True)
+        (dx,) = torch.autograd.grad(qb.mx_quaternion_linear(xg, q), xg, gy)
+        want = ref.gradients(ref.f64(gy), ref.f64(x), v)[0]
+        assert ref.rel(ref.f64(dx), want) <= ref.tolerance("f16", 4 * N_g) + small, k
