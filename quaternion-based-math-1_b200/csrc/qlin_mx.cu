@@ -71,13 +71,17 @@ struct Carve {
   }
 };
 
+// SM count that the rules below reckon with: they size workspaces, which do not depend
+// on the device.  (Launches take the device's own.)
+constexpr int64_t kRuleSms = 148;
+
 // 16-bit inputs of up to 32 tokens take the streaming kernels (qlin_mx_few.cuh; 5120 ->
 // 27648 at 32 tokens 39 against 47 us), and up to 64 where the layer has at most a tile
 // of 16 output quaternions per SM (4096 -> 4096 at 64 tokens 13 against 21 us, 5120 ->
 // 27648 70 against 47); more take the CTA-pair kernel (qlin_mx_pair.cuh).  fp32 always
 // streams.
 bool streams(int dtype, int64_t M, int64_t N_g) {
-  return dtype == QLIN_F32 || M <= 32 || (M <= 64 && N_g <= 148 * kMxRows);
+  return dtype == QLIN_F32 || M <= 32 || (M <= 64 && N_g <= kRuleSms * kMxRows);
 }
 
 // Tokens of a tile of the streaming kernels (one or two tokens apart).  16 bits: two
@@ -90,8 +94,8 @@ bool streams(int dtype, int64_t M, int64_t N_g) {
 int few_tile(int dtype, int64_t M, int64_t N_g) {
   if (M <= 16) return M <= 8 ? 8 : 16;
   if (dtype != QLIN_F32) return M <= 32 ? 16 : 32;
-  const int64_t waves16 = ceil_div(ceil_div(N_g, 2 * kMxRows) * ceil_div(M, 16), 148);
-  const int64_t waves32 = ceil_div(ceil_div(N_g, 4 * kMxRows) * ceil_div(M, 32), 148);
+  const int64_t waves16 = ceil_div(ceil_div(N_g, 2 * kMxRows) * ceil_div(M, 16), kRuleSms);
+  const int64_t waves32 = ceil_div(ceil_div(N_g, 4 * kMxRows) * ceil_div(M, 32), kRuleSms);
   return 2 * waves16 <= 7 * waves32 ? 16 : 32;
 }
 
