@@ -14,7 +14,7 @@
 // what the first has left in L2; a set that L2 holds is read from HBM once.
 // 48 bf16 gradients, 270 MB: 136 us (4.0 TB/s if only one read and the write count;
 // three passes at HBM's rate: 124 us).  48 fp32 gradients of adapters, 25 MB, which L2
-// holds: 16.5 us.
+// holds: 17 us.
 // (Evict-first hints for all but the last 40 or 72 MB of the first pass changed
 // nothing: 134 to 142 us for 270 MB either way.)
 //

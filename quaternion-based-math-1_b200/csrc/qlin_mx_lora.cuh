@@ -7,17 +7,17 @@
 // t and u are kept as parts (or in fp32): rounded to one they would add an error of the
 // size of the results' own rounding.  The CTA-pair kernel takes them as three bf16 parts
 // (exact), dA and dB as three bf16 ones or two f16 ones with a power of two per rank and
-// 16 tokens (mx_top_scale).  x and gy are read
-// once for t and u and once for the gradients, which bounds these kernels; the
-// products are warp-level tensor-core ones (m16n8k16) whose k slots are numbered
-// so that a lane reads eight consecutive elements of a row in one 16-byte piece
-// for both operands (2 M r (K + N) operations are too few for tcgen05 tiles: rank 32
-// fills a quarter of one).
+// 16 tokens (mx_top_scale).  x and gy are read once for t and u and once for the
+// gradients, which bounds the down projections; the products are warp-level tensor-core
+// ones (m16n8k16) whose k slots are numbered so that a lane reads eight consecutive
+// elements of a row in one 16-byte piece for both operands (2 M r (K + N) operations are
+// too few for tcgen05 tiles: rank 32 fills a quarter of one).
 //
 // 4096 layer, 2048 bf16 tokens, rank 32 (x and gy: 16.8 MB each), each launch by
-// itself: t in the forward pass 11.0 us, everything turned 6.5 us, t and u 13.3 us
-// (2.5 TB/s), dA, dB and dbias 15.0 us and the sum of their parts 4.5 us.  The first
-// runs under the product's start, dA and dB partly beside the input gradient's end.
+// itself: t in the forward pass 10.0 us, everything turned 6.8 us, t and u 14.5 us
+// (2.3 TB/s), dA, dB and dbias 20.1 us (15.0 with two parts: their products bound it) and
+// the sum of their partial sums 5.7 us.  The first runs under the product's start, dA and
+// dB partly beside the input gradient's end.
 //
 // (Inputs are not declared restrict: the compiler may read through such pointers
 // before the dependency wait.)

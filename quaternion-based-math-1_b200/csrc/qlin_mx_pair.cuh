@@ -18,7 +18,7 @@
 //
 // Bound by the tensor pipe at 256 tokens (84 % of all cycles): 4096 -> 11008 at 2048
 // bf16 tokens 113 us in a burst (1630 TFLOP/s), 134 us sustained (1380, at the power
-// limit); 5120 -> 27648 with an adapter of rank 32 368 and 421 us.
+// limit); 5120 -> 27648 with an adapter of rank 32 365 and 424 us.
 //
 // Adapter: y += t B^T with t = s x A^T and B as sums of bf16 parts, for fp16 too: bf16
 // has fp32's range, so that neither a large B nor a small or large t leaves it.  t =
