@@ -456,7 +456,9 @@ int qlin_mx_dequantize(int dtype, const void* mx, int64_t K_g, int64_t N_g,
  * At most 2^31 - 1024 tokens and rank 2^24 (QLIN_ERR_SHAPE).
  * 16-bit types with more than 32 tokens want y 8-byte aligned and ld_y a multiple
  * of 4 (QLIN_ERR_ALIGN).  The down projection is kept in fp32's range and precision
- * for every type.  Waits inside the kernels are bounded (qlin_get_device_error).
+ * for every type.  fp16 and three tokens or more: blocks whose scale is below 2^-36 of
+ * the layer's largest are rounded at 2^-37 of that.  Waits inside the kernels are
+ * bounded (qlin_get_device_error).
  */
 int qlin_mx_workspace_size(int dtype, int64_t M, int64_t K_g, int64_t N_g, int rank, size_t* bytes);
 int qlin_mx_forward(int dtype,

@@ -22,10 +22,12 @@ def clip_grad_norm(parameters, max_norm: float, error_if_nonfinite: bool = False
     are skipped, one that comes up twice counts once.  Gradients may be
     float32, bfloat16 and float16 side by side; sums are kept in 64 bits in a
     fixed order.  An infinite ``max_norm`` gives the norm and leaves the
-    gradients; with a NaN norm every gradient becomes NaN otherwise;
+    gradients; otherwise a NaN norm makes every gradient NaN and an infinite
+    one (past float32's range, too) zero, infinite ones NaN;
     ``error_if_nonfinite`` raises ``RuntimeError`` instead (the host then waits
     for the norm; the gradients are unchanged).  Gradients of different
-    parameters must not overlap in memory.
+    parameters must not overlap in memory; one that cannot be written in place
+    is refused before any is scaled.
     """
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]

@@ -8,8 +8,11 @@ bits a weight.  They serve inference and, with
 constant, gradients reach the input, the bias and the LoRA factors.
 
 ``x``, bias, LoRA factors and outputs are float32, bfloat16 or float16, sums
-are fp32; with float32 inputs the products are those of fp32 arithmetic.  CPU
-tensors raise ``RuntimeError`` -- there is no CPU path.
+are fp32; with float32 inputs the products are those of fp32 arithmetic.  The
+weights enter exactly; with float16 inputs of three tokens or more that holds
+for blocks whose scale is at least 2^-36 of the layer's largest (all float16
+weights below 8192), others are rounded at 2^-37 of it.  CPU tensors raise
+``RuntimeError`` -- there is no CPU path.
 """
 
 from __future__ import annotations
