@@ -317,7 +317,7 @@ at::Tensor clip_grad_norm(const pybind11::iterable& parameters, double max_norm,
     check_cuda(g, grads[0], false);
     types.push_back(dtype_code(g.scalar_type()));
     // nothing is written before every gradient is known to be writable
-    at::assert_no_internal_overlap(g);
+    if (!g.is_contiguous()) at::assert_no_internal_overlap(g);
     TORCH_CHECK(!g.is_inference() || c10::InferenceMode::is_enabled(),
                 "a gradient made in inference mode cannot be clipped outside it");
   }
